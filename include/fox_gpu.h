@@ -389,6 +389,78 @@ fox_gpu_status fox_gpu_batch_attention(fox_gpu_ctx *ctx, float *out, size_t out_
                                        size_t head_dim, size_t M, const uint32_t *pos,
                                        size_t n_ctx);
 
+/* --------------------------------------------------- quantised caches */
+
+/* A layer's keys and values in 4 or 8 bits instead of 32, for contexts whose
+ * float caches would fill the GPU or bound its decode (no counterpart in
+ * RustFox, whose cache is f32).  One block of device memory per layer, of
+ * fox_gpu_kvq_bytes bytes (4.25 and 8.25 bits a value, head_dim taken up to
+ * the next of 32, 64, 96, 128, 192, 256), 16-byte aligned; its contents need no
+ * clearing, its layout is the library's own (read it with fox_gpu_kvq_read).
+ *
+ * Each head's dimensions are quantised in groups of 32 per position.  A
+ * group's scale d has 5 exponent and 3 mantissa bits: the least one, from
+ * 2^-19 on, with max <= (h - 1/2) d and -min <= (h + 1/2) d, h = 8 or 128; a value x is
+ * held as d round(x / d), ties to even, so to within d / 2.  Scales end at 224 (Q4) and
+ * 120 (Q8): values past 1680 and 15300 saturate.  A group that holds a NaN
+ * or an infinity reads as NaN.
+ *
+ * head_dim is even and at most 256 (else FOX_GPU_ERR_UNSUPPORTED), n_ctx at
+ * most 2^30.  Strides are in floats, used when there is more than one row,
+ * and at least the row's width.  pos[0] is the position of the first row,
+ * read on the device (one graph serves every step); rows whose position is
+ * not below n_ctx are not stored. */
+enum { FOX_GPU_KV_Q4 = 4, FOX_GPU_KV_Q8 = 8 };
+
+/* bytes of a layer's cache; 0 for a shape that is not taken */
+size_t fox_gpu_kvq_bytes(int kv_type, size_t n_ctx, size_t n_head_kv, size_t head_dim);
+
+/* M <= n_ctx rows of n_head_kv * head_dim floats into positions pos[0] + i.
+ * Other positions keep what they hold. */
+fox_gpu_status fox_gpu_kvq_write(fox_gpu_ctx *ctx, int kv_type, void *cache, size_t n_ctx,
+                                 size_t n_head_kv, size_t head_dim, const uint32_t *pos, size_t M,
+                                 const float *k, size_t k_stride, const float *v, size_t v_stride);
+
+/* Rows p0 .. p0+n-1 as floats; k or v may be NULL. */
+fox_gpu_status fox_gpu_kvq_read(fox_gpu_ctx *ctx, int kv_type, const void *cache, size_t n_ctx,
+                                size_t n_head_kv, size_t head_dim, size_t p0, size_t n,
+                                float *k, size_t k_stride, float *v, size_t v_stride);
+
+/* Queries and keys normed head by head, rotated, and keys and values stored,
+ * in one launch, for M <= FOX_GPU_BATCH_TOKENS tokens at positions pos[0] + t:
+ *   x' = x / sqrt(mean(x^2) + eps) * w over each head of q and k, with
+ *   w = q_norm, k_norm (head_dim floats; NULL: that one is not normed),
+ * then every pair of dimensions rotated by its position's angle: (2j, 2j+1), as
+ * fox_gpu_rope_store does, or (j, j + head_dim/2).  Computed in double and
+ * rounded once.  Queries go to q_out (which may be q, with its stride), keys
+ * and values to the float caches of fox_gpu_rope_store or to a quantised
+ * one; k and v are left as they are.  Tables are n_ctx rows of
+ * head_dim/2 cosines and sines.  A token whose position is not below n_ctx is
+ * neither turned nor stored. */
+enum { FOX_GPU_PAIRS_ADJACENT = 0, FOX_GPU_PAIRS_HALVES = 1 };
+fox_gpu_status fox_gpu_norm_rope_store(
+    fox_gpu_ctx *ctx, const float *q, size_t q_stride, float *q_out, size_t q_out_stride,
+    const float *k, size_t k_stride, const float *v, size_t v_stride, size_t n_head,
+    size_t n_head_kv, size_t head_dim, size_t M, const float *q_norm, const float *k_norm, float eps,
+    int pairs, const float *cos_t, const float *sin_t, const uint32_t *pos, size_t n_ctx,
+    float *k_cache, float *v_cache);
+fox_gpu_status fox_gpu_kvq_norm_rope_store(
+    fox_gpu_ctx *ctx, const float *q, size_t q_stride, float *q_out, size_t q_out_stride,
+    const float *k, size_t k_stride, const float *v, size_t v_stride, size_t n_head,
+    size_t n_head_kv, size_t head_dim, size_t M, const float *q_norm, const float *k_norm, float eps,
+    int pairs, const float *cos_t, const float *sin_t, const uint32_t *pos, int kv_type,
+    void *cache, size_t n_ctx);
+
+/* Causal GQA attention of M <= FOX_GPU_BATCH_TOKENS tokens at positions
+ * pos[0] + t over positions 0 .. pos[0] + t of a quantised cache:
+ * softmax(q.k / sqrt(hd)) v, for any number of query heads per kv head.  The
+ * cache's values are multiplied as they are; sums, maxima and the softmax are in
+ * 32 bits.  out must not overlap q. */
+fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, size_t out_stride,
+                                     const float *q, size_t q_stride, int kv_type,
+                                     const void *cache, size_t n_head, size_t n_head_kv,
+                                     size_t head_dim, size_t M, const uint32_t *pos, size_t n_ctx);
+
 /* ------------------------------------------------------------- graphs */
 
 /* Record the work queued on the context's stream between begin and end into

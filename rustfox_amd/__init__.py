@@ -25,6 +25,8 @@ F32, F16, Q4_K, Q6_K, TQ1_0, TQ2_0 = 0, 1, 12, 14, 34, 35
 ACT_PER_VECTOR, ACT_PER_BLOCK = 0, 1
 GEMV_ACCUMULATE = 1
 ATTN_SPLIT, ATTN_EXACT = 0, 1
+KV_Q4, KV_Q8 = 4, 8
+PAIRS_ADJACENT, PAIRS_HALVES = 0, 1
 MAX_TOKENS = 8
 BATCH_TOKENS = 1024
 
@@ -118,6 +120,13 @@ def gpu_lib() -> C.CDLL:
         "fox_gpu_batch_rope_store": [vp, vp, sz, vp, sz, vp, sz, sz, sz, sz, sz, vp, vp, vp, sz,
                                      vp, vp],
         "fox_gpu_batch_attention": [vp, vp, sz, vp, sz, vp, vp, sz, sz, sz, sz, vp, sz],
+        "fox_gpu_kvq_write": [vp, C.c_int, vp, sz, sz, sz, vp, sz, vp, sz, vp, sz],
+        "fox_gpu_kvq_read": [vp, C.c_int, vp, sz, sz, sz, sz, sz, vp, sz, vp, sz],
+        "fox_gpu_norm_rope_store": [vp, vp, sz, vp, sz, vp, sz, vp, sz, sz, sz, sz, sz, vp, vp,
+                                    C.c_float, C.c_int, vp, vp, vp, sz, vp, vp],
+        "fox_gpu_kvq_norm_rope_store": [vp, vp, sz, vp, sz, vp, sz, vp, sz, sz, sz, sz, sz, vp, vp,
+                                        C.c_float, C.c_int, vp, vp, vp, C.c_int, vp, sz],
+        "fox_gpu_kvq_attention": [vp, vp, sz, vp, sz, C.c_int, vp, sz, sz, sz, sz, vp, sz],
         "fox_gpu_silu_mul": [vp, vp, vp, sz, sz, sz],
         "fox_gpu_add": [vp, vp, vp, sz, sz, sz],
         "fox_gpu_argmax": [vp, vp, sz, vp, vp, C.c_uint32, vp],
@@ -137,6 +146,8 @@ def gpu_lib() -> C.CDLL:
                                      "fox_gpu_graph_free", "fox_gpu_event_destroy") else C.c_int
     L.fox_gpu_last_error.restype = C.c_char_p
     L.fox_gpu_last_error.argtypes = []
+    L.fox_gpu_kvq_bytes.restype = C.c_size_t
+    L.fox_gpu_kvq_bytes.argtypes = [C.c_int, sz, sz, sz]
     L.fox_gpu_workspace_bytes.restype = C.c_size_t
     L.fox_gpu_workspace_bytes.argtypes = [vp]
     _gpu = L
@@ -403,6 +414,62 @@ class Gpu:
         _check(self.lib.fox_gpu_batch_attention(self.ctx, out.ptr, n_head * hd, q.ptr, n_head * hd,
                                                 kc.ptr, vc.ptr, n_head, n_head_kv, hd, M, pos.ptr,
                                                 n_ctx))
+
+    # -- quantised caches (kv_type KV_Q4 or KV_Q8; strides default to the row's width)
+    def kvq_bytes(self, kv_type, n_ctx, n_head_kv, head_dim) -> int:
+        """Bytes of a layer's quantised cache (0: a shape that is not taken)."""
+        return int(self.lib.fox_gpu_kvq_bytes(kv_type, n_ctx, n_head_kv, head_dim))
+
+    def kvq_write(self, kv_type, cache: DeviceArray, n_ctx, n_head_kv, head_dim, pos: DeviceArray,
+                  M, k: DeviceArray, v: DeviceArray, k_stride=None, v_stride=None):
+        """M rows of keys and values into positions pos[0] .. of a quantised cache."""
+        w = n_head_kv * head_dim
+        _check(self.lib.fox_gpu_kvq_write(self.ctx, kv_type, cache.ptr, n_ctx, n_head_kv, head_dim,
+                                          pos.ptr, M, k.ptr, k_stride or w, v.ptr, v_stride or w))
+
+    def kvq_read(self, kv_type, cache: DeviceArray, n_ctx, n_head_kv, head_dim, p0, n,
+                 k: DeviceArray = None, v: DeviceArray = None, k_stride=None, v_stride=None):
+        """Rows p0 .. p0 + n - 1 of a quantised cache as floats."""
+        w = n_head_kv * head_dim
+        _check(self.lib.fox_gpu_kvq_read(self.ctx, kv_type, cache.ptr, n_ctx, n_head_kv, head_dim,
+                                         p0, n, k.ptr if k else None, k_stride or w,
+                                         v.ptr if v else None, v_stride or w))
+
+    def norm_rope_store(self, q: DeviceArray, k: DeviceArray, v: DeviceArray, q_out: DeviceArray,
+                        n_head, n_head_kv, head_dim, M, q_norm: DeviceArray, k_norm: DeviceArray,
+                        eps, pairs, cos_t: DeviceArray, sin_t: DeviceArray, pos: DeviceArray,
+                        n_ctx, kc: DeviceArray, vc: DeviceArray, q_stride=None, q_out_stride=None,
+                        k_stride=None, v_stride=None):
+        """Head norms (None: none), rotation and the store into the float caches."""
+        nq, nk = n_head * head_dim, n_head_kv * head_dim
+        _check(self.lib.fox_gpu_norm_rope_store(
+            self.ctx, q.ptr, q_stride or nq, q_out.ptr, q_out_stride or nq, k.ptr, k_stride or nk,
+            v.ptr, v_stride or nk, n_head, n_head_kv, head_dim, M, q_norm.ptr if q_norm else None,
+            k_norm.ptr if k_norm else None, eps, pairs, cos_t.ptr, sin_t.ptr, pos.ptr, n_ctx,
+            kc.ptr, vc.ptr))
+
+    def kvq_norm_rope_store(self, q: DeviceArray, k: DeviceArray, v: DeviceArray,
+                            q_out: DeviceArray, n_head, n_head_kv, head_dim, M,
+                            q_norm: DeviceArray, k_norm: DeviceArray, eps, pairs,
+                            cos_t: DeviceArray, sin_t: DeviceArray, pos: DeviceArray, kv_type,
+                            cache: DeviceArray, n_ctx, q_stride=None, q_out_stride=None,
+                            k_stride=None, v_stride=None):
+        """Head norms (None: none), rotation and the store into a quantised cache."""
+        nq, nk = n_head * head_dim, n_head_kv * head_dim
+        _check(self.lib.fox_gpu_kvq_norm_rope_store(
+            self.ctx, q.ptr, q_stride or nq, q_out.ptr, q_out_stride or nq, k.ptr, k_stride or nk,
+            v.ptr, v_stride or nk, n_head, n_head_kv, head_dim, M, q_norm.ptr if q_norm else None,
+            k_norm.ptr if k_norm else None, eps, pairs, cos_t.ptr, sin_t.ptr, pos.ptr, kv_type,
+            cache.ptr, n_ctx))
+
+    def kvq_attention(self, out: DeviceArray, q: DeviceArray, kv_type, cache: DeviceArray, n_head,
+                      n_head_kv, head_dim, M, pos: DeviceArray, n_ctx, q_stride=None,
+                      out_stride=None):
+        """Causal attention of M tokens at positions pos[0] .. over a quantised cache."""
+        w = n_head * head_dim
+        _check(self.lib.fox_gpu_kvq_attention(self.ctx, out.ptr, out_stride or w, q.ptr,
+                                              q_stride or w, kv_type, cache.ptr, n_head, n_head_kv,
+                                              head_dim, M, pos.ptr, n_ctx))
 
     def event(self):
         e = C.c_void_p()

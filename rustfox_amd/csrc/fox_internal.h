@@ -197,3 +197,6 @@ fox_gpu_status fox_float_gemv(fox_gpu_ctx *ctx, const fox_gpu_tensor *w, const f
 fox_gpu_status fox_few_gemv(fox_gpu_ctx *ctx, size_t n, const fox_gpu_tensor *const *ws,
                             const float *x, size_t x_stride, size_t M, float *const *outs,
                             const size_t *out_strides, unsigned flags, uint8_t *fixed);
+// the shapes quantised caches take (fox_kvq.hip); `what` names the caller in the message
+fox_gpu_status fox_kvq_shape(const char *what, int kv_type, size_t n_ctx, size_t n_head_kv,
+                             size_t head_dim);
