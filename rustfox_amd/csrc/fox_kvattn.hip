@@ -1,72 +1,425 @@
-// fox_kvattn.hip -- causal attention over a quantised cache.
+// fox_kvattn.hip -- causal attention over a quantised cache on the matrix
+// cores.
+//
+// Arithmetic.  The cache's values are exactly halves (fox_kvq_dev.h), so an
+// f16 MFMA multiplies them without rounding; the other operand, the query or the
+// softmax's weight, is the sum of two halves (22 bits of it), each its own MFMA into
+// the same float sums.  A query head's row is scaled by a power of two first, its
+// largest value to 2^14, so that the lower half is not lost below the half's range.
+//
+// Layout of one step, 32 positions (a tile) of one kv head by 16 query rows (row =
+// token * G + head in the group of G = n_head / n_head_kv that share it):
+//   S[pos][row] = sum_d K[pos][d] q[row][d]   two 16x16x32 MFMA rows of 16
+//     positions; lane (r, c) = (lane % 16, lane / 16) supplies position r's
+//     dimensions of chunk c, a contiguous quarter of the row, and holds row r's
+//     scores of positions 16 i + 4 c + 0..3 afterwards
+//   O[dim][row] += sum_pos V[dim][pos] P[pos][row]   the weights of those eight
+//     positions are that lane's operand as they stand, since a V word holds
+//     just those positions (fox_kvq_dev.h).
+// The running maximum only follows scores that pass it by 8 (in powers of two):
+// weights are exp2(s - m + 7) <= 2^15, within a half; between updates no lane
+// needs another's maximum.
 #include "fox_kvq_dev.h"
 #include "fox_internal.h"
 
 #include <cfloat>
 #include <cmath>
 
-// One workgroup per (query head, token): a position a thread for the scores,
-// a running maximum and sum, a column a thread for the values.
+typedef _Float16 h2v __attribute__((ext_vector_type(2)));
+typedef _Float16 h8v __attribute__((ext_vector_type(8)));
+typedef float f4v __attribute__((ext_vector_type(4)));
+typedef uint32_t u4v __attribute__((ext_vector_type(4)));
+
+#define KA_WAVES 4
+#define KA_ROOM 8.0f            // how far scores may pass the running maximum
+#define KA_LIFT 7.0f            // weights are scaled by 2^7: 2^(8 + 7) is within a half
+
+struct AttnArgs {
+    float *out, *part;
+    size_t out_stride, q_stride;
+    const float *q;
+    const uint8_t *cache;
+    const uint32_t *pos;
+    size_t n_ctx;
+    int n_head_kv, G, hd, M, splits, q_wide;
+};
+
+__device__ __forceinline__ h2v as_h2(uint32_t v) { return __builtin_bit_cast(h2v, v); }
+__device__ __forceinline__ uint32_t as_u(h2v v) { return __builtin_bit_cast(uint32_t, v); }
+
+// eight values 4 d (c) as halves from their codes w and the scales' halves d
+// (a pair per two values): 4 bits as (64 + n) d - 72 d, one rounding of an
+// exact result; 8 bits as ((1024 + n) - 1152) d
 template <int BITS>
-__global__ __launch_bounds__(256) void kv_attn_plain(float *out, size_t out_stride, const float *q,
-                                                     size_t q_stride, const uint8_t *cache,
-                                                     int n_head, int n_head_kv, int hd,
-                                                     const uint32_t *pos, size_t n_ctx)
+__device__ __forceinline__ h8v unpack(const uint32_t *w, const h2v d[4], const h2v m72[4])
 {
-    constexpr int H = 1 << (BITS - 1);
-    __shared__ float qs[KVQ_MAXHD], ps[256], red[4];
-    const int tid = threadIdx.x, h = blockIdx.x, t = blockIdx.y, kvh = h / (n_head / n_head_kv);
-    const size_t upto = min((size_t)pos[0] + (size_t)t + 1, n_ctx);
-    const KvqLayout L = kvq_layout(BITS, hd);
-    const uint8_t *base = cache + (size_t)kvh * ((n_ctx + KVQ_TILE - 1) / KVQ_TILE) * L.record;
-    if (tid < hd) qs[tid] = q[(size_t)t * q_stride + (size_t)h * hd + tid];
-    __syncthreads();
-    float m = -FLT_MAX, l = 0.0f, o = 0.0f;
-    for (size_t p0 = 0; p0 < upto; p0 += 256) {
-        const size_t p = p0 + tid;
-        float s = -INFINITY;
-        if (p < upto) {
-            const uint8_t *rec = base + p / KVQ_TILE * L.record;
-            const int r = (int)(p % KVQ_TILE);
-            s = 0.0f;
-            for (int d = 0; d < hd; d++) {
-                const int e = d & 7;
-                const uint8_t *w = rec + (size_t)r * (L.width * BITS / 8) + (d >> 3) * BITS;
-                const int c = BITS == 4 ? (int)(*(const uint32_t *)w >> (4 * (e / 2 + 4 * (e & 1))) & 15u)
-                                        : (int)w[e];
-                s = __builtin_fmaf(qs[d], (float)(c - H) * kvq_scale(rec[L.ks + kvq_k_scale(d >> 5, r)]), s);
-            }
-            s /= sqrtf((float)hd);
+    uint32_t r[4];
+    if (BITS == 4) {
+        const uint32_t x[4] = {w[0] << 4, w[0], w[0] >> 4, w[0] >> 8};
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            r[i] = as_u(__builtin_elementwise_fma(as_h2((x[i] & 0x00F000F0u) | 0x54005400u), d[i],
+                                                  m72[i]));
+    } else {
+        const h2v off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            r[i] = as_u((as_h2(__builtin_amdgcn_perm(0x64646464u, w[i >> 1],
+                                                     i & 1 ? 0x07030702u : 0x05010500u)) + off) * d[i]);
+    }
+    return __builtin_bit_cast(h8v, *(u4v *)r);
+}
+
+__device__ __forceinline__ float quad_max(float v)
+{
+    v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float quad_sum(float v)
+{
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+
+// One tile's bytes as a lane holds them.
+template <int BITS, int NG>
+struct Tile {
+    static constexpr int NS = NG % 4 == 0 ? NG / 4 : NG < 3 ? 1 : NG;   // K scale pairs of a lane
+    uint32_t k[2][NG * BITS / 4], v[2 * NG][BITS / 4];
+    uint16_t ks[NS];
+    uint2 vs[NG];
+
+    __device__ __forceinline__ void load(const uint8_t *rec, int lane)
+    {
+        constexpr int CODES = KVQ_TILE * NG * 32 * BITS / 8;
+        const int r = lane & 15, c = lane >> 4;
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+            __builtin_memcpy(k[i], __builtin_assume_aligned(rec + (16 * i + r) * (4 * NG * BITS) + c * NG * BITS, 4 * (NG % 4 == 0 ? 4 : NG % 2 == 0 ? 2 : 1)),
+                             sizeof(k[i]));
+#pragma unroll
+        for (int s = 0; s < NS; s++) {
+            const int g = NS == NG ? (NG * c + s) / 4 : NG % 4 == 0 ? c * (NG / 4) + s : NG * c / 4;
+            ks[s] = *(const uint16_t *)(rec + 2 * CODES + g * 32 + r * 2);
         }
-        float mx = s;
-        for (int k = 32; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor(mx, k));
-        if ((tid & 63) == 0) red[tid >> 6] = mx;
-        __syncthreads();
-        const float mn = fmaxf(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), m);
-        const float e = p < upto ? expf(s - mn) : 0.0f, f = expf(m - mn);
-        ps[tid] = e;
-        float sum = e;
-        for (int k = 32; k > 0; k >>= 1) sum += __shfl_xor(sum, k);
-        __syncthreads();
-        if ((tid & 63) == 0) red[tid >> 6] = sum;
-        __syncthreads();
-        l = l * f + (red[0] + red[1] + red[2] + red[3]);
-        m = mn;
-        if (tid < hd) {
-            o *= f;
-            const int n = (int)min((size_t)256, upto - p0);
-            for (int i = 0; i < n; i++) {
-                const uint8_t *rec = base + (p0 + i) / KVQ_TILE * L.record;
-                const int r = (int)((p0 + i) % KVQ_TILE), pl = kvq_v_place(r);
-                const uint8_t *w = rec + L.v + ((size_t)tid * 4 + kvq_v_chunk(r)) * BITS;
-                const int c = BITS == 4 ? (int)(*(const uint32_t *)w >> (4 * (pl / 2 + 4 * (pl & 1))) & 15u)
-                                        : (int)w[pl];
-                o = __builtin_fmaf(ps[i], (float)(c - H) * kvq_scale(rec[L.vs + kvq_v_scale(tid >> 5, r)]), o);
+#pragma unroll
+        for (int t = 0; t < 2 * NG; t++)
+            __builtin_memcpy(v[t], __builtin_assume_aligned(rec + CODES + ((16 * t + r) * 4 + c) * BITS, BITS),
+                             sizeof(v[t]));
+#pragma unroll
+        for (int g = 0; g < NG; g++)
+            vs[g] = *(const uint2 *)(rec + 2 * CODES + 32 * NG + g * 32 + c * 8);
+    }
+    // scale pair of MFMA step j's dimensions
+    __device__ __forceinline__ uint32_t kscale(int j) const
+    {
+        return ks[NS == NG ? j : NG % 4 == 0 ? j / 4 : 0];
+    }
+};
+
+// Partial attention of T x 16 query rows over the tiles that fall to one wave
+// (tiles w0, w0 + step, ...); the four waves of a workgroup are merged through
+// LDS, and with several splits per kv head a record (m, l, -, -, o) goes to
+// the workspace for kv_merge_k.
+template <int BITS, int NG, int T>
+__global__ __launch_bounds__(64 * KA_WAVES) void kv_attn_few(AttnArgs A)
+{
+    constexpr int WIDTH = 32 * NG;
+    __shared__ f4v so[KA_WAVES][NG][64];
+    __shared__ float sm[KA_WAVES][T][16], sl[KA_WAVES][T][16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, c = lane >> 4;
+    const int split = blockIdx.x, kvh = blockIdx.y, row0 = blockIdx.z * 16 * T;
+    const int rows = A.M * A.G;
+    const size_t p0 = A.pos[0];
+    auto end_of = [&](int row) { return (int)min(p0 + (size_t)(row / A.G) + 1, A.n_ctx); };
+    const int last = end_of(min(row0 + 16 * T, rows) - 1);       // positions any row sees
+    const int first = end_of(row0);                              // and all rows see
+    const int n_tiles = (last + KVQ_TILE - 1) / KVQ_TILE, step = A.splits * KA_WAVES;
+    if (split * KA_WAVES >= n_tiles) return;                     // (uniform)
+    const int used = min(A.splits, (n_tiles + KA_WAVES - 1) / KA_WAVES);
+    const size_t recs = (A.n_ctx + KVQ_TILE - 1) / KVQ_TILE;
+    constexpr int REC = 2 * (KVQ_TILE * WIDTH * BITS / 8 + KVQ_TILE * NG);
+    const uint8_t *base = A.cache + (size_t)kvh * recs * REC;
+
+    int tile = split * KA_WAVES + wave;
+    Tile<BITS, NG> cur;
+    cur.load(base + (size_t)min(tile, n_tiles - 1) * REC, lane);
+
+    // queries: row r's dimensions of chunk c, MFMA step j the eight from 8 j on
+    h8v qh[T][NG], ql[T][NG];
+    float sc[T], m[T], l[T];
+    int end[T];
+    f4v o[T][2 * NG];
+#pragma unroll
+    for (int t = 0; t < T; t++) {
+        const int row = min(row0 + 16 * t + r, rows - 1);
+        end[t] = end_of(row);
+        const float *qr = A.q + (size_t)(row / A.G) * A.q_stride + ((size_t)kvh * A.G + row % A.G) * A.hd;
+        float x[NG][8], top = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NG; j++) {
+            const int d = 8 * (NG * c + j);
+            if (A.q_wide) {
+                const bool in = d < A.hd;
+                *(float4 *)x[j] = in ? *(const float4 *)(qr + d) : float4{0, 0, 0, 0};
+                *(float4 *)(x[j] + 4) = in ? *(const float4 *)(qr + d + 4) : float4{0, 0, 0, 0};
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[j][e] = d + e < A.hd ? qr[d + e] : 0.0f;
             }
+#pragma unroll
+            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[j][e]));
+        }
+        top = quad_max(top);
+        // 2^(14 - exponent of the largest), the exponent kept within range
+        const int ex = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 113);
+        const float up = __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
+        sc[t] = 1.44269504f / sqrtf((float)A.hd) * 0.25f * __uint_as_float((uint32_t)(127 - 14 + ex) << 23);
+#pragma unroll
+        for (int j = 0; j < NG; j++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float y = x[j][e] * up;
+                const _Float16 hi = (_Float16)y;
+                qh[t][j][e] = hi;
+                ql[t][j][e] = (_Float16)(y - (float)hi);
+            }
+        m[t] = -FLT_MAX;
+        l[t] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < 2 * NG; d++) o[t][d] = f4v{0, 0, 0, 0};
+    }
+
+    for (; tile < n_tiles; tile += step) {
+        Tile<BITS, NG> next;
+        next.load(base + (size_t)min(tile + step, n_tiles - 1) * REC, lane);
+        const int tp = tile * KVQ_TILE;
+        const bool edge = tp + KVQ_TILE > first;                 // (uniform)
+        if (edge) {
+            // positions no row sees: whatever the cache holds there counts
+            // as zero.  NaN values that only some rows see are taken out of
+            // the product and put into those rows' sums.
+            uint32_t keep[2], nan[NG][2], any = 0;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int n = min(max(last - (tp + 16 * i + 4 * c), 0), 4);    // seen ones of four
+                keep[i] = n == 4 ? ~0u : (1u << 8 * n) - 1;
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    uint32_t &b = i ? cur.vs[g].y : cur.vs[g].x;
+                    b &= keep[i];
+                    nan[g][i] = ((b & 0x78787878u) + 0x08080808u) & b & 0x80808080u;   // from 0xF8 on
+                    b &= ~((nan[g][i] << 1) - (nan[g][i] >> 7));
+                    any |= nan[g][i];
+                }
+            }
+            if (__any(any != 0)) {
+                const float bad = __uint_as_float(0x7FC00000u);
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    int p = nan[g][0] ? tp + 4 * c + (__builtin_ctz(nan[g][0]) >> 3)
+                          : nan[g][1] ? tp + 16 + 4 * c + (__builtin_ctz(nan[g][1]) >> 3) : 0x7FFFFFFF;
+                    p = min(p, __shfl_xor(p, 16));               // the group's first one
+                    p = min(p, __shfl_xor(p, 32));
+#pragma unroll
+                    for (int t = 0; t < T; t++)
+                        if (p < end[t]) o[t][2 * g] = o[t][2 * g + 1] = f4v{bad, bad, bad, bad};
+                }
+            }
+        }
+        // scores
+        f4v s[T][2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+#pragma unroll
+            for (int t = 0; t < T; t++) s[t][i] = f4v{0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < NG; j++) {
+                const uint32_t b = __builtin_amdgcn_perm(0, cur.kscale(j), i ? 0x0C010C01u : 0x0C000C00u);
+                const h2v d1 = as_h2(b << 7), m1 = d1 * (h2v){(_Float16)-72.0f, (_Float16)-72.0f};
+                const h2v d[4] = {d1, d1, d1, d1}, mm[4] = {m1, m1, m1, m1};
+                const h8v kf = unpack<BITS>(cur.k[i] + j * BITS / 4, d, mm);
+#pragma unroll
+                for (int t = 0; t < T; t++) {
+                    s[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[t][j], s[t][i], 0, 0, 0);
+                    s[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[t][j], s[t][i], 0, 0, 0);
+                }
+            }
+        }
+        // weights
+        h8v ph[T], pl[T];
+#pragma unroll
+        for (int t = 0; t < T; t++) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = s[t][e >> 2][e & 3];
+            if (edge) {
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (tp + 16 * (e >> 2) + 4 * c + (e & 3) >= end[t]) x[e] = -INFINITY;
+            }
+            float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
+                              fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))) * sc[t];
+            if (__any(top > m[t] + KA_ROOM)) {
+                const float mn = fmaxf(m[t], quad_max(top)), f = __builtin_amdgcn_exp2f(m[t] - mn);
+                m[t] = mn;
+                l[t] *= f;
+#pragma unroll
+                for (int d = 0; d < 2 * NG; d++) o[t][d] *= f;
+            }
+            const float off = KA_LIFT - m[t];
+            h2v hi[4], lo[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i], sc[t], off));
+                const float b = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i + 1], sc[t], off));
+                l[t] += a + b;
+                hi[i] = __builtin_bit_cast(h2v, __builtin_amdgcn_cvt_pkrtz(a, b));
+                lo[i] = __builtin_bit_cast(h2v, __builtin_amdgcn_cvt_pkrtz(
+                            __builtin_fmaf((float)hi[i][0], -1.0f, a),
+                            __builtin_fmaf((float)hi[i][1], -1.0f, b)));
+            }
+            ph[t] = __builtin_bit_cast(h8v, *(u4v *)hi);
+            pl[t] = __builtin_bit_cast(h8v, *(u4v *)lo);
+        }
+        // values
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            h2v d[4], mm[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                d[i] = as_h2(__builtin_amdgcn_perm(0, i < 2 ? cur.vs[g].x : cur.vs[g].y,
+                                                   i & 1 ? 0x0C030C02u : 0x0C010C00u) << 7);
+                mm[i] = d[i] * (h2v){(_Float16)-72.0f, (_Float16)-72.0f};
+            }
+#pragma unroll
+            for (int k = 2 * g; k < 2 * g + 2; k++) {
+                const h8v vf = unpack<BITS>(cur.v[k], d, mm);
+#pragma unroll
+                for (int t = 0; t < T; t++) {
+                    o[t][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[t], o[t][k], 0, 0, 0);
+                    o[t][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[t], o[t][k], 0, 0, 0);
+                }
+            }
+        }
+        cur = next;
+    }
+
+    // the four waves' sums at their common maximum (a wave without tiles has
+    // m = -FLT_MAX and l = 0), NG 16-dimension tiles of 16 rows at a time
+#pragma unroll
+    for (int t = 0; t < T; t++) {
+        l[t] = quad_sum(l[t]);
+        if (c == 0) {
+            sm[wave][t][r] = m[t];
+            sl[wave][t][r] = l[t];
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < T; t++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            if (t + h) __syncthreads();
+#pragma unroll
+            for (int d = 0; d < NG; d++) so[wave][d][lane] = o[t][h * NG + d];
+            __syncthreads();
+            const int row = row0 + 16 * t + r;
+            for (int k = wave; k < NG && row < rows; k += KA_WAVES) {
+                float mx = sm[0][t][r], sum = 0.0f;
+#pragma unroll
+                for (int w = 1; w < KA_WAVES; w++) mx = fmaxf(mx, sm[w][t][r]);
+                f4v v = {0, 0, 0, 0};
+#pragma unroll
+                for (int w = 0; w < KA_WAVES; w++) {
+                    const float f = __builtin_amdgcn_exp2f(sm[w][t][r] - mx);
+                    sum += sl[w][t][r] * f;
+                    v += so[w][k][lane] * f;
+                }
+                const int dim = 16 * (h * NG + k) + 4 * c;
+                if (used == 1) {
+                    float *dst = A.out + (size_t)(row / A.G) * A.out_stride +
+                                 ((size_t)kvh * A.G + row % A.G) * A.hd;
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (dim + e < A.hd) dst[dim + e] = v[e] * 0.25f / sum;
+                } else {
+                    float *dst = A.part + (((size_t)kvh * rows + row) * A.splits + split) * (4 + WIDTH);
+                    if (dim == 0) {
+                        dst[0] = mx;
+                        dst[1] = sum;
+                    }
+                    *(f4v *)(dst + 4 + dim) = v;
+                }
+            }
+        }
+}
+
+// One workgroup per (row, kv head): the splits' records at their common
+// maximum.  32 threads to a column quad's splits, eight split groups.
+__global__ __launch_bounds__(256) void kv_merge_k(AttnArgs A, int width, int rows_per)
+{
+    __shared__ float sm[8], sl[8];
+    __shared__ f4v so[8][32];
+    const int row = blockIdx.x, kvh = blockIdx.y, rows = A.M * A.G;
+    const int tid = threadIdx.x, sg = tid >> 5, cq = tid & 31;
+    // the splits kv_attn_few used for this row's block of rows_per
+    const int row_last = min(row / rows_per * rows_per + rows_per, rows) - 1;
+    const int last = (int)min((size_t)A.pos[0] + (size_t)(row_last / A.G) + 1, A.n_ctx);
+    const int n_tiles = (last + KVQ_TILE - 1) / KVQ_TILE;
+    const int used = min(A.splits, (n_tiles + KA_WAVES - 1) / KA_WAVES);
+    if (used == 1) return;
+    const size_t rec = 4 + (size_t)width;
+    const float *base = A.part + ((size_t)kvh * rows + row) * A.splits * rec;
+    for (int c0 = 0; c0 < width / 4; c0 += 32) {
+        const int c4 = c0 + cq;
+        float m = -FLT_MAX, l = 0.0f;
+        f4v o = {0, 0, 0, 0};
+        if (c4 < width / 4)
+            for (int s = sg; s < used; s += 8) {
+                const float *p = base + (size_t)s * rec;
+                const float ms = p[0], mn = fmaxf(m, ms), f = __builtin_amdgcn_exp2f(m - mn),
+                            g = __builtin_amdgcn_exp2f(ms - mn);
+                l = l * f + p[1] * g;
+                o = o * f + *(const f4v *)(p + 4 + 4 * c4) * g;
+                m = mn;
+            }
+        if (cq == 0) {
+            sm[sg] = m;
+            sl[sg] = l;
+        }
+        so[sg][cq] = o;
+        __syncthreads();
+        if (sg == 0 && c4 < width / 4) {
+            float mx = sm[0], sum = 0.0f;
+            for (int g = 1; g < 8; g++) mx = fmaxf(mx, sm[g]);
+            f4v v = {0, 0, 0, 0};
+            for (int g = 0; g < 8; g++) {
+                const float f = __builtin_amdgcn_exp2f(sm[g] - mx);
+                sum += sl[g] * f;
+                v += so[g][cq] * f;
+            }
+            float *dst = A.out + (size_t)(row / A.G) * A.out_stride + ((size_t)kvh * A.G + row % A.G) * A.hd;
+            for (int e = 0; e < 4; e++)
+                if (4 * c4 + e < A.hd) dst[4 * c4 + e] = v[e] * 0.25f / sum;
         }
         __syncthreads();
     }
-    if (tid < hd) out[(size_t)t * out_stride + (size_t)h * hd + tid] = o / l;
+}
+
+template <int BITS>
+static const void *few_kernel(int ng, int T)
+{
+#define FOX_FEW(n) (T == 1 ? (const void *)kv_attn_few<BITS, n, 1> : (const void *)kv_attn_few<BITS, n, 2>)
+    switch (ng) {
+    case 1: return FOX_FEW(1);
+    case 2: return FOX_FEW(2);
+    case 3: return FOX_FEW(3);
+    case 4: return FOX_FEW(4);
+    case 6: return FOX_FEW(6);
+    default: return (const void *)kv_attn_few<BITS, 8, 1>;
+    }
+#undef FOX_FEW
 }
 
 extern "C" fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, size_t out_stride,
@@ -88,15 +441,42 @@ extern "C" fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, si
     if ((uintptr_t)cache % 16)
         return fox_fail(FOX_GPU_ERR_ARG, "kvq_attention: the cache must be 16-byte aligned");
     FOX_HIP(hipSetDevice(ctx->device));
-    const dim3 grid((unsigned)n_head, (unsigned)M);
-    if (kv_type == FOX_GPU_KV_Q4)
-        hipLaunchKernelGGL(kv_attn_plain<4>, grid, dim3(256), 0, ctx->stream, out, out_stride, q,
-                           q_stride, (const uint8_t *)cache, (int)n_head, (int)n_head_kv,
-                           (int)head_dim, pos, n_ctx);
-    else
-        hipLaunchKernelGGL(kv_attn_plain<8>, grid, dim3(256), 0, ctx->stream, out, out_stride, q,
-                           q_stride, (const uint8_t *)cache, (int)n_head, (int)n_head_kv,
-                           (int)head_dim, pos, n_ctx);
-    FOX_LAUNCHED("kvq attention");
+    AttnArgs A = {};
+    A.out = out;
+    A.out_stride = out_stride;
+    A.q = q;
+    A.q_stride = q_stride;
+    A.cache = (const uint8_t *)cache;
+    A.pos = pos;
+    A.n_ctx = n_ctx;
+    A.n_head_kv = (int)n_head_kv;
+    A.G = (int)(n_head / n_head_kv);
+    A.hd = (int)head_dim;
+    A.M = (int)M;
+    A.q_wide = head_dim % 8 == 0 && (uintptr_t)q % 16 == 0 && (M == 1 || q_stride % 4 == 0);
+    const int width = kvq_width((int)head_dim), ng = width / 32;
+    const size_t rows = M * (size_t)A.G;
+    const int T = rows <= 16 || ng > 6 ? 1 : 2;
+    const size_t blocks = (rows + 16 * T - 1) / (16 * T);
+    size_t splits = 2 * (size_t)ctx->n_cu / (n_head_kv * blocks);
+    const size_t most = (n_ctx + KVQ_TILE * KA_WAVES - 1) / (KVQ_TILE * KA_WAVES);
+    if (splits > most) splits = most;
+    if (splits < 1) splits = 1;
+    A.splits = (int)splits;
+    if (splits > 1) {
+        st = fox_ws_reserve(ctx, n_head_kv * rows * splits * (4 + (size_t)width) * sizeof(float));
+        if (st) return st;
+        A.part = (float *)ctx->ws;
+    }
+    const void *k = kv_type == FOX_GPU_KV_Q4 ? few_kernel<4>(ng, T)
+                                             : few_kernel<8>(ng, T);
+    void *args[] = {&A};
+    FOX_HIP(hipLaunchKernel(k, dim3((unsigned)splits, (unsigned)n_head_kv, (unsigned)blocks),
+                            dim3(64 * KA_WAVES), args, 0, ctx->stream));
+    if (splits > 1) {
+        hipLaunchKernelGGL(kv_merge_k, dim3((unsigned)rows, (unsigned)n_head_kv), dim3(256), 0,
+                           ctx->stream, A, width, 16 * T);
+        FOX_LAUNCHED("kvq attention merge");
+    }
     return FOX_GPU_OK;
 }

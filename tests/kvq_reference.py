@@ -51,11 +51,12 @@ def norm_rope(x, hd, w, eps, cos, sin, halves):
 
 
 def attention(q, K, V, n_head, n_kv, hd, pos, n_ctx):
-    """(result, sum of weight |value|, largest sum of |q k| / sqrt(hd)) of every token's heads:
-    [M][n_head hd] twice and [M][n_head]; K, V [n_ctx][n_kv hd]."""
+    """(result, what attention_bound needs) of every token's heads, [M][n_head hd]; K, V
+    [n_ctx][n_kv hd]."""
     q, K, V = (np.asarray(a, np.float64) for a in (q, K, V))
     M = q.shape[0]
-    out, mag, top = np.empty((M, n_head * hd)), np.empty((M, n_head * hd)), np.empty((M, n_head))
+    out, mag, flat = (np.empty((M, n_head * hd)) for _ in range(3))
+    top = np.empty((M, n_head))
     for t in range(M):
         upto = min(pos + t + 1, n_ctx)
         for h in range(n_head):
@@ -66,17 +67,24 @@ def attention(q, K, V, n_head, n_kv, hd, pos, n_ctx):
             p = np.exp(s - s.max())
             p /= p.sum()
             at = slice(h * hd, (h + 1) * hd)
-            out[t, at], mag[t, at] = p @ v, p @ np.abs(v)
+            out[t, at], mag[t, at], flat[t, at] = p @ v, p @ np.abs(v), np.abs(v).sum(0)
             top[t, h] = (np.abs(k) @ np.abs(x)).max() / np.sqrt(hd)
-    return out, mag, top
+    return out, dict(mag=mag, flat=flat, top=top)
 
 
-def attention_bound(mag, top, n, hd):
+def attention_bound(sizes, n, hd):
     """How far a result may be off, element by element.  A score's products and sums in 32 bits,
     from a query held to 2^-21 of each value, are off by at most (hd + 12) 2^-23 of the sum of
-    their sizes, and by 4 roundings of the score where it is scaled and shifted, 2^-22 of it twice;
-    a weight is off by that, relatively, twice (its own and the maximum's), and by 2^-21 for the exponential and its
-    split; n weights and products are summed with at most n + 8 roundings each, above and below
-    the quotient."""
-    hd_n = np.repeat(top, mag.shape[1] // top.shape[1], 1)
-    return mag * (2 * hd_n * (hd + 16) * 2.0 ** -23 + 2 * (n + 8) * 2.0 ** -24 + 2.0 ** -20) + 1e-30
+    their sizes (top), and by 4 roundings of the score where it is scaled and shifted, 2^-22 of it
+    twice; a weight is off by that, relatively, twice (its own and the maximum's), and by 2^-21 for
+    the exponential and its split; n weights and products are summed with at most n + 8 roundings
+    each, above and below the quotient: all relative to the sum of weight |value| (mag).
+
+    The split is absolute at its end: a weight is held as two halves, the largest weight of a row as at
+    least 2^7 (its maximum may lag by 2^8, 2^15 being the most), and halves end at 2^-24, so a
+    weight is off by up to 2^-24 / 2^7 = 2^-31 of the largest, whatever its own size; the sum of
+    the weights is at least the largest, so a result by 2^-31 of the sum of |value| (flat)."""
+    mag, top = sizes["mag"], sizes["top"]
+    rows = np.repeat(top, mag.shape[1] // top.shape[1], 1)
+    return (mag * (2 * rows * (hd + 16) * 2.0 ** -23 + 2 * (n + 8) * 2.0 ** -24 + 2.0 ** -20) +
+            sizes["flat"] * 2.0 ** -31)

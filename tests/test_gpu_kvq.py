@@ -275,13 +275,13 @@ def attend(gpu, bits, c, q, n_head, n_kv, hd, n_ctx, pos, pad=0):
 
 
 def check(got, q, K, V, n_head, n_kv, hd, pos, n_ctx):
-    want, mag, top = kr.attention(q, K, V, n_head, n_kv, hd, pos, n_ctx)
+    want, sizes = kr.attention(q, K, V, n_head, n_kv, hd, pos, n_ctx)
     n = min(pos + q.shape[0], n_ctx)
     off = np.abs(got - want)
-    assert np.all(off <= kr.attention_bound(mag, top, n, hd)), (off / kr.attention_bound(mag, top, n, hd)).max()
+    assert np.all(off <= kr.attention_bound(sizes, n, hd)), (off / kr.attention_bound(sizes, n, hd)).max()
     # roundings fall either way: over all outputs they add up as their number's root
-    rel = np.linalg.norm(off) / np.linalg.norm(mag)
-    assert rel <= 2.0 ** -24 * (32 + 4 * np.sqrt(n) + 8 * np.sqrt(hd) * max(1.0, top.max())), rel
+    rel = np.linalg.norm(off) / np.linalg.norm(sizes["mag"])
+    assert rel <= 2.0 ** -24 * (32 + 4 * np.sqrt(n) + 8 * np.sqrt(hd) * max(1.0, sizes["top"].max())), rel
 
 
 @pytest.mark.parametrize("case", ATTN_CASES, ids=str)
@@ -315,11 +315,11 @@ def test_a_nan_row_reaches_only_those_who_see_it(gpu, bits, side, M):
     hit[j:, n_head // 2:, 0 if side == "k" else 32:] = True
     assert np.array_equal(np.isnan(got), hit.reshape(M, -1))
     Kz, Vz = (np.nan_to_num(kr.held(x, bits, hd)) for x in (K, V))
-    want, mag, top = kr.attention(q, Kz, Vz, n_head, n_kv, hd, pos, n_ctx)
+    want, sizes = kr.attention(q, Kz, Vz, n_head, n_kv, hd, pos, n_ctx)
     seen = ~hit.reshape(M, -1)
     if side == "k":
         seen[j:, n_head // 2 * hd:] = False
-    assert np.all(np.abs(got - want)[seen] <= kr.attention_bound(mag, top, pos + M, hd)[seen])
+    assert np.all(np.abs(got - want)[seen] <= kr.attention_bound(sizes, pos + M, hd)[seen])
 
 
 @pytest.mark.parametrize("M", [1, 5, 70])
@@ -340,8 +340,8 @@ def test_scores_far_apart(gpu, M):
     q[:, 4 * hd] = 1e6
     c = fill(gpu, 4, n_ctx, n_kv, hd, K, V)
     got = attend(gpu, 4, c, q, n_head, n_kv, hd, n_ctx, pos)
-    want, mag, top = kr.attention(q, kr.held(K, 4, hd), kr.held(V, 4, hd), n_head, n_kv, hd, pos, n_ctx)
-    assert np.all(np.abs(got - want) <= kr.attention_bound(mag, top, n, hd))
+    want, sizes = kr.attention(q, kr.held(K, 4, hd), kr.held(V, 4, hd), n_head, n_kv, hd, pos, n_ctx)
+    assert np.all(np.abs(got - want) <= kr.attention_bound(sizes, n, hd))
 
 
 @pytest.mark.parametrize("M", [1, 40])
@@ -401,8 +401,8 @@ def test_a_prompt_and_steps(gpu, bits):
         qt = kr.norm_rope(q, hd, qn, EPS, cos[at], sin[at], True).astype(np.float32)
         K[at] = kr.held(kr.norm_rope(k, hd, kn, EPS, cos[at], sin[at], True).astype(np.float32), bits, hd)
         V[at] = kr.held(v, bits, hd)
-        want, mag, top = kr.attention(qt, K, V, n_head, n_kv, hd, p, n_ctx)
-        assert np.all(np.abs(got - want) <= kr.attention_bound(mag, top, p + M, hd)), p
+        want, sizes = kr.attention(qt, K, V, n_head, n_kv, hd, p, n_ctx)
+        assert np.all(np.abs(got - want) <= kr.attention_bound(sizes, p + M, hd)), p
 
     def data(M):
         return rows(rng, M, nq), rows(rng, M, nk), rows(rng, M, nk)
