@@ -100,11 +100,11 @@ struct StoreArgs {
     size_t M, n_ctx;
     uint8_t *cache;             // quantised cache, or
     float *k_cache, *v_cache;   // the float ones
-    int wide;                   // rows take 16-byte loads and stores
+    bool wide;                  // rows take 16-byte loads and stores
 };
 
 // eight values of a row from column d on (zero past hd)
-__device__ __forceinline__ void load_8(float x[8], const float *row, int d, int hd, int wide)
+__device__ __forceinline__ void load_8(float x[8], const float *row, int d, int hd, bool wide)
 {
     if (wide) {
         *(float4 *)x = *(const float4 *)(row + d);
@@ -119,7 +119,7 @@ __device__ __forceinline__ void load_8(float x[8], const float *row, int d, int 
 // (both laid out by dimension): first members a, second members b; zero past
 // the last pair.
 __device__ __forceinline__ void load_pairs(float a[8], float b[8], const float *row, int j0, int hd,
-                                           int halves, int wide)
+                                           int halves, bool wide)
 {
     const int half = hd >> 1;
     if (wide) {
@@ -144,7 +144,7 @@ __device__ __forceinline__ void load_pairs(float a[8], float b[8], const float *
 }
 
 __device__ __forceinline__ void store_pairs(float *row, const float a[8], const float b[8], int j0,
-                                            int hd, int halves, int wide)
+                                            int hd, int halves, bool wide)
 {
     const int half = hd >> 1;
     if (wide) {
@@ -167,198 +167,259 @@ __device__ __forceinline__ void store_pairs(float *row, const float a[8], const 
 }
 
 #define KS_PAIRS 16                                    // pair items of a token, at most
-#define KS_ROW (KVQ_MAXHD + 4)
 
-// One workgroup per (tile of 32 positions, head): the tile's tokens of a kv
-// head (blockIdx.y < n_head_kv), quantised into the tile's record (BITS 4, 8)
-// or stored as floats (32); or of a query head.  ROPE: keys and queries are
-// normed and rotated on the way, eight pairs of a token an item, so a query
-// may be turned in place.  That arithmetic is in double, rounded to float
-// once: a key's code may hang on its last bit.  A quantiser's item is eight
-// columns of one token, a group of 32 a lane quad.  The V codes of a position
-// share their words with other positions', so a workgroup owns its tile's
-// words: codes pass through LDS, and words that hold positions outside the
-// pass keep those.
-template <int BITS, bool ROPE>
+// One workgroup per (tile of 32 positions, row of heads): the tile's tokens of
+// one head's keys (blockIdx.y < n_head_kv), values (< 2 n_head_kv) or queries.
+// Keys and values are quantised into the tile's record (BITS 4, 8) or stored
+// as floats (32).  ROPE: keys and queries are normed and rotated on the way, eight
+// pairs of a token an item, so a query may be turned in place.  That
+// arithmetic is in double, rounded to float once: a key's code may hang on
+// its last bit (the vector unit adds and multiplies doubles at the rate of
+// floats).  A quantiser's item is eight columns of one token, a group of 32 a
+// lane quad.  The V codes of a position share their words with other
+// positions', so a workgroup owns its tile's words: codes pass through LDS, and
+// words that hold positions outside the pass keep those.
+// HD: head_dim where rows take 16-byte loads and head_dim is a stored width, else 0.
+template <int BITS, bool ROPE, int HD>
 __global__ __launch_bounds__(KS_THREADS) void kv_store_k(StoreArgs A)
 {
-    __shared__ double ss[32 * KS_PAIRS];               // sums of squares, [token][item]
-    __shared__ float kf[ROPE && BITS != 32 ? 32 * KS_ROW : 1];   // turned keys, [token][dim]
-    __shared__ uint8_t vc[BITS != 32 ? 32 * KS_ROW : 1];   // V codes, [position in tile][dim]
-    const int tid = threadIdx.x, head = blockIdx.y, hd = A.hd;
+    constexpr int LROW = (HD ? HD : KVQ_MAXHD) + 4;
+    constexpr bool WIDE = HD != 0;
+    __shared__ double ss[ROPE ? 32 * KS_PAIRS : 1];    // sums of squares, [token][item]
+    // turned keys [token][dim], or V codes [position in tile][dim]
+    __shared__ __attribute__((aligned(16))) uint8_t lds[BITS != 32 ? 32 * LROW * (ROPE ? 4 : 1) : 16];
+    const int tid = threadIdx.x, hd = HD ? HD : A.hd;
     const size_t p_first = A.pos[0], p_end = min(p_first + A.M, A.n_ctx);
     const size_t t0 = (p_first / KVQ_TILE + blockIdx.x) * KVQ_TILE;
     const size_t lo = max(p_first, t0), hi = min(p_end, t0 + KVQ_TILE);
     if (lo >= hi) return;                              // (uniform)
     const int nt = (int)(hi - lo), r0 = (int)(lo - t0);
     const KvqLayout L = kvq_layout(BITS == 32 ? 8 : BITS, hd);
-    const bool is_q = ROPE && head >= A.n_head_kv;
-    const int h = is_q ? head - A.n_head_kv : head;
+    const int part = blockIdx.y < A.n_head_kv ? 0 : blockIdx.y < 2 * A.n_head_kv ? 1 : 2;
+    const bool is_q = part == 2;
+    const int h = blockIdx.y - part * A.n_head_kv;
     const size_t tok0 = lo - p_first;                  // first token of the tile
+    const size_t kvd = (size_t)A.n_head_kv * hd;
     if constexpr (ROPE) {
-        const float *src = is_q ? A.q : A.k, *w = is_q ? A.q_norm : A.k_norm;
-        const size_t stride = is_q ? A.q_stride : A.k_stride;
-        const int ni = (hd + 15) / 16, half = hd >> 1;
-        const size_t kvd = (size_t)A.n_head_kv * hd;
-        float a[2][8], b[2][8];
+        if (part != 1) {
+            const float *src = is_q ? A.q : A.k, *w = is_q ? A.q_norm : A.k_norm;
+            const size_t stride = is_q ? A.q_stride : A.k_stride;
+            const int ni = (hd + 15) / 16, half = hd >> 1;
+            constexpr int SLOTS = HD ? (2 * HD + KS_THREADS - 1) / KS_THREADS : 2;
+            float a[SLOTS][8], b[SLOTS][8];
 #pragma unroll
-        for (int s = 0; s < 2; s++) {
-            const int it = tid + s * KS_THREADS;
-            if (it >= nt * ni) continue;
-            const int t = it / ni, i = it % ni;
-            load_pairs(a[s], b[s], src + (tok0 + t) * stride + (size_t)h * hd, 8 * i, hd, A.halves,
-                       A.wide);
-            double x = 0.0;
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                x += (double)a[s][j] * (double)a[s][j] + (double)b[s][j] * (double)b[s][j];
-            ss[t * KS_PAIRS + i] = x;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int s = 0; s < 2; s++) {
-            const int it = tid + s * KS_THREADS;
-            if (it >= nt * ni) continue;
-            const int t = it / ni, i = it % ni;
-            double inv = 1.0;
-            float wa[8], wb[8], ya[8], yb[8];
-            if (w) {
+            for (int s = 0; s < SLOTS; s++) {
+                const int it = tid + s * KS_THREADS;
+                if (it >= nt * ni) continue;
+                const int t = it / ni, i = it % ni;
+                load_pairs(a[s], b[s], src + (tok0 + t) * stride + (size_t)h * hd, 8 * i, hd, A.halves,
+                           WIDE);
                 double x = 0.0;
-                for (int j = 0; j < ni; j++) x += ss[t * KS_PAIRS + j];
-                inv = 1.0 / sqrt(x / (double)hd + (double)A.eps);
-                load_pairs(wa, wb, w, 8 * i, hd, A.halves, 0);
-            }
-            const float *cr = A.cos_t + (lo + t) * half, *sr = A.sin_t + (lo + t) * half;
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int at = min(8 * i + j, half - 1);
-                double x = (double)a[s][j] * inv, y = (double)b[s][j] * inv;
-                if (w) {
-                    x *= (double)wa[j];
-                    y *= (double)wb[j];
-                }
-                const double c = cr[at], sn = sr[at];
-                ya[j] = (float)(x * c - y * sn);
-                yb[j] = (float)(x * sn + y * c);
+                for (int j = 0; j < 8; j++)
+                    x += (double)a[s][j] * (double)a[s][j] + (double)b[s][j] * (double)b[s][j];
+                ss[t * KS_PAIRS + i] = x;
             }
-            float *dst;
-            if (is_q) dst = A.q_out + (tok0 + t) * A.qo_stride + (size_t)h * hd;
-            else if (BITS == 32) dst = A.k_cache + (lo + t) * kvd + (size_t)h * hd;
-            else dst = kf + t * KS_ROW;
-            store_pairs(dst, ya, yb, 8 * i, hd, A.halves, is_q ? A.wide : 0);
+            __syncthreads();
+#pragma unroll
+            for (int s = 0; s < SLOTS; s++) {
+                const int it = tid + s * KS_THREADS;
+                if (it >= nt * ni) continue;
+                const int t = it / ni, i = it % ni;
+                float wa[8], wb[8], cs[8], sn[8], ya[8], yb[8];
+                const float *cr = A.cos_t + (lo + t) * half, *sr = A.sin_t + (lo + t) * half;
+                if (w) load_pairs(wa, wb, w, 8 * i, hd, A.halves, WIDE);
+                load_8(cs, cr, 8 * i, half, WIDE);
+                load_8(sn, sr, 8 * i, half, WIDE);
+                double inv = 1.0;
+                if (w) {
+                    double x = 0.0;
+#pragma unroll
+                    for (int j = 0; j < (HD ? HD / 16 : KS_PAIRS); j++)
+                        if (HD || j < ni) x += ss[t * KS_PAIRS + j];
+                    inv = 1.0 / sqrt(x / (double)hd + (double)A.eps);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    double x = (double)a[s][j] * inv, y = (double)b[s][j] * inv;
+                    if (w) {
+                        x *= (double)wa[j];
+                        y *= (double)wb[j];
+                    }
+                    ya[j] = (float)(x * (double)cs[j] - y * (double)sn[j]);
+                    yb[j] = (float)(x * (double)sn[j] + y * (double)cs[j]);
+                }
+                float *dst;
+                if (is_q) dst = A.q_out + (tok0 + t) * A.qo_stride + (size_t)h * hd;
+                else if (BITS == 32) dst = A.k_cache + (lo + t) * kvd + (size_t)h * hd;
+                else dst = (float *)lds + t * LROW;
+                store_pairs(dst, ya, yb, 8 * i, hd, A.halves, WIDE);
+            }
+            if (is_q || BITS == 32) return;
+            __syncthreads();
         }
-        if (is_q) return;
-        __syncthreads();
     }
-    const int no = (hd + 7) / 8, nw = BITS == 32 ? no : L.width / 8;
-    if constexpr (BITS == 32) {
-        const size_t kvd = (size_t)A.n_head_kv * hd;
-        for (int it = tid; it < nt * no; it += KS_THREADS) {
-            const int t = it / no, d = it % no * 8;
-            const size_t p = lo + t;
-            float x[8];
-            load_8(x, A.v + (tok0 + t) * A.v_stride + (size_t)h * hd, d, hd, A.wide);
-            for (int i = 0; i < 8 && d + i < hd; i++)
-                A.v_cache[((p >> 2) * kvd + (size_t)h * hd + d + i) * 4 + (p & 3)] = x[i];
+    if constexpr (BITS == 32) {                        // values: a column of four positions
+        const float *row = A.v + tok0 * A.v_stride + (size_t)h * hd;
+        for (int it = tid; it < KVQ_TILE / 4 * hd; it += KS_THREADS) {
+            const int r = it / hd * 4 - r0, c = it % hd;   // first token of the four
+            if (r <= -4 || r >= nt) continue;
+            float *dst = A.v_cache + (((lo + r) >> 2) * kvd + (size_t)h * hd + c) * 4;
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (r + i >= 0 && r + i < nt) x[i] = row[(size_t)(r + i) * A.v_stride + c];
+            if (WIDE && r >= 0 && r + 4 <= nt) {
+                *(float4 *)dst = *(const float4 *)x;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (r + i >= 0 && r + i < nt) dst[i] = x[i];
+            }
         }
     } else {
+        const int nw = HD ? HD / 8 : L.width / 8;
         uint8_t *rec = A.cache + ((size_t)h * ((A.n_ctx + KVQ_TILE - 1) / KVQ_TILE) +
                                   t0 / KVQ_TILE) * (size_t)L.record;
-        for (int it = tid; it < 2 * nt * nw; it += KS_THREADS) {
-            const bool is_v = it >= nt * nw;
-            const int u = is_v ? it - nt * nw : it, t = u / nw, o = u % nw, d = 8 * o, r = r0 + t;
-            float x[8] = {};
-            if (d < hd) {
-                if (is_v) {
-                    load_8(x, A.v + (tok0 + t) * A.v_stride + (size_t)h * hd, d, hd, A.wide);
-                } else if (ROPE) {
+        const float *row = part ? A.v + tok0 * A.v_stride : A.k + tok0 * A.k_stride;
+        const size_t stride = part ? A.v_stride : A.k_stride;
+        // (the words of a tile partly outside the pass are read early)
+        constexpr int NWORD = (HD ? HD : KVQ_MAXHD) * 4 / KS_THREADS + (HD * 4 % KS_THREADS != 0);
+        uint2 old[NWORD];
+        const bool whole = nt == KVQ_TILE;
+        if (part && !whole) {
 #pragma unroll
-                    for (int i = 0; i < 8; i++) x[i] = d + i < hd ? kf[t * KS_ROW + d + i] : 0.0f;
-                } else {
-                    load_8(x, A.k + (tok0 + t) * A.k_stride + (size_t)h * hd, d, hd, A.wide);
-                }
+            for (int s = 0; s < NWORD; s++) {
+                const int it = tid + s * KS_THREADS;
+                if (it >= L.width * 4) continue;
+                if (BITS == 4) old[s].x = *(const uint32_t *)(rec + L.v + (size_t)it * 4);
+                else old[s] = *(const uint2 *)(rec + L.v + (size_t)it * 8);
+            }
+        }
+        for (int it = tid; it < nt * nw; it += KS_THREADS) {
+            const int t = it / nw, o = it % nw, d = 8 * o, r = r0 + t;
+            float x[8] = {};
+            if (ROPE && !part) {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    x[i] = HD || d + i < hd ? ((const float *)lds)[t * LROW + d + i] : 0.0f;
+            } else if (HD || d < hd) {
+                load_8(x, row + t * stride + (size_t)h * hd, d, hd, WIDE);
             }
             uint32_t code[8];
             const uint32_t b = quantise_8<BITS>(x, code);
             const int g = o >> 2;
-            if (!is_v) {
+            if (!part) {
                 put_codes<BITS>(rec + (size_t)r * (L.width * BITS / 8) + o * BITS, code);
                 if ((o & 3) == 0) rec[L.ks + kvq_k_scale(g, r)] = (uint8_t)b;
             } else {
                 if ((o & 3) == 0) rec[L.vs + kvq_v_scale(g, r)] = (uint8_t)b;
+                uint32_t *dst = (uint32_t *)(lds + r * LROW + d);
 #pragma unroll
-                for (int i = 0; i < 8; i++) vc[r * KS_ROW + d + i] = (uint8_t)code[i];
+                for (int i = 0; i < 2; i++)
+                    dst[i] = code[4 * i] | code[4 * i + 1] << 8 | code[4 * i + 2] << 16 |
+                             code[4 * i + 3] << 24;
             }
         }
+        if (!part) return;
         __syncthreads();
         // V words: item (dim, chunk) has eight positions
-        for (int it = tid; it < L.width * 4; it += KS_THREADS) {
+#pragma unroll
+        for (int s = 0; s < NWORD; s++) {
+            const int it = tid + s * KS_THREADS;
+            if (it >= L.width * 4) continue;
             const int dim = it >> 2, c = it & 3;
-            uint8_t *dst = rec + L.v + (size_t)it * BITS;
             uint32_t code[8];
-            bool any = false, all = true, on[8];
+            bool any = whole;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const int r = (e & 3) + 4 * c + 16 * (e >> 2);
-                on[e] = r >= r0 && r < r0 + nt;
-                any |= on[e];
-                all &= on[e];
-                code[e] = on[e] ? vc[r * KS_ROW + dim] : 0;
+                const bool on = whole || (r >= r0 && r < r0 + nt);
+                any |= on;
+                code[e] = on ? lds[r * LROW + dim]
+                        : BITS == 4 ? old[s].x >> (4 * (e / 2 + 4 * (e & 1))) & 15u
+                                    : (e < 4 ? old[s].x >> (8 * e) : old[s].y >> (8 * e - 32)) & 255u;
             }
-            if (!any) continue;
-            if (!all) {
-                if (BITS == 4) {
-                    const uint32_t old = *(const uint32_t *)dst;
-#pragma unroll
-                    for (int e = 0; e < 8; e++)
-                        if (!on[e]) code[e] = old >> (4 * (e / 2 + 4 * (e & 1))) & 15u;
-                } else {
-                    const uint2 old = *(const uint2 *)dst;
-#pragma unroll
-                    for (int e = 0; e < 8; e++)
-                        if (!on[e]) code[e] = (e < 4 ? old.x >> (8 * e) : old.y >> (8 * e - 32)) & 255u;
-                }
-            }
-            put_codes<BITS>(dst, code);
+            if (any) put_codes<BITS>(rec + L.v + (size_t)it * BITS, code);
         }
     }
 }
 
 // ----------------------------------------------------------------- reading
 
-// One workgroup per (tile, kv head): rows p0 .. p0 + n - 1 as floats.
+// value e of eight
 template <int BITS>
+__device__ __forceinline__ int code_of(const uint32_t *w, int e)
+{
+    return BITS == 4 ? (int)(w[0] >> (4 * (e / 2 + 4 * (e & 1))) & 15u)
+                     : (int)(w[e >> 2] >> (8 * (e & 3)) & 255u);
+}
+
+__device__ __forceinline__ void put_row(float *dst, const float *x, int n, int d, int hd, bool wide)
+{
+    if (wide) {
+        for (int i = 0; i < n; i += 4) *(float4 *)(dst + d + i) = *(const float4 *)(x + i);
+        return;
+    }
+    for (int i = 0; i < n; i++)
+        if (d + i < hd) dst[d + i] = x[i];
+}
+
+// One workgroup per (tile, kv head): rows p0 .. p0 + n - 1 as floats.  Half of
+// the waves take the keys, an item eight columns of a row; half the values,
+// an item four columns of a chunk's eight rows: 8 x 16 bytes stored by a thread either
+// way (head_dim 128), whole 512-byte row pieces by half a wave.
+template <int BITS, int HD>
 __global__ __launch_bounds__(KS_THREADS) void kv_read_k(const uint8_t *__restrict__ cache,
-                                                        size_t n_ctx, int hd, size_t p0, size_t n,
+                                                        size_t n_ctx, int hd_, size_t p0, size_t n,
                                                         float *__restrict__ k, size_t k_stride,
                                                         float *__restrict__ v, size_t v_stride)
 {
-    constexpr int H = 1 << (BITS - 1);
-    const int tid = threadIdx.x, h = blockIdx.y;
+    constexpr int H = 1 << (BITS - 1), HALF_WG = KS_THREADS / 2;
+    constexpr bool WIDE = HD != 0;
+    const int hd = HD ? HD : hd_, h = blockIdx.y;
     const size_t t0 = (p0 / KVQ_TILE + blockIdx.x) * KVQ_TILE;
     const KvqLayout L = kvq_layout(BITS, hd);
     const uint8_t *rec = cache + ((size_t)h * ((n_ctx + KVQ_TILE - 1) / KVQ_TILE) +
                                   t0 / KVQ_TILE) * (size_t)L.record;
     const int lo = t0 < p0 ? (int)(p0 - t0) : 0;
     const int hi = (int)min((size_t)KVQ_TILE, p0 + n - t0);
-    for (int it = tid; it < KVQ_TILE * L.width; it += KS_THREADS) {
-        const int r = it / L.width, d = it % L.width, e = d & 7;
-        if (r < lo || r >= hi || d >= hd) continue;
-        const size_t row = t0 + r - p0;
-        if (k) {
-            const uint8_t *w = rec + (size_t)r * (L.width * BITS / 8) + (d >> 3) * BITS;
-            const int c = BITS == 4 ? (int)(*(const uint32_t *)w >> (4 * (e / 2 + 4 * (e & 1))) & 15u)
-                                    : (int)w[e];
-            k[row * k_stride + (size_t)h * hd + d] =
-                (float)(c - H) * kvq_scale(rec[L.ks + kvq_k_scale(d >> 5, r)]);
+    const int tid = threadIdx.x & (HALF_WG - 1);
+    if (threadIdx.x < HALF_WG) {
+        if (!k) return;
+        const int no = HD ? HD / 8 : (hd + 7) / 8;
+        k += (t0 - p0) * k_stride + (size_t)h * hd;    // (row r of the tile; may wrap, r >= lo does not)
+#pragma unroll 4
+        for (int it = tid; it < KVQ_TILE * no; it += HALF_WG) {
+            const int r = it / no, o = it % no;
+            uint32_t w[2];
+            __builtin_memcpy(w, __builtin_assume_aligned(rec + (size_t)r * (L.width * BITS / 8) + o * BITS, BITS), BITS);
+            const float d = kvq_scale(rec[L.ks + kvq_k_scale(o >> 2, r)]);
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = (float)(code_of<BITS>(w, e) - H) * d;
+            if (r >= lo && r < hi) put_row(k + (size_t)r * k_stride, x, 8, 8 * o, hd, WIDE);
         }
-        if (v) {
-            const int pl = kvq_v_place(r);
-            const uint8_t *w = rec + L.v + ((size_t)d * 4 + kvq_v_chunk(r)) * BITS;
-            const int c = BITS == 4 ? (int)(*(const uint32_t *)w >> (4 * (pl / 2 + 4 * (pl & 1))) & 15u)
-                                    : (int)w[pl];
-            v[row * v_stride + (size_t)h * hd + d] =
-                (float)(c - H) * kvq_scale(rec[L.vs + kvq_v_scale(d >> 5, r)]);
+    } else {
+        if (!v) return;
+        const int nq = HD ? HD / 4 : (hd + 3) / 4;
+        v += (t0 - p0) * v_stride + (size_t)h * hd;
+        for (int it = tid; it < 4 * nq; it += HALF_WG) {
+            const int c = it / nq, d0 = it % nq * 4;
+            uint32_t w[4][2];
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                __builtin_memcpy(w[i], __builtin_assume_aligned(rec + L.v + ((size_t)(d0 + i) * 4 + c) * BITS, BITS), BITS);
+            const uint2 s = *(const uint2 *)(rec + L.vs + (d0 >> 5) * 32 + c * 8);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int r = (e & 3) + 4 * c + 16 * (e >> 2);
+                const float d = kvq_scale((e < 4 ? s.x : s.y) >> (8 * (e & 3)) & 255u);
+                float x[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[i] = (float)(code_of<BITS>(w[i], e) - H) * d;
+                if (r >= lo && r < hi) put_row(v + (size_t)r * v_stride, x, 4, d0, hd, WIDE);
+            }
         }
     }
 }
@@ -391,16 +452,25 @@ extern "C" size_t fox_gpu_kvq_bytes(int kv_type, size_t n_ctx, size_t n_head_kv,
 
 static bool wide_rows(const float *p, size_t stride) { return (uintptr_t)p % 16 == 0 && stride % 4 == 0; }
 
+// A kernel's instance for a head_dim that is a stored width, where rows take
+// 16-byte accesses (wide), else the one for any.
+#define FOX_BY_WIDTH(wide, hd, F)                                                            \
+    (!(wide) ? F(0) : (hd) == 32 ? F(32) : (hd) == 64 ? F(64) : (hd) == 96 ? F(96)           \
+                    : (hd) == 128 ? F(128) : (hd) == 192 ? F(192) : (hd) == 256 ? F(256) : F(0))
+
 template <int BITS, bool ROPE>
-static fox_gpu_status launch_store(fox_gpu_ctx *ctx, const StoreArgs &A)
+static fox_gpu_status launch_store(fox_gpu_ctx *ctx, StoreArgs A)
 {
     const size_t most = A.M < A.n_ctx ? A.M : A.n_ctx;       // rows that can be stored
-    const size_t tiles = (most + KVQ_TILE - 1) / KVQ_TILE + 1;
+    // (the position is not known here: the rows may begin at a tile's end)
+    const size_t tiles = (most + KVQ_TILE - 2) / KVQ_TILE + 1;
+#define FOX_STORE(hd) ((const void *)kv_store_k<BITS, ROPE, hd>)
+    const void *k = FOX_BY_WIDTH(A.wide, A.hd, FOX_STORE);
+#undef FOX_STORE
+    void *args[] = {&A};
     FOX_HIP(hipSetDevice(ctx->device));
-    hipLaunchKernelGGL((kv_store_k<BITS, ROPE>),
-                       dim3((unsigned)tiles, (unsigned)(A.n_head_kv + (ROPE ? A.n_head : 0))),
-                       dim3(KS_THREADS), 0, ctx->stream, A);
-    FOX_LAUNCHED("kv store");
+    FOX_HIP(hipLaunchKernel(k, dim3((unsigned)tiles, (unsigned)(2 * A.n_head_kv + (ROPE ? A.n_head : 0))),
+                            dim3(KS_THREADS), args, 0, ctx->stream));
     return FOX_GPU_OK;
 }
 
@@ -429,7 +499,7 @@ extern "C" fox_gpu_status fox_gpu_kvq_write(fox_gpu_ctx *ctx, int kv_type, void 
     A.M = M;
     A.n_ctx = n_ctx;
     A.cache = (uint8_t *)cache;
-    A.wide = head_dim % 8 == 0 && wide_rows(k, M > 1 ? k_stride : 0) && wide_rows(v, M > 1 ? v_stride : 0);
+    A.wide = wide_rows(k, M > 1 ? k_stride : 0) && wide_rows(v, M > 1 ? v_stride : 0);
     return kv_type == FOX_GPU_KV_Q4 ? launch_store<4, false>(ctx, A) : launch_store<8, false>(ctx, A);
 }
 
@@ -450,16 +520,18 @@ extern "C" fox_gpu_status fox_gpu_kvq_read(fox_gpu_ctx *ctx, int kv_type, const 
     if ((uintptr_t)cache % 16)
         return fox_fail(FOX_GPU_ERR_ARG, "kvq_read: the cache must be 16-byte aligned");
     const unsigned tiles = (unsigned)((p0 + n - 1) / KVQ_TILE - p0 / KVQ_TILE + 1);
+    const bool wide = wide_rows(k, n > 1 ? k_stride : 0) && wide_rows(v, n > 1 ? v_stride : 0);
+    int hd = (int)head_dim;
+#define FOX_READ4(hd) ((const void *)kv_read_k<4, hd>)
+#define FOX_READ8(hd) ((const void *)kv_read_k<8, hd>)
+    const void *f = kv_type == FOX_GPU_KV_Q4 ? FOX_BY_WIDTH(wide, hd, FOX_READ4)
+                                             : FOX_BY_WIDTH(wide, hd, FOX_READ8);
+#undef FOX_READ4
+#undef FOX_READ8
+    void *args[] = {(void *)&cache, &n_ctx, &hd, &p0, &n, &k, &k_stride, &v, &v_stride};
     FOX_HIP(hipSetDevice(ctx->device));
-    if (kv_type == FOX_GPU_KV_Q4)
-        hipLaunchKernelGGL(kv_read_k<4>, dim3(tiles, (unsigned)n_head_kv), dim3(KS_THREADS), 0,
-                           ctx->stream, (const uint8_t *)cache, n_ctx, (int)head_dim, p0, n, k,
-                           k_stride, v, v_stride);
-    else
-        hipLaunchKernelGGL(kv_read_k<8>, dim3(tiles, (unsigned)n_head_kv), dim3(KS_THREADS), 0,
-                           ctx->stream, (const uint8_t *)cache, n_ctx, (int)head_dim, p0, n, k,
-                           k_stride, v, v_stride);
-    FOX_LAUNCHED("kv read");
+    FOX_HIP(hipLaunchKernel(f, dim3(tiles, (unsigned)n_head_kv), dim3(KS_THREADS), args, 0,
+                            ctx->stream));
     return FOX_GPU_OK;
 }
 
@@ -503,9 +575,10 @@ static fox_gpu_status rope_args(const char *what, fox_gpu_ctx *ctx, const float 
     A->pos = pos;
     A->M = M;
     A->n_ctx = n_ctx;
-    A->wide = head_dim % 16 == 0 && wide_rows(q, M > 1 ? q_stride : 0) &&
-              wide_rows(q_out, M > 1 ? qo_stride : 0) && wide_rows(k, M > 1 ? k_stride : 0) &&
-              wide_rows(v, M > 1 ? v_stride : 0);
+    A->wide = wide_rows(q, M > 1 ? q_stride : 0) && wide_rows(q_out, M > 1 ? qo_stride : 0) &&
+              wide_rows(k, M > 1 ? k_stride : 0) && wide_rows(v, M > 1 ? v_stride : 0) &&
+              wide_rows(q_norm, 0) && wide_rows(k_norm, 0) && wide_rows(cos_t, 0) &&
+              wide_rows(sin_t, 0);
     return FOX_GPU_OK;
 }
 
@@ -523,6 +596,7 @@ extern "C" fox_gpu_status fox_gpu_norm_rope_store(
     if (st) return st;
     if (!k_cache || !v_cache) return fox_fail(FOX_GPU_ERR_ARG, "norm_rope_store: null cache");
     A.k_cache = k_cache;
+    A.wide = A.wide && wide_rows(k_cache, 0) && wide_rows(v_cache, 0);
     A.v_cache = v_cache;
     return launch_store<32, true>(ctx, A);
 }
