@@ -81,6 +81,149 @@ __device__ __forceinline__ float quad_sum(float v)
     return v + __shfl_xor(v, 32);
 }
 
+// A tile's K scale byte pair (positions r and 16 + r) of chunk c's dimensions
+// in MFMA step j: the group it lies in.
+template <int NG>
+__device__ __forceinline__ int k_group(int c, int j) { return (NG * c + j) / 4; }
+
+// eight scales' halves as pairs, and -72 of them
+__device__ __forceinline__ void v_scales(uint2 b, h2v d[4], h2v m72[4])
+{
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        d[i] = as_h2(__builtin_amdgcn_perm(0, i < 2 ? b.x : b.y, i & 1 ? 0x0C030C02u : 0x0C010C00u) << 7);
+        m72[i] = d[i] * (h2v){(_Float16)-72.0f, (_Float16)-72.0f};
+    }
+}
+template <int BITS>
+__device__ __forceinline__ h8v unpack_k(const uint32_t *w, uint32_t pair, int i)
+{
+    const h2v d1 = as_h2(__builtin_amdgcn_perm(0, pair, i ? 0x0C010C01u : 0x0C000C00u) << 7);
+    const h2v m1 = d1 * (h2v){(_Float16)-72.0f, (_Float16)-72.0f};
+    const h2v d[4] = {d1, d1, d1, d1}, mm[4] = {m1, m1, m1, m1};
+    return unpack<BITS>(w, d, mm);
+}
+
+// A tile that not every row sees whole: scale bytes b of V's group, of
+// positions tp + 4 c + 0..3 and tp + 16 + 4 c + 0..3.  Positions from `last` on, that no row
+// sees, count as zero whatever the cache holds there; NaN scales are taken
+// out of the product.  Returns the first position of those (or INT_MAX), to be put into the
+// sums of the rows that see it.
+__device__ __forceinline__ int trim_scales(uint2 &b2, int tp, int c, int last)
+{
+    int at = 0x7FFFFFFF;
+#pragma unroll
+    for (int i = 1; i >= 0; i--) {
+        const int p = tp + 16 * i + 4 * c, n = min(max(last - p, 0), 4);
+        uint32_t b = (i ? b2.y : b2.x) & (n == 4 ? ~0u : (1u << 8 * n) - 1);
+        const uint32_t nan = ((b & 0x78787878u) + 0x08080808u) & b & 0x80808080u;   // from 0xF8 on
+        b &= ~((nan << 1) - (nan >> 7));
+        if (nan) at = p + (__builtin_ctz(nan) >> 3);
+        (i ? b2.y : b2.x) = b;
+    }
+    return at;
+}
+
+// One query row's dimensions of chunk c as two halves each, MFMA step j the
+// eight from 8 (NG c + j) on, scaled by a power of two; returns what turns a score of
+// theirs into powers of two.
+template <int NG>
+__device__ __forceinline__ float load_query(h8v qh[NG], h8v ql[NG], const float *qr, int c,
+                                            const AttnArgs &A)
+{
+    float x[NG][8], top = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NG; j++) {
+        const int d = 8 * (NG * c + j);
+        if (A.q_wide) {
+            const bool in = d < A.hd;
+            *(float4 *)x[j] = in ? *(const float4 *)(qr + d) : float4{0, 0, 0, 0};
+            *(float4 *)(x[j] + 4) = in ? *(const float4 *)(qr + d + 4) : float4{0, 0, 0, 0};
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[j][e] = d + e < A.hd ? qr[d + e] : 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[j][e]));
+    }
+    top = quad_max(top);
+    // 2^(14 - exponent of the largest), the exponent kept within range
+    const int ex = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 113);
+    const float up = __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
+#pragma unroll
+    for (int j = 0; j < NG; j++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float y = x[j][e] * up;
+            const _Float16 hi = (_Float16)y;
+            qh[j][e] = hi;
+            ql[j][e] = (_Float16)(y - (float)hi);
+        }
+    return 1.44269504f / sqrtf((float)A.hd) * 0.25f * __uint_as_float((uint32_t)(127 - 14 + ex) << 23);
+}
+
+// The weights of a row's eight positions from their scores, as two halves each;
+// the running maximum m, the sum l and the row's sums o follow.
+template <int ND>
+__device__ __forceinline__ void weigh(const f4v s[2], float sc, bool edge, int tp, int c, int end,
+                                      float &m, float &l, f4v o[ND], h8v &ph, h8v &pl)
+{
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) x[e] = s[e >> 2][e & 3];
+    if (edge) {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            if (tp + 16 * (e >> 2) + 4 * c + (e & 3) >= end) x[e] = -INFINITY;
+    }
+    const float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
+                            fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))) * sc;
+    if (__any(top > m + KA_ROOM)) {
+        const float mn = fmaxf(m, quad_max(top)), f = __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < ND; d++) o[d] *= f;
+    }
+    const float off = KA_LIFT - m;
+    h2v hi[4], lo[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i], sc, off));
+        const float b = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i + 1], sc, off));
+        l += a + b;
+        hi[i] = __builtin_bit_cast(h2v, __builtin_amdgcn_cvt_pkrtz(a, b));
+        lo[i] = __builtin_bit_cast(h2v, __builtin_amdgcn_cvt_pkrtz(
+                    __builtin_fmaf((float)hi[i][0], -1.0f, a), __builtin_fmaf((float)hi[i][1], -1.0f, b)));
+    }
+    ph = __builtin_bit_cast(h8v, *(u4v *)hi);
+    pl = __builtin_bit_cast(h8v, *(u4v *)lo);
+}
+
+__device__ __forceinline__ f4v mfma(h8v a, h8v b, f4v c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// Four sums of one row at dimension `dim` of kv head kvh: the result, or a split's record.
+__device__ __forceinline__ void put_sums(const AttnArgs &A, int kvh, int row, int dim, f4v v, float m,
+                                         float l, bool whole, int split, int width)
+{
+    if (whole) {
+        float *dst = A.out + (size_t)(row / A.G) * A.out_stride + ((size_t)kvh * A.G + row % A.G) * A.hd;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (dim + e < A.hd) dst[dim + e] = v[e] * 0.25f / l;
+    } else {
+        float *dst = A.part + (((size_t)kvh * A.M * A.G + row) * A.splits + split) * (4 + width);
+        if (dim == 0) {
+            dst[0] = m;
+            dst[1] = l;
+        }
+        *(f4v *)(dst + 4 + dim) = v;
+    }
+}
+
 // One tile's bytes as a lane holds them.
 template <int BITS, int NG>
 struct Tile {
@@ -146,7 +289,6 @@ __global__ __launch_bounds__(64 * KA_WAVES) void kv_attn_few(AttnArgs A)
     Tile<BITS, NG> cur;
     cur.load(base + (size_t)min(tile, n_tiles - 1) * REC, lane);
 
-    // queries: row r's dimensions of chunk c, MFMA step j the eight from 8 j on
     h8v qh[T][NG], ql[T][NG];
     float sc[T], m[T], l[T];
     int end[T];
@@ -155,36 +297,8 @@ __global__ __launch_bounds__(64 * KA_WAVES) void kv_attn_few(AttnArgs A)
     for (int t = 0; t < T; t++) {
         const int row = min(row0 + 16 * t + r, rows - 1);
         end[t] = end_of(row);
-        const float *qr = A.q + (size_t)(row / A.G) * A.q_stride + ((size_t)kvh * A.G + row % A.G) * A.hd;
-        float x[NG][8], top = 0.0f;
-#pragma unroll
-        for (int j = 0; j < NG; j++) {
-            const int d = 8 * (NG * c + j);
-            if (A.q_wide) {
-                const bool in = d < A.hd;
-                *(float4 *)x[j] = in ? *(const float4 *)(qr + d) : float4{0, 0, 0, 0};
-                *(float4 *)(x[j] + 4) = in ? *(const float4 *)(qr + d + 4) : float4{0, 0, 0, 0};
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; e++) x[j][e] = d + e < A.hd ? qr[d + e] : 0.0f;
-            }
-#pragma unroll
-            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[j][e]));
-        }
-        top = quad_max(top);
-        // 2^(14 - exponent of the largest), the exponent kept within range
-        const int ex = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 113);
-        const float up = __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
-        sc[t] = 1.44269504f / sqrtf((float)A.hd) * 0.25f * __uint_as_float((uint32_t)(127 - 14 + ex) << 23);
-#pragma unroll
-        for (int j = 0; j < NG; j++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float y = x[j][e] * up;
-                const _Float16 hi = (_Float16)y;
-                qh[t][j][e] = hi;
-                ql[t][j][e] = (_Float16)(y - (float)hi);
-            }
+        sc[t] = load_query<NG>(qh[t], ql[t], A.q + (size_t)(row / A.G) * A.q_stride +
+                                                 ((size_t)kvh * A.G + row % A.G) * A.hd, c, A);
         m[t] = -FLT_MAX;
         l[t] = 0.0f;
 #pragma unroll
@@ -197,30 +311,14 @@ __global__ __launch_bounds__(64 * KA_WAVES) void kv_attn_few(AttnArgs A)
         const int tp = tile * KVQ_TILE;
         const bool edge = tp + KVQ_TILE > first;                 // (uniform)
         if (edge) {
-            // positions no row sees: whatever the cache holds there counts
-            // as zero.  NaN values that only some rows see are taken out of
-            // the product and put into those rows' sums.
-            uint32_t keep[2], nan[NG][2], any = 0;
+            int at[NG], any = 0x7FFFFFFF;
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const int n = min(max(last - (tp + 16 * i + 4 * c), 0), 4);    // seen ones of four
-                keep[i] = n == 4 ? ~0u : (1u << 8 * n) - 1;
-#pragma unroll
-                for (int g = 0; g < NG; g++) {
-                    uint32_t &b = i ? cur.vs[g].y : cur.vs[g].x;
-                    b &= keep[i];
-                    nan[g][i] = ((b & 0x78787878u) + 0x08080808u) & b & 0x80808080u;   // from 0xF8 on
-                    b &= ~((nan[g][i] << 1) - (nan[g][i] >> 7));
-                    any |= nan[g][i];
-                }
-            }
-            if (__any(any != 0)) {
+            for (int g = 0; g < NG; g++) any = min(any, at[g] = trim_scales(cur.vs[g], tp, c, last));
+            if (__any(any != 0x7FFFFFFF)) {
                 const float bad = __uint_as_float(0x7FC00000u);
 #pragma unroll
                 for (int g = 0; g < NG; g++) {
-                    int p = nan[g][0] ? tp + 4 * c + (__builtin_ctz(nan[g][0]) >> 3)
-                          : nan[g][1] ? tp + 16 + 4 * c + (__builtin_ctz(nan[g][1]) >> 3) : 0x7FFFFFFF;
-                    p = min(p, __shfl_xor(p, 16));               // the group's first one
+                    int p = min(at[g], __shfl_xor(at[g], 16));   // the group's first one
                     p = min(p, __shfl_xor(p, 32));
 #pragma unroll
                     for (int t = 0; t < T; t++)
@@ -228,7 +326,6 @@ __global__ __launch_bounds__(64 * KA_WAVES) void kv_attn_few(AttnArgs A)
                 }
             }
         }
-        // scores
         f4v s[T][2];
 #pragma unroll
         for (int i = 0; i < 2; i++) {
@@ -236,70 +333,29 @@ __global__ __launch_bounds__(64 * KA_WAVES) void kv_attn_few(AttnArgs A)
             for (int t = 0; t < T; t++) s[t][i] = f4v{0, 0, 0, 0};
 #pragma unroll
             for (int j = 0; j < NG; j++) {
-                const uint32_t b = __builtin_amdgcn_perm(0, cur.kscale(j), i ? 0x0C010C01u : 0x0C000C00u);
-                const h2v d1 = as_h2(b << 7), m1 = d1 * (h2v){(_Float16)-72.0f, (_Float16)-72.0f};
-                const h2v d[4] = {d1, d1, d1, d1}, mm[4] = {m1, m1, m1, m1};
-                const h8v kf = unpack<BITS>(cur.k[i] + j * BITS / 4, d, mm);
+                const h8v kf = unpack_k<BITS>(cur.k[i] + j * BITS / 4, cur.kscale(j), i);
 #pragma unroll
                 for (int t = 0; t < T; t++) {
-                    s[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[t][j], s[t][i], 0, 0, 0);
-                    s[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[t][j], s[t][i], 0, 0, 0);
+                    s[t][i] = mfma(kf, qh[t][j], s[t][i]);
+                    s[t][i] = mfma(kf, ql[t][j], s[t][i]);
                 }
             }
         }
-        // weights
         h8v ph[T], pl[T];
 #pragma unroll
-        for (int t = 0; t < T; t++) {
-            float x[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = s[t][e >> 2][e & 3];
-            if (edge) {
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    if (tp + 16 * (e >> 2) + 4 * c + (e & 3) >= end[t]) x[e] = -INFINITY;
-            }
-            float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
-                              fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))) * sc[t];
-            if (__any(top > m[t] + KA_ROOM)) {
-                const float mn = fmaxf(m[t], quad_max(top)), f = __builtin_amdgcn_exp2f(m[t] - mn);
-                m[t] = mn;
-                l[t] *= f;
-#pragma unroll
-                for (int d = 0; d < 2 * NG; d++) o[t][d] *= f;
-            }
-            const float off = KA_LIFT - m[t];
-            h2v hi[4], lo[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i], sc[t], off));
-                const float b = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i + 1], sc[t], off));
-                l[t] += a + b;
-                hi[i] = __builtin_bit_cast(h2v, __builtin_amdgcn_cvt_pkrtz(a, b));
-                lo[i] = __builtin_bit_cast(h2v, __builtin_amdgcn_cvt_pkrtz(
-                            __builtin_fmaf((float)hi[i][0], -1.0f, a),
-                            __builtin_fmaf((float)hi[i][1], -1.0f, b)));
-            }
-            ph[t] = __builtin_bit_cast(h8v, *(u4v *)hi);
-            pl[t] = __builtin_bit_cast(h8v, *(u4v *)lo);
-        }
-        // values
+        for (int t = 0; t < T; t++)
+            weigh<2 * NG>(s[t], sc[t], edge, tp, c, end[t], m[t], l[t], o[t], ph[t], pl[t]);
 #pragma unroll
         for (int g = 0; g < NG; g++) {
             h2v d[4], mm[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                d[i] = as_h2(__builtin_amdgcn_perm(0, i < 2 ? cur.vs[g].x : cur.vs[g].y,
-                                                   i & 1 ? 0x0C030C02u : 0x0C010C00u) << 7);
-                mm[i] = d[i] * (h2v){(_Float16)-72.0f, (_Float16)-72.0f};
-            }
+            v_scales(cur.vs[g], d, mm);
 #pragma unroll
             for (int k = 2 * g; k < 2 * g + 2; k++) {
                 const h8v vf = unpack<BITS>(cur.v[k], d, mm);
 #pragma unroll
                 for (int t = 0; t < T; t++) {
-                    o[t][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[t], o[t][k], 0, 0, 0);
-                    o[t][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[t], o[t][k], 0, 0, 0);
+                    o[t][k] = mfma(vf, ph[t], o[t][k]);
+                    o[t][k] = mfma(vf, pl[t], o[t][k]);
                 }
             }
         }
@@ -336,38 +392,204 @@ __global__ __launch_bounds__(64 * KA_WAVES) void kv_attn_few(AttnArgs A)
                     sum += sl[w][t][r] * f;
                     v += so[w][k][lane] * f;
                 }
-                const int dim = 16 * (h * NG + k) + 4 * c;
-                if (used == 1) {
-                    float *dst = A.out + (size_t)(row / A.G) * A.out_stride +
-                                 ((size_t)kvh * A.G + row % A.G) * A.hd;
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        if (dim + e < A.hd) dst[dim + e] = v[e] * 0.25f / sum;
-                } else {
-                    float *dst = A.part + (((size_t)kvh * rows + row) * A.splits + split) * (4 + WIDTH);
-                    if (dim == 0) {
-                        dst[0] = mx;
-                        dst[1] = sum;
-                    }
-                    *(f4v *)(dst + 4 + dim) = v;
-                }
+                put_sums(A, kvh, row, 16 * (h * NG + k) + 4 * c, v, mx, sum, used == 1, split, WIDTH);
             }
         }
 }
 
+// Many rows: a workgroup of eight waves takes 16 RT RW rows; RW waves share a
+// tile's unpacked halves in LDS, a piece unpacked by each of them, and PW = 8 / RW
+// such groups take tiles in turn, merged at the end.  Two waves a SIMD, so
+// that one's softmax runs beside the other's products.  A tile is unpacked
+// while the one before it is multiplied, its words read a step earlier still.
+template <int BITS, int NG, int RW>
+__global__ __launch_bounds__(512, 2) void kv_attn_many(AttnArgs A)
+{
+    constexpr int WIDTH = 32 * NG, PW = 8 / RW, RT = NG > 4 ? 1 : 2, NF = 2 * NG;
+    constexpr int FW = (NF + RW - 1) / RW;                       // fragments a wave unpacks, of K and V each
+    constexpr int CODES = KVQ_TILE * WIDTH * BITS / 8, REC = 2 * (CODES + KVQ_TILE * NG);
+    static_assert(2 * PW * 2 * NF * 1024 + 4096 <= 160 * 1024, "LDS");
+    // [buffer][group][K fragments, V fragments][lane]: a fragment is an MFMA operand
+    extern __shared__ h8v frag[];
+    __shared__ int nan_at[2][PW][NG];
+    __shared__ float sm[PW][RW][RT][16], sl[PW][RW][RT][16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, c = lane >> 4, rw = wave % RW, pw = wave / RW;
+    // workgroups that share a kv head's cache get the same blockIdx % n_head_kv; the
+    // longest rows first
+    const int rows = A.M * A.G, blocks = (rows + 16 * RT * RW - 1) / (16 * RT * RW);
+    const int kvh = blockIdx.x % A.n_head_kv, item = blockIdx.x / A.n_head_kv;
+    const int split = item % A.splits, row0 = (blocks - 1 - item / A.splits) * 16 * RT * RW;
+    const size_t p0 = A.pos[0];
+    auto end_of = [&](int row) { return (int)min(p0 + (size_t)(row / A.G) + 1, A.n_ctx); };
+    const int last = end_of(min(row0 + 16 * RT * RW, rows) - 1), first = end_of(row0);
+    const int n_tiles = (last + KVQ_TILE - 1) / KVQ_TILE, step = A.splits * PW;
+    if (split * PW >= n_tiles) return;                           // (uniform)
+    const int used = min(A.splits, (n_tiles + PW - 1) / PW);
+    const int my_row0 = row0 + 16 * RT * rw;
+    const int my_last = my_row0 < rows ? end_of(min(my_row0 + 16 * RT, rows) - 1) : 0;
+    const uint8_t *base = A.cache + (size_t)kvh * ((A.n_ctx + KVQ_TILE - 1) / KVQ_TILE) * REC;
+
+    // the words of this wave's fragments
+    uint32_t kw[FW][BITS / 4], vw[FW][BITS / 4];
+    uint16_t ks[FW];
+    uint2 vs[FW];
+    auto fetch = [&](int tile) __attribute__((always_inline)) {
+        const uint8_t *rec = base + (size_t)min(tile, n_tiles - 1) * REC;
+#pragma unroll
+        for (int u = 0; u < FW; u++) {
+            const int f = min(rw * FW + u, NF - 1), i = f / NG, j = f % NG;
+            __builtin_memcpy(kw[u], __builtin_assume_aligned(rec + (16 * i + r) * (4 * NG * BITS) + (c * NG + j) * BITS, BITS), BITS);
+            ks[u] = *(const uint16_t *)(rec + 2 * CODES + k_group<NG>(c, j) * 32 + r * 2);
+            __builtin_memcpy(vw[u], __builtin_assume_aligned(rec + CODES + ((16 * f + r) * 4 + c) * BITS, BITS), BITS);
+            vs[u] = *(const uint2 *)(rec + 2 * CODES + 32 * NG + (f >> 1) * 32 + c * 8);
+        }
+    };
+    auto stage = [&](int tile, int buf) __attribute__((always_inline)) {
+        const int tp = tile * KVQ_TILE;
+        h8v *dst = frag + (size_t)(buf * PW + pw) * 2 * NF * 64 + lane;
+#pragma unroll
+        for (int u = 0; u < FW; u++) {
+            const int f = rw * FW + u;
+            if (FW * RW > NF && f >= NF) break;
+            dst[f * 64] = unpack_k<BITS>(kw[u], ks[u], f / NG);
+            if (tp + KVQ_TILE > first) {                         // (uniform)
+                int p = trim_scales(vs[u], tp, c, last);
+                p = min(p, __shfl_xor(p, 16));
+                p = min(p, __shfl_xor(p, 32));
+                if (lane == 0 && (f & 1) == 0) nan_at[buf][pw][f >> 1] = p;
+            }
+            h2v d[4], mm[4];
+            v_scales(vs[u], d, mm);
+            dst[(NF + f) * 64] = unpack<BITS>(vw[u], d, mm);
+        }
+    };
+
+    int tile = split * PW + pw;
+    fetch(tile);
+    h8v qh[RT][NG], ql[RT][NG];
+    float sc[RT], m[RT], l[RT];
+    int end[RT];
+    f4v o[RT][NF];
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        const int row = min(my_row0 + 16 * t + r, rows - 1);
+        end[t] = end_of(row);
+        sc[t] = load_query<NG>(qh[t], ql[t], A.q + (size_t)(row / A.G) * A.q_stride +
+                                                 ((size_t)kvh * A.G + row % A.G) * A.hd, c, A);
+        m[t] = -FLT_MAX;
+        l[t] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < NF; d++) o[t][d] = f4v{0, 0, 0, 0};
+    }
+    stage(tile, 0);
+    fetch(tile + step);
+    __syncthreads();
+    const int n_steps = (n_tiles - split * PW + step - 1) / step;
+    for (int n = 0; n < n_steps; n++, tile += step) {
+        const int buf = n & 1, tp = tile * KVQ_TILE;
+        if (n + 1 < n_steps) {
+            stage(tile + step, buf ^ 1);
+            fetch(tile + 2 * step);
+        }
+        if (tp < my_last) {                                      // (uniform in a wave)
+            const h8v *src = frag + (size_t)(buf * PW + pw) * 2 * NF * 64 + lane;
+            const bool edge = tp + KVQ_TILE > first;
+            f4v s[RT][2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+#pragma unroll
+                for (int t = 0; t < RT; t++) s[t][i] = f4v{0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < NG; j++) {
+                    const h8v kf = src[(i * NG + j) * 64];
+#pragma unroll
+                    for (int t = 0; t < RT; t++) {
+                        s[t][i] = mfma(kf, qh[t][j], s[t][i]);
+                        s[t][i] = mfma(kf, ql[t][j], s[t][i]);
+                    }
+                }
+            }
+            h8v ph[RT], pl[RT];
+#pragma unroll
+            for (int t = 0; t < RT; t++)
+                weigh<NF>(s[t], sc[t], edge, tp, c, end[t], m[t], l[t], o[t], ph[t], pl[t]);
+            if (edge) {
+                const float bad = __uint_as_float(0x7FC00000u);
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    const int p = nan_at[buf][pw][g];
+#pragma unroll
+                    for (int t = 0; t < RT; t++)
+                        if (p < end[t]) o[t][2 * g] = o[t][2 * g + 1] = f4v{bad, bad, bad, bad};
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < NF; k++) {
+                const h8v vf = src[(NF + k) * 64];
+#pragma unroll
+                for (int t = 0; t < RT; t++) {
+                    o[t][k] = mfma(vf, ph[t], o[t][k]);
+                    o[t][k] = mfma(vf, pl[t], o[t][k]);
+                }
+            }
+        }
+        __syncthreads();
+    }
+
+    // the groups' sums at their common maximum, group 0's waves adding them up
+    f4v *so = (f4v *)frag;
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        l[t] = quad_sum(l[t]);
+        if (c == 0) {
+            sm[pw][rw][t][r] = m[t];
+            sl[pw][rw][t][r] = l[t];
+        }
+        if (pw) {
+#pragma unroll
+            for (int k = 0; k < NF; k++) so[(((pw - 1) * RW + rw) * RT * NF + t * NF + k) * 64 + lane] = o[t][k];
+        }
+    }
+    __syncthreads();
+    if (pw) return;
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        const int row = my_row0 + 16 * t + r;
+        if (row >= rows) continue;
+        float mx = m[t], sum = 0.0f, f[PW];
+#pragma unroll
+        for (int w = 1; w < PW; w++) mx = fmaxf(mx, sm[w][rw][t][r]);
+#pragma unroll
+        for (int w = 0; w < PW; w++) {
+            f[w] = __builtin_amdgcn_exp2f(sm[w][rw][t][r] - mx);
+            sum += sl[w][rw][t][r] * f[w];
+        }
+#pragma unroll
+        for (int k = 0; k < NF; k++) {
+            f4v v = o[t][k] * f[0];
+#pragma unroll
+            for (int w = 1; w < PW; w++)
+                v += so[(((w - 1) * RW + rw) * RT * NF + t * NF + k) * 64 + lane] * f[w];
+            put_sums(A, kvh, row, 16 * k + 4 * c, v, mx, sum, used == 1, split, WIDTH);
+        }
+    }
+}
+
 // One workgroup per (row, kv head): the splits' records at their common
 // maximum.  32 threads to a column quad's splits, eight split groups.
-__global__ __launch_bounds__(256) void kv_merge_k(AttnArgs A, int width, int rows_per)
+__global__ __launch_bounds__(256) void kv_merge_k(AttnArgs A, int width, int rows_per, int tiles_per)
 {
     __shared__ float sm[8], sl[8];
     __shared__ f4v so[8][32];
     const int row = blockIdx.x, kvh = blockIdx.y, rows = A.M * A.G;
     const int tid = threadIdx.x, sg = tid >> 5, cq = tid & 31;
-    // the splits kv_attn_few used for this row's block of rows_per
+    // the splits that hold this row: of its block of rows_per rows, tiles_per
+    // tiles of a split at a time
     const int row_last = min(row / rows_per * rows_per + rows_per, rows) - 1;
     const int last = (int)min((size_t)A.pos[0] + (size_t)(row_last / A.G) + 1, A.n_ctx);
     const int n_tiles = (last + KVQ_TILE - 1) / KVQ_TILE;
-    const int used = min(A.splits, (n_tiles + KA_WAVES - 1) / KA_WAVES);
+    const int used = min(A.splits, (n_tiles + tiles_per - 1) / tiles_per);
     if (used == 1) return;
     const size_t rec = 4 + (size_t)width;
     const float *base = A.part + ((size_t)kvh * rows + row) * A.splits * rec;
@@ -422,6 +644,19 @@ static const void *few_kernel(int ng, int T)
 #undef FOX_FEW
 }
 
+template <int BITS>
+static const void *many_kernel(int ng)
+{
+    switch (ng) {
+    case 1: return (const void *)kv_attn_many<BITS, 1, 4>;
+    case 2: return (const void *)kv_attn_many<BITS, 2, 4>;
+    case 3: return (const void *)kv_attn_many<BITS, 3, 4>;
+    case 4: return (const void *)kv_attn_many<BITS, 4, 4>;
+    case 6: return (const void *)kv_attn_many<BITS, 6, 4>;
+    default: return (const void *)kv_attn_many<BITS, 8, 4>;
+    }
+}
+
 extern "C" fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, size_t out_stride,
                                                 const float *q, size_t q_stride, int kv_type,
                                                 const void *cache, size_t n_head, size_t n_head_kv,
@@ -456,10 +691,28 @@ extern "C" fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, si
     A.q_wide = head_dim % 8 == 0 && (uintptr_t)q % 16 == 0 && (M == 1 || q_stride % 4 == 0);
     const int width = kvq_width((int)head_dim), ng = width / 32;
     const size_t rows = M * (size_t)A.G;
+    const bool many = rows > 32, q4 = kv_type == FOX_GPU_KV_Q4;
     const int T = rows <= 16 || ng > 6 ? 1 : 2;
-    const size_t blocks = (rows + 16 * T - 1) / (16 * T);
-    size_t splits = 2 * (size_t)ctx->n_cu / (n_head_kv * blocks);
-    const size_t most = (n_ctx + KVQ_TILE * KA_WAVES - 1) / (KVQ_TILE * KA_WAVES);
+    const int per = many ? 16 * (ng > 4 ? 1 : 2) * 4 : 16 * T;          // rows of a workgroup
+    const int tiles_per = many ? 2 : KA_WAVES;                        // tiles it takes side by side
+    const size_t blocks = (rows + per - 1) / per, items = n_head_kv * blocks;
+    size_t splits = 1;
+    const size_t most = (n_ctx + KVQ_TILE * tiles_per - 1) / (KVQ_TILE * tiles_per);
+    if (!many) {
+        splits = 2 * (size_t)ctx->n_cu / items;
+    } else {
+        // one workgroup to a compute unit: the number of splits whose rounds
+        // leave the fewest of them idle, each split's records priced at 1/32
+        double best = 1e30;
+        for (size_t s = 1; s <= 16; s++) {
+            const double cost = (double)((items * s + ctx->n_cu - 1) / ctx->n_cu) / (double)s +
+                                (s > 1 ? 0.03 * (double)s * (double)items / ctx->n_cu : 0.0);
+            if (cost < best) {
+                best = cost;
+                splits = s;
+            }
+        }
+    }
     if (splits > most) splits = most;
     if (splits < 1) splits = 1;
     A.splits = (int)splits;
@@ -468,14 +721,20 @@ extern "C" fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, si
         if (st) return st;
         A.part = (float *)ctx->ws;
     }
-    const void *k = kv_type == FOX_GPU_KV_Q4 ? few_kernel<4>(ng, T)
-                                             : few_kernel<8>(ng, T);
     void *args[] = {&A};
-    FOX_HIP(hipLaunchKernel(k, dim3((unsigned)splits, (unsigned)n_head_kv, (unsigned)blocks),
-                            dim3(64 * KA_WAVES), args, 0, ctx->stream));
+    if (many) {
+        const void *k = q4 ? many_kernel<4>(ng) : many_kernel<8>(ng);
+        const size_t lds = 2 * (size_t)tiles_per * 4 * ng * 1024;
+        FOX_HIP(hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+        FOX_HIP(hipLaunchKernel(k, dim3((unsigned)(items * splits)), dim3(512), args, lds, ctx->stream));
+    } else {
+        FOX_HIP(hipLaunchKernel(q4 ? few_kernel<4>(ng, T) : few_kernel<8>(ng, T),
+                                dim3((unsigned)splits, (unsigned)n_head_kv, (unsigned)blocks),
+                                dim3(64 * KA_WAVES), args, 0, ctx->stream));
+    }
     if (splits > 1) {
         hipLaunchKernelGGL(kv_merge_k, dim3((unsigned)rows, (unsigned)n_head_kv), dim3(256), 0,
-                           ctx->stream, A, width, 16 * T);
+                           ctx->stream, A, width, per, tiles_per);
         FOX_LAUNCHED("kvq attention merge");
     }
     return FOX_GPU_OK;
