@@ -162,22 +162,21 @@ __device__ __forceinline__ float load_query(h8v qh[NG], h8v ql[NG], const float 
     return 1.44269504f / sqrtf((float)A.hd) * 0.25f * __uint_as_float((uint32_t)(127 - 14 + ex) << 23);
 }
 
-// The weights of a row's eight positions from their scores, as two halves each;
-// the running maximum m, the sum l and the row's sums o follow.
-template <int ND>
-__device__ __forceinline__ void weigh(const f4v s[2], float sc, bool edge, int tp, int c, int end,
-                                      float &m, float &l, f4v o[ND], h8v &ph, h8v &pl)
+// Scores of positions a row does not see.
+__device__ __forceinline__ void hide(f4v s[2], int tp, int c, int end)
 {
-    float x[8];
 #pragma unroll
-    for (int e = 0; e < 8; e++) x[e] = s[e >> 2][e & 3];
-    if (edge) {
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-            if (tp + 16 * (e >> 2) + 4 * c + (e & 3) >= end) x[e] = -INFINITY;
-    }
-    const float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
-                            fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))) * sc;
+    for (int e = 0; e < 8; e++)
+        if (tp + 16 * (e >> 2) + 4 * c + (e & 3) >= end) s[e >> 2][e & 3] = -INFINITY;
+}
+
+// The running maximum m, with the sum l and the row's sums o, after scores that
+// pass it by KA_ROOM.
+template <int ND>
+__device__ __forceinline__ void follow(const f4v s[2], float sc, float &m, float &l, f4v o[ND])
+{
+    const float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                            fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3]))) * sc;
     if (__any(top > m + KA_ROOM)) {
         const float mn = fmaxf(m, quad_max(top)), f = __builtin_amdgcn_exp2f(m - mn);
         m = mn;
@@ -185,16 +184,35 @@ __device__ __forceinline__ void weigh(const f4v s[2], float sc, bool edge, int t
 #pragma unroll
         for (int d = 0; d < ND; d++) o[d] *= f;
     }
+}
+
+// a - (float)h for the two halves of h
+__device__ __forceinline__ float less_lo(float a, h2v h)
+{
+    float d;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(d) : "v"(as_u(h)), "v"(a));
+    return d;
+}
+__device__ __forceinline__ float less_hi(float a, h2v h)
+{
+    float d;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
+        : "=v"(d) : "v"(as_u(h)), "v"(a));
+    return d;
+}
+
+// The weights of a row's eight positions, as two halves each, and their sum.
+__device__ __forceinline__ void weigh(const f4v s[2], float sc, float m, float &l, h8v &ph, h8v &pl)
+{
     const float off = KA_LIFT - m;
     h2v hi[4], lo[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i], sc, off));
-        const float b = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i + 1], sc, off));
+        const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 1][2 * (i & 1)], sc, off));
+        const float b = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 1][2 * (i & 1) + 1], sc, off));
         l += a + b;
         hi[i] = __builtin_bit_cast(h2v, __builtin_amdgcn_cvt_pkrtz(a, b));
-        lo[i] = __builtin_bit_cast(h2v, __builtin_amdgcn_cvt_pkrtz(
-                    __builtin_fmaf((float)hi[i][0], -1.0f, a), __builtin_fmaf((float)hi[i][1], -1.0f, b)));
+        lo[i] = __builtin_bit_cast(h2v, __builtin_amdgcn_cvt_pkrtz(less_lo(a, hi[i]), less_hi(b, hi[i])));
     }
     ph = __builtin_bit_cast(h8v, *(u4v *)hi);
     pl = __builtin_bit_cast(h8v, *(u4v *)lo);
@@ -343,8 +361,11 @@ __global__ __launch_bounds__(64 * KA_WAVES) void kv_attn_few(AttnArgs A)
         }
         h8v ph[T], pl[T];
 #pragma unroll
-        for (int t = 0; t < T; t++)
-            weigh<2 * NG>(s[t], sc[t], edge, tp, c, end[t], m[t], l[t], o[t], ph[t], pl[t]);
+        for (int t = 0; t < T; t++) {
+            if (edge) hide(s[t], tp, c, end[t]);
+            follow<2 * NG>(s[t], sc[t], m[t], l[t], o[t]);
+            weigh(s[t], sc[t], m[t], l[t], ph[t], pl[t]);
+        }
 #pragma unroll
         for (int g = 0; g < NG; g++) {
             h2v d[4], mm[4];
@@ -427,50 +448,75 @@ __global__ __launch_bounds__(512, 2) void kv_attn_many(AttnArgs A)
     if (split * PW >= n_tiles) return;                           // (uniform)
     const int used = min(A.splits, (n_tiles + PW - 1) / PW);
     const int my_row0 = row0 + 16 * RT * rw;
-    const int my_last = my_row0 < rows ? end_of(min(my_row0 + 16 * RT, rows) - 1) : 0;
     const uint8_t *base = A.cache + (size_t)kvh * ((A.n_ctx + KVQ_TILE - 1) / KVQ_TILE) * REC;
 
-    // the words of this wave's fragments
+    // the words of this wave's fragments; fragment f of K is step j = f % NG
+    // of positions 16 (f / NG) + 0..15, of V the dimensions 16 f + 0..15
     uint32_t kw[FW][BITS / 4], vw[FW][BITS / 4];
     uint16_t ks[FW];
     uint2 vs[FW];
-    auto fetch = [&](int tile) __attribute__((always_inline)) {
-        const uint8_t *rec = base + (size_t)min(tile, n_tiles - 1) * REC;
+    auto record = [&](int tile) __attribute__((always_inline)) {
+        return base + (size_t)min(tile, n_tiles - 1) * REC;
+    };
+    auto fetch_k = [&](int tile) __attribute__((always_inline)) {
+        const uint8_t *rec = record(tile);
 #pragma unroll
         for (int u = 0; u < FW; u++) {
             const int f = min(rw * FW + u, NF - 1), i = f / NG, j = f % NG;
             __builtin_memcpy(kw[u], __builtin_assume_aligned(rec + (16 * i + r) * (4 * NG * BITS) + (c * NG + j) * BITS, BITS), BITS);
             ks[u] = *(const uint16_t *)(rec + 2 * CODES + k_group<NG>(c, j) * 32 + r * 2);
+        }
+    };
+    auto fetch_v = [&](int tile) __attribute__((always_inline)) {
+        const uint8_t *rec = record(tile);
+#pragma unroll
+        for (int u = 0; u < FW; u++) {
+            const int f = min(rw * FW + u, NF - 1);
             __builtin_memcpy(vw[u], __builtin_assume_aligned(rec + CODES + ((16 * f + r) * 4 + c) * BITS, BITS), BITS);
             vs[u] = *(const uint2 *)(rec + 2 * CODES + 32 * NG + (f >> 1) * 32 + c * 8);
         }
     };
-    auto stage = [&](int tile, int buf) __attribute__((always_inline)) {
-        const int tp = tile * KVQ_TILE;
-        h8v *dst = frag + (size_t)(buf * PW + pw) * 2 * NF * 64 + lane;
+    auto place = [&](int buf) __attribute__((always_inline)) {   // a tile's K fragments; V's NF further on
+        return frag + (size_t)(buf * PW + pw) * 2 * NF * 64 + lane;
+    };
+    auto stage_k = [&](int buf) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < FW; u++) {
             const int f = rw * FW + u;
             if (FW * RW > NF && f >= NF) break;
-            dst[f * 64] = unpack_k<BITS>(kw[u], ks[u], f / NG);
-            if (tp + KVQ_TILE > first) {                         // (uniform)
-                int p = trim_scales(vs[u], tp, c, last);
-                p = min(p, __shfl_xor(p, 16));
-                p = min(p, __shfl_xor(p, 32));
-                if (lane == 0 && (f & 1) == 0) nan_at[buf][pw][f >> 1] = p;
-            }
+            place(buf)[f * 64] = unpack_k<BITS>(kw[u], ks[u], f / NG);
+        }
+    };
+    auto stage_v = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < FW; u++) {
+            const int f = rw * FW + u;
+            if (FW * RW > NF && f >= NF) break;
             h2v d[4], mm[4];
             v_scales(vs[u], d, mm);
-            dst[(NF + f) * 64] = unpack<BITS>(vw[u], d, mm);
+            place(buf)[(NF + f) * 64] = unpack<BITS>(vw[u], d, mm);
+        }
+    };
+    auto trim = [&](int tile, int buf) __attribute__((always_inline)) {   // the fetched V words' scales
+        const int tp = tile * KVQ_TILE;
+        if (tp + KVQ_TILE <= first) return;                      // (uniform)
+#pragma unroll
+        for (int u = 0; u < FW; u++) {
+            const int f = rw * FW + u;
+            int p = trim_scales(vs[u], tp, c, last);
+            p = min(p, __shfl_xor(p, 16));
+            p = min(p, __shfl_xor(p, 32));
+            if (lane == 0 && (f & 1) == 0 && f < NF) nan_at[buf][pw][f >> 1] = p;
         }
     };
 
     int tile = split * PW + pw;
-    fetch(tile);
+    fetch_k(tile);
+    fetch_v(tile);
     h8v qh[RT][NG], ql[RT][NG];
     float sc[RT], m[RT], l[RT];
     int end[RT];
-    f4v o[RT][NF];
+    f4v o[RT][NF], s[RT][2];
 #pragma unroll
     for (int t = 0; t < RT; t++) {
         const int row = min(my_row0 + 16 * t + r, rows - 1);
@@ -482,57 +528,66 @@ __global__ __launch_bounds__(512, 2) void kv_attn_many(AttnArgs A)
 #pragma unroll
         for (int d = 0; d < NF; d++) o[t][d] = f4v{0, 0, 0, 0};
     }
-    stage(tile, 0);
-    fetch(tile + step);
+    auto score = [&](int buf) __attribute__((always_inline)) {
+        const h8v *src = place(buf);
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+#pragma unroll
+            for (int t = 0; t < RT; t++) s[t][i] = f4v{0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < NG; j++) {
+                const h8v kf = src[(i * NG + j) * 64];
+#pragma unroll
+                for (int t = 0; t < RT; t++) s[t][i] = mfma(kf, qh[t][j], s[t][i]);
+#pragma unroll
+                for (int t = 0; t < RT; t++) s[t][i] = mfma(kf, ql[t][j], s[t][i]);
+            }
+        }
+    };
+    trim(tile, 0);
+    stage_k(0);
+    stage_v(0);
+    fetch_k(tile + step);
+    stage_k(1);
+    fetch_k(tile + 2 * step);
+    fetch_v(tile + step);
     __syncthreads();
+    score(0);
+    __syncthreads();                                             // (the loop writes K's buffer 0 again)
     const int n_steps = (n_tiles - split * PW + step - 1) / step;
     for (int n = 0; n < n_steps; n++, tile += step) {
         const int buf = n & 1, tp = tile * KVQ_TILE;
-        if (n + 1 < n_steps) {
-            stage(tile + step, buf ^ 1);
-            fetch(tile + 2 * step);
+        if (tp + KVQ_TILE > first) {                             // (uniform)
+            const float bad = __uint_as_float(0x7FC00000u);
+#pragma unroll
+            for (int t = 0; t < RT; t++) {
+                hide(s[t], tp, c, end[t]);
+#pragma unroll
+                for (int g = 0; g < NG; g++)
+                    if (nan_at[buf][pw][g] < end[t]) o[t][2 * g] = o[t][2 * g + 1] = f4v{bad, bad, bad, bad};
+            }
         }
-        if (tp < my_last) {                                      // (uniform in a wave)
-            const h8v *src = frag + (size_t)(buf * PW + pw) * 2 * NF * 64 + lane;
-            const bool edge = tp + KVQ_TILE > first;
-            f4v s[RT][2];
+        trim(tile + step, buf ^ 1);
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
+        for (int t = 0; t < RT; t++) follow<NF>(s[t], sc[t], m[t], l[t], o[t]);
+        // this tile's weights beside the next one's scores
+        h8v ph[RT], pl[RT];
 #pragma unroll
-                for (int t = 0; t < RT; t++) s[t][i] = f4v{0, 0, 0, 0};
+        for (int t = 0; t < RT; t++) weigh(s[t], sc[t], m[t], l[t], ph[t], pl[t]);
+        score(buf ^ 1);
+        // its values beside the unpacking of the next one's, and of the keys after those
+        stage_k(buf);
+        stage_v(buf ^ 1);
+        fetch_k(tile + 3 * step);
+        fetch_v(tile + 2 * step);
+        const h8v *src = place(buf) + NF * 64;
 #pragma unroll
-                for (int j = 0; j < NG; j++) {
-                    const h8v kf = src[(i * NG + j) * 64];
+        for (int k = 0; k < NF; k++) {
+            const h8v vf = src[k * 64];
 #pragma unroll
-                    for (int t = 0; t < RT; t++) {
-                        s[t][i] = mfma(kf, qh[t][j], s[t][i]);
-                        s[t][i] = mfma(kf, ql[t][j], s[t][i]);
-                    }
-                }
-            }
-            h8v ph[RT], pl[RT];
+            for (int t = 0; t < RT; t++) o[t][k] = mfma(vf, ph[t], o[t][k]);
 #pragma unroll
-            for (int t = 0; t < RT; t++)
-                weigh<NF>(s[t], sc[t], edge, tp, c, end[t], m[t], l[t], o[t], ph[t], pl[t]);
-            if (edge) {
-                const float bad = __uint_as_float(0x7FC00000u);
-#pragma unroll
-                for (int g = 0; g < NG; g++) {
-                    const int p = nan_at[buf][pw][g];
-#pragma unroll
-                    for (int t = 0; t < RT; t++)
-                        if (p < end[t]) o[t][2 * g] = o[t][2 * g + 1] = f4v{bad, bad, bad, bad};
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < NF; k++) {
-                const h8v vf = src[(NF + k) * 64];
-#pragma unroll
-                for (int t = 0; t < RT; t++) {
-                    o[t][k] = mfma(vf, ph[t], o[t][k]);
-                    o[t][k] = mfma(vf, pl[t], o[t][k]);
-                }
-            }
+            for (int t = 0; t < RT; t++) o[t][k] = mfma(vf, pl[t], o[t][k]);
         }
         __syncthreads();
     }
