@@ -7,18 +7,15 @@
 // the same float sums.  A query head's row is scaled by a power of two first, its
 // largest value to 2^14, so that the lower half is not lost below the half's range.
 //
-// Layout of one step, 32 positions (a tile) of one kv head by 16 query rows (row =
+// A step is 32 positions (a tile) of one kv head by 16 or 32 query rows (row =
 // token * G + head in the group of G = n_head / n_head_kv that share it):
-//   S[pos][row] = sum_d K[pos][d] q[row][d]   two 16x16x32 MFMA rows of 16
-//     positions; lane (r, c) = (lane % 16, lane / 16) supplies position r's
-//     dimensions of chunk c, a contiguous quarter of the row, and holds row r's
-//     scores of positions 16 i + 4 c + 0..3 afterwards
-//   O[dim][row] += sum_pos V[dim][pos] P[pos][row]   the weights of those eight
-//     positions are that lane's operand as they stand, since a V word holds
-//     just those positions (fox_kvq_dev.h).
+//   S[pos][row] = sum_d K[pos][d] q[row][d]
+//   O[dim][row] += sum_pos V[dim][pos] P[pos][row]
+// A lane's scores in S are of the eight positions of a V word (kvq_v_pos), so the
+// weights of those positions are the second product's operand as they stand.
 // The running maximum only follows scores that pass it by 8 (in powers of two):
 // weights are exp2(s - m + 7) <= 2^15, within a half; between updates no lane
-// needs another's maximum.
+// needs another's maximum.  A weight ends at 2^-24, 2^-31 of the largest.
 #include "fox_kvq_dev.h"
 #include "fox_internal.h"
 
@@ -28,6 +25,7 @@
 typedef _Float16 h2v __attribute__((ext_vector_type(2)));
 typedef _Float16 h8v __attribute__((ext_vector_type(8)));
 typedef float f4v __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
 typedef uint32_t u4v __attribute__((ext_vector_type(4)));
 
 #define KA_WAVES 4
@@ -41,7 +39,8 @@ struct AttnArgs {
     const uint8_t *cache;
     const uint32_t *pos;
     size_t n_ctx;
-    int n_head_kv, G, hd, M, splits, q_wide;
+    int n_head_kv, G, hd, M, splits;
+    bool q_wide, out_wide;        // rows take 16-byte accesses
 };
 
 __device__ __forceinline__ h2v as_h2(uint32_t v) { return __builtin_bit_cast(h2v, v); }
@@ -55,11 +54,14 @@ __device__ __forceinline__ h8v unpack(const uint32_t *w, const h2v d[4], const h
 {
     uint32_t r[4];
     if (BITS == 4) {
+        // (in registers, where one instruction takes both: of two literals it takes neither)
+        uint32_t mask = 0x00F000F0u, base = 0x54005400u;
+        asm("" : "+s"(mask));
+        asm("" : "+v"(base));
         const uint32_t x[4] = {w[0] << 4, w[0], w[0] >> 4, w[0] >> 8};
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            r[i] = as_u(__builtin_elementwise_fma(as_h2((x[i] & 0x00F000F0u) | 0x54005400u), d[i],
-                                                  m72[i]));
+            r[i] = as_u(__builtin_elementwise_fma(as_h2((x[i] & mask) | base), d[i], m72[i]));
     } else {
         const h2v off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
 #pragma unroll
@@ -81,11 +83,6 @@ __device__ __forceinline__ float quad_sum(float v)
     return v + __shfl_xor(v, 32);
 }
 
-// A tile's K scale byte pair (positions r and 16 + r) of chunk c's dimensions
-// in MFMA step j: the group it lies in.
-template <int NG>
-__device__ __forceinline__ int k_group(int c, int j) { return (NG * c + j) / 4; }
-
 // eight scales' halves as pairs, and -72 of them
 __device__ __forceinline__ void v_scales(uint2 b, h2v d[4], h2v m72[4])
 {
@@ -95,26 +92,26 @@ __device__ __forceinline__ void v_scales(uint2 b, h2v d[4], h2v m72[4])
         m72[i] = d[i] * (h2v){(_Float16)-72.0f, (_Float16)-72.0f};
     }
 }
+// (one scale for the eight: byte i of `bytes`)
 template <int BITS>
-__device__ __forceinline__ h8v unpack_k(const uint32_t *w, uint32_t pair, int i)
+__device__ __forceinline__ h8v unpack_k(const uint32_t *w, uint32_t bytes, int i)
 {
-    const h2v d1 = as_h2(__builtin_amdgcn_perm(0, pair, i ? 0x0C010C01u : 0x0C000C00u) << 7);
+    const h2v d1 = as_h2(__builtin_amdgcn_perm(0, bytes, i ? 0x0C010C01u : 0x0C000C00u) << 7);
     const h2v m1 = d1 * (h2v){(_Float16)-72.0f, (_Float16)-72.0f};
     const h2v d[4] = {d1, d1, d1, d1}, mm[4] = {m1, m1, m1, m1};
     return unpack<BITS>(w, d, mm);
 }
 
-// A tile that not every row sees whole: scale bytes b of V's group, of
-// positions tp + 4 c + 0..3 and tp + 16 + 4 c + 0..3.  Positions from `last` on, that no row
-// sees, count as zero whatever the cache holds there; NaN scales are taken
-// out of the product.  Returns the first position of those (or INT_MAX), to be put into the
-// sums of the rows that see it.
+// A tile that not every row sees whole: V's scale bytes of chunk c of a group.
+// Positions from `last` on, that no row sees, count as zero whatever the cache
+// holds there; NaN scales are taken out of the product.  Returns the first
+// position of those (or INT_MAX), to be put into the sums of the rows that see it.
 __device__ __forceinline__ int trim_scales(uint2 &b2, int tp, int c, int last)
 {
     int at = 0x7FFFFFFF;
 #pragma unroll
     for (int i = 1; i >= 0; i--) {
-        const int p = tp + 16 * i + 4 * c, n = min(max(last - p, 0), 4);
+        const int p = tp + kvq_v_pos(c, 4 * i), n = min(max(last - p, 0), 4);
         uint32_t b = (i ? b2.y : b2.x) & (n == 4 ? ~0u : (1u << 8 * n) - 1);
         const uint32_t nan = ((b & 0x78787878u) + 0x08080808u) & b & 0x80808080u;   // from 0xF8 on
         b &= ~((nan << 1) - (nan >> 7));
@@ -124,34 +121,24 @@ __device__ __forceinline__ int trim_scales(uint2 &b2, int tp, int c, int last)
     return at;
 }
 
-// One query row's dimensions of chunk c as two halves each, MFMA step j the
-// eight from 8 (NG c + j) on, scaled by a power of two; returns what turns a score of
-// theirs into powers of two.
-template <int NG>
-__device__ __forceinline__ float load_query(h8v qh[NG], h8v ql[NG], const float *qr, int c,
-                                            const AttnArgs &A)
+// A lane's part c of a query row's dimensions as two halves each, the eight from
+// 8 (N c + j) on for product step j, scaled by a power of two; the row's PARTS parts
+// are in lanes 64 / PARTS apart.  x: the part's floats.  Returns what turns a
+// score of theirs into powers of two.
+template <int N, int PARTS>
+__device__ __forceinline__ float split_query(h8v qh[N], h8v ql[N], const float (*x)[8], int hd)
 {
-    float x[NG][8], top = 0.0f;
+    float top = 0.0f;
 #pragma unroll
-    for (int j = 0; j < NG; j++) {
-        const int d = 8 * (NG * c + j);
-        if (A.q_wide) {
-            const bool in = d < A.hd;
-            *(float4 *)x[j] = in ? *(const float4 *)(qr + d) : float4{0, 0, 0, 0};
-            *(float4 *)(x[j] + 4) = in ? *(const float4 *)(qr + d + 4) : float4{0, 0, 0, 0};
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[j][e] = d + e < A.hd ? qr[d + e] : 0.0f;
-        }
+    for (int j = 0; j < N; j++)
 #pragma unroll
         for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[j][e]));
-    }
-    top = quad_max(top);
+    top = PARTS == 4 ? quad_max(top) : fmaxf(top, __shfl_xor(top, 32));
     // 2^(14 - exponent of the largest), the exponent kept within range
     const int ex = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 113);
     const float up = __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
 #pragma unroll
-    for (int j = 0; j < NG; j++)
+    for (int j = 0; j < N; j++)
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const float y = x[j][e] * up;
@@ -159,31 +146,27 @@ __device__ __forceinline__ float load_query(h8v qh[NG], h8v ql[NG], const float 
             qh[j][e] = hi;
             ql[j][e] = (_Float16)(y - (float)hi);
         }
-    return 1.44269504f / sqrtf((float)A.hd) * 0.25f * __uint_as_float((uint32_t)(127 - 14 + ex) << 23);
+    return 1.44269504f / sqrtf((float)hd) * 0.25f * __uint_as_float((uint32_t)(127 - 14 + ex) << 23);
 }
 
-// Scores of positions a row does not see.
-__device__ __forceinline__ void hide(f4v s[2], int tp, int c, int end)
+// four floats of a query row from dimension d on (zero past hd)
+__device__ __forceinline__ float4 query_quad(const float *row, int d, const AttnArgs &A)
 {
-#pragma unroll
-    for (int e = 0; e < 8; e++)
-        if (tp + 16 * (e >> 2) + 4 * c + (e & 3) >= end) s[e >> 2][e & 3] = -INFINITY;
+    if (A.q_wide) return d < A.hd ? *(const float4 *)(row + d) : float4{0, 0, 0, 0};
+    return float4{d < A.hd ? row[d] : 0.0f, d + 1 < A.hd ? row[d + 1] : 0.0f,
+                  d + 2 < A.hd ? row[d + 2] : 0.0f, d + 3 < A.hd ? row[d + 3] : 0.0f};
+}
+__device__ __forceinline__ const float *query_row(const AttnArgs &A, int kvh, int row)
+{
+    return A.q + (size_t)(row / A.G) * A.q_stride + ((size_t)kvh * A.G + row % A.G) * A.hd;
 }
 
-// The running maximum m, with the sum l and the row's sums o, after scores that
-// pass it by KA_ROOM.
-template <int ND>
-__device__ __forceinline__ void follow(const f4v s[2], float sc, float &m, float &l, f4v o[ND])
+// (fmaxf quiets its operands first; the instruction passes a NaN over by itself)
+__device__ __forceinline__ float max3(float a, float b, float c)
 {
-    const float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                            fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3]))) * sc;
-    if (__any(top > m + KA_ROOM)) {
-        const float mn = fmaxf(m, quad_max(top)), f = __builtin_amdgcn_exp2f(m - mn);
-        m = mn;
-        l *= f;
-#pragma unroll
-        for (int d = 0; d < ND; d++) o[d] *= f;
-    }
+    float d;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+    return d;
 }
 
 // a - (float)h for the two halves of h
@@ -201,15 +184,14 @@ __device__ __forceinline__ float less_hi(float a, h2v h)
     return d;
 }
 
-// The weights of a row's eight positions, as two halves each, and their sum.
-__device__ __forceinline__ void weigh(const f4v s[2], float sc, float m, float &l, h8v &ph, h8v &pl)
+// The weights of eight positions from their scores, as two halves each, and their sum.
+__device__ __forceinline__ void weigh(const float s[8], float sc, float off, float &l, h8v &ph, h8v &pl)
 {
-    const float off = KA_LIFT - m;
     h2v hi[4], lo[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 1][2 * (i & 1)], sc, off));
-        const float b = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 1][2 * (i & 1) + 1], sc, off));
+        const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i], sc, off));
+        const float b = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i + 1], sc, off));
         l += a + b;
         hi[i] = __builtin_bit_cast(h2v, __builtin_amdgcn_cvt_pkrtz(a, b));
         lo[i] = __builtin_bit_cast(h2v, __builtin_amdgcn_cvt_pkrtz(less_lo(a, hi[i]), less_hi(b, hi[i])));
@@ -221,6 +203,10 @@ __device__ __forceinline__ void weigh(const f4v s[2], float sc, float m, float &
 __device__ __forceinline__ f4v mfma(h8v a, h8v b, f4v c)
 {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f16v mfma(h8v a, h8v b, f16v c)
+{
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
 // Four sums of one row at dimension `dim` of kv head kvh: the result, or a split's record.
@@ -256,7 +242,7 @@ struct Tile {
         const int r = lane & 15, c = lane >> 4;
 #pragma unroll
         for (int i = 0; i < 2; i++)
-            __builtin_memcpy(k[i], __builtin_assume_aligned(rec + (16 * i + r) * (4 * NG * BITS) + c * NG * BITS, 4 * (NG % 4 == 0 ? 4 : NG % 2 == 0 ? 2 : 1)),
+            __builtin_memcpy(k[i], __builtin_assume_aligned(rec + (16 * (r >> 3) + 8 * i + (r & 7)) * (4 * NG * BITS) + c * NG * BITS, 4 * (NG % 4 == 0 ? 4 : NG % 2 == 0 ? 2 : 1)),
                              sizeof(k[i]));
 #pragma unroll
         for (int s = 0; s < NS; s++) {
@@ -315,8 +301,11 @@ __global__ __launch_bounds__(64 * KA_WAVES) void kv_attn_few(AttnArgs A)
     for (int t = 0; t < T; t++) {
         const int row = min(row0 + 16 * t + r, rows - 1);
         end[t] = end_of(row);
-        sc[t] = load_query<NG>(qh[t], ql[t], A.q + (size_t)(row / A.G) * A.q_stride +
-                                                 ((size_t)kvh * A.G + row % A.G) * A.hd, c, A);
+        const float *qr = query_row(A, kvh, row);
+        float x[NG][8];
+#pragma unroll
+        for (int j = 0; j < 2 * NG; j++) *(float4 *)&x[j >> 1][4 * (j & 1)] = query_quad(qr, 8 * NG * c + 4 * j, A);
+        sc[t] = split_query<NG, 4>(qh[t], ql[t], x, A.hd);
         m[t] = -FLT_MAX;
         l[t] = 0.0f;
 #pragma unroll
@@ -362,9 +351,22 @@ __global__ __launch_bounds__(64 * KA_WAVES) void kv_attn_few(AttnArgs A)
         h8v ph[T], pl[T];
 #pragma unroll
         for (int t = 0; t < T; t++) {
-            if (edge) hide(s[t], tp, c, end[t]);
-            follow<2 * NG>(s[t], sc[t], m[t], l[t], o[t]);
-            weigh(s[t], sc[t], m[t], l[t], ph[t], pl[t]);
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                x[e] = s[t][e >> 2][e & 3];
+                if (edge && tp + kvq_v_pos(c, e) >= end[t]) x[e] = -INFINITY;
+            }
+            const float top = max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]),
+                                   max3(x[6], x[7], x[7])) * sc[t];
+            if (__any(top > m[t] + KA_ROOM)) {
+                const float mn = fmaxf(m[t], quad_max(top)), f = __builtin_amdgcn_exp2f(m[t] - mn);
+                m[t] = mn;
+                l[t] *= f;
+#pragma unroll
+                for (int d = 0; d < 2 * NG; d++) o[t][d] *= f;
+            }
+            weigh(x, sc[t], KA_LIFT - m[t], l[t], ph[t], pl[t]);
         }
 #pragma unroll
         for (int g = 0; g < NG; g++) {
@@ -418,43 +420,58 @@ __global__ __launch_bounds__(64 * KA_WAVES) void kv_attn_few(AttnArgs A)
         }
 }
 
-// Many rows: a workgroup of eight waves takes 16 RT RW rows; RW waves share a
-// tile's unpacked halves in LDS, a piece unpacked by each of them, and PW = 8 / RW
-// such groups take tiles in turn, merged at the end.  Two waves a SIMD, so
-// that one's softmax runs beside the other's products.  A tile is unpacked
-// while the one before it is multiplied, its words read a step earlier still.
-template <int BITS, int NG, int RW>
-__global__ __launch_bounds__(512, 2) void kv_attn_many(AttnArgs A)
+// Many rows: RW waves of 32 rows each share a tile's unpacked halves in LDS, a
+// piece unpacked by each of them, and PW such groups of a workgroup take tiles in
+// turn, merged at the end.  Products are 32x32x16: at the 16x16x32 form's
+// back-to-back rate the matrix cores idle half the time (32 cycles an
+// instruction against 16, measured; with vector instructions between, 19 to 23
+// against 17 to 19).  A tile's weights are formed beside the next one's scores; a tile is
+// unpacked while the one before it is multiplied, its words read a step
+// earlier still.
+template <int BITS, int NG, int RW, int PW>
+__global__ __launch_bounds__(64 * RW * PW, NG > 4 ? 1 : 2) void kv_attn_many(AttnArgs A)
 {
-    constexpr int WIDTH = 32 * NG, PW = 8 / RW, RT = NG > 4 ? 1 : 2, NF = 2 * NG;
+    constexpr int WIDTH = 32 * NG, NF = 2 * NG;
     constexpr int FW = (NF + RW - 1) / RW;                       // fragments a wave unpacks, of K and V each
     constexpr int CODES = KVQ_TILE * WIDTH * BITS / 8, REC = 2 * (CODES + KVQ_TILE * NG);
-    static_assert(2 * PW * 2 * NF * 1024 + 4096 <= 160 * 1024, "LDS");
-    // [buffer][group][K fragments, V fragments][lane]: a fragment is an MFMA operand
+    static_assert(2 * PW * 2 * NF * 1024 + 4096 <= 160 * 1024 &&
+                  32 * RW * (PW > 2 ? PW - 1 : 1) * (WIDTH + 4) * 4 + 4096 <= 160 * 1024, "LDS");
+    // [buffer][group][K fragments, V fragments][lane]: a fragment is an MFMA
+    // operand; f of K holds 8 dimensions of each half of the 32 positions' rows, from
+    // 8 f and from WIDTH / 2 + 8 f on; f of V dimensions 32 (f / 2) + 0..31 of
+    // positions 16 (f % 2) + 0..15
     extern __shared__ h8v frag[];
+    constexpr int ROW = WIDTH + 4;                               // floats of a row in LDS, when rows pass through it
     __shared__ int nan_at[2][PW][NG];
-    __shared__ float sm[PW][RW][RT][16], sl[PW][RW][RT][16];
+    __shared__ float sm[PW][RW][32], sl[PW][RW][32];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int r = lane & 15, c = lane >> 4, rw = wave % RW, pw = wave / RW;
+    const int r = lane & 31, c = lane >> 5, rw = wave % RW, pw = wave / RW;
     // workgroups that share a kv head's cache get the same blockIdx % n_head_kv; the
     // longest rows first
-    const int rows = A.M * A.G, blocks = (rows + 16 * RT * RW - 1) / (16 * RT * RW);
+    const int rows = A.M * A.G, blocks = (rows + 32 * RW - 1) / (32 * RW);
     const int kvh = blockIdx.x % A.n_head_kv, item = blockIdx.x / A.n_head_kv;
-    const int split = item % A.splits, row0 = (blocks - 1 - item / A.splits) * 16 * RT * RW;
+    const int split = item % A.splits, row0 = (blocks - 1 - item / A.splits) * 32 * RW;
     const size_t p0 = A.pos[0];
     auto end_of = [&](int row) { return (int)min(p0 + (size_t)(row / A.G) + 1, A.n_ctx); };
-    const int last = end_of(min(row0 + 16 * RT * RW, rows) - 1), first = end_of(row0);
+    const int last = end_of(min(row0 + 32 * RW, rows) - 1), first = end_of(row0);
     const int n_tiles = (last + KVQ_TILE - 1) / KVQ_TILE, step = A.splits * PW;
     if (split * PW >= n_tiles) return;                           // (uniform)
     const int used = min(A.splits, (n_tiles + PW - 1) / PW);
-    const int my_row0 = row0 + 16 * RT * rw;
+    const int row = row0 + 32 * rw + r, end = end_of(min(row, rows - 1));
     const uint8_t *base = A.cache + (size_t)kvh * ((A.n_ctx + KVQ_TILE - 1) / KVQ_TILE) * REC;
 
-    // the words of this wave's fragments; fragment f of K is step j = f % NG
-    // of positions 16 (f / NG) + 0..15, of V the dimensions 16 f + 0..15
-    uint32_t kw[FW][BITS / 4], vw[FW][BITS / 4];
-    uint16_t ks[FW];
+    // the words of this wave's fragments, and where they are in a record
+    uint32_t kw[FW][BITS / 4], vw[FW][BITS / 4], kat[FW], sat[FW], vat[FW], wat[FW];
+    uint8_t ks[FW];
     uint2 vs[FW];
+#pragma unroll
+    for (int u = 0; u < FW; u++) {
+        const int f = min(rw * FW + u, NF - 1), oct = c * NF + f;
+        kat[u] = r * (4 * NG * BITS) + oct * BITS;
+        sat[u] = 2 * CODES + kvq_k_scale(oct >> 2, r);
+        vat[u] = CODES + ((32 * (f >> 1) + r) * 4 + 2 * (f & 1) + c) * BITS;
+        wat[u] = 2 * CODES + 32 * NG + (f >> 1) * 32 + (2 * (f & 1) + c) * 8;
+    }
     auto record = [&](int tile) __attribute__((always_inline)) {
         return base + (size_t)min(tile, n_tiles - 1) * REC;
     };
@@ -462,18 +479,16 @@ __global__ __launch_bounds__(512, 2) void kv_attn_many(AttnArgs A)
         const uint8_t *rec = record(tile);
 #pragma unroll
         for (int u = 0; u < FW; u++) {
-            const int f = min(rw * FW + u, NF - 1), i = f / NG, j = f % NG;
-            __builtin_memcpy(kw[u], __builtin_assume_aligned(rec + (16 * i + r) * (4 * NG * BITS) + (c * NG + j) * BITS, BITS), BITS);
-            ks[u] = *(const uint16_t *)(rec + 2 * CODES + k_group<NG>(c, j) * 32 + r * 2);
+            __builtin_memcpy(kw[u], __builtin_assume_aligned(rec + kat[u], BITS), BITS);
+            ks[u] = rec[sat[u]];
         }
     };
     auto fetch_v = [&](int tile) __attribute__((always_inline)) {
         const uint8_t *rec = record(tile);
 #pragma unroll
         for (int u = 0; u < FW; u++) {
-            const int f = min(rw * FW + u, NF - 1);
-            __builtin_memcpy(vw[u], __builtin_assume_aligned(rec + CODES + ((16 * f + r) * 4 + c) * BITS, BITS), BITS);
-            vs[u] = *(const uint2 *)(rec + 2 * CODES + 32 * NG + (f >> 1) * 32 + c * 8);
+            __builtin_memcpy(vw[u], __builtin_assume_aligned(rec + vat[u], BITS), BITS);
+            vs[u] = *(const uint2 *)(rec + wat[u]);
         }
     };
     auto place = [&](int buf) __attribute__((always_inline)) {   // a tile's K fragments; V's NF further on
@@ -484,7 +499,7 @@ __global__ __launch_bounds__(512, 2) void kv_attn_many(AttnArgs A)
         for (int u = 0; u < FW; u++) {
             const int f = rw * FW + u;
             if (FW * RW > NF && f >= NF) break;
-            place(buf)[f * 64] = unpack_k<BITS>(kw[u], ks[u], f / NG);
+            place(buf)[f * 64] = unpack_k<BITS>(kw[u], ks[u], 0);
         }
     };
     auto stage_v = [&](int buf) __attribute__((always_inline)) {
@@ -497,53 +512,56 @@ __global__ __launch_bounds__(512, 2) void kv_attn_many(AttnArgs A)
             place(buf)[(NF + f) * 64] = unpack<BITS>(vw[u], d, mm);
         }
     };
-    auto trim = [&](int tile, int buf) __attribute__((always_inline)) {   // the fetched V words' scales
+    // the fetched V words' scales, where not every row sees the tile whole
+    auto trim = [&](int tile, int buf) __attribute__((always_inline)) {
         const int tp = tile * KVQ_TILE;
         if (tp + KVQ_TILE <= first) return;                      // (uniform)
 #pragma unroll
         for (int u = 0; u < FW; u++) {
             const int f = rw * FW + u;
-            int p = trim_scales(vs[u], tp, c, last);
-            p = min(p, __shfl_xor(p, 16));
+            int p = trim_scales(vs[u], tp, 2 * (f & 1) + c, last);
             p = min(p, __shfl_xor(p, 32));
-            if (lane == 0 && (f & 1) == 0 && f < NF) nan_at[buf][pw][f >> 1] = p;
+            if (lane == 0 && f < NF) atomicMin(&nan_at[buf][pw][f >> 1], p);
         }
     };
 
+    if (threadIdx.x < 2 * PW * NG) (&nan_at[0][0][0])[threadIdx.x] = 0x7FFFFFFF;
     int tile = split * PW + pw;
     fetch_k(tile);
     fetch_v(tile);
-    h8v qh[RT][NG], ql[RT][NG];
-    float sc[RT], m[RT], l[RT];
-    int end[RT];
-    f4v o[RT][NF], s[RT][2];
-#pragma unroll
-    for (int t = 0; t < RT; t++) {
-        const int row = min(my_row0 + 16 * t + r, rows - 1);
-        end[t] = end_of(row);
-        sc[t] = load_query<NG>(qh[t], ql[t], A.q + (size_t)(row / A.G) * A.q_stride +
-                                                 ((size_t)kvh * A.G + row % A.G) * A.hd, c, A);
-        m[t] = -FLT_MAX;
-        l[t] = 0.0f;
-#pragma unroll
-        for (int d = 0; d < NF; d++) o[t][d] = f4v{0, 0, 0, 0};
+    // queries, through LDS: a row's pieces side by side from memory (a lane a
+    // row touches 64 lines with every load)
+    float *rowbuf = (float *)frag;
+    for (int it = threadIdx.x; it < 32 * RW * WIDTH / 4; it += 64 * RW * PW) {
+        const int rr = it / (WIDTH / 4), d = it % (WIDTH / 4) * 4;
+        *(float4 *)(rowbuf + rr * ROW + d) = query_quad(query_row(A, kvh, min(row0 + rr, rows - 1)), d, A);
     }
+    __syncthreads();
+    h8v qh[NF], ql[NF];
+    float sc;
+    {
+        float x[NF][8];
+#pragma unroll
+        for (int j = 0; j < 2 * NF; j++)
+            *(float4 *)&x[j >> 1][4 * (j & 1)] =
+                *(const float4 *)(rowbuf + (32 * rw + r) * ROW + 8 * NF * c + 4 * j);
+        sc = split_query<NF, 2>(qh, ql, x, A.hd);
+    }
+    float m = -FLT_MAX, l = 0.0f;
+    f16v o[NG], s;
+#pragma unroll
+    for (int d = 0; d < NG; d++) o[d] = f16v{};
     auto score = [&](int buf) __attribute__((always_inline)) {
         const h8v *src = place(buf);
+        s = f16v{};
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-#pragma unroll
-            for (int t = 0; t < RT; t++) s[t][i] = f4v{0, 0, 0, 0};
-#pragma unroll
-            for (int j = 0; j < NG; j++) {
-                const h8v kf = src[(i * NG + j) * 64];
-#pragma unroll
-                for (int t = 0; t < RT; t++) s[t][i] = mfma(kf, qh[t][j], s[t][i]);
-#pragma unroll
-                for (int t = 0; t < RT; t++) s[t][i] = mfma(kf, ql[t][j], s[t][i]);
-            }
+        for (int f = 0; f < NF; f++) {
+            const h8v kf = src[f * 64];
+            s = mfma(kf, qh[f], s);
+            s = mfma(kf, ql[f], s);
         }
     };
+    __syncthreads();                                             // (nan_at; the queries are read)
     trim(tile, 0);
     stage_k(0);
     stage_v(0);
@@ -558,22 +576,35 @@ __global__ __launch_bounds__(512, 2) void kv_attn_many(AttnArgs A)
     for (int n = 0; n < n_steps; n++, tile += step) {
         const int buf = n & 1, tp = tile * KVQ_TILE;
         if (tp + KVQ_TILE > first) {                             // (uniform)
-            const float bad = __uint_as_float(0x7FC00000u);
 #pragma unroll
-            for (int t = 0; t < RT; t++) {
-                hide(s[t], tp, c, end[t]);
+            for (int e = 0; e < 16; e++)
+                if (tp + 8 * (e >> 2) + 4 * c + (e & 3) >= end) s[e] = -INFINITY;
 #pragma unroll
-                for (int g = 0; g < NG; g++)
-                    if (nan_at[buf][pw][g] < end[t]) o[t][2 * g] = o[t][2 * g + 1] = f4v{bad, bad, bad, bad};
-            }
+            for (int g = 0; g < NG; g++)
+                if (nan_at[buf][pw][g] < end) o[g] = f16v{} + __uint_as_float(0x7FC00000u);
         }
         trim(tile + step, buf ^ 1);
+        float top = max3(s[0], s[1], s[2]);
 #pragma unroll
-        for (int t = 0; t < RT; t++) follow<NF>(s[t], sc[t], m[t], l[t], o[t]);
+        for (int e = 3; e < 15; e += 2) top = max3(top, s[e], s[e + 1]);
+        top = max3(top, s[15], s[15]) * sc;
+        if (__any(top > m + KA_ROOM)) {
+            const float mn = fmaxf(m, fmaxf(top, __shfl_xor(top, 32))), f = __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < NG; d++) o[d] *= f;
+        }
         // this tile's weights beside the next one's scores
-        h8v ph[RT], pl[RT];
+        h8v ph[2], pl[2];
+        {
+            float x[16];
 #pragma unroll
-        for (int t = 0; t < RT; t++) weigh(s[t], sc[t], m[t], l[t], ph[t], pl[t]);
+            for (int e = 0; e < 16; e++) x[e] = s[e];
+            const float off = KA_LIFT - m;
+            weigh(x, sc, off, l, ph[0], pl[0]);
+            weigh(x + 8, sc, off, l, ph[1], pl[1]);
+        }
         score(buf ^ 1);
         // its values beside the unpacking of the next one's, and of the keys after those
         stage_k(buf);
@@ -582,51 +613,70 @@ __global__ __launch_bounds__(512, 2) void kv_attn_many(AttnArgs A)
         fetch_v(tile + 2 * step);
         const h8v *src = place(buf) + NF * 64;
 #pragma unroll
-        for (int k = 0; k < NF; k++) {
-            const h8v vf = src[k * 64];
+        for (int i = 0; i < 2; i++)
 #pragma unroll
-            for (int t = 0; t < RT; t++) o[t][k] = mfma(vf, ph[t], o[t][k]);
-#pragma unroll
-            for (int t = 0; t < RT; t++) o[t][k] = mfma(vf, pl[t], o[t][k]);
-        }
+            for (int d = 0; d < NG; d++) {
+                const h8v vf = src[(2 * d + i) * 64];
+                o[d] = mfma(vf, ph[i], o[d]);
+                o[d] = mfma(vf, pl[i], o[d]);
+            }
         __syncthreads();
     }
 
-    // the groups' sums at their common maximum, group 0's waves adding them up
-    f4v *so = (f4v *)frag;
+    // the groups' sums at their common maximum, group 0's waves adding them
+    // up; a wave's rows in LDS, then whole to memory
+    l += __shfl_xor(l, 32);
+    if (c == 0) {
+        sm[pw][rw][r] = m;
+        sl[pw][rw][r] = l;
+    }
+    float *mine = rowbuf + 32 * rw * ROW + r * ROW + 4 * c;      // (group 1's sums, then the result)
+    auto quad = [&](int k) { return f4v{o[k >> 2][4 * (k & 3)], o[k >> 2][4 * (k & 3) + 1],
+                                        o[k >> 2][4 * (k & 3) + 2], o[k >> 2][4 * (k & 3) + 3]}; };
+    if (pw) {
 #pragma unroll
-    for (int t = 0; t < RT; t++) {
-        l[t] = quad_sum(l[t]);
-        if (c == 0) {
-            sm[pw][rw][t][r] = m[t];
-            sl[pw][rw][t][r] = l[t];
-        }
-        if (pw) {
-#pragma unroll
-            for (int k = 0; k < NF; k++) so[(((pw - 1) * RW + rw) * RT * NF + t * NF + k) * 64 + lane] = o[t][k];
-        }
+        for (int k = 0; k < 4 * NG; k++) *(f4v *)(mine + (pw - 1) * 32 * RW * ROW + 8 * k) = quad(k);
     }
     __syncthreads();
     if (pw) return;
+    float mx = m, sum = 0.0f, f[PW];
 #pragma unroll
-    for (int t = 0; t < RT; t++) {
-        const int row = my_row0 + 16 * t + r;
-        if (row >= rows) continue;
-        float mx = m[t], sum = 0.0f, f[PW];
+    for (int w = 1; w < PW; w++) mx = fmaxf(mx, sm[w][rw][r]);
 #pragma unroll
-        for (int w = 1; w < PW; w++) mx = fmaxf(mx, sm[w][rw][t][r]);
+    for (int w = 0; w < PW; w++) {
+        f[w] = __builtin_amdgcn_exp2f(sm[w][rw][r] - mx);
+        sum += sl[w][rw][r] * f[w];
+    }
+    const float by = used == 1 ? 0.25f / sum : 1.0f;
 #pragma unroll
-        for (int w = 0; w < PW; w++) {
-            f[w] = __builtin_amdgcn_exp2f(sm[w][rw][t][r] - mx);
-            sum += sl[w][rw][t][r] * f[w];
-        }
+    for (int k = 0; k < 4 * NG; k++) {
+        f4v v = quad(k) * f[0];
 #pragma unroll
-        for (int k = 0; k < NF; k++) {
-            f4v v = o[t][k] * f[0];
+        for (int w = 1; w < PW; w++) v += *(const f4v *)(mine + (w - 1) * 32 * RW * ROW + 8 * k) * f[w];
+        *(f4v *)(mine + 8 * k) = v * by;
+    }
+    if (used > 1 && c == 0 && row < rows) {
+        float *dst = A.part + (((size_t)kvh * rows + row) * A.splits + split) * (4 + WIDTH);
+        dst[0] = mx;
+        dst[1] = sum;
+    }
+    __builtin_amdgcn_wave_barrier();
+    // (this wave's own rows: no other wave's writes to wait for)
+    for (int it = lane; it < 32 * WIDTH / 4; it += 64) {
+        const int rr = 32 * rw + it / (WIDTH / 4), d = it % (WIDTH / 4) * 4, at = row0 + rr;
+        if (at >= rows) continue;
+        const f4v v = *(const f4v *)(rowbuf + rr * ROW + d);
+        if (used > 1) {
+            *(f4v *)(A.part + (((size_t)kvh * rows + at) * A.splits + split) * (4 + WIDTH) + 4 + d) = v;
+        } else {
+            float *dst = A.out + (size_t)(at / A.G) * A.out_stride + ((size_t)kvh * A.G + at % A.G) * A.hd + d;
+            if (A.out_wide) {
+                if (d < A.hd) *(f4v *)dst = v;
+            } else {
 #pragma unroll
-            for (int w = 1; w < PW; w++)
-                v += so[(((w - 1) * RW + rw) * RT * NF + t * NF + k) * 64 + lane] * f[w];
-            put_sums(A, kvh, row, 16 * k + 4 * c, v, mx, sum, used == 1, split, WIDTH);
+                for (int e = 0; e < 4; e++)
+                    if (d + e < A.hd) dst[e] = v[e];
+            }
         }
     }
 }
@@ -684,6 +734,52 @@ __global__ __launch_bounds__(256) void kv_merge_k(AttnArgs A, int width, int row
     }
 }
 
+// The same for up to 16 splits: 32 threads to a row, eight rows to a workgroup,
+// a column quad's records read together.
+__global__ __launch_bounds__(256) void kv_merge_rows_k(AttnArgs A, int width, int rows_per, int tiles_per)
+{
+    const int rows = A.M * A.G, row = blockIdx.x * 8 + (threadIdx.x >> 5), kvh = blockIdx.y;
+    if (row >= rows) return;
+    const int row_last = min(row / rows_per * rows_per + rows_per, rows) - 1;
+    const int last = (int)min((size_t)A.pos[0] + (size_t)(row_last / A.G) + 1, A.n_ctx);
+    const int n_tiles = (last + KVQ_TILE - 1) / KVQ_TILE;
+    const int used = min(A.splits, (n_tiles + tiles_per - 1) / tiles_per);
+    if (used == 1) return;
+    const size_t rec = 4 + (size_t)width;
+    const float *base = A.part + ((size_t)kvh * rows + row) * A.splits * rec;
+    float *dst = A.out + (size_t)(row / A.G) * A.out_stride + ((size_t)kvh * A.G + row % A.G) * A.hd;
+    for (int c4 = threadIdx.x & 31; c4 < width / 4; c4 += 32) {
+        float m = -FLT_MAX, l = 0.0f;
+        f4v o = {0, 0, 0, 0};
+        for (int s0 = 0; s0 < used; s0 += 4) {
+            float ms[4], ls[4];
+            f4v os[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const float *p = base + (size_t)min(s0 + k, used - 1) * rec;
+                ms[k] = p[0];
+                ls[k] = p[1];
+                os[k] = *(const f4v *)(p + 4 + 4 * c4);
+            }
+            const float mn = fmaxf(fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3])), m);
+            const float f = __builtin_amdgcn_exp2f(m - mn);
+            l *= f;
+            o *= f;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const float g = s0 + k < used ? __builtin_amdgcn_exp2f(ms[k] - mn) : 0.0f;
+                if (s0 + k < used) {
+                    l += ls[k] * g;
+                    o += os[k] * g;
+                }
+            }
+            m = mn;
+        }
+        for (int e = 0; e < 4; e++)
+            if (4 * c4 + e < A.hd) dst[4 * c4 + e] = o[e] * 0.25f / l;
+    }
+}
+
 template <int BITS>
 static const void *few_kernel(int ng, int T)
 {
@@ -699,16 +795,16 @@ static const void *few_kernel(int ng, int T)
 #undef FOX_FEW
 }
 
-template <int BITS>
+template <int BITS, int RW>
 static const void *many_kernel(int ng)
 {
     switch (ng) {
-    case 1: return (const void *)kv_attn_many<BITS, 1, 4>;
-    case 2: return (const void *)kv_attn_many<BITS, 2, 4>;
-    case 3: return (const void *)kv_attn_many<BITS, 3, 4>;
-    case 4: return (const void *)kv_attn_many<BITS, 4, 4>;
-    case 6: return (const void *)kv_attn_many<BITS, 6, 4>;
-    default: return (const void *)kv_attn_many<BITS, 8, 4>;
+    case 1: return (const void *)kv_attn_many<BITS, 1, RW, 8 / RW>;
+    case 2: return (const void *)kv_attn_many<BITS, 2, RW, 8 / RW>;
+    case 3: return (const void *)kv_attn_many<BITS, 3, RW, 8 / RW>;
+    case 4: return (const void *)kv_attn_many<BITS, 4, RW, 8 / RW>;
+    case 6: return (const void *)kv_attn_many<BITS, 6, 4, 1>;
+    default: return (const void *)kv_attn_many<BITS, 8, 4, 1>;
     }
 }
 
@@ -743,27 +839,34 @@ extern "C" fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, si
     A.G = (int)(n_head / n_head_kv);
     A.hd = (int)head_dim;
     A.M = (int)M;
-    A.q_wide = head_dim % 8 == 0 && (uintptr_t)q % 16 == 0 && (M == 1 || q_stride % 4 == 0);
+    A.q_wide = head_dim % 4 == 0 && (uintptr_t)q % 16 == 0 && (M == 1 || q_stride % 4 == 0);
+    A.out_wide = head_dim % 4 == 0 && (uintptr_t)out % 16 == 0 && (M == 1 || out_stride % 4 == 0);
     const int width = kvq_width((int)head_dim), ng = width / 32;
     const size_t rows = M * (size_t)A.G;
     const bool many = rows > 32, q4 = kv_type == FOX_GPU_KV_Q4;
     const int T = rows <= 16 || ng > 6 ? 1 : 2;
-    const int per = many ? 16 * (ng > 4 ? 1 : 2) * 4 : 16 * T;          // rows of a workgroup
-    const int tiles_per = many ? 2 : KA_WAVES;                        // tiles it takes side by side
+    // many rows: 128 of them in four waves, tiles in two groups; up to 64 in two
+    // waves and four groups; heads past 128 dimensions hold one group's registers only
+    const int rw = ng > 4 || rows > 64 ? 4 : 2, pw = ng > 4 ? 1 : 8 / rw;
+    const int per = many ? 32 * rw : 16 * T;                            // rows of a workgroup
+    const int tiles_per = many ? pw : KA_WAVES;                         // tiles it takes side by side
     const size_t blocks = (rows + per - 1) / per, items = n_head_kv * blocks;
-    size_t splits = 1;
     const size_t most = (n_ctx + KVQ_TILE * tiles_per - 1) / (KVQ_TILE * tiles_per);
+    size_t splits = 1;
     if (!many) {
         splits = 2 * (size_t)ctx->n_cu / items;
     } else {
-        // one workgroup to a compute unit: the number of splits whose rounds
-        // leave the fewest of them idle, each split's records priced at 1/32
-        double best = 1e30;
-        for (size_t s = 1; s <= 16; s++) {
-            const double cost = (double)((items * s + ctx->n_cu - 1) / ctx->n_cu) / (double)s +
-                                (s > 1 ? 0.03 * (double)s * (double)items / ctx->n_cu : 0.0);
-            if (cost < best) {
-                best = cost;
+        // One workgroup to a compute unit.  More splits fill the last round, at
+        // the price of their records, which leave the caches at the kernel's end
+        // and come back: measured 1.65 us a step of a workgroup, 1 us a MB of records
+        // (a 1024-token prompt of 32 heads over 8 of 128 in 2 splits: 38.7 -> 71 us).
+        double best = 0.0;
+        for (size_t s = 1; s <= 64 && s <= most; s++) {
+            const double rounds = (double)((items * s + ctx->n_cu - 1) / ctx->n_cu);
+            const double us = rounds * (8.0 + 1.65 * (double)((most + s - 1) / s)) +
+                              (s > 1 ? 5.0 + 1e-6 * (double)(items * s * per) * (4 + width) * 4 : 0.0);
+            if (s == 1 || us < best) {
+                best = us;
                 splits = s;
             }
         }
@@ -778,18 +881,25 @@ extern "C" fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, si
     }
     void *args[] = {&A};
     if (many) {
-        const void *k = q4 ? many_kernel<4>(ng) : many_kernel<8>(ng);
-        const size_t lds = 2 * (size_t)tiles_per * 4 * ng * 1024;
+        const void *k = rw == 2 ? (q4 ? many_kernel<4, 2>(ng) : many_kernel<8, 2>(ng))
+                                : (q4 ? many_kernel<4, 4>(ng) : many_kernel<8, 4>(ng));
+        const size_t tiles_lds = 2 * (size_t)tiles_per * 4 * ng * 1024;
+        const size_t rows_lds = 32 * (size_t)rw * (pw > 2 ? pw - 1 : 1) * (width + 4) * sizeof(float);
+        const size_t lds = tiles_lds > rows_lds ? tiles_lds : rows_lds;
         FOX_HIP(hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-        FOX_HIP(hipLaunchKernel(k, dim3((unsigned)(items * splits)), dim3(512), args, lds, ctx->stream));
+        FOX_HIP(hipLaunchKernel(k, dim3((unsigned)(items * splits)), dim3(64 * rw * pw), args, lds, ctx->stream));
     } else {
         FOX_HIP(hipLaunchKernel(q4 ? few_kernel<4>(ng, T) : few_kernel<8>(ng, T),
                                 dim3((unsigned)splits, (unsigned)n_head_kv, (unsigned)blocks),
                                 dim3(64 * KA_WAVES), args, 0, ctx->stream));
     }
     if (splits > 1) {
-        hipLaunchKernelGGL(kv_merge_k, dim3((unsigned)rows, (unsigned)n_head_kv), dim3(256), 0,
-                           ctx->stream, A, width, per, tiles_per);
+        if (splits <= 16)
+            hipLaunchKernelGGL(kv_merge_rows_k, dim3((unsigned)((rows + 7) / 8), (unsigned)n_head_kv),
+                               dim3(256), 0, ctx->stream, A, width, per, tiles_per);
+        else
+            hipLaunchKernelGGL(kv_merge_k, dim3((unsigned)rows, (unsigned)n_head_kv), dim3(256), 0,
+                               ctx->stream, A, width, per, tiles_per);
         FOX_LAUNCHED("kvq attention merge");
     }
     return FOX_GPU_OK;

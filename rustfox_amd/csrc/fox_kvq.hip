@@ -333,7 +333,7 @@ __global__ __launch_bounds__(KS_THREADS) void kv_store_k(StoreArgs A)
             bool any = whole;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const int r = (e & 3) + 4 * c + 16 * (e >> 2);
+                const int r = kvq_v_pos(c, e);
                 const bool on = whole || (r >= r0 && r < r0 + nt);
                 any |= on;
                 code[e] = on ? lds[r * LROW + dim]
@@ -413,7 +413,7 @@ __global__ __launch_bounds__(KS_THREADS) void kv_read_k(const uint8_t *__restric
             const uint2 s = *(const uint2 *)(rec + L.vs + (d0 >> 5) * 32 + c * 8);
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const int r = (e & 3) + 4 * c + 16 * (e >> 2);
+                const int r = kvq_v_pos(c, e);
                 const float d = kvq_scale((e < 4 ? s.x : s.y) >> (8 * (e & 3)) & 255u);
                 float x[4];
 #pragma unroll

@@ -20,12 +20,11 @@
 // Layout.  A layer's cache is [n_head_kv][tiles of 32 positions] records, each
 //   K codes  [32 positions][width BITS / 8 bytes]
 //   V codes  [width dims][4 chunks][8 positions: BITS bytes]
-//   K scales [width / 32 groups][16][2]       position 16 i + r at [g][r][i]
+//   K scales [width / 32 groups][16][2]       position 16 (r / 8) + 8 i + r % 8 at [g][r][i]
 //   V scales [width / 32 groups][4 chunks][8]
-// with the eight positions of V chunk c being 4 c + r and 16 + 4 c + r
-// (r < 4) in that order: the positions whose scores a lane of the matrix core's
-// result holds for two 16-position tiles, so the softmax's weights are the
-// next product's operand where they are.  Eight values of 4 bits make a dword
+// with the eight positions of V chunk c (kvq_v_pos) being those whose scores a
+// lane of the matrix cores' result holds, so that the softmax's weights are
+// the next product's operand where they are.  Eight values of 4 bits make a dword
 // whose nibble e / 2 + 4 (e % 2) holds value e, so that a mask takes values
 // 2 i and 2 i + 1 as the halves of one register; 8-bit values are in order.
 // Codes are stored as c + h.
@@ -68,10 +67,20 @@ __host__ __device__ inline KvqLayout kvq_layout(int bits, int hd)
     return l;
 }
 
-// chunk c and place e of a tile's position r in the V codes and scales
-__device__ __forceinline__ int kvq_v_chunk(int r) { return (r & 15) >> 2; }
-__device__ __forceinline__ int kvq_v_place(int r) { return (r & 3) + 4 * (r >> 4); }
-__device__ __forceinline__ int kvq_k_scale(int g, int r) { return g * 32 + (r & 15) * 2 + (r >> 4); }
+// Position of place e in chunk c of a tile.  A 32x32 result holds, in lane half
+// c % 2, rows 8 a + 4 (c % 2) + 0..3 for a = 0..3, and an operand's lane eight of
+// 16 summands: chunk c is a = 2 (c / 2) and the next.
+__host__ __device__ inline int kvq_v_pos(int c, int e)
+{
+    return 16 * (c >> 1) + 8 * (e >> 2) + 4 * (c & 1) + (e & 3);
+}
+// and back: chunk and place of a tile's position r
+__device__ __forceinline__ int kvq_v_chunk(int r) { return 2 * (r >> 4) + (r >> 2 & 1); }
+__device__ __forceinline__ int kvq_v_place(int r) { return (r & 3) + 4 * (r >> 3 & 1); }
+__device__ __forceinline__ int kvq_k_scale(int g, int r)
+{
+    return g * 32 + (8 * (r >> 4) + (r & 7)) * 2 + (r >> 3 & 1);
+}
 __device__ __forceinline__ int kvq_v_scale(int g, int r)
 {
     return g * 32 + kvq_v_chunk(r) * 8 + kvq_v_place(r);
