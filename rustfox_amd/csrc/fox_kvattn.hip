@@ -121,32 +121,42 @@ __device__ __forceinline__ int trim_scales(uint2 &b2, int tp, int c, int last)
     return at;
 }
 
-// A lane's part c of a query row's dimensions as two halves each, the eight from
-// 8 (N c + j) on for product step j, scaled by a power of two; the row's PARTS parts
-// are in lanes 64 / PARTS apart.  x: the part's floats.  Returns what turns a
-// score of theirs into powers of two.
-template <int N, int PARTS>
-__device__ __forceinline__ float split_query(h8v qh[N], h8v ql[N], const float (*x)[8], int hd)
+// a - (float)h for the two halves of h
+__device__ __forceinline__ float less_lo(float a, h2v h)
 {
-    float top = 0.0f;
-#pragma unroll
-    for (int j = 0; j < N; j++)
-#pragma unroll
-        for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[j][e]));
-    top = PARTS == 4 ? quad_max(top) : fmaxf(top, __shfl_xor(top, 32));
-    // 2^(14 - exponent of the largest), the exponent kept within range
+    float d;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(d) : "v"(as_u(h)), "v"(a));
+    return d;
+}
+__device__ __forceinline__ float less_hi(float a, h2v h)
+{
+    float d;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
+        : "=v"(d) : "v"(as_u(h)), "v"(a));
+    return d;
+}
+
+// 2^(14 - exponent of a row's largest value), the exponent kept within range;
+// back turns a score of the scaled row into powers of two
+__device__ __forceinline__ float query_scale(float top, int hd, float &back)
+{
     const int ex = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 113);
-    const float up = __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
+    back = 1.44269504f / sqrtf((float)hd) * 0.25f * __uint_as_float((uint32_t)(127 - 14 + ex) << 23);
+    return __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
+}
+
+// eight scaled values as two halves each
+__device__ __forceinline__ void split_8(const float x[8], float up, h8v &hi, h8v &lo)
+{
+    h2v h[4], d[4];
 #pragma unroll
-    for (int j = 0; j < N; j++)
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float y = x[j][e] * up;
-            const _Float16 hi = (_Float16)y;
-            qh[j][e] = hi;
-            ql[j][e] = (_Float16)(y - (float)hi);
-        }
-    return 1.44269504f / sqrtf((float)hd) * 0.25f * __uint_as_float((uint32_t)(127 - 14 + ex) << 23);
+    for (int i = 0; i < 4; i++) {
+        const float a = x[2 * i] * up, b = x[2 * i + 1] * up;
+        h[i] = h2v{(_Float16)a, (_Float16)b};
+        d[i] = h2v{(_Float16)less_lo(a, h[i]), (_Float16)less_hi(b, h[i])};
+    }
+    hi = __builtin_bit_cast(h8v, *(u4v *)h);
+    lo = __builtin_bit_cast(h8v, *(u4v *)d);
 }
 
 // four floats of a query row from dimension d on (zero past hd)
@@ -169,21 +179,6 @@ __device__ __forceinline__ float max3(float a, float b, float c)
     return d;
 }
 
-// a - (float)h for the two halves of h
-__device__ __forceinline__ float less_lo(float a, h2v h)
-{
-    float d;
-    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(d) : "v"(as_u(h)), "v"(a));
-    return d;
-}
-__device__ __forceinline__ float less_hi(float a, h2v h)
-{
-    float d;
-    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
-        : "=v"(d) : "v"(as_u(h)), "v"(a));
-    return d;
-}
-
 // The weights of eight positions from their scores, as two halves each, and their sum.
 __device__ __forceinline__ void weigh(const float s[8], float sc, float off, float &l, h8v &ph, h8v &pl)
 {
@@ -198,6 +193,12 @@ __device__ __forceinline__ void weigh(const float s[8], float sc, float off, flo
     }
     ph = __builtin_bit_cast(h8v, *(u4v *)hi);
     pl = __builtin_bit_cast(h8v, *(u4v *)lo);
+}
+
+// the value of lane r ^ 8 of each 16
+__device__ __forceinline__ float other_half(float v)
+{
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x128, 0xF, 0xF, true));
 }
 
 __device__ __forceinline__ f4v mfma(h8v a, h8v b, f4v c)
@@ -264,23 +265,44 @@ struct Tile {
     }
 };
 
-// Partial attention of T x 16 query rows over the tiles that fall to one wave
-// (tiles w0, w0 + step, ...); the four waves of a workgroup are merged through
-// LDS, and with several splits per kv head a record (m, l, -, -, o) goes to
-// the workspace for kv_merge_k.
-template <int BITS, int NG, int T>
+// Few rows: partial attention of ROWS query rows over the tiles that fall to one
+// wave (w0, w0 + step, ...), unpacked in its registers; the four waves of a
+// workgroup are merged through LDS, and with several splits per kv head a record
+// (m, l, -, -, o) goes to the workspace for the merge kernels.
+// ROWS 8: the columns of one product hold the rows' upper halves and their
+// lower ones, so a tile takes half the products; the two columns of a row are
+// added where a score is used and at the end.
+template <int BITS, int NG, int ROWS>
 __global__ __launch_bounds__(64 * KA_WAVES) void kv_attn_few(AttnArgs A)
 {
-    constexpr int WIDTH = 32 * NG;
-    __shared__ f4v so[KA_WAVES][NG][64];
+    constexpr bool PACK = ROWS == 8;
+    constexpr int WIDTH = 32 * NG, T = ROWS == 32 ? 2 : 1, NT = T * 2 * NG, NQ = PACK ? 1 : 2;
+    constexpr int ROUND = NT < 8 ? NT : 8;                       // tiles of sums merged at a time
+    constexpr int JW = (NG + KA_WAVES - 1) / KA_WAVES;           // product steps a wave prepares
+    constexpr int QF = T * NG * NQ, SH = ROUND * KA_WAVES > QF ? ROUND * KA_WAVES : QF;
+    __shared__ f4v shared[SH][64];                               // query operands, then sums
     __shared__ float sm[KA_WAVES][T][16], sl[KA_WAVES][T][16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, c = lane >> 4;
-    const int split = blockIdx.x, kvh = blockIdx.y, row0 = blockIdx.z * 16 * T;
+    const int split = blockIdx.x, kvh = blockIdx.y, row0 = blockIdx.z * ROWS;
     const int rows = A.M * A.G;
+    // queries: lane (r, c) has row r's dimensions of chunk c, product step j the
+    // eight from 8 (NG c + j) on; a wave prepares some steps for all
+    float x[T][JW][8];
+    const int rq = PACK ? r & 7 : r;
+#pragma unroll
+    for (int t = 0; t < T; t++) {
+        const float *qr = query_row(A, kvh, min(row0 + 16 * t + rq, rows - 1));
+#pragma unroll
+        for (int u = 0; u < JW; u++) {
+            const int j = min(wave + KA_WAVES * u, NG - 1);
+            *(float4 *)x[t][u] = query_quad(qr, 8 * (NG * c + j), A);
+            *(float4 *)(x[t][u] + 4) = query_quad(qr, 8 * (NG * c + j) + 4, A);
+        }
+    }
     const size_t p0 = A.pos[0];
     auto end_of = [&](int row) { return (int)min(p0 + (size_t)(row / A.G) + 1, A.n_ctx); };
-    const int last = end_of(min(row0 + 16 * T, rows) - 1);       // positions any row sees
+    const int last = end_of(min(row0 + ROWS, rows) - 1);         // positions any row sees
     const int first = end_of(row0);                              // and all rows see
     const int n_tiles = (last + KVQ_TILE - 1) / KVQ_TILE, step = A.splits * KA_WAVES;
     if (split * KA_WAVES >= n_tiles) return;                     // (uniform)
@@ -291,30 +313,57 @@ __global__ __launch_bounds__(64 * KA_WAVES) void kv_attn_few(AttnArgs A)
 
     int tile = split * KA_WAVES + wave;
     Tile<BITS, NG> cur;
-    cur.load(base + (size_t)min(tile, n_tiles - 1) * REC, lane);
+    if (tile < n_tiles) cur.load(base + (size_t)tile * REC, lane);
 
-    h8v qh[T][NG], ql[T][NG];
+    h8v q[T][NQ][NG];
     float sc[T], m[T], l[T];
     int end[T];
     f4v o[T][2 * NG];
 #pragma unroll
     for (int t = 0; t < T; t++) {
-        const int row = min(row0 + 16 * t + r, rows - 1);
-        end[t] = end_of(row);
-        const float *qr = query_row(A, kvh, row);
-        float x[NG][8];
+        float top = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 2 * NG; j++) *(float4 *)&x[j >> 1][4 * (j & 1)] = query_quad(qr, 8 * NG * c + 4 * j, A);
-        sc[t] = split_query<NG, 4>(qh[t], ql[t], x, A.hd);
+        for (int u = 0; u < JW; u++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[t][u][e]));
+        top = quad_max(top);
+        if (c == 0) sm[wave][t][r] = top;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < T; t++) {
+        const float top = fmaxf(fmaxf(sm[0][t][r], sm[1][t][r]), fmaxf(sm[2][t][r], sm[3][t][r]));
+        const float up = query_scale(top, A.hd, sc[t]);
+#pragma unroll
+        for (int u = 0; u < JW; u++) {
+            const int j = wave + KA_WAVES * u;
+            h8v hi, lo;
+            split_8(x[t][u], up, hi, lo);
+            if (j >= NG) continue;
+            if (PACK) {
+                *(h8v *)&shared[t * NG + j][lane] = r < 8 ? hi : lo;
+            } else {
+                *(h8v *)&shared[(t * NG + j) * 2][lane] = hi;
+                *(h8v *)&shared[(t * NG + j) * 2 + 1][lane] = lo;
+            }
+        }
+        end[t] = end_of(min(row0 + 16 * t + rq, rows - 1));
         m[t] = -FLT_MAX;
         l[t] = 0.0f;
 #pragma unroll
         for (int d = 0; d < 2 * NG; d++) o[t][d] = f4v{0, 0, 0, 0};
     }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < T; t++)
+#pragma unroll
+        for (int j = 0; j < NG; j++)
+#pragma unroll
+            for (int i = 0; i < NQ; i++) q[t][i][j] = *(const h8v *)&shared[(t * NG + j) * NQ + i][lane];
 
     for (; tile < n_tiles; tile += step) {
         Tile<BITS, NG> next;
-        next.load(base + (size_t)min(tile + step, n_tiles - 1) * REC, lane);
+        if (tile + step < n_tiles) next.load(base + (size_t)(tile + step) * REC, lane);
         const int tp = tile * KVQ_TILE;
         const bool edge = tp + KVQ_TILE > first;                 // (uniform)
         if (edge) {
@@ -342,23 +391,23 @@ __global__ __launch_bounds__(64 * KA_WAVES) void kv_attn_few(AttnArgs A)
             for (int j = 0; j < NG; j++) {
                 const h8v kf = unpack_k<BITS>(cur.k[i] + j * BITS / 4, cur.kscale(j), i);
 #pragma unroll
-                for (int t = 0; t < T; t++) {
-                    s[t][i] = mfma(kf, qh[t][j], s[t][i]);
-                    s[t][i] = mfma(kf, ql[t][j], s[t][i]);
-                }
+                for (int u = 0; u < NQ; u++)
+#pragma unroll
+                    for (int t = 0; t < T; t++) s[t][i] = mfma(kf, q[t][u][j], s[t][i]);
             }
         }
-        h8v ph[T], pl[T];
+        h8v p[T][NQ];
 #pragma unroll
         for (int t = 0; t < T; t++) {
-            float x[8];
+            float y[8];
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                x[e] = s[t][e >> 2][e & 3];
-                if (edge && tp + kvq_v_pos(c, e) >= end[t]) x[e] = -INFINITY;
+                y[e] = s[t][e >> 2][e & 3];
+                if (PACK) y[e] += other_half(y[e]);
+                if (edge && tp + kvq_v_pos(c, e) >= end[t]) y[e] = -INFINITY;
             }
-            const float top = max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]),
-                                   max3(x[6], x[7], x[7])) * sc[t];
+            const float top = max3(max3(y[0], y[1], y[2]), max3(y[3], y[4], y[5]),
+                                   max3(y[6], y[7], y[7])) * sc[t];
             if (__any(top > m[t] + KA_ROOM)) {
                 const float mn = fmaxf(m[t], quad_max(top)), f = __builtin_amdgcn_exp2f(m[t] - mn);
                 m[t] = mn;
@@ -366,27 +415,34 @@ __global__ __launch_bounds__(64 * KA_WAVES) void kv_attn_few(AttnArgs A)
 #pragma unroll
                 for (int d = 0; d < 2 * NG; d++) o[t][d] *= f;
             }
-            weigh(x, sc[t], KA_LIFT - m[t], l[t], ph[t], pl[t]);
+            h8v hi, lo;
+            weigh(y, sc[t], KA_LIFT - m[t], l[t], hi, lo);
+            if (PACK) {
+                p[t][0] = r < 8 ? hi : lo;
+            } else {
+                p[t][0] = hi;
+                p[t][NQ - 1] = lo;
+            }
         }
 #pragma unroll
         for (int g = 0; g < NG; g++) {
             h2v d[4], mm[4];
             v_scales(cur.vs[g], d, mm);
+            h8v vf[2];
 #pragma unroll
-            for (int k = 2 * g; k < 2 * g + 2; k++) {
-                const h8v vf = unpack<BITS>(cur.v[k], d, mm);
+            for (int k = 0; k < 2; k++) vf[k] = unpack<BITS>(cur.v[2 * g + k], d, mm);
 #pragma unroll
-                for (int t = 0; t < T; t++) {
-                    o[t][k] = mfma(vf, ph[t], o[t][k]);
-                    o[t][k] = mfma(vf, pl[t], o[t][k]);
-                }
-            }
+            for (int u = 0; u < NQ; u++)
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+#pragma unroll
+                    for (int t = 0; t < T; t++) o[t][2 * g + k] = mfma(vf[k], p[t][u], o[t][2 * g + k]);
         }
         cur = next;
     }
 
     // the four waves' sums at their common maximum (a wave without tiles has
-    // m = -FLT_MAX and l = 0), NG 16-dimension tiles of 16 rows at a time
+    // m = -FLT_MAX and l = 0), ROUND 16-dimension tiles of 16 rows at a time
 #pragma unroll
     for (int t = 0; t < T; t++) {
         l[t] = quad_sum(l[t]);
@@ -396,28 +452,31 @@ __global__ __launch_bounds__(64 * KA_WAVES) void kv_attn_few(AttnArgs A)
         }
     }
 #pragma unroll
-    for (int t = 0; t < T; t++)
+    for (int k0 = 0; k0 < NT; k0 += ROUND) {
+        __syncthreads();                                         // (the queries, or the last round, are read)
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            if (t + h) __syncthreads();
+        for (int k = k0; k < k0 + ROUND && k < NT; k++)
+            shared[wave * ROUND + k - k0][lane] = o[k / (2 * NG)][k % (2 * NG)];
+        __syncthreads();
 #pragma unroll
-            for (int d = 0; d < NG; d++) so[wave][d][lane] = o[t][h * NG + d];
-            __syncthreads();
-            const int row = row0 + 16 * t + r;
-            for (int k = wave; k < NG && row < rows; k += KA_WAVES) {
-                float mx = sm[0][t][r], sum = 0.0f;
+        for (int u = 0; u < (ROUND + KA_WAVES - 1) / KA_WAVES; u++) {
+            const int k = k0 + wave + KA_WAVES * u, t = k / (2 * NG), row = row0 + 16 * t + r;
+            if (k >= NT || k >= k0 + ROUND || row >= rows || (PACK && r >= 8)) continue;
+            float mx = sm[0][t][r], sum = 0.0f;
 #pragma unroll
-                for (int w = 1; w < KA_WAVES; w++) mx = fmaxf(mx, sm[w][t][r]);
-                f4v v = {0, 0, 0, 0};
+            for (int w = 1; w < KA_WAVES; w++) mx = fmaxf(mx, sm[w][t][r]);
+            f4v v = {0, 0, 0, 0};
 #pragma unroll
-                for (int w = 0; w < KA_WAVES; w++) {
-                    const float f = __builtin_amdgcn_exp2f(sm[w][t][r] - mx);
-                    sum += sl[w][t][r] * f;
-                    v += so[w][k][lane] * f;
-                }
-                put_sums(A, kvh, row, 16 * (h * NG + k) + 4 * c, v, mx, sum, used == 1, split, WIDTH);
+            for (int w = 0; w < KA_WAVES; w++) {
+                const float f = __builtin_amdgcn_exp2f(sm[w][t][r] - mx);
+                sum += sl[w][t][r] * f;
+                f4v part = shared[w * ROUND + k - k0][lane];
+                if (PACK) part += shared[w * ROUND + k - k0][lane + 8];
+                v += part * f;
             }
+            put_sums(A, kvh, row, 16 * (k % (2 * NG)) + 4 * c, v, mx, sum, used == 1, split, WIDTH);
         }
+    }
 }
 
 // Many rows: RW waves of 32 rows each share a tile's unpacked halves in LDS, a
@@ -545,7 +604,14 @@ __global__ __launch_bounds__(64 * RW * PW, NG > 4 ? 1 : 2) void kv_attn_many(Att
         for (int j = 0; j < 2 * NF; j++)
             *(float4 *)&x[j >> 1][4 * (j & 1)] =
                 *(const float4 *)(rowbuf + (32 * rw + r) * ROW + 8 * NF * c + 4 * j);
-        sc = split_query<NF, 2>(qh, ql, x, A.hd);
+        float top = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NF; j++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[j][e]));
+        const float up = query_scale(fmaxf(top, __shfl_xor(top, 32)), A.hd, sc);
+#pragma unroll
+        for (int j = 0; j < NF; j++) split_8(x[j], up, qh[j], ql[j]);
     }
     float m = -FLT_MAX, l = 0.0f;
     f16v o[NG], s;
@@ -703,12 +769,30 @@ __global__ __launch_bounds__(256) void kv_merge_k(AttnArgs A, int width, int row
         float m = -FLT_MAX, l = 0.0f;
         f4v o = {0, 0, 0, 0};
         if (c4 < width / 4)
-            for (int s = sg; s < used; s += 8) {
-                const float *p = base + (size_t)s * rec;
-                const float ms = p[0], mn = fmaxf(m, ms), f = __builtin_amdgcn_exp2f(m - mn),
-                            g = __builtin_amdgcn_exp2f(ms - mn);
-                l = l * f + p[1] * g;
-                o = o * f + *(const f4v *)(p + 4 + 4 * c4) * g;
+            for (int s0 = sg; s0 < used; s0 += 8 * 8) {
+                float ms[8], ls[8];
+                f4v os[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) {                     // (read together)
+                    const float *p = base + (size_t)min(s0 + 8 * k, used - 1) * rec;
+                    ms[k] = p[0];
+                    ls[k] = p[1];
+                    os[k] = *(const f4v *)(p + 4 + 4 * c4);
+                }
+                float mn = m;
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    if (s0 + 8 * k < used) mn = fmaxf(mn, ms[k]);
+                const float f = __builtin_amdgcn_exp2f(m - mn);
+                l *= f;
+                o *= f;
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    if (s0 + 8 * k >= used) continue;
+                    const float g = __builtin_amdgcn_exp2f(ms[k] - mn);
+                    l += ls[k] * g;
+                    o += os[k] * g;
+                }
                 m = mn;
             }
         if (cq == 0) {
@@ -781,16 +865,18 @@ __global__ __launch_bounds__(256) void kv_merge_rows_k(AttnArgs A, int width, in
 }
 
 template <int BITS>
-static const void *few_kernel(int ng, int T)
+static const void *few_kernel(int ng, int per)
 {
-#define FOX_FEW(n) (T == 1 ? (const void *)kv_attn_few<BITS, n, 1> : (const void *)kv_attn_few<BITS, n, 2>)
+#define FOX_FEW(n)                                                                     \
+    (per == 8 ? (const void *)kv_attn_few<BITS, n, 8>                                  \
+              : per == 16 ? (const void *)kv_attn_few<BITS, n, 16> : (const void *)kv_attn_few<BITS, n, 32>)
     switch (ng) {
     case 1: return FOX_FEW(1);
     case 2: return FOX_FEW(2);
     case 3: return FOX_FEW(3);
     case 4: return FOX_FEW(4);
     case 6: return FOX_FEW(6);
-    default: return (const void *)kv_attn_few<BITS, 8, 1>;
+    default: return per == 8 ? (const void *)kv_attn_few<BITS, 8, 8> : (const void *)kv_attn_few<BITS, 8, 16>;
     }
 #undef FOX_FEW
 }
@@ -844,11 +930,10 @@ extern "C" fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, si
     const int width = kvq_width((int)head_dim), ng = width / 32;
     const size_t rows = M * (size_t)A.G;
     const bool many = rows > 32, q4 = kv_type == FOX_GPU_KV_Q4;
-    const int T = rows <= 16 || ng > 6 ? 1 : 2;
     // many rows: 128 of them in four waves, tiles in two groups; up to 64 in two
     // waves and four groups; heads past 128 dimensions hold one group's registers only
     const int rw = ng > 4 || rows > 64 ? 4 : 2, pw = ng > 4 ? 1 : 8 / rw;
-    const int per = many ? 32 * rw : 16 * T;                            // rows of a workgroup
+    const int per = many ? 32 * rw : rows <= 8 ? 8 : rows <= 16 || ng > 6 ? 16 : 32;   // rows of a workgroup
     const int tiles_per = many ? pw : KA_WAVES;                         // tiles it takes side by side
     const size_t blocks = (rows + per - 1) / per, items = n_head_kv * blocks;
     const size_t most = (n_ctx + KVQ_TILE * tiles_per - 1) / (KVQ_TILE * tiles_per);
@@ -889,7 +974,7 @@ extern "C" fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, si
         FOX_HIP(hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
         FOX_HIP(hipLaunchKernel(k, dim3((unsigned)(items * splits)), dim3(64 * rw * pw), args, lds, ctx->stream));
     } else {
-        FOX_HIP(hipLaunchKernel(q4 ? few_kernel<4>(ng, T) : few_kernel<8>(ng, T),
+        FOX_HIP(hipLaunchKernel(q4 ? few_kernel<4>(ng, per) : few_kernel<8>(ng, per),
                                 dim3((unsigned)splits, (unsigned)n_head_kv, (unsigned)blocks),
                                 dim3(64 * KA_WAVES), args, 0, ctx->stream));
     }
