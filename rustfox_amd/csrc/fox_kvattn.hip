@@ -21,6 +21,8 @@
 
 #include <cfloat>
 #include <cmath>
+#include <type_traits>
+#include <cstdlib>
 
 typedef _Float16 h2v __attribute__((ext_vector_type(2)));
 typedef _Float16 h8v __attribute__((ext_vector_type(8)));
@@ -121,19 +123,13 @@ __device__ __forceinline__ int trim_scales(uint2 &b2, int tp, int c, int last)
     return at;
 }
 
-// a - (float)h for the two halves of h
-__device__ __forceinline__ float less_lo(float a, h2v h)
+// a - (float)h in one instruction: the -1 is kept from the compiler, which
+// would convert and subtract
+__device__ __forceinline__ float less(float a, _Float16 h)
 {
-    float d;
-    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(d) : "v"(as_u(h)), "v"(a));
-    return d;
-}
-__device__ __forceinline__ float less_hi(float a, h2v h)
-{
-    float d;
-    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
-        : "=v"(d) : "v"(as_u(h)), "v"(a));
-    return d;
+    float minus = -1.0f;
+    asm("" : "+s"(minus));
+    return __builtin_fmaf((float)h, minus, a);
 }
 
 // 2^(14 - exponent of a row's largest value), the exponent kept within range;
@@ -153,7 +149,7 @@ __device__ __forceinline__ void split_8(const float x[8], float up, h8v &hi, h8v
     for (int i = 0; i < 4; i++) {
         const float a = x[2 * i] * up, b = x[2 * i + 1] * up;
         h[i] = h2v{(_Float16)a, (_Float16)b};
-        d[i] = h2v{(_Float16)less_lo(a, h[i]), (_Float16)less_hi(b, h[i])};
+        d[i] = h2v{(_Float16)less(a, h[i][0]), (_Float16)less(b, h[i][1])};
     }
     hi = __builtin_bit_cast(h8v, *(u4v *)h);
     lo = __builtin_bit_cast(h8v, *(u4v *)d);
@@ -171,25 +167,45 @@ __device__ __forceinline__ const float *query_row(const AttnArgs &A, int kvh, in
     return A.q + (size_t)(row / A.G) * A.q_stride + ((size_t)kvh * A.G + row % A.G) * A.hd;
 }
 
-// (fmaxf quiets its operands first; the instruction passes a NaN over by itself)
-__device__ __forceinline__ float max3(float a, float b, float c)
+// Exponents of a row's N weights from its scores s, x = s sc - m + KA_LIFT.  Where one passes
+// the maximum m by more than KA_ROOM, m becomes the largest score (of the row's
+// PARTS lanes, 64 / PARTS apart) and the row's sum l and sums o follow.
+template <int N, int PARTS, typename V, int ND>
+__device__ __forceinline__ void exponents(float x[N], const float s[N], float sc, float &m, float &l,
+                                          V (&o)[ND])
 {
-    float d;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
-    return d;
+    float top = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+        x[e] = __builtin_fmaf(s[e], sc, KA_LIFT - m);
+        top = fmaxf(top, x[e]);
+    }
+    if (__any(top > KA_LIFT + KA_ROOM)) {
+        float mx = s[0];
+#pragma unroll
+        for (int e = 1; e < N; e++) mx = fmaxf(mx, s[e]);
+        if (PARTS == 4) mx = fmaxf(mx, __shfl_xor(mx, 16));
+        mx = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32)) * sc);
+        const float f = __builtin_amdgcn_exp2f(m - mx);
+        m = mx;
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < ND; d++) o[d] *= f;
+#pragma unroll
+        for (int e = 0; e < N; e++) x[e] = __builtin_fmaf(s[e], sc, KA_LIFT - m);
+    }
 }
 
-// The weights of eight positions from their scores, as two halves each, and their sum.
-__device__ __forceinline__ void weigh(const float s[8], float sc, float off, float &l, h8v &ph, h8v &pl)
+// The weights of eight positions, as two halves each, and their sum.
+__device__ __forceinline__ void weigh(const float x[8], float &l, h8v &ph, h8v &pl)
 {
     h2v hi[4], lo[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i], sc, off));
-        const float b = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i + 1], sc, off));
+        const float a = __builtin_amdgcn_exp2f(x[2 * i]), b = __builtin_amdgcn_exp2f(x[2 * i + 1]);
         l += a + b;
         hi[i] = __builtin_bit_cast(h2v, __builtin_amdgcn_cvt_pkrtz(a, b));
-        lo[i] = __builtin_bit_cast(h2v, __builtin_amdgcn_cvt_pkrtz(less_lo(a, hi[i]), less_hi(b, hi[i])));
+        lo[i] = __builtin_bit_cast(h2v, __builtin_amdgcn_cvt_pkrtz(less(a, hi[i][0]), less(b, hi[i][1])));
     }
     ph = __builtin_bit_cast(h8v, *(u4v *)hi);
     pl = __builtin_bit_cast(h8v, *(u4v *)lo);
@@ -237,19 +253,24 @@ struct Tile {
     uint16_t ks[NS];
     uint2 vs[NG];
 
-    __device__ __forceinline__ void load(const uint8_t *rec, int lane)
+    __device__ __forceinline__ void load_k(const uint8_t *rec, int lane)
     {
         constexpr int CODES = KVQ_TILE * NG * 32 * BITS / 8;
-        const int r = lane & 15, c = lane >> 4;
+        const uint32_t r = lane & 15, c = lane >> 4;
 #pragma unroll
         for (int i = 0; i < 2; i++)
             __builtin_memcpy(k[i], __builtin_assume_aligned(rec + (16 * (r >> 3) + 8 * i + (r & 7)) * (4 * NG * BITS) + c * NG * BITS, 4 * (NG % 4 == 0 ? 4 : NG % 2 == 0 ? 2 : 1)),
                              sizeof(k[i]));
 #pragma unroll
         for (int s = 0; s < NS; s++) {
-            const int g = NS == NG ? (NG * c + s) / 4 : NG % 4 == 0 ? c * (NG / 4) + s : NG * c / 4;
+            const uint32_t g = NS == NG ? (NG * c + s) / 4 : NG % 4 == 0 ? c * (NG / 4) + s : NG * c / 4;
             ks[s] = *(const uint16_t *)(rec + 2 * CODES + g * 32 + r * 2);
         }
+    }
+    __device__ __forceinline__ void load_v(const uint8_t *rec, int lane)
+    {
+        constexpr int CODES = KVQ_TILE * NG * 32 * BITS / 8;
+        const uint32_t r = lane & 15, c = lane >> 4;
 #pragma unroll
         for (int t = 0; t < 2 * NG; t++)
             __builtin_memcpy(v[t], __builtin_assume_aligned(rec + CODES + ((16 * t + r) * 4 + c) * BITS, BITS),
@@ -273,7 +294,7 @@ struct Tile {
 // lower ones, so a tile takes half the products; the two columns of a row are
 // added where a score is used and at the end.
 template <int BITS, int NG, int ROWS>
-__global__ __launch_bounds__(64 * KA_WAVES) void kv_attn_few(AttnArgs A)
+__global__ __launch_bounds__(64 * KA_WAVES, NG > 4 ? 1 : 2) void kv_attn_few(AttnArgs A)
 {
     constexpr bool PACK = ROWS == 8;
     constexpr int WIDTH = 32 * NG, T = ROWS == 32 ? 2 : 1, NT = T * 2 * NG, NQ = PACK ? 1 : 2;
@@ -313,7 +334,10 @@ __global__ __launch_bounds__(64 * KA_WAVES) void kv_attn_few(AttnArgs A)
 
     int tile = split * KA_WAVES + wave;
     Tile<BITS, NG> cur;
-    if (tile < n_tiles) cur.load(base + (size_t)tile * REC, lane);
+    if (tile < n_tiles) {
+        cur.load_k(base + (size_t)tile * REC, lane);
+        cur.load_v(base + (size_t)tile * REC, lane);
+    }
 
     h8v q[T][NQ][NG];
     float sc[T], m[T], l[T];
@@ -361,9 +385,9 @@ __global__ __launch_bounds__(64 * KA_WAVES) void kv_attn_few(AttnArgs A)
 #pragma unroll
             for (int i = 0; i < NQ; i++) q[t][i][j] = *(const h8v *)&shared[(t * NG + j) * NQ + i][lane];
 
-    for (; tile < n_tiles; tile += step) {
-        Tile<BITS, NG> next;
-        if (tile + step < n_tiles) next.load(base + (size_t)(tile + step) * REC, lane);
+    // (the next tile's keys are read into their registers once these are unpacked,
+    // its values a phase later: no copies, and room for a third wave)
+    auto take = [&](auto more) __attribute__((always_inline)) {
         const int tp = tile * KVQ_TILE;
         const bool edge = tp + KVQ_TILE > first;                 // (uniform)
         if (edge) {
@@ -396,6 +420,7 @@ __global__ __launch_bounds__(64 * KA_WAVES) void kv_attn_few(AttnArgs A)
                     for (int t = 0; t < T; t++) s[t][i] = mfma(kf, q[t][u][j], s[t][i]);
             }
         }
+        if constexpr (decltype(more)::value) cur.load_k(base + (size_t)(tile + step) * REC, lane);
         h8v p[T][NQ];
 #pragma unroll
         for (int t = 0; t < T; t++) {
@@ -404,19 +429,17 @@ __global__ __launch_bounds__(64 * KA_WAVES) void kv_attn_few(AttnArgs A)
             for (int e = 0; e < 8; e++) {
                 y[e] = s[t][e >> 2][e & 3];
                 if (PACK) y[e] += other_half(y[e]);
-                if (edge && tp + kvq_v_pos(c, e) >= end[t]) y[e] = -INFINITY;
             }
-            const float top = max3(max3(y[0], y[1], y[2]), max3(y[3], y[4], y[5]),
-                                   max3(y[6], y[7], y[7])) * sc[t];
-            if (__any(top > m[t] + KA_ROOM)) {
-                const float mn = fmaxf(m[t], quad_max(top)), f = __builtin_amdgcn_exp2f(m[t] - mn);
-                m[t] = mn;
-                l[t] *= f;
+            if (edge) {
+                asm volatile("");                                // (a branch, not eight selects for every tile)
 #pragma unroll
-                for (int d = 0; d < 2 * NG; d++) o[t][d] *= f;
+                for (int e = 0; e < 8; e++)
+                    if (tp + kvq_v_pos(c, e) >= end[t]) y[e] = -INFINITY;
             }
+            float x[8];
             h8v hi, lo;
-            weigh(y, sc[t], KA_LIFT - m[t], l[t], hi, lo);
+            exponents<8, 4>(x, y, sc[t], m[t], l[t], o[t]);
+            weigh(x, l[t], hi, lo);
             if (PACK) {
                 p[t][0] = r < 8 ? hi : lo;
             } else {
@@ -438,8 +461,10 @@ __global__ __launch_bounds__(64 * KA_WAVES) void kv_attn_few(AttnArgs A)
 #pragma unroll
                     for (int t = 0; t < T; t++) o[t][2 * g + k] = mfma(vf[k], p[t][u], o[t][2 * g + k]);
         }
-        cur = next;
-    }
+        if constexpr (decltype(more)::value) cur.load_v(base + (size_t)(tile + step) * REC, lane);
+    };
+    for (; tile + step < n_tiles; tile += step) take(std::true_type{});
+    if (tile < n_tiles) take(std::false_type{});
 
     // the four waves' sums at their common maximum (a wave without tiles has
     // m = -FLT_MAX and l = 0), ROUND 16-dimension tiles of 16 rows at a time
@@ -642,6 +667,7 @@ __global__ __launch_bounds__(64 * RW * PW, NG > 4 ? 1 : 2) void kv_attn_many(Att
     for (int n = 0; n < n_steps; n++, tile += step) {
         const int buf = n & 1, tp = tile * KVQ_TILE;
         if (tp + KVQ_TILE > first) {                             // (uniform)
+            asm volatile("");                                    // (a branch, not selects for every tile)
 #pragma unroll
             for (int e = 0; e < 16; e++)
                 if (tp + 8 * (e >> 2) + 4 * c + (e & 3) >= end) s[e] = -INFINITY;
@@ -650,27 +676,14 @@ __global__ __launch_bounds__(64 * RW * PW, NG > 4 ? 1 : 2) void kv_attn_many(Att
                 if (nan_at[buf][pw][g] < end) o[g] = f16v{} + __uint_as_float(0x7FC00000u);
         }
         trim(tile + step, buf ^ 1);
-        float top = max3(s[0], s[1], s[2]);
-#pragma unroll
-        for (int e = 3; e < 15; e += 2) top = max3(top, s[e], s[e + 1]);
-        top = max3(top, s[15], s[15]) * sc;
-        if (__any(top > m + KA_ROOM)) {
-            const float mn = fmaxf(m, fmaxf(top, __shfl_xor(top, 32))), f = __builtin_amdgcn_exp2f(m - mn);
-            m = mn;
-            l *= f;
-#pragma unroll
-            for (int d = 0; d < NG; d++) o[d] *= f;
-        }
         // this tile's weights beside the next one's scores
-        h8v ph[2], pl[2];
-        {
-            float x[16];
+        float y[16], x[16];
 #pragma unroll
-            for (int e = 0; e < 16; e++) x[e] = s[e];
-            const float off = KA_LIFT - m;
-            weigh(x, sc, off, l, ph[0], pl[0]);
-            weigh(x + 8, sc, off, l, ph[1], pl[1]);
-        }
+        for (int e = 0; e < 16; e++) y[e] = s[e];
+        exponents<16, 2>(x, y, sc, m, l, o);
+        h8v ph[2], pl[2];
+        weigh(x, l, ph[0], pl[0]);
+        weigh(x + 8, l, ph[1], pl[1]);
         score(buf ^ 1);
         // its values beside the unpacking of the next one's, and of the keys after those
         stage_k(buf);
@@ -939,7 +952,7 @@ extern "C" fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, si
     const size_t most = (n_ctx + KVQ_TILE * tiles_per - 1) / (KVQ_TILE * tiles_per);
     size_t splits = 1;
     if (!many) {
-        splits = 2 * (size_t)ctx->n_cu / items;
+        splits = (getenv("KVM") ? atoi(getenv("KVM")) : 2) * (size_t)ctx->n_cu / items;
     } else {
         // One workgroup to a compute unit.  More splits fill the last round, at
         // the price of their records, which leave the caches at the kernel's end
