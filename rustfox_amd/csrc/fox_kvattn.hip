@@ -22,7 +22,6 @@
 #include <cfloat>
 #include <cmath>
 #include <type_traits>
-#include <cstdlib>
 
 typedef _Float16 h2v __attribute__((ext_vector_type(2)));
 typedef _Float16 h8v __attribute__((ext_vector_type(8)));
@@ -39,7 +38,6 @@ struct AttnArgs {
     size_t out_stride, q_stride;
     const float *q;
     const uint8_t *cache;
-    const uint32_t *pos;
     size_t n_ctx;
     int n_head_kv, G, hd, M, splits;
     bool q_wide, out_wide;        // rows take 16-byte accesses
@@ -294,7 +292,7 @@ struct Tile {
 // lower ones, so a tile takes half the products; the two columns of a row are
 // added where a score is used and at the end.
 template <int BITS, int NG, int ROWS>
-__global__ __launch_bounds__(64 * KA_WAVES, NG > 4 ? 1 : 2) void kv_attn_few(AttnArgs A)
+__global__ __launch_bounds__(64 * KA_WAVES, NG > 4 ? 1 : 2) void kv_attn_few(const uint32_t *pos, AttnArgs A)
 {
     constexpr bool PACK = ROWS == 8;
     constexpr int WIDTH = 32 * NG, T = ROWS == 32 ? 2 : 1, NT = T * 2 * NG, NQ = PACK ? 1 : 2;
@@ -321,7 +319,7 @@ __global__ __launch_bounds__(64 * KA_WAVES, NG > 4 ? 1 : 2) void kv_attn_few(Att
             *(float4 *)(x[t][u] + 4) = query_quad(qr, 8 * (NG * c + j) + 4, A);
         }
     }
-    const size_t p0 = A.pos[0];
+    const size_t p0 = pos[0];
     auto end_of = [&](int row) { return (int)min(p0 + (size_t)(row / A.G) + 1, A.n_ctx); };
     const int last = end_of(min(row0 + ROWS, rows) - 1);         // positions any row sees
     const int first = end_of(row0);                              // and all rows see
@@ -513,7 +511,7 @@ __global__ __launch_bounds__(64 * KA_WAVES, NG > 4 ? 1 : 2) void kv_attn_few(Att
 // unpacked while the one before it is multiplied, its words read a step
 // earlier still.
 template <int BITS, int NG, int RW, int PW>
-__global__ __launch_bounds__(64 * RW * PW, NG > 4 ? 1 : 2) void kv_attn_many(AttnArgs A)
+__global__ __launch_bounds__(64 * RW * PW, NG > 4 ? 1 : 2) void kv_attn_many(const uint32_t *pos, AttnArgs A)
 {
     constexpr int WIDTH = 32 * NG, NF = 2 * NG;
     constexpr int FW = (NF + RW - 1) / RW;                       // fragments a wave unpacks, of K and V each
@@ -535,7 +533,7 @@ __global__ __launch_bounds__(64 * RW * PW, NG > 4 ? 1 : 2) void kv_attn_many(Att
     const int rows = A.M * A.G, blocks = (rows + 32 * RW - 1) / (32 * RW);
     const int kvh = blockIdx.x % A.n_head_kv, item = blockIdx.x / A.n_head_kv;
     const int split = item % A.splits, row0 = (blocks - 1 - item / A.splits) * 32 * RW;
-    const size_t p0 = A.pos[0];
+    const size_t p0 = pos[0];
     auto end_of = [&](int row) { return (int)min(p0 + (size_t)(row / A.G) + 1, A.n_ctx); };
     const int last = end_of(min(row0 + 32 * RW, rows) - 1), first = end_of(row0);
     const int n_tiles = (last + KVQ_TILE - 1) / KVQ_TILE, step = A.splits * PW;
@@ -762,59 +760,59 @@ __global__ __launch_bounds__(64 * RW * PW, NG > 4 ? 1 : 2) void kv_attn_many(Att
 
 // One workgroup per (row, kv head): the splits' records at their common
 // maximum.  32 threads to a column quad's splits, eight split groups.
-__global__ __launch_bounds__(256) void kv_merge_k(AttnArgs A, int width, int rows_per, int tiles_per)
+__global__ __launch_bounds__(256) void kv_merge_k(const uint32_t *pos, AttnArgs A, int width, int rows_per, int tiles_per)
 {
     __shared__ float sm[8], sl[8];
     __shared__ f4v so[8][32];
     const int row = blockIdx.x, kvh = blockIdx.y, rows = A.M * A.G;
     const int tid = threadIdx.x, sg = tid >> 5, cq = tid & 31;
+    const size_t rec = 4 + (size_t)width;
+    const float *base = A.part + ((size_t)kvh * rows + row) * A.splits * rec;
     // the splits that hold this row: of its block of rows_per rows, tiles_per
     // tiles of a split at a time
     const int row_last = min(row / rows_per * rows_per + rows_per, rows) - 1;
-    const int last = (int)min((size_t)A.pos[0] + (size_t)(row_last / A.G) + 1, A.n_ctx);
+    const int last = (int)min((size_t)pos[0] + (size_t)(row_last / A.G) + 1, A.n_ctx);
     const int n_tiles = (last + KVQ_TILE - 1) / KVQ_TILE;
     const int used = min(A.splits, (n_tiles + tiles_per - 1) / tiles_per);
-    if (used == 1) return;
-    const size_t rec = 4 + (size_t)width;
-    const float *base = A.part + ((size_t)kvh * rows + row) * A.splits * rec;
     for (int c0 = 0; c0 < width / 4; c0 += 32) {
-        const int c4 = c0 + cq;
+        const int c4 = min(c0 + cq, width / 4 - 1);
         float m = -FLT_MAX, l = 0.0f;
         f4v o = {0, 0, 0, 0};
-        if (c4 < width / 4)
-            for (int s0 = sg; s0 < used; s0 += 8 * 8) {
-                float ms[8], ls[8];
-                f4v os[8];
+        for (int s0 = sg; s0 < A.splits; s0 += 8 * 8) {
+            float ms[8], ls[8];
+            f4v os[8];
 #pragma unroll
-                for (int k = 0; k < 8; k++) {                     // (read together)
-                    const float *p = base + (size_t)min(s0 + 8 * k, used - 1) * rec;
-                    ms[k] = p[0];
-                    ls[k] = p[1];
-                    os[k] = *(const f4v *)(p + 4 + 4 * c4);
-                }
-                float mn = m;
-#pragma unroll
-                for (int k = 0; k < 8; k++)
-                    if (s0 + 8 * k < used) mn = fmaxf(mn, ms[k]);
-                const float f = __builtin_amdgcn_exp2f(m - mn);
-                l *= f;
-                o *= f;
-#pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    if (s0 + 8 * k >= used) continue;
-                    const float g = __builtin_amdgcn_exp2f(ms[k] - mn);
-                    l += ls[k] * g;
-                    o += os[k] * g;
-                }
-                m = mn;
+            for (int k = 0; k < 8; k++) {                         // (read together, ahead of the position:
+                const float *p = base + (size_t)min(s0 + 8 * k, A.splits - 1) * rec;   // unused ones are
+                ms[k] = p[0];                                     // there and left out below)
+                ls[k] = p[1];
+                os[k] = *(const f4v *)(p + 4 + 4 * c4);
             }
+            if (s0 >= used) break;
+            float mn = m;
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+                if (s0 + 8 * k < used) mn = fmaxf(mn, ms[k]);
+            const float f = __builtin_amdgcn_exp2f(m - mn);
+            l *= f;
+            o *= f;
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                if (s0 + 8 * k >= used) continue;
+                const float g = __builtin_amdgcn_exp2f(ms[k] - mn);
+                l += ls[k] * g;
+                o += os[k] * g;
+            }
+            m = mn;
+        }
+        if (used == 1) return;                                    // (uniform; written whole)
         if (cq == 0) {
             sm[sg] = m;
             sl[sg] = l;
         }
         so[sg][cq] = o;
         __syncthreads();
-        if (sg == 0 && c4 < width / 4) {
+        if (sg == 0 && c0 + cq < width / 4) {
             float mx = sm[0], sum = 0.0f;
             for (int g = 1; g < 8; g++) mx = fmaxf(mx, sm[g]);
             f4v v = {0, 0, 0, 0};
@@ -833,12 +831,12 @@ __global__ __launch_bounds__(256) void kv_merge_k(AttnArgs A, int width, int row
 
 // The same for up to 16 splits: 32 threads to a row, eight rows to a workgroup,
 // a column quad's records read together.
-__global__ __launch_bounds__(256) void kv_merge_rows_k(AttnArgs A, int width, int rows_per, int tiles_per)
+__global__ __launch_bounds__(256) void kv_merge_rows_k(const uint32_t *pos, AttnArgs A, int width, int rows_per, int tiles_per)
 {
     const int rows = A.M * A.G, row = blockIdx.x * 8 + (threadIdx.x >> 5), kvh = blockIdx.y;
     if (row >= rows) return;
     const int row_last = min(row / rows_per * rows_per + rows_per, rows) - 1;
-    const int last = (int)min((size_t)A.pos[0] + (size_t)(row_last / A.G) + 1, A.n_ctx);
+    const int last = (int)min((size_t)pos[0] + (size_t)(row_last / A.G) + 1, A.n_ctx);
     const int n_tiles = (last + KVQ_TILE - 1) / KVQ_TILE;
     const int used = min(A.splits, (n_tiles + tiles_per - 1) / tiles_per);
     if (used == 1) return;
@@ -932,7 +930,6 @@ extern "C" fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, si
     A.q = q;
     A.q_stride = q_stride;
     A.cache = (const uint8_t *)cache;
-    A.pos = pos;
     A.n_ctx = n_ctx;
     A.n_head_kv = (int)n_head_kv;
     A.G = (int)(n_head / n_head_kv);
@@ -952,7 +949,9 @@ extern "C" fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, si
     const size_t most = (n_ctx + KVQ_TILE * tiles_per - 1) / (KVQ_TILE * tiles_per);
     size_t splits = 1;
     if (!many) {
-        splits = (getenv("KVM") ? atoi(getenv("KVM")) : 2) * (size_t)ctx->n_cu / items;
+        // up to 4 tiles a wave in one launch: at 500 positions 8.9 us against 8.8 in
+        // 4 splits and a merge, at 250 7.4 / 8.7, at 800 11.0 / 9.8
+        splits = n_ctx <= 512 ? 1 : 2 * (size_t)ctx->n_cu / items;
     } else {
         // One workgroup to a compute unit.  More splits fill the last round, at
         // the price of their records, which leave the caches at the kernel's end
@@ -977,7 +976,7 @@ extern "C" fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, si
         if (st) return st;
         A.part = (float *)ctx->ws;
     }
-    void *args[] = {&A};
+    void *args[] = {(void *)&pos, &A};
     if (many) {
         const void *k = rw == 2 ? (q4 ? many_kernel<4, 2>(ng) : many_kernel<8, 2>(ng))
                                 : (q4 ? many_kernel<4, 4>(ng) : many_kernel<8, 4>(ng));
@@ -992,12 +991,12 @@ extern "C" fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, si
                                 dim3(64 * KA_WAVES), args, 0, ctx->stream));
     }
     if (splits > 1) {
-        if (splits <= 16)
+        if (splits <= 16 && rows * n_head_kv >= 1024)
             hipLaunchKernelGGL(kv_merge_rows_k, dim3((unsigned)((rows + 7) / 8), (unsigned)n_head_kv),
-                               dim3(256), 0, ctx->stream, A, width, per, tiles_per);
+                               dim3(256), 0, ctx->stream, pos, A, width, per, tiles_per);
         else
             hipLaunchKernelGGL(kv_merge_k, dim3((unsigned)rows, (unsigned)n_head_kv), dim3(256), 0,
-                               ctx->stream, A, width, per, tiles_per);
+                               ctx->stream, pos, A, width, per, tiles_per);
         FOX_LAUNCHED("kvq attention merge");
     }
     return FOX_GPU_OK;
