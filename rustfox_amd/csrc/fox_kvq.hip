@@ -21,28 +21,32 @@ __device__ __forceinline__ uint32_t quad_u(uint32_t v)
     return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xF, 0xF, true);
 }
 
-// Codes (c + h) of the eight values x of one lane, whose group of 32 is held
-// by its four-lane quad (all four active); returns the scale byte.  Every
-// decision is exact: (h +- 1/2) d and r d are products of few bits, and
-// x - r d, within d / 2 of a border, is a multiple of d 2^-24.
+// Codes (c + h), a byte each, of the eight values x of one lane, whose group of
+// 32 is held by its four-lane quad (all four active); returns the scale byte.
+//
+// x / d is rounded by adding 1.5 2^23 + h, which leaves the code in the float's
+// low byte.  That quotient, from an approximate 1 / d, is off by less than
+// h 2^-21, so only codes that close to a half (and saturating groups, and ones
+// that are not finite) take the exact way: x against the borders (r +- 1/2) d,
+// where r d has few bits and x - r d is a multiple of d 2^-24.
 template <int BITS>
-__device__ __forceinline__ uint32_t quantise_8(const float x[8], uint32_t code[8])
+__device__ __forceinline__ uint32_t quantise_8(const float x[8], uint32_t code[2])
 {
     constexpr int H = 1 << (BITS - 1);
-    float hi = 0.0f, lo = 0.0f;
-    uint32_t top = 0;                                   // largest |x| as bits: NaN above infinity
+    constexpr float MAGIC = 12582912.0f + H, NEAR = 0.5f - H * 0x1p-21f;
+    float hi = fmaxf(x[0], 0.0f), lo = fminf(x[0], 0.0f), sum = x[0];
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
+    for (int i = 1; i < 8; i++) {
         hi = fmaxf(hi, x[i]);
         lo = fminf(lo, x[i]);
-        top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+        sum += x[i];
     }
     hi = fmaxf(hi, quad_f<0xB1>(hi));
     lo = fminf(lo, quad_f<0xB1>(lo));
-    top = max(top, quad_u<0xB1>(top));
+    sum += quad_f<0xB1>(sum);
     hi = fmaxf(hi, quad_f<0x4E>(hi));
     lo = fminf(lo, quad_f<0x4E>(lo));
-    top = max(top, quad_u<0x4E>(top));
+    sum += quad_f<0x4E>(sum);
     // the scale byte: truncated from the needed scale, which rounding may have
     // put one byte low, then raised while it does not cover the group
     const float need = fmaxf(hi * (1.0f / (H - 0.5f)), lo * (-1.0f / (H + 0.5f))) * 4.0f;
@@ -50,43 +54,78 @@ __device__ __forceinline__ uint32_t quantise_8(const float x[8], uint32_t code[8
                             : (int)(__float_as_uint(need) >> 20) - ((127 - 15) << 3);
     b = min(b, KVQ_CAP(BITS));
     float d = kvq_scale((uint32_t)b);
+    bool over = hi > (H - 0.5f) * d || -lo > (H + 0.5f) * d;
 #pragma unroll
-    for (int k = 0; k < 2; k++)
-        if ((hi > (H - 0.5f) * d || -lo > (H + 0.5f) * d) && b < KVQ_CAP(BITS))
-            d = kvq_scale((uint32_t)++b);
-    const float inv = b ? 1.0f / d : 0.0f, half = 0.5f * d;
-    const bool bad = top >= 0x7F800000u;
+    for (int k = 0; k < 2; k++) {
+        b += over && b < KVQ_CAP(BITS);
+        d = kvq_scale((uint32_t)b);
+        over = hi > (H - 0.5f) * d || -lo > (H + 0.5f) * d;
+    }
+    const float inv = b ? __builtin_amdgcn_rcpf(d) : 0.0f;
+    uint32_t c[8];
+    float off = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        float r = rintf(fminf(fmaxf(x[i] * inv, -H - 1.0f), H + 1.0f));
-        const float e = __builtin_fmaf(-r, d, x[i]);
-        const bool odd = ((int)r & 1) != 0;
-        if (e > half || (e == half && odd)) r += 1.0f;
-        else if (e < -half || (e == -half && odd)) r -= 1.0f;
-        const int c = (int)fminf(fmaxf(r, (float)-H), (float)(H - 1));
-        code[i] = bad ? (uint32_t)H : (uint32_t)(c + H);
+        const float y = __builtin_fmaf(x[i], inv, MAGIC);
+        off = fmaxf(off, fabsf(__builtin_fmaf(x[i], inv, MAGIC - y)));
+        c[i] = __float_as_uint(y);
     }
+    const bool odd_sum = !(fabsf(sum) <= 3.4028235e38f);
+    if (off > NEAR || over || odd_sum) {
+        const float half = 0.5f * d;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            float r = rintf(fminf(fmaxf(x[i] * inv, -H - 1.0f), H + 1.0f));
+            const float e = __builtin_fmaf(-r, d, x[i]);
+            const bool odd = ((int)r & 1) != 0;
+            if (e > half || (e == half && odd)) r += 1.0f;
+            else if (e < -half || (e == -half && odd)) r -= 1.0f;
+            c[i] = (uint32_t)((int)fminf(fmaxf(r, (float)-H), (float)(H - 1)) + H);
+        }
+    }
+    bool bad = false;
+    if (odd_sum) {                                      // (the quad has one sum: all of it or none is here)
+        uint32_t top = 0;                               // largest |x| as bits: NaN above infinity
+#pragma unroll
+        for (int i = 0; i < 8; i++) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+        top = max(top, quad_u<0xB1>(top));
+        top = max(top, quad_u<0x4E>(top));
+        bad = top >= 0x7F800000u;
+        if (bad)
+#pragma unroll
+            for (int i = 0; i < 8; i++) c[i] = H;
+    }
+#pragma unroll
+    for (int k = 0; k < 2; k++)
+        code[k] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(c[4 * k + 3], c[4 * k + 2], 0x0C0C0400u),
+                                        __builtin_amdgcn_perm(c[4 * k + 1], c[4 * k], 0x0C0C0400u),
+                                        0x05040100u);
     return bad ? (uint32_t)KVQ_NAN : (uint32_t)b;
 }
 
-// Eight codes as the bytes of a K row or a V chunk.
+// Eight codes in bytes as they are held in a K row.
 template <int BITS>
-__device__ __forceinline__ void put_codes(uint8_t *dst, const uint32_t code[8])
+__device__ __forceinline__ void put_codes(uint8_t *dst, const uint32_t code[2])
 {
     if (BITS == 4) {
-        uint32_t w = 0;
-#pragma unroll
-        for (int e = 0; e < 8; e++) w |= code[e] << (4 * (e / 2 + 4 * (e & 1)));
-        *(uint32_t *)dst = w;
+        // values 0 2 4 6 to the nibbles of the lower half, 1 3 5 7 of the upper
+        const uint32_t even = __builtin_amdgcn_perm(code[1], code[0], 0x06040200u);
+        const uint32_t odd = __builtin_amdgcn_perm(code[1], code[0], 0x07050301u);
+        *(uint32_t *)dst = __builtin_amdgcn_perm(odd | odd >> 4, even | even >> 4, 0x06040200u);
     } else {
-        uint2 w = {0, 0};
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            w.x |= code[e] << (8 * e);
-            w.y |= code[e + 4] << (8 * e);
-        }
-        *(uint2 *)dst = w;
+        *(uint2 *)dst = uint2{code[0], code[1]};
     }
+}
+
+// column k of the 4x4 bytes a, b, c, d for k = 0..3
+__device__ __forceinline__ void transpose_4(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t o[4])
+{
+    const uint32_t p = __builtin_amdgcn_perm(b, a, 0x05010400u), q = __builtin_amdgcn_perm(b, a, 0x07030602u);
+    const uint32_t r = __builtin_amdgcn_perm(d, c, 0x05010400u), s = __builtin_amdgcn_perm(d, c, 0x07030602u);
+    o[0] = __builtin_amdgcn_perm(r, p, 0x05040100u);
+    o[1] = __builtin_amdgcn_perm(r, p, 0x07060302u);
+    o[2] = __builtin_amdgcn_perm(s, q, 0x05040100u);
+    o[3] = __builtin_amdgcn_perm(s, q, 0x07060302u);
 }
 
 // ----------------------------------------------------------------- storing
@@ -285,17 +324,30 @@ __global__ __launch_bounds__(KS_THREADS) void kv_store_k(StoreArgs A)
                                   t0 / KVQ_TILE) * (size_t)L.record;
         const float *row = part ? A.v + tok0 * A.v_stride : A.k + tok0 * A.k_stride;
         const size_t stride = part ? A.v_stride : A.k_stride;
-        // (the words of a tile partly outside the pass are read early)
-        constexpr int NWORD = (HD ? HD : KVQ_MAXHD) * 4 / KS_THREADS + (HD * 4 % KS_THREADS != 0);
-        uint2 old[NWORD];
+        // V words: item (four dims, chunk).  Those of a tile partly outside the
+        // pass are read early, and keep what `on` leaves out
+        constexpr int NWORD = (HD ? HD : KVQ_MAXHD) / KS_THREADS + (HD % KS_THREADS != 0);
+        uint32_t old[NWORD][4][BITS / 4], on[BITS / 4] = {};
         const bool whole = nt == KVQ_TILE;
+        {
+            // (a thread's items have one chunk: KS_THREADS is a multiple of 4)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int r = kvq_v_pos(tid & 3, e);
+                if (r < r0 || r >= r0 + nt) continue;
+                if (BITS == 4) on[0] |= 15u << (4 * (e / 2 + 4 * (e & 1)));
+                else on[(e >> 2) & (BITS / 4 - 1)] |= 255u << (8 * (e & 3));
+            }
+        }
         if (part && !whole) {
 #pragma unroll
             for (int s = 0; s < NWORD; s++) {
                 const int it = tid + s * KS_THREADS;
-                if (it >= L.width * 4) continue;
-                if (BITS == 4) old[s].x = *(const uint32_t *)(rec + L.v + (size_t)it * 4);
-                else old[s] = *(const uint2 *)(rec + L.v + (size_t)it * 8);
+                if (it >= L.width || !(on[0] | on[BITS / 4 - 1])) continue;
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    __builtin_memcpy(old[s][k], __builtin_assume_aligned(
+                        rec + L.v + (size_t)((it & ~3) * 4 + 4 * k + (it & 3)) * BITS, BITS), BITS);
             }
         }
         // (a thread's loads together)
@@ -317,7 +369,7 @@ __global__ __launch_bounds__(KS_THREADS) void kv_store_k(StoreArgs A)
             for (int u = 0; u < IT; u++) {
                 const int it = it0 + u * KS_THREADS, t = it / nw, o = it % nw, r = r0 + t, g = o >> 2;
                 if (it >= nt * nw) break;
-                uint32_t code[8];
+                uint32_t code[2];
                 const uint32_t b = quantise_8<BITS>(x[u], code);
                 if (!part) {
                     put_codes<BITS>(rec + (size_t)r * (L.width * BITS / 8) + o * BITS, code);
@@ -325,33 +377,39 @@ __global__ __launch_bounds__(KS_THREADS) void kv_store_k(StoreArgs A)
                 } else {
                     if ((o & 3) == 0) rec[L.vs + kvq_v_scale(g, r)] = (uint8_t)b;
                     uint32_t *dst = (uint32_t *)(lds + r * LROW + 8 * o);
-#pragma unroll
-                    for (int i = 0; i < 2; i++)
-                        dst[i] = code[4 * i] | code[4 * i + 1] << 8 | code[4 * i + 2] << 16 |
-                                 code[4 * i + 3] << 24;
+                    dst[0] = code[0];
+                    dst[1] = code[1];
                 }
             }
         }
         if (!part) return;
         __syncthreads();
-        // V words: item (dim, chunk) has eight positions
 #pragma unroll
         for (int s = 0; s < NWORD; s++) {
             const int it = tid + s * KS_THREADS;
-            if (it >= L.width * 4) continue;
-            const int dim = it >> 2, c = it & 3;
-            uint32_t code[8];
-            bool any = whole;
+            if (it >= L.width || !(on[0] | on[BITS / 4 - 1])) continue;
+            const int d0 = it & ~3, c = it & 3;
+            uint32_t w[8], o[2][4];
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const int r = kvq_v_pos(c, e);
-                const bool on = whole || (r >= r0 && r < r0 + nt);
-                any |= on;
-                code[e] = on ? lds[r * LROW + dim]
-                        : BITS == 4 ? old[s].x >> (4 * (e / 2 + 4 * (e & 1))) & 15u
-                                    : (e < 4 ? old[s].x >> (8 * e) : old[s].y >> (8 * e - 32)) & 255u;
+                w[e] = *(const uint32_t *)(lds + kvq_v_pos(c, e) * LROW + d0);
+                if (BITS == 4 && !whole) w[e] &= 0x0F0F0F0Fu;    // (rows outside the pass: anything)
             }
-            if (any) put_codes<BITS>(rec + L.v + (size_t)it * BITS, code);
+            if (BITS == 4)
+                transpose_4(w[0] | w[2] << 4, w[4] | w[6] << 4, w[1] | w[3] << 4, w[5] | w[7] << 4, o[0]);
+            else {
+                transpose_4(w[0], w[1], w[2], w[3], o[0]);
+                transpose_4(w[4], w[5], w[6], w[7], o[1]);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                uint32_t v[BITS / 4];
+#pragma unroll
+                for (int i = 0; i < BITS / 4; i++)
+                    v[i] = whole ? o[i][k] : (o[i][k] & on[i]) | (old[s][k][i] & ~on[i]);
+                __builtin_memcpy(__builtin_assume_aligned(rec + L.v + (size_t)((d0 + k) * 4 + c) * BITS, BITS),
+                                 v, BITS);
+            }
         }
     }
 }
