@@ -148,8 +148,9 @@ struct StoreArgs {
 __device__ __forceinline__ void load_8(float x[8], const float *row, int d, int hd, bool wide)
 {
     if (wide) {
-        *(float4 *)x = *(const float4 *)(row + d);
-        *(float4 *)(x + 4) = *(const float4 *)(row + d + 4);
+        const bool in = d < hd;                        // (whole eights)
+        *(float4 *)x = in ? *(const float4 *)(row + d) : float4{0, 0, 0, 0};
+        *(float4 *)(x + 4) = in ? *(const float4 *)(row + d + 4) : float4{0, 0, 0, 0};
         return;
     }
 #pragma unroll
@@ -220,16 +221,17 @@ __device__ __forceinline__ void store_pairs(float *row, const float a[8], const 
 // lane quad.  The V codes of a position share their words with other
 // positions', so a workgroup owns its tile's words: codes pass through LDS, and
 // words that hold positions outside the pass keep those.
-// HD: head_dim where rows take 16-byte loads and head_dim is a stored width, else 0.
+// HD: head_dim where rows take 16-byte loads and head_dim is a stored width, else
+// 0: any head_dim, by 16 bytes where that is a multiple of 16.
 template <int BITS, bool ROPE, int HD>
 __global__ __launch_bounds__(KS_THREADS) void kv_store_k(StoreArgs A)
 {
     constexpr int LROW = (HD ? HD : KVQ_MAXHD) + 4;
-    constexpr bool WIDE = HD != 0;
     __shared__ double ss[ROPE ? 32 * KS_PAIRS : 1];    // sums of squares, [token][item]
     // turned keys [token][dim], or V codes [position in tile][dim]
     __shared__ __attribute__((aligned(16))) uint8_t lds[BITS != 32 ? 32 * LROW * (ROPE ? 4 : 1) : 16];
     const int tid = threadIdx.x, hd = HD ? HD : A.hd;
+    const bool wide = HD || (A.wide && hd % 16 == 0);
     const size_t p_first = A.pos[0], p_end = min(p_first + A.M, A.n_ctx);
     const size_t t0 = (p_first / KVQ_TILE + blockIdx.x) * KVQ_TILE;
     const size_t lo = max(p_first, t0), hi = min(p_end, t0 + KVQ_TILE);
@@ -254,7 +256,7 @@ __global__ __launch_bounds__(KS_THREADS) void kv_store_k(StoreArgs A)
                 if (it >= nt * ni) continue;
                 const int t = it / ni, i = it % ni;
                 load_pairs(a[s], b[s], src + (tok0 + t) * stride + (size_t)h * hd, 8 * i, hd, A.halves,
-                           WIDE);
+                           wide);
                 double x = 0.0;
 #pragma unroll
                 for (int j = 0; j < 8; j++)
@@ -269,9 +271,9 @@ __global__ __launch_bounds__(KS_THREADS) void kv_store_k(StoreArgs A)
                 const int t = it / ni, i = it % ni;
                 float wa[8], wb[8], cs[8], sn[8], ya[8], yb[8];
                 const float *cr = A.cos_t + (lo + t) * half, *sr = A.sin_t + (lo + t) * half;
-                if (w) load_pairs(wa, wb, w, 8 * i, hd, A.halves, WIDE);
-                load_8(cs, cr, 8 * i, half, WIDE);
-                load_8(sn, sr, 8 * i, half, WIDE);
+                if (w) load_pairs(wa, wb, w, 8 * i, hd, A.halves, wide);
+                load_8(cs, cr, 8 * i, half, wide);
+                load_8(sn, sr, 8 * i, half, wide);
                 double inv = 1.0;
                 if (w) {
                     double x = 0.0;
@@ -294,7 +296,7 @@ __global__ __launch_bounds__(KS_THREADS) void kv_store_k(StoreArgs A)
                 if (is_q) dst = A.q_out + (tok0 + t) * A.qo_stride + (size_t)h * hd;
                 else if (BITS == 32) dst = A.k_cache + (lo + t) * kvd + (size_t)h * hd;
                 else dst = (float *)lds + t * LROW;
-                store_pairs(dst, ya, yb, 8 * i, hd, A.halves, WIDE);
+                store_pairs(dst, ya, yb, 8 * i, hd, A.halves, wide);
             }
             if (is_q || BITS == 32) return;
             __syncthreads();
@@ -310,7 +312,7 @@ __global__ __launch_bounds__(KS_THREADS) void kv_store_k(StoreArgs A)
 #pragma unroll
             for (int i = 0; i < 4; i++)
                 if (r + i >= 0 && r + i < nt) x[i] = row[(size_t)(r + i) * A.v_stride + c];
-            if (WIDE && r >= 0 && r + 4 <= nt) {
+            if (wide && r >= 0 && r + 4 <= nt) {
                 *(float4 *)dst = *(const float4 *)x;
             } else {
 #pragma unroll
@@ -362,7 +364,7 @@ __global__ __launch_bounds__(KS_THREADS) void kv_store_k(StoreArgs A)
                     for (int i = 0; i < 8; i++)
                         x[u][i] = HD || d + i < hd ? ((const float *)lds)[t * LROW + d + i] : 0.0f;
                 } else {
-                    load_8(x[u], row + t * stride + (size_t)h * hd, d, hd, WIDE);
+                    load_8(x[u], row + t * stride + (size_t)h * hd, d, hd, wide);
                 }
             }
 #pragma unroll
@@ -444,11 +446,12 @@ template <int BITS, int HD>
 __global__ __launch_bounds__(KS_THREADS) void kv_read_k(const uint8_t *__restrict__ cache,
                                                         size_t n_ctx, int hd_, size_t p0, size_t n,
                                                         float *__restrict__ k, size_t k_stride,
-                                                        float *__restrict__ v, size_t v_stride)
+                                                        float *__restrict__ v, size_t v_stride,
+                                                        bool wide_)
 {
     constexpr int H = 1 << (BITS - 1), HALF_WG = KS_THREADS / 2;
-    constexpr bool WIDE = HD != 0;
     const int hd = HD ? HD : hd_, h = blockIdx.y;
+    const bool wide = HD || (wide_ && hd % 4 == 0);
     const size_t t0 = (p0 / KVQ_TILE + blockIdx.x) * KVQ_TILE;
     const KvqLayout L = kvq_layout(BITS, hd);
     const uint8_t *rec = cache + ((size_t)h * ((n_ctx + KVQ_TILE - 1) / KVQ_TILE) +
@@ -471,7 +474,7 @@ __global__ __launch_bounds__(KS_THREADS) void kv_read_k(const uint8_t *__restric
             float x[4];
 #pragma unroll
             for (int e = 0; e < 4; e++) x[e] = (float)(code_of<BITS>(&w, e) - H) * d;
-            if (r >= lo && r < hi) put_quad(k + (size_t)r * k_stride, x, 4 * q, hd, WIDE);
+            if (r >= lo && r < hi) put_quad(k + (size_t)r * k_stride, x, 4 * q, hd, wide);
         }
     } else {
         if (!v) return;
@@ -491,7 +494,7 @@ __global__ __launch_bounds__(KS_THREADS) void kv_read_k(const uint8_t *__restric
                 float x[4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) x[i] = (float)(code_of<BITS>(w[i], e) - H) * d;
-                if (r >= lo && r < hi) put_quad(v + (size_t)r * v_stride, x, d0, hd, WIDE);
+                if (r >= lo && r < hi) put_quad(v + (size_t)r * v_stride, x, d0, hd, wide);
             }
         }
     }
@@ -593,7 +596,7 @@ extern "C" fox_gpu_status fox_gpu_kvq_read(fox_gpu_ctx *ctx, int kv_type, const 
     if ((uintptr_t)cache % 16)
         return fox_fail(FOX_GPU_ERR_ARG, "kvq_read: the cache must be 16-byte aligned");
     const unsigned tiles = (unsigned)((p0 + n - 1) / KVQ_TILE - p0 / KVQ_TILE + 1);
-    const bool wide = wide_rows(k, n > 1 ? k_stride : 0) && wide_rows(v, n > 1 ? v_stride : 0);
+    bool wide = wide_rows(k, n > 1 ? k_stride : 0) && wide_rows(v, n > 1 ? v_stride : 0);
     int hd = (int)head_dim;
 #define FOX_READ4(hd) ((const void *)kv_read_k<4, hd>)
 #define FOX_READ8(hd) ((const void *)kv_read_k<8, hd>)
@@ -601,7 +604,7 @@ extern "C" fox_gpu_status fox_gpu_kvq_read(fox_gpu_ctx *ctx, int kv_type, const 
                                              : FOX_BY_WIDTH(wide, hd, FOX_READ8);
 #undef FOX_READ4
 #undef FOX_READ8
-    void *args[] = {(void *)&cache, &n_ctx, &hd, &p0, &n, &k, &k_stride, &v, &v_stride};
+    void *args[] = {(void *)&cache, &n_ctx, &hd, &p0, &n, &k, &k_stride, &v, &v_stride, &wide};
     FOX_HIP(hipSetDevice(ctx->device));
     FOX_HIP(hipLaunchKernel(f, dim3(tiles, (unsigned)n_head_kv), dim3(KS_THREADS), args, 0,
                             ctx->stream));
