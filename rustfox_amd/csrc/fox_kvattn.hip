@@ -40,6 +40,7 @@ struct AttnArgs {
     const uint8_t *cache;
     size_t n_ctx;
     int n_head_kv, G, hd, M, splits;
+    float score;                  // log2(e) / sqrt(hd) / 4 (the halves are 4 times the values)
     bool q_wide, out_wide;        // rows take 16-byte accesses
 };
 
@@ -132,10 +133,10 @@ __device__ __forceinline__ float less(float a, _Float16 h)
 
 // 2^(14 - exponent of a row's largest value), the exponent kept within range;
 // back turns a score of the scaled row into powers of two
-__device__ __forceinline__ float query_scale(float top, int hd, float &back)
+__device__ __forceinline__ float query_scale(float top, float score, float &back)
 {
     const int ex = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 113);
-    back = 1.44269504f / sqrtf((float)hd) * 0.25f * __uint_as_float((uint32_t)(127 - 14 + ex) << 23);
+    back = score * __uint_as_float((uint32_t)(127 - 14 + ex) << 23);
     return __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
 }
 
@@ -298,9 +299,9 @@ __global__ __launch_bounds__(64 * KA_WAVES, NG > 4 ? 1 : 2) void kv_attn_few(con
     constexpr int WIDTH = 32 * NG, T = ROWS == 32 ? 2 : 1, NT = T * 2 * NG, NQ = PACK ? 1 : 2;
     constexpr int ROUND = NT < 8 ? NT : 8;                       // tiles of sums merged at a time
     constexpr int JW = (NG + KA_WAVES - 1) / KA_WAVES;           // product steps a wave prepares
-    constexpr int QF = T * NG * NQ, SH = ROUND * KA_WAVES > QF ? ROUND * KA_WAVES : QF;
-    __shared__ f4v shared[SH][64];                               // query operands, then sums
-    __shared__ float sm[KA_WAVES][T][16], sl[KA_WAVES][T][16];
+    __shared__ h8v sq[T * NG * NQ][64];                          // query operands
+    __shared__ f4v so[KA_WAVES][ROUND][PACK ? 32 : 64];
+    __shared__ float tops[KA_WAVES][T][16], sm[KA_WAVES][T][16], sl[KA_WAVES][T][16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, c = lane >> 4;
     const int split = blockIdx.x, kvh = blockIdx.y, row0 = blockIdx.z * ROWS;
@@ -349,13 +350,13 @@ __global__ __launch_bounds__(64 * KA_WAVES, NG > 4 ? 1 : 2) void kv_attn_few(con
 #pragma unroll
             for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[t][u][e]));
         top = quad_max(top);
-        if (c == 0) sm[wave][t][r] = top;
+        if (c == 0) tops[wave][t][r] = top;
     }
     __syncthreads();
 #pragma unroll
     for (int t = 0; t < T; t++) {
-        const float top = fmaxf(fmaxf(sm[0][t][r], sm[1][t][r]), fmaxf(sm[2][t][r], sm[3][t][r]));
-        const float up = query_scale(top, A.hd, sc[t]);
+        const float top = fmaxf(fmaxf(tops[0][t][r], tops[1][t][r]), fmaxf(tops[2][t][r], tops[3][t][r]));
+        const float up = query_scale(top, A.score, sc[t]);
 #pragma unroll
         for (int u = 0; u < JW; u++) {
             const int j = wave + KA_WAVES * u;
@@ -363,10 +364,10 @@ __global__ __launch_bounds__(64 * KA_WAVES, NG > 4 ? 1 : 2) void kv_attn_few(con
             split_8(x[t][u], up, hi, lo);
             if (j >= NG) continue;
             if (PACK) {
-                *(h8v *)&shared[t * NG + j][lane] = r < 8 ? hi : lo;
+                sq[t * NG + j][lane] = r < 8 ? hi : lo;
             } else {
-                *(h8v *)&shared[(t * NG + j) * 2][lane] = hi;
-                *(h8v *)&shared[(t * NG + j) * 2 + 1][lane] = lo;
+                sq[(t * NG + j) * 2][lane] = hi;
+                sq[(t * NG + j) * 2 + 1][lane] = lo;
             }
         }
         end[t] = end_of(min(row0 + 16 * t + rq, rows - 1));
@@ -381,7 +382,7 @@ __global__ __launch_bounds__(64 * KA_WAVES, NG > 4 ? 1 : 2) void kv_attn_few(con
 #pragma unroll
         for (int j = 0; j < NG; j++)
 #pragma unroll
-            for (int i = 0; i < NQ; i++) q[t][i][j] = *(const h8v *)&shared[(t * NG + j) * NQ + i][lane];
+            for (int i = 0; i < NQ; i++) q[t][i][j] = sq[(t * NG + j) * NQ + i][lane];
 
     // (the next tile's keys are read into their registers once these are unpacked,
     // its values a phase later: no copies, and room for a third wave)
@@ -474,30 +475,42 @@ __global__ __launch_bounds__(64 * KA_WAVES, NG > 4 ? 1 : 2) void kv_attn_few(con
             sl[wave][t][r] = l[t];
         }
     }
+    // (PACK: a row's two columns first; its sums are in lanes r < 8)
+    const int sums = PACK ? 8 * c + r : lane;
 #pragma unroll
     for (int k0 = 0; k0 < NT; k0 += ROUND) {
-        __syncthreads();                                         // (the queries, or the last round, are read)
+        if (k0) __syncthreads();                                 // (the last round is read)
 #pragma unroll
-        for (int k = k0; k < k0 + ROUND && k < NT; k++)
-            shared[wave * ROUND + k - k0][lane] = o[k / (2 * NG)][k % (2 * NG)];
+        for (int k = k0; k < k0 + ROUND && k < NT; k++) {
+            f4v v = o[k / (2 * NG)][k % (2 * NG)];
+            if (PACK) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] += other_half(v[e]);
+                if (r < 8) so[wave][k - k0][sums] = v;
+            } else {
+                so[wave][k - k0][sums] = v;
+            }
+        }
         __syncthreads();
+        // item: four sums of a row; in a PACK round's 32 of a tile, half a wave
+        constexpr int PER = PACK ? 32 : 64;
 #pragma unroll
-        for (int u = 0; u < (ROUND + KA_WAVES - 1) / KA_WAVES; u++) {
-            const int k = k0 + wave + KA_WAVES * u, t = k / (2 * NG), row = row0 + 16 * t + r;
-            if (k >= NT || k >= k0 + ROUND || row >= rows || (PACK && r >= 8)) continue;
-            float mx = sm[0][t][r], sum = 0.0f;
+        for (int it = 0; it < (ROUND * PER + 64 * KA_WAVES - 1) / (64 * KA_WAVES); it++) {
+            const int at = threadIdx.x + it * 64 * KA_WAVES, k = k0 + at / PER, i = at % PER;
+            const int rr = PACK ? i & 7 : i & 15, cc = PACK ? i >> 3 : i >> 4;
+            const int t = T == 1 ? 0 : k / (2 * NG), row = row0 + 16 * t + rr;
+            if (k >= NT || k >= k0 + ROUND || row >= rows) continue;
+            float mx = sm[0][t][rr], sum = 0.0f;
 #pragma unroll
-            for (int w = 1; w < KA_WAVES; w++) mx = fmaxf(mx, sm[w][t][r]);
+            for (int w = 1; w < KA_WAVES; w++) mx = fmaxf(mx, sm[w][t][rr]);
             f4v v = {0, 0, 0, 0};
 #pragma unroll
             for (int w = 0; w < KA_WAVES; w++) {
-                const float f = __builtin_amdgcn_exp2f(sm[w][t][r] - mx);
-                sum += sl[w][t][r] * f;
-                f4v part = shared[w * ROUND + k - k0][lane];
-                if (PACK) part += shared[w * ROUND + k - k0][lane + 8];
-                v += part * f;
+                const float f = __builtin_amdgcn_exp2f(sm[w][t][rr] - mx);
+                sum += sl[w][t][rr] * f;
+                v += so[w][k - k0][i] * f;
             }
-            put_sums(A, kvh, row, 16 * (k % (2 * NG)) + 4 * c, v, mx, sum, used == 1, split, WIDTH);
+            put_sums(A, kvh, row, 16 * (k % (2 * NG)) + 4 * cc, v, mx, sum, used == 1, split, WIDTH);
         }
     }
 }
@@ -632,7 +645,7 @@ __global__ __launch_bounds__(64 * RW * PW, NG > 4 ? 1 : 2) void kv_attn_many(con
         for (int j = 0; j < NF; j++)
 #pragma unroll
             for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[j][e]));
-        const float up = query_scale(fmaxf(top, __shfl_xor(top, 32)), A.hd, sc);
+        const float up = query_scale(fmaxf(top, __shfl_xor(top, 32)), A.score, sc);
 #pragma unroll
         for (int j = 0; j < NF; j++) split_8(x[j], up, qh[j], ql[j]);
     }
@@ -934,6 +947,7 @@ extern "C" fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, si
     A.n_head_kv = (int)n_head_kv;
     A.G = (int)(n_head / n_head_kv);
     A.hd = (int)head_dim;
+    A.score = (float)(1.4426950408889634 / std::sqrt((double)head_dim) / 4);
     A.M = (int)M;
     A.q_wide = head_dim % 4 == 0 && (uintptr_t)q % 16 == 0 && (M == 1 || q_stride % 4 == 0);
     A.out_wide = head_dim % 4 == 0 && (uintptr_t)out % 16 == 0 && (M == 1 || out_stride % 4 == 0);
