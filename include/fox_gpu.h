@@ -415,13 +415,13 @@ enum { FOX_GPU_KV_Q4 = 4, FOX_GPU_KV_Q8 = 8 };
 /* bytes of a layer's cache; 0 for a shape that is not taken */
 size_t fox_gpu_kvq_bytes(int kv_type, size_t n_ctx, size_t n_head_kv, size_t head_dim);
 
-/* M <= n_ctx rows of n_head_kv * head_dim floats into positions pos[0] + i.
- * Other positions keep what they hold. */
+/* M <= n_ctx rows (at most 2^28) of n_head_kv * head_dim floats into positions
+ * pos[0] + i.  Other positions keep what they hold. */
 fox_gpu_status fox_gpu_kvq_write(fox_gpu_ctx *ctx, int kv_type, void *cache, size_t n_ctx,
                                  size_t n_head_kv, size_t head_dim, const uint32_t *pos, size_t M,
                                  const float *k, size_t k_stride, const float *v, size_t v_stride);
 
-/* Rows p0 .. p0+n-1 as floats; k or v may be NULL. */
+/* Rows p0 .. p0+n-1 (at most 2^28) as floats; k or v may be NULL. */
 fox_gpu_status fox_gpu_kvq_read(fox_gpu_ctx *ctx, int kv_type, const void *cache, size_t n_ctx,
                                 size_t n_head_kv, size_t head_dim, size_t p0, size_t n,
                                 float *k, size_t k_stride, float *v, size_t v_stride);

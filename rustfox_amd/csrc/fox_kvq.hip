@@ -7,6 +7,7 @@
 typedef float f4v __attribute__((ext_vector_type(4)));
 
 #define KS_THREADS 256
+#define KVQ_MAXROWS (1u << 28)       // rows of one call (2^32 threads are a launch's most)
 
 // ------------------------------------------------------------- quantising
 
@@ -559,7 +560,9 @@ extern "C" fox_gpu_status fox_gpu_kvq_write(fox_gpu_ctx *ctx, int kv_type, void 
         return fox_fail(FOX_GPU_ERR_ARG, "kvq_write: bad argument");
     fox_gpu_status st = fox_kvq_shape("kvq_write", kv_type, n_ctx, n_head_kv, head_dim);
     if (st) return st;
-    if (M > n_ctx) return fox_fail(FOX_GPU_ERR_ARG, "kvq_write: %zu rows of %zu", M, n_ctx);
+    if (M > n_ctx || M > KVQ_MAXROWS)
+        return fox_fail(FOX_GPU_ERR_ARG, "kvq_write: %zu rows of %zu, at most %u a call", M, n_ctx,
+                        KVQ_MAXROWS);
     if (M > 1 && (k_stride < n_head_kv * head_dim || v_stride < n_head_kv * head_dim))
         return fox_fail(FOX_GPU_ERR_ARG, "kvq_write: a stride below the row's width");
     if ((uintptr_t)cache % 16)
@@ -591,6 +594,8 @@ extern "C" fox_gpu_status fox_gpu_kvq_read(fox_gpu_ctx *ctx, int kv_type, const 
     if (p0 >= n_ctx || n > n_ctx - p0)
         return fox_fail(FOX_GPU_ERR_ARG, "kvq_read: %zu rows from %zu on are outside the %zu-row "
                         "cache", n, p0, n_ctx);
+    if (n > KVQ_MAXROWS)
+        return fox_fail(FOX_GPU_ERR_ARG, "kvq_read: %zu rows, at most %u a call", n, KVQ_MAXROWS);
     if (n > 1 && ((k && k_stride < n_head_kv * head_dim) || (v && v_stride < n_head_kv * head_dim)))
         return fox_fail(FOX_GPU_ERR_ARG, "kvq_read: a stride below the row's width");
     if ((uintptr_t)cache % 16)
@@ -627,7 +632,9 @@ static fox_gpu_status rope_args(const char *what, fox_gpu_ctx *ctx, const float 
     if (pairs != FOX_GPU_PAIRS_ADJACENT && pairs != FOX_GPU_PAIRS_HALVES)
         return fox_fail(FOX_GPU_ERR_ARG, "%s: unknown pairing %d", what, pairs);
     if (M > FOX_GPU_BATCH_TOKENS) return fox_fail(FOX_GPU_ERR_ARG, "%s: too many tokens", what);
-    if (n_head > 32767) return fox_fail(FOX_GPU_ERR_ARG, "%s: too many heads", what);
+    if (n_head + 2 * n_head_kv > 65535)                      // (rows of the grid)
+        return fox_fail(FOX_GPU_ERR_ARG, "%s: %zu heads beside %zu kv heads are too many", what, n_head,
+                        n_head_kv);
     if (M > 1 && (q_stride < nq || qo_stride < nq || k_stride < nkv || v_stride < nkv))
         return fox_fail(FOX_GPU_ERR_ARG, "%s: a stride below the row's width", what);
     *A = {};

@@ -69,10 +69,11 @@ def test_rows_come_back_as_held(gpu, bits, n_kv, hd):
     n_ctx, w = 101, n_kv * hd
     c = poisoned(gpu, bits, n_ctx, n_kv, hd)
     want_k, want_v = (np.full((n_ctx, w), np.nan, np.float32) for _ in range(2))
-    for p, n in [(37, 1), (38, 2), (40, 33), (0, 5), (4, 30), (95, 6), (70, 1), (39, 1)]:
+    for p, n in [(37, 1), (38, 2), (40, 33), (0, 5), (4, 30), (95, 6), (70, 1), (39, 1), (33, 64)]:
         K, V = rows(rng, n, w), rows(rng, n, w)
-        gpu.kvq_write(bits, c, n_ctx, n_kv, hd, u32(gpu, p), n, padded(gpu, K, w + 3),
-                      padded(gpu, V, w + 4), w + 3, w + 4)
+        ks, vs = (w + 3, w + 4) if n % 2 else (w + 4 - w % 4, w + 8 - w % 4)
+        gpu.kvq_write(bits, c, n_ctx, n_kv, hd, u32(gpu, p), n, padded(gpu, K, ks),
+                      padded(gpu, V, vs), ks, vs)
         want_k[p:p + n], want_v[p:p + n] = kr.held(K, bits, hd), kr.held(V, bits, hd)
         for p0, m in [(0, n_ctx), (p, n), (max(p - 1, 0), 2)]:
             k, v = read(gpu, bits, c, n_ctx, n_kv, hd, p0, m)
@@ -179,13 +180,15 @@ def test_norm_rope_store(gpu, bits, case, halves):
     qn, kn = ((1 + 0.2 * rng.standard_normal(hd)).astype(np.float32) for _ in range(2))
     cos, sin = kr.tables(n_ctx, hd)
     m = max(0, min(M, n_ctx - pos))
-    for wq, wk, place in [(qn, kn, False), (None, kn, True), (qn, None, False), (None, None, True)]:
-        dq, dk, dv = padded(gpu, q, nq + 4), padded(gpu, k, nk + 8), padded(gpu, v, nk + 1)
+    # rows 16 bytes apart (wide accesses where head_dim allows them), then a float off that
+    for wq, wk, place, off in [(qn, kn, False, 0), (None, kn, True, 0), (qn, None, False, 1),
+                               (None, None, True, 1), (qn, kn, True, 0)]:
+        dq, dk, dv = padded(gpu, q, nq + 4), padded(gpu, k, nk + 8), padded(gpu, v, nk + 4 + off)
         dqn, dkn = (gpu.array(x) if x is not None else None for x in (wq, wk))
         do = dq if place else gpu.array(np.full((M, nq + 4), 7.5, np.float32))
         dc, ds = gpu.array(cos), gpu.array(sin)
         args = (dq, dk, dv, do, n_head, n_kv, hd, M, dqn, dkn, EPS, halves, dc, ds, u32(gpu, pos))
-        st = (nq + 4, nq + 4, nk + 8, nk + 1)
+        st = (nq + 4, nq + 4, nk + 8, nk + 4 + off)
         if bits == 32:
             kc = gpu.array(np.full((n_ctx, nk), 9.0, np.float32))
             vc = gpu.array(np.full(((n_ctx + 3) // 4, nk, 4), 9.0, np.float32))
@@ -259,6 +262,10 @@ ATTN_CASES = [  # n_head, n_kv, hd, n_ctx, pos, M
     (8, 2, 128, 513, 1, 511), (2, 1, 32, 1100, 70, 1000),
     (16, 4, 64, 2100, 2000, 1), (32, 8, 128, 5000, 4900, 1),                   # many splits
     (32, 16, 128, 4200, 4100, 8), (8, 2, 128, 6000, 5900, 33),
+    (32, 8, 128, 5000, 10, 1), (32, 8, 128, 5000, 100, 2), (8, 2, 128, 6000, 3, 33),   # short in a long cache
+    (32, 2, 128, 3000, 2900, 2), (64, 2, 64, 3000, 2950, 1), (24, 2, 192, 2000, 1990, 2),  # 32 rows, several tiles a wave
+    (8, 1, 128, 40000, 39990, 1), (16, 1, 96, 40000, 39990, 1), (20, 1, 64, 20000, 19990, 3),
+    (8, 4, 256, 1500, 1400, 20), (16, 2, 128, 1500, 1450, 8), (64, 16, 128, 300, 30, 256),
     (4, 2, 64, 50, 47, 6),                    # tokens past the context see all of it
     (4, 2, 64, 50, 60, 2),
 ]
@@ -433,6 +440,71 @@ def test_a_prompt_and_steps(gpu, bits):
         gpu.kvq_attention(other, dq, bits, c, n_head, n_kv, hd, 1, pos, n_ctx)
         assert np.array_equal(other.numpy(), got)
     gpu.lib.fox_gpu_graph_free(g)
+
+
+def test_a_captured_prompt_pass(gpu):
+    """A pass of many tokens whose records fill the workspace, captured beside a single token's and
+    replayed in turn, each against the eager call."""
+    n_head, n_kv, hd, n_ctx = 8, 1, 128, 4000
+    rng = np.random.default_rng(12)
+    K, V = rows(rng, n_ctx, hd), rows(rng, n_ctx, hd)
+    c = fill(gpu, 4, n_ctx, n_kv, hd, K, V)
+    jobs = []
+    for M, pos in ((20, 3900), (1, 3950)):
+        dq = gpu.array(rng.standard_normal((M, n_head * hd)).astype(np.float32))
+        out, dpos = gpu.empty((M, n_head * hd), np.float32), u32(gpu, pos)
+        call = lambda M=M, dq=dq, out=out, dpos=dpos: gpu.kvq_attention(  # noqa: E731
+            out, dq, 4, c, n_head, n_kv, hd, M, dpos, n_ctx)
+        call()
+        want = out.numpy()
+        check(want, dq.numpy(), kr.held(K, 4, hd), kr.held(V, 4, hd), n_head, n_kv, hd, pos, n_ctx)
+        g = C.c_void_p()
+        assert gpu.lib.fox_gpu_graph_begin(gpu.ctx) == 0
+        call()
+        assert gpu.lib.fox_gpu_graph_end(gpu.ctx, C.byref(g)) == 0
+        jobs.append((g, out, want, call))
+    for turn in range(4):
+        for g, out, want, call in jobs:
+            out.fill(0xFF)
+            assert gpu.lib.fox_gpu_graph_launch(gpu.ctx, g) == 0
+            assert np.array_equal(out.numpy(), want)
+            call()
+            assert np.array_equal(out.numpy(), want)
+    for g, *_ in jobs:
+        gpu.lib.fox_gpu_graph_free(g)
+
+
+def test_a_cache_past_four_gigabytes(gpu):
+    """Offsets that need more than 32 bits: rows at both ends of a zeroed cache, whose other keys
+    score 0 and whose other values add nothing."""
+    n_head, n_kv, hd, n_ctx, bits = 2, 1, 256, 9_000_000, 8
+    size = gpu.kvq_bytes(bits, n_ctx, n_kv, hd)
+    assert size > 1 << 32
+    rng = np.random.default_rng(8)
+    c = gpu.empty(size, np.uint8).fill(0)
+    n = 40
+    K, V = (rng.standard_normal((2 * n, hd)).astype(np.float32) for _ in range(2))
+    for i, p in ((0, 0), (n, n_ctx - n)):
+        gpu.kvq_write(bits, c, n_ctx, n_kv, hd, u32(gpu, p), n, gpu.array(K[i:i + n]), gpu.array(V[i:i + n]))
+        k, v = read(gpu, bits, c, n_ctx, n_kv, hd, p, n)
+        assert same(k, kr.held(K[i:i + n], bits, hd)) and same(v, kr.held(V[i:i + n], bits, hd))
+    Kh, Vh = np.float64(kr.held(K, bits, hd)), np.float64(kr.held(V, bits, hd))
+    for M in (1, 20):
+        q = (6 * rng.standard_normal((M, n_head * hd))).astype(np.float32)
+        got = attend(gpu, bits, c, q, n_head, n_kv, hd, n_ctx, n_ctx - M)
+        for t in range(M):
+            for h in range(n_head):
+                m = 2 * n - (M - 1 - t)
+                s = Kh[:m] @ np.float64(q[t, h * hd:(h + 1) * hd]) / np.sqrt(hd)
+                e = np.exp(s)
+                want, mag = e @ Vh[:m], e @ np.abs(Vh[:m])
+                total = e.sum() + n_ctx - M + 1 + t - m
+                # 9e6 weights: each of the 512 .. 16384 running sums of a row adds at most 2^15 of them, a
+                # half step each time; the scores' own error as in attention_bound
+                top = (np.abs(Kh[:m]) @ np.abs(q[t, h * hd:(h + 1) * hd])).max() / np.sqrt(hd)
+                rel = 2 * top * (hd + 16) * 2.0 ** -23 + 2 * 2.0 ** 15 * 2.0 ** -24 + 2.0 ** -20
+                off = np.abs(got[t, h * hd:(h + 1) * hd] - want / total)
+                assert np.all(off <= rel * mag / total + np.abs(Vh[:m]).sum(0) * 2.0 ** -31), (M, t, h)
 
 
 def test_two_contexts_at_once(gpu):

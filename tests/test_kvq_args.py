@@ -48,11 +48,13 @@ CALLS = {
     "write": ("fox_gpu_kvq_write", WRITE, SHAPE + [
         (dict(ctx=None), ARG), (dict(cache=None), ARG), (dict(pos=None), ARG), (dict(k=None), ARG),
         (dict(v=None), ARG), (dict(M=0), ARG), (dict(M=101), ARG), (dict(ks=127), ARG),
-        (dict(vs=127), ARG), (dict(cache=P + 8), ARG), (dict(nkv=32768, ks=1 << 22, vs=1 << 22), ARG)]),
+        (dict(vs=127), ARG), (dict(cache=P + 8), ARG), (dict(nkv=32768, ks=1 << 22, vs=1 << 22), ARG),
+        (dict(n_ctx=1 << 30, M=(1 << 28) + 1), ARG)]),
     "read": ("fox_gpu_kvq_read", READ, SHAPE + [
         (dict(ctx=None), ARG), (dict(cache=None), ARG), (dict(k=None, v=None), ARG), (dict(n=0), ARG),
         (dict(p0=98), ARG), (dict(p0=100), ARG), (dict(n=101), ARG), (dict(n=2 ** 64 - 1), ARG),
-        (dict(ks=127), ARG), (dict(vs=127), ARG), (dict(cache=P + 4), ARG)]),
+        (dict(ks=127), ARG), (dict(vs=127), ARG), (dict(cache=P + 4), ARG),
+        (dict(n_ctx=1 << 30, n=(1 << 28) + 1), ARG)]),
     "rope": ("fox_gpu_norm_rope_store", ROPE_F, [s for s in SHAPE if "kv" not in s[0]] + [
         (dict(ctx=None), ARG), (dict(q=None), ARG), (dict(o=None), ARG), (dict(k=None), ARG),
         (dict(v=None), ARG), (dict(cos=None), ARG), (dict(sin=None), ARG), (dict(pos=None), ARG),
@@ -62,6 +64,7 @@ CALLS = {
     "kvq_rope": ("fox_gpu_kvq_norm_rope_store", ROPE_Q, SHAPE + [
         (dict(ctx=None), ARG), (dict(q=None), ARG), (dict(cache=None), ARG), (dict(cache=P + 8), ARG),
         (dict(nh=0), ARG), (dict(M=0), ARG), (dict(M=1025), ARG), (dict(pairs=-1), ARG),
+        (dict(nh=65533, qs=1 << 24, os=1 << 24), ARG),
         (dict(ks=127), ARG)]),
     "attention": ("fox_gpu_kvq_attention", ATTN, SHAPE + [
         (dict(ctx=None), ARG), (dict(o=None), ARG), (dict(q=None), ARG), (dict(cache=None), ARG),
