@@ -40,9 +40,17 @@ struct AttnArgs {
     const uint8_t *cache;
     size_t n_ctx;
     int n_head_kv, G, hd, M, splits;
+    uint32_t by_g, g_shift;       // row / G: see token_of
     float score;                  // log2(e) / sqrt(hd) / 4 (the halves are 4 times the values)
     bool q_wide, out_wide;        // rows take 16-byte accesses
 };
+
+// row / G without a division (some thirty instructions, each met cold in a short
+// call): by_g = 2^(30 + g_shift) / G rounded up, 2^g_shift >= G, which is exact for row < 2^30
+__device__ __forceinline__ int token_of(const AttnArgs &A, int row)
+{
+    return (int)(__umulhi((uint32_t)row << 2, A.by_g) >> A.g_shift);
+}
 
 __device__ __forceinline__ h2v as_h2(uint32_t v) { return __builtin_bit_cast(h2v, v); }
 __device__ __forceinline__ uint32_t as_u(h2v v) { return __builtin_bit_cast(uint32_t, v); }
@@ -163,7 +171,13 @@ __device__ __forceinline__ float4 query_quad(const float *row, int d, const Attn
 }
 __device__ __forceinline__ const float *query_row(const AttnArgs &A, int kvh, int row)
 {
-    return A.q + (size_t)(row / A.G) * A.q_stride + ((size_t)kvh * A.G + row % A.G) * A.hd;
+    const int tok = token_of(A, row);
+    return A.q + (size_t)tok * A.q_stride + (uint32_t)((kvh * A.G + row - tok * A.G) * A.hd);
+}
+__device__ __forceinline__ float *out_row(const AttnArgs &A, int kvh, int row)
+{
+    const int tok = token_of(A, row);
+    return A.out + (size_t)tok * A.out_stride + (uint32_t)((kvh * A.G + row - tok * A.G) * A.hd);
 }
 
 // Exponents of a row's N weights from its scores s, x = s sc - m + KA_LIFT.  Where one passes
@@ -230,7 +244,7 @@ __device__ __forceinline__ void put_sums(const AttnArgs &A, int kvh, int row, in
                                          float l, bool whole, int split, int width)
 {
     if (whole) {
-        float *dst = A.out + (size_t)(row / A.G) * A.out_stride + ((size_t)kvh * A.G + row % A.G) * A.hd;
+        float *dst = out_row(A, kvh, row);
 #pragma unroll
         for (int e = 0; e < 4; e++)
             if (dim + e < A.hd) dst[dim + e] = v[e] * 0.25f / l;
@@ -321,7 +335,7 @@ __global__ __launch_bounds__(64 * KA_WAVES, NG > 4 ? 1 : 2) void kv_attn_few(con
         }
     }
     const size_t p0 = pos[0];
-    auto end_of = [&](int row) { return (int)min(p0 + (size_t)(row / A.G) + 1, A.n_ctx); };
+    auto end_of = [&](int row) { return (int)min(p0 + (size_t)token_of(A, row) + 1, A.n_ctx); };
     const int last = end_of(min(row0 + ROWS, rows) - 1);         // positions any row sees
     const int first = end_of(row0);                              // and all rows see
     const int n_tiles = (last + KVQ_TILE - 1) / KVQ_TILE, step = A.splits * KA_WAVES;
@@ -530,7 +544,7 @@ __global__ __launch_bounds__(64 * RW * PW, NG > 4 ? 1 : 2) void kv_attn_many(con
     constexpr int FW = (NF + RW - 1) / RW;                       // fragments a wave unpacks, of K and V each
     constexpr int CODES = KVQ_TILE * WIDTH * BITS / 8, REC = 2 * (CODES + KVQ_TILE * NG);
     static_assert(2 * PW * 2 * NF * 1024 + 4096 <= 160 * 1024 &&
-                  32 * RW * (PW > 2 ? PW - 1 : 1) * (WIDTH + 4) * 4 + 4096 <= 160 * 1024, "LDS");
+                  32 * RW * PW * (WIDTH + 4) * 4 + 4096 <= 160 * 1024, "LDS");
     // [buffer][group][K fragments, V fragments][lane]: a fragment is an MFMA
     // operand; f of K holds 8 dimensions of each half of the 32 positions' rows, from
     // 8 f and from WIDTH / 2 + 8 f on; f of V dimensions 32 (f / 2) + 0..31 of
@@ -547,7 +561,7 @@ __global__ __launch_bounds__(64 * RW * PW, NG > 4 ? 1 : 2) void kv_attn_many(con
     const int kvh = blockIdx.x % A.n_head_kv, item = blockIdx.x / A.n_head_kv;
     const int split = item % A.splits, row0 = (blocks - 1 - item / A.splits) * 32 * RW;
     const size_t p0 = pos[0];
-    auto end_of = [&](int row) { return (int)min(p0 + (size_t)(row / A.G) + 1, A.n_ctx); };
+    auto end_of = [&](int row) { return (int)min(p0 + (size_t)token_of(A, row) + 1, A.n_ctx); };
     const int last = end_of(min(row0 + 32 * RW, rows) - 1), first = end_of(row0);
     const int n_tiles = (last + KVQ_TILE - 1) / KVQ_TILE, step = A.splits * PW;
     if (split * PW >= n_tiles) return;                           // (uniform)
@@ -627,9 +641,20 @@ __global__ __launch_bounds__(64 * RW * PW, NG > 4 ? 1 : 2) void kv_attn_many(con
     // queries, through LDS: a row's pieces side by side from memory (a lane a
     // row touches 64 lines with every load)
     float *rowbuf = (float *)frag;
-    for (int it = threadIdx.x; it < 32 * RW * WIDTH / 4; it += 64 * RW * PW) {
-        const int rr = it / (WIDTH / 4), d = it % (WIDTH / 4) * 4;
-        *(float4 *)(rowbuf + rr * ROW + d) = query_quad(query_row(A, kvh, min(row0 + rr, rows - 1)), d, A);
+    constexpr int QUADS = WIDTH / 4, AT_ONCE = 64 * RW * PW / QUADS;   // rows that the threads cover at once
+    const int rr0 = threadIdx.x / QUADS, d0 = threadIdx.x % QUADS * 4;
+    if (rr0 < AT_ONCE) {
+        if (A.q_wide) {
+#pragma unroll 8
+            for (int rr = rr0; rr < 32 * RW; rr += AT_ONCE)
+                *(f4v *)(rowbuf + rr * ROW + d0) =
+                    d0 < A.hd ? *(const f4v *)(query_row(A, kvh, min(row0 + rr, rows - 1)) + d0) : f4v{0, 0, 0, 0};
+        } else {
+#pragma unroll 1
+            for (int rr = rr0; rr < 32 * RW; rr += AT_ONCE)
+                *(float4 *)(rowbuf + rr * ROW + d0) =
+                    query_quad(query_row(A, kvh, min(row0 + rr, rows - 1)), d0, A);
+        }
     }
     __syncthreads();
     h8v qh[NF], ql[NF];
@@ -713,59 +738,54 @@ __global__ __launch_bounds__(64 * RW * PW, NG > 4 ? 1 : 2) void kv_attn_many(con
         __syncthreads();
     }
 
-    // the groups' sums at their common maximum, group 0's waves adding them
-    // up; a wave's rows in LDS, then whole to memory
+    // the groups' sums through LDS, added at their common maximum; rows whole to
+    // memory, every thread a column quad of some (in loops: code that a workgroup
+    // runs once costs its way to the instruction cache, 0.2 us a 128 bytes)
     l += __shfl_xor(l, 32);
     if (c == 0) {
         sm[pw][rw][r] = m;
         sl[pw][rw][r] = l;
     }
-    float *mine = rowbuf + 32 * rw * ROW + r * ROW + 4 * c;      // (group 1's sums, then the result)
-    auto quad = [&](int k) { return f4v{o[k >> 2][4 * (k & 3)], o[k >> 2][4 * (k & 3) + 1],
-                                        o[k >> 2][4 * (k & 3) + 2], o[k >> 2][4 * (k & 3) + 3]}; };
-    if (pw) {
+    float *mine = rowbuf + ((pw * RW + rw) * 32 + r) * ROW + 4 * c;
 #pragma unroll
-        for (int k = 0; k < 4 * NG; k++) *(f4v *)(mine + (pw - 1) * 32 * RW * ROW + 8 * k) = quad(k);
-    }
+    for (int k = 0; k < 4 * NG; k++)
+        *(f4v *)(mine + 8 * k) = f4v{o[k >> 2][4 * (k & 3)], o[k >> 2][4 * (k & 3) + 1],
+                                     o[k >> 2][4 * (k & 3) + 2], o[k >> 2][4 * (k & 3) + 3]};
     __syncthreads();
-    if (pw) return;
-    float mx = m, sum = 0.0f, f[PW];
+    int thread = threadIdx.x;
+    asm("" : "+v"(thread));                                      // (found again, not kept through the loop)
+    const int d1 = thread % QUADS * 4;
+    if (thread / QUADS >= AT_ONCE) return;
+#pragma unroll 2
+    for (int rr = thread / QUADS; rr < 32 * RW; rr += AT_ONCE) {
+        const int at = row0 + rr;
+        if (at >= rows) break;
+        float mx = sm[0][0][rr], sum = 0.0f;
 #pragma unroll
-    for (int w = 1; w < PW; w++) mx = fmaxf(mx, sm[w][rw][r]);
+        for (int w = 1; w < PW; w++) mx = fmaxf(mx, sm[w][0][rr]);
+        f4v v = {0, 0, 0, 0};
 #pragma unroll
-    for (int w = 0; w < PW; w++) {
-        f[w] = __builtin_amdgcn_exp2f(sm[w][rw][r] - mx);
-        sum += sl[w][rw][r] * f[w];
-    }
-    const float by = used == 1 ? 0.25f / sum : 1.0f;
-#pragma unroll
-    for (int k = 0; k < 4 * NG; k++) {
-        f4v v = quad(k) * f[0];
-#pragma unroll
-        for (int w = 1; w < PW; w++) v += *(const f4v *)(mine + (w - 1) * 32 * RW * ROW + 8 * k) * f[w];
-        *(f4v *)(mine + 8 * k) = v * by;
-    }
-    if (used > 1 && c == 0 && row < rows) {
-        float *dst = A.part + (((size_t)kvh * rows + row) * A.splits + split) * (4 + WIDTH);
-        dst[0] = mx;
-        dst[1] = sum;
-    }
-    __builtin_amdgcn_wave_barrier();
-    // (this wave's own rows: no other wave's writes to wait for)
-    for (int it = lane; it < 32 * WIDTH / 4; it += 64) {
-        const int rr = 32 * rw + it / (WIDTH / 4), d = it % (WIDTH / 4) * 4, at = row0 + rr;
-        if (at >= rows) continue;
-        const f4v v = *(const f4v *)(rowbuf + rr * ROW + d);
+        for (int w = 0; w < PW; w++) {
+            const float f = __builtin_amdgcn_exp2f(sm[w][0][rr] - mx);
+            sum += sl[w][0][rr] * f;
+            v += *(const f4v *)(rowbuf + (w * 32 * RW + rr) * ROW + d1) * f;
+        }
         if (used > 1) {
-            *(f4v *)(A.part + (((size_t)kvh * rows + at) * A.splits + split) * (4 + WIDTH) + 4 + d) = v;
+            float *dst = A.part + (((size_t)kvh * rows + at) * A.splits + split) * (4 + WIDTH);
+            *(f4v *)(dst + 4 + d1) = v;
+            if (d1 == 0) {
+                dst[0] = mx;
+                dst[1] = sum;
+            }
         } else {
-            float *dst = A.out + (size_t)(at / A.G) * A.out_stride + ((size_t)kvh * A.G + at % A.G) * A.hd + d;
+            float *dst = out_row(A, kvh, at) + d1;
+            v *= 0.25f / sum;
             if (A.out_wide) {
-                if (d < A.hd) *(f4v *)dst = v;
+                if (d1 < A.hd) *(f4v *)dst = v;
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; e++)
-                    if (d + e < A.hd) dst[e] = v[e];
+                    if (d1 + e < A.hd) dst[e] = v[e];
             }
         }
     }
@@ -784,7 +804,7 @@ __global__ __launch_bounds__(256) void kv_merge_k(const uint32_t *pos, AttnArgs 
     // the splits that hold this row: of its block of rows_per rows, tiles_per
     // tiles of a split at a time
     const int row_last = min(row / rows_per * rows_per + rows_per, rows) - 1;
-    const int last = (int)min((size_t)pos[0] + (size_t)(row_last / A.G) + 1, A.n_ctx);
+    const int last = (int)min((size_t)pos[0] + (size_t)token_of(A, row_last) + 1, A.n_ctx);
     const int n_tiles = (last + KVQ_TILE - 1) / KVQ_TILE;
     const int used = min(A.splits, (n_tiles + tiles_per - 1) / tiles_per);
     for (int c0 = 0; c0 < width / 4; c0 += 32) {
@@ -834,7 +854,7 @@ __global__ __launch_bounds__(256) void kv_merge_k(const uint32_t *pos, AttnArgs 
                 sum += sl[g] * f;
                 v += so[g][cq] * f;
             }
-            float *dst = A.out + (size_t)(row / A.G) * A.out_stride + ((size_t)kvh * A.G + row % A.G) * A.hd;
+            float *dst = out_row(A, kvh, row);
             for (int e = 0; e < 4; e++)
                 if (4 * c4 + e < A.hd) dst[4 * c4 + e] = v[e] * 0.25f / sum;
         }
@@ -849,13 +869,13 @@ __global__ __launch_bounds__(256) void kv_merge_rows_k(const uint32_t *pos, Attn
     const int rows = A.M * A.G, row = blockIdx.x * 8 + (threadIdx.x >> 5), kvh = blockIdx.y;
     if (row >= rows) return;
     const int row_last = min(row / rows_per * rows_per + rows_per, rows) - 1;
-    const int last = (int)min((size_t)pos[0] + (size_t)(row_last / A.G) + 1, A.n_ctx);
+    const int last = (int)min((size_t)pos[0] + (size_t)token_of(A, row_last) + 1, A.n_ctx);
     const int n_tiles = (last + KVQ_TILE - 1) / KVQ_TILE;
     const int used = min(A.splits, (n_tiles + tiles_per - 1) / tiles_per);
     if (used == 1) return;
     const size_t rec = 4 + (size_t)width;
     const float *base = A.part + ((size_t)kvh * rows + row) * A.splits * rec;
-    float *dst = A.out + (size_t)(row / A.G) * A.out_stride + ((size_t)kvh * A.G + row % A.G) * A.hd;
+    float *dst = out_row(A, kvh, row);
     for (int c4 = threadIdx.x & 31; c4 < width / 4; c4 += 32) {
         float m = -FLT_MAX, l = 0.0f;
         f4v o = {0, 0, 0, 0};
@@ -947,6 +967,8 @@ extern "C" fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, si
     A.n_head_kv = (int)n_head_kv;
     A.G = (int)(n_head / n_head_kv);
     A.hd = (int)head_dim;
+    while (((uint32_t)1 << A.g_shift) < (uint32_t)A.G) A.g_shift++;
+    A.by_g = (uint32_t)((((uint64_t)1 << (30 + A.g_shift)) + (uint32_t)A.G - 1) / (uint32_t)A.G);
     A.score = (float)(1.4426950408889634 / std::sqrt((double)head_dim) / 4);
     A.M = (int)M;
     A.q_wide = head_dim % 4 == 0 && (uintptr_t)q % 16 == 0 && (M == 1 || q_stride % 4 == 0);
@@ -995,7 +1017,7 @@ extern "C" fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, si
         const void *k = rw == 2 ? (q4 ? many_kernel<4, 2>(ng) : many_kernel<8, 2>(ng))
                                 : (q4 ? many_kernel<4, 4>(ng) : many_kernel<8, 4>(ng));
         const size_t tiles_lds = 2 * (size_t)tiles_per * 4 * ng * 1024;
-        const size_t rows_lds = 32 * (size_t)rw * (pw > 2 ? pw - 1 : 1) * (width + 4) * sizeof(float);
+        const size_t rows_lds = 32 * (size_t)rw * pw * (width + 4) * sizeof(float);
         const size_t lds = tiles_lds > rows_lds ? tiles_lds : rows_lds;
         FOX_HIP(hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
         FOX_HIP(hipLaunchKernel(k, dim3((unsigned)(items * splits)), dim3(64 * rw * pw), args, lds, ctx->stream));
