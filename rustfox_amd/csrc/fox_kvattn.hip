@@ -20,6 +20,7 @@
 #include "fox_internal.h"
 
 #include <cfloat>
+#include <climits>
 #include <cmath>
 #include <type_traits>
 
@@ -33,17 +34,27 @@ typedef uint32_t u4v __attribute__((ext_vector_type(4)));
 #define KA_ROOM 8.0f            // how far scores may pass the running maximum
 #define KA_LIFT 7.0f            // weights are scaled by 2^7: 2^(8 + 7) is within a half
 
+// how a kernel's rows and positions are divided
+struct Parts {
+    int splits, rows, tiles;      // splits of the positions; rows of a workgroup, tiles it takes side by side
+};
+
 struct AttnArgs {
     float *out, *part;
     size_t out_stride, q_stride;
     const float *q;
     const uint8_t *cache;
-    size_t n_ctx;
-    int n_head_kv, G, hd, M, splits;
-    uint32_t by_g, g_shift;       // row / G: see token_of
+    int n_ctx, n_head_kv, G, splits;
+    uint32_t by_g;                // row / G: see token_of
     float score;                  // log2(e) / sqrt(hd) / 4 (the halves are 4 times the values)
+    int from;                     // positions from which kv_attn_many takes the call, kv_attn_few below
+    uint16_t hd, M;
+    uint8_t g_shift;
     bool q_wide, out_wide;        // rows take 16-byte accesses
 };
+
+// positions that the call's last token sees
+__device__ __forceinline__ int seen_of(const AttnArgs &A, size_t p0) { return (int)min(p0 + A.M, (size_t)A.n_ctx); }
 
 // row / G without a division (some thirty instructions, each met cold in a short
 // call): by_g = 2^(30 + g_shift) / G rounded up, 2^g_shift >= G, which is exact for row < 2^30
@@ -335,11 +346,11 @@ __global__ __launch_bounds__(64 * KA_WAVES, NG > 4 ? 1 : 2) void kv_attn_few(con
         }
     }
     const size_t p0 = pos[0];
-    auto end_of = [&](int row) { return (int)min(p0 + (size_t)token_of(A, row) + 1, A.n_ctx); };
+    auto end_of = [&](int row) { return (int)min(p0 + (size_t)token_of(A, row) + 1, (size_t)A.n_ctx); };
     const int last = end_of(min(row0 + ROWS, rows) - 1);         // positions any row sees
     const int first = end_of(row0);                              // and all rows see
     const int n_tiles = (last + KVQ_TILE - 1) / KVQ_TILE, step = A.splits * KA_WAVES;
-    if (split * KA_WAVES >= n_tiles) return;                     // (uniform)
+    if (split * KA_WAVES >= n_tiles || seen_of(A, p0) >= A.from) return;   // (uniform)
     const int used = min(A.splits, (n_tiles + KA_WAVES - 1) / KA_WAVES);
     const size_t recs = (A.n_ctx + KVQ_TILE - 1) / KVQ_TILE;
     constexpr int REC = 2 * (KVQ_TILE * WIDTH * BITS / 8 + KVQ_TILE * NG);
@@ -537,10 +548,10 @@ __global__ __launch_bounds__(64 * KA_WAVES, NG > 4 ? 1 : 2) void kv_attn_few(con
 // against 17 to 19).  A tile's weights are formed beside the next one's scores; a tile is
 // unpacked while the one before it is multiplied, its words read a step
 // earlier still.
-template <int BITS, int NG, int RW, int PW>
-__global__ __launch_bounds__(64 * RW * PW, NG > 4 ? 1 : 2) void kv_attn_many(const uint32_t *pos, AttnArgs A)
+template <int BITS, int NG, int PW>
+__global__ __launch_bounds__(256 * PW, NG > 4 ? 1 : 2) void kv_attn_many(const uint32_t *pos, AttnArgs A)
 {
-    constexpr int WIDTH = 32 * NG, NF = 2 * NG;
+    constexpr int WIDTH = 32 * NG, NF = 2 * NG, RW = 4;
     constexpr int FW = (NF + RW - 1) / RW;                       // fragments a wave unpacks, of K and V each
     constexpr int CODES = KVQ_TILE * WIDTH * BITS / 8, REC = 2 * (CODES + KVQ_TILE * NG);
     static_assert(2 * PW * 2 * NF * 1024 + 4096 <= 160 * 1024 &&
@@ -561,10 +572,10 @@ __global__ __launch_bounds__(64 * RW * PW, NG > 4 ? 1 : 2) void kv_attn_many(con
     const int kvh = blockIdx.x % A.n_head_kv, item = blockIdx.x / A.n_head_kv;
     const int split = item % A.splits, row0 = (blocks - 1 - item / A.splits) * 32 * RW;
     const size_t p0 = pos[0];
-    auto end_of = [&](int row) { return (int)min(p0 + (size_t)token_of(A, row) + 1, A.n_ctx); };
+    auto end_of = [&](int row) { return (int)min(p0 + (size_t)token_of(A, row) + 1, (size_t)A.n_ctx); };
     const int last = end_of(min(row0 + 32 * RW, rows) - 1), first = end_of(row0);
     const int n_tiles = (last + KVQ_TILE - 1) / KVQ_TILE, step = A.splits * PW;
-    if (split * PW >= n_tiles) return;                           // (uniform)
+    if (split * PW >= n_tiles || seen_of(A, p0) < A.from) return;   // (uniform)
     const int used = min(A.splits, (n_tiles + PW - 1) / PW);
     const int row = row0 + 32 * rw + r, end = end_of(min(row, rows - 1));
     const uint8_t *base = A.cache + (size_t)kvh * ((A.n_ctx + KVQ_TILE - 1) / KVQ_TILE) * REC;
@@ -792,31 +803,34 @@ __global__ __launch_bounds__(64 * RW * PW, NG > 4 ? 1 : 2) void kv_attn_many(con
 }
 
 // One workgroup per (row, kv head): the splits' records at their common
-// maximum.  32 threads to a column quad's splits, eight split groups.
-__global__ __launch_bounds__(256) void kv_merge_k(const uint32_t *pos, AttnArgs A, int width, int rows_per, int tiles_per)
+// maximum.  32 threads to a column quad's splits, eight split groups.  (EITHER: both
+// kernels were launched; otherwise the position is not waited for.)
+template <bool EITHER>
+__global__ __launch_bounds__(256) void kv_merge_k(const uint32_t *pos, AttnArgs A, int width, Parts few, Parts many)
 {
     __shared__ float sm[8], sl[8];
     __shared__ f4v so[8][32];
     const int row = blockIdx.x, kvh = blockIdx.y, rows = A.M * A.G;
     const int tid = threadIdx.x, sg = tid >> 5, cq = tid & 31;
     const size_t rec = 4 + (size_t)width;
-    const float *base = A.part + ((size_t)kvh * rows + row) * A.splits * rec;
-    // the splits that hold this row: of its block of rows_per rows, tiles_per
-    // tiles of a split at a time
-    const int row_last = min(row / rows_per * rows_per + rows_per, rows) - 1;
-    const int last = (int)min((size_t)pos[0] + (size_t)token_of(A, row_last) + 1, A.n_ctx);
+    // the splits that hold this row: of its block of P.rows rows, P.tiles tiles
+    // of a split at a time
+    const Parts P = EITHER && seen_of(A, pos[0]) >= A.from ? many : few;
+    const float *base = A.part + ((size_t)kvh * rows + row) * P.splits * rec;
+    const int row_last = min(row / P.rows * P.rows + P.rows, rows) - 1;
+    const int last = (int)min((size_t)pos[0] + (size_t)token_of(A, row_last) + 1, (size_t)A.n_ctx);
     const int n_tiles = (last + KVQ_TILE - 1) / KVQ_TILE;
-    const int used = min(A.splits, (n_tiles + tiles_per - 1) / tiles_per);
+    const int used = min(P.splits, (n_tiles + P.tiles - 1) / P.tiles);
     for (int c0 = 0; c0 < width / 4; c0 += 32) {
         const int c4 = min(c0 + cq, width / 4 - 1);
         float m = -FLT_MAX, l = 0.0f;
         f4v o = {0, 0, 0, 0};
-        for (int s0 = sg; s0 < A.splits; s0 += 8 * 8) {
+        for (int s0 = sg; s0 < P.splits; s0 += 8 * 8) {
             float ms[8], ls[8];
             f4v os[8];
 #pragma unroll
             for (int k = 0; k < 8; k++) {                         // (read together, ahead of the position:
-                const float *p = base + (size_t)min(s0 + 8 * k, A.splits - 1) * rec;   // unused ones are
+                const float *p = base + (size_t)min(s0 + 8 * k, P.splits - 1) * rec;   // unused ones are
                 ms[k] = p[0];                                     // there and left out below)
                 ls[k] = p[1];
                 os[k] = *(const f4v *)(p + 4 + 4 * c4);
@@ -864,17 +878,19 @@ __global__ __launch_bounds__(256) void kv_merge_k(const uint32_t *pos, AttnArgs 
 
 // The same for up to 16 splits: 32 threads to a row, eight rows to a workgroup,
 // a column quad's records read together.
-__global__ __launch_bounds__(256) void kv_merge_rows_k(const uint32_t *pos, AttnArgs A, int width, int rows_per, int tiles_per)
+template <bool EITHER>
+__global__ __launch_bounds__(256) void kv_merge_rows_k(const uint32_t *pos, AttnArgs A, int width, Parts few, Parts many)
 {
     const int rows = A.M * A.G, row = blockIdx.x * 8 + (threadIdx.x >> 5), kvh = blockIdx.y;
     if (row >= rows) return;
-    const int row_last = min(row / rows_per * rows_per + rows_per, rows) - 1;
-    const int last = (int)min((size_t)pos[0] + (size_t)token_of(A, row_last) + 1, A.n_ctx);
+    const Parts P = EITHER && seen_of(A, pos[0]) >= A.from ? many : few;
+    const int row_last = min(row / P.rows * P.rows + P.rows, rows) - 1;
+    const int last = (int)min((size_t)pos[0] + (size_t)token_of(A, row_last) + 1, (size_t)A.n_ctx);
     const int n_tiles = (last + KVQ_TILE - 1) / KVQ_TILE;
-    const int used = min(A.splits, (n_tiles + tiles_per - 1) / tiles_per);
+    const int used = min(P.splits, (n_tiles + P.tiles - 1) / P.tiles);
     if (used == 1) return;
     const size_t rec = 4 + (size_t)width;
-    const float *base = A.part + ((size_t)kvh * rows + row) * A.splits * rec;
+    const float *base = A.part + ((size_t)kvh * rows + row) * P.splits * rec;
     float *dst = out_row(A, kvh, row);
     for (int c4 = threadIdx.x & 31; c4 < width / 4; c4 += 32) {
         float m = -FLT_MAX, l = 0.0f;
@@ -925,17 +941,44 @@ static const void *few_kernel(int ng, int per)
 #undef FOX_FEW
 }
 
-template <int BITS, int RW>
+template <int BITS>
 static const void *many_kernel(int ng)
 {
     switch (ng) {
-    case 1: return (const void *)kv_attn_many<BITS, 1, RW, 8 / RW>;
-    case 2: return (const void *)kv_attn_many<BITS, 2, RW, 8 / RW>;
-    case 3: return (const void *)kv_attn_many<BITS, 3, RW, 8 / RW>;
-    case 4: return (const void *)kv_attn_many<BITS, 4, RW, 8 / RW>;
-    case 6: return (const void *)kv_attn_many<BITS, 6, 4, 1>;
-    default: return (const void *)kv_attn_many<BITS, 8, 4, 1>;
+    case 1: return (const void *)kv_attn_many<BITS, 1, 2>;
+    case 2: return (const void *)kv_attn_many<BITS, 2, 2>;
+    case 3: return (const void *)kv_attn_many<BITS, 3, 2>;
+    case 4: return (const void *)kv_attn_many<BITS, 4, 2>;
+    default: return (const void *)kv_attn_many<BITS, 8, 1>;
     }
+}
+
+// Into how many splits of `most` side-by-side steps at most each item's positions go, by the
+// microseconds (as measured) of a workgroup's way in and out, of a step of it, of the
+// merge and of a split's records.  A compute unit takes w workgroups one after another, or
+// two at a time at 1.7 times one's time; tried are the fewest splits
+// that give the steps that w = 1..4 workgroups each can have.
+static int split_count(size_t items, size_t most, int n_cu, bool pairs, double way, double step, double merge,
+                          double records)
+{
+    size_t best = 1;
+    double least = 0.0;
+    for (int w = 0; w <= 4; w++) {                               // (w = 0: one split)
+        size_t s = w ? w * (size_t)n_cu / items : 1;
+        if (s > most) s = most;
+        if (s == 0) continue;
+        const size_t steps = (most + s - 1) / s;
+        s = (most + steps - 1) / steps;
+        const size_t load = (items * s + n_cu - 1) / n_cu;
+        const double us = (pairs ? 1.7 * (double)(load / 2) + (double)(load % 2) : (double)load) *
+                              (way + step * (double)steps) +
+                          (s > 1 ? merge + records * (double)s : 0.0);
+        if (w == 0 || us < least) {
+            least = us;
+            best = s;
+        }
+    }
+    return (int)best;
 }
 
 extern "C" fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, size_t out_stride,
@@ -963,77 +1006,76 @@ extern "C" fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, si
     A.q = q;
     A.q_stride = q_stride;
     A.cache = (const uint8_t *)cache;
-    A.n_ctx = n_ctx;
+    A.n_ctx = (int)n_ctx;
     A.n_head_kv = (int)n_head_kv;
     A.G = (int)(n_head / n_head_kv);
-    A.hd = (int)head_dim;
+    A.hd = (uint16_t)head_dim;
     while (((uint32_t)1 << A.g_shift) < (uint32_t)A.G) A.g_shift++;
     A.by_g = (uint32_t)((((uint64_t)1 << (30 + A.g_shift)) + (uint32_t)A.G - 1) / (uint32_t)A.G);
     A.score = (float)(1.4426950408889634 / std::sqrt((double)head_dim) / 4);
-    A.M = (int)M;
+    A.M = (uint16_t)M;
     A.q_wide = head_dim % 4 == 0 && (uintptr_t)q % 16 == 0 && (M == 1 || q_stride % 4 == 0);
     A.out_wide = head_dim % 4 == 0 && (uintptr_t)out % 16 == 0 && (M == 1 || out_stride % 4 == 0);
     const int width = kvq_width((int)head_dim), ng = width / 32;
     const size_t rows = M * (size_t)A.G;
-    const bool many = rows > 32, q4 = kv_type == FOX_GPU_KV_Q4;
-    // many rows: 128 of them in four waves, tiles in two groups; up to 64 in two
-    // waves and four groups; heads past 128 dimensions hold one group's registers only
-    const int rw = ng > 4 || rows > 64 ? 4 : 2, pw = ng > 4 ? 1 : 8 / rw;
-    const int per = many ? 32 * rw : rows <= 8 ? 8 : rows <= 16 || ng > 6 ? 16 : 32;   // rows of a workgroup
-    const int tiles_per = many ? pw : KA_WAVES;                         // tiles it takes side by side
-    const size_t blocks = (rows + per - 1) / per, items = n_head_kv * blocks;
-    const size_t most = (n_ctx + KVQ_TILE * tiles_per - 1) / (KVQ_TILE * tiles_per);
-    size_t splits = 1;
-    if (!many) {
-        // up to 4 tiles a wave in one launch: at 500 positions 8.9 us against 8.8 in
-        // 4 splits and a merge, at 250 7.4 / 8.7, at 800 11.0 / 9.8
-        splits = n_ctx <= 512 ? 1 : 2 * (size_t)ctx->n_cu / items;
-    } else {
-        // One workgroup to a compute unit.  More splits fill the last round, at
-        // the price of their records, which leave the caches at the kernel's end
-        // and come back: measured 1.65 us a step of a workgroup, 1 us a MB of records
-        // (a 1024-token prompt of 32 heads over 8 of 128 in 2 splits: 38.7 -> 71 us).
-        double best = 0.0;
-        for (size_t s = 1; s <= 64 && s <= most; s++) {
-            const double rounds = (double)((items * s + ctx->n_cu - 1) / ctx->n_cu);
-            const double us = rounds * (8.0 + 1.65 * (double)((most + s - 1) / s)) +
-                              (s > 1 ? 5.0 + 1e-6 * (double)(items * s * per) * (4 + width) * 4 : 0.0);
-            if (s == 1 || us < best) {
-                best = us;
-                splits = s;
-            }
-        }
+    const bool q4 = kv_type == FOX_GPU_KV_Q4;
+    // Unpacking a tile once for 128 rows costs a long way in and out (a workgroup of
+    // one tile 9 us against 4), so only long work pays for it: from 4.2e7 pairs of
+    // a row and a position on, and where the last 128 rows are not mostly empty.
+    // Heads of 128 dimensions, kv heads x rows x positions, in tiles by the wave and
+    // unpacked once: 8 x 64 x 128 8.3 / 12.7 us, 8 x 4000 x 1024 38.1 / 38.2,
+    // 8 x 4000 x 2500 88 / 79, 8 x 192 x 40000 79 / 88, 8 x 256 x 40000 97 / 91.
+    // Heads of 256, where a wave holds 16 rows: 4 x 192 x 2500 30 / 47, 4 x 768 x
+    // 2500 57 / 60, 16 x 96 x 16000 110 / 107, 4 x 768 x 16000 254 / 143.  Of 192, never
+    // (4 x 6000 x 16000 675 / 716).  Where the position decides, both are launched
+    // and the one that it is not for ends at once (2 us).
+    const size_t per = rows <= 8 ? 8 : rows <= 16 || ng > 6 ? 16 : 32, turns = ng > 4 ? 1 : 2;
+    const bool wide = ng != 6 && 2 * ((rows + per - 1) / per) > (ng > 6 ? 10 : 7) * ((rows + 127) / 128);
+    const double from = (ng > 6 ? 1.6e7 : 4.2e7) / ((double)rows * (double)n_head_kv);
+    A.from = wide && from < (double)n_ctx ? (int)from + 1 : INT_MAX;
+    const bool many = A.from <= (int64_t)n_ctx, few = A.from > (int64_t)M;   // (a call has M positions at least)
+    Parts few_parts = {}, many_parts = {};
+    const double record = 1e-6 * (double)(rows * n_head_kv) * (4 + width) * sizeof(float);   // MB of a split's
+    const size_t few_blocks = (rows + per - 1) / per, many_blocks = (rows + 127) / 128;
+    if (few) {
+        const size_t n = A.from < (int64_t)n_ctx ? (size_t)A.from : n_ctx;
+        few_parts = {split_count(n_head_kv * few_blocks, (n + KVQ_TILE * KA_WAVES - 1) / (KVQ_TILE * KA_WAVES), ctx->n_cu,
+                             ng <= 4, 0.45 * ng, per == 32 ? 0.35 + 0.19 * ng : 0.2 + 0.18 * ng, 1.9, 0.5 * record),
+                 (int)per, KA_WAVES};
     }
-    if (splits > most) splits = most;
-    if (splits < 1) splits = 1;
-    A.splits = (int)splits;
+    if (many)
+        many_parts = {split_count(n_head_kv * many_blocks, (n_ctx + KVQ_TILE * turns - 1) / (KVQ_TILE * turns), ctx->n_cu,
+                              false, 8.0, 1.65, 5.0, record),
+                  128, (int)turns};
+    const int splits = few_parts.splits > many_parts.splits ? few_parts.splits : many_parts.splits;
     if (splits > 1) {
         st = fox_ws_reserve(ctx, n_head_kv * rows * splits * (4 + (size_t)width) * sizeof(float));
         if (st) return st;
         A.part = (float *)ctx->ws;
     }
     void *args[] = {(void *)&pos, &A};
+    A.splits = few_parts.splits;
+    if (few)
+        FOX_HIP(hipLaunchKernel(q4 ? few_kernel<4>(ng, (int)per) : few_kernel<8>(ng, (int)per),
+                                dim3((unsigned)few_parts.splits, (unsigned)n_head_kv, (unsigned)few_blocks),
+                                dim3(64 * KA_WAVES), args, 0, ctx->stream));
     if (many) {
-        const void *k = rw == 2 ? (q4 ? many_kernel<4, 2>(ng) : many_kernel<8, 2>(ng))
-                                : (q4 ? many_kernel<4, 4>(ng) : many_kernel<8, 4>(ng));
-        const size_t tiles_lds = 2 * (size_t)tiles_per * 4 * ng * 1024;
-        const size_t rows_lds = 32 * (size_t)rw * pw * (width + 4) * sizeof(float);
+        A.splits = many_parts.splits;
+        const void *k = q4 ? many_kernel<4>(ng) : many_kernel<8>(ng);
+        const size_t tiles_lds = 2 * turns * 4 * ng * 1024, rows_lds = 128 * turns * (width + 4) * sizeof(float);
         const size_t lds = tiles_lds > rows_lds ? tiles_lds : rows_lds;
         FOX_HIP(hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-        FOX_HIP(hipLaunchKernel(k, dim3((unsigned)(items * splits)), dim3(64 * rw * pw), args, lds, ctx->stream));
-    } else {
-        FOX_HIP(hipLaunchKernel(q4 ? few_kernel<4>(ng, per) : few_kernel<8>(ng, per),
-                                dim3((unsigned)splits, (unsigned)n_head_kv, (unsigned)blocks),
-                                dim3(64 * KA_WAVES), args, 0, ctx->stream));
+        FOX_HIP(hipLaunchKernel(k, dim3((unsigned)(n_head_kv * many_blocks * many_parts.splits)), dim3(256 * turns), args,
+                                lds, ctx->stream));
     }
     if (splits > 1) {
-        if (splits <= 16 && rows * n_head_kv >= 1024)
-            hipLaunchKernelGGL(kv_merge_rows_k, dim3((unsigned)((rows + 7) / 8), (unsigned)n_head_kv),
-                               dim3(256), 0, ctx->stream, pos, A, width, per, tiles_per);
-        else
-            hipLaunchKernelGGL(kv_merge_k, dim3((unsigned)rows, (unsigned)n_head_kv), dim3(256), 0,
-                               ctx->stream, pos, A, width, per, tiles_per);
-        FOX_LAUNCHED("kvq attention merge");
+        const bool by_rows = splits <= 16 && rows * n_head_kv >= 1024, either = few && many;
+        if (!few) few_parts = many_parts;
+        const void *k = by_rows ? either ? (const void *)kv_merge_rows_k<true> : (const void *)kv_merge_rows_k<false>
+                                : either ? (const void *)kv_merge_k<true> : (const void *)kv_merge_k<false>;
+        void *merge_args[] = {(void *)&pos, &A, (void *)&width, &few_parts, &many_parts};
+        FOX_HIP(hipLaunchKernel(k, dim3((unsigned)(by_rows ? (rows + 7) / 8 : rows), (unsigned)n_head_kv), dim3(256),
+                                merge_args, 0, ctx->stream));
     }
     return FOX_GPU_OK;
 }

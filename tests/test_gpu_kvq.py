@@ -380,6 +380,95 @@ def test_small_and_large_values(gpu):
             check(got, q, kr.held(K, bits, hd), kr.held(V, bits, hd), n_head, n_kv, hd, n_ctx - 1, n_ctx)
 
 
+LONG_WORK = [  # n_head, n_kv, hd, n_ctx, pos, M: 4.2e7 pairs of a row and a position (1.6e7 of 256 dimensions)
+    (1100, 1, 32, 520, 310, 100), (1100, 1, 32, 520, 100, 100),     # past them, and below in the same cache
+    (512, 1, 64, 700, 500, 192), (520, 1, 90, 930, 800, 101), (512, 2, 128, 1200, 1000, 100),
+    (130, 1, 256, 1300, 1200, 101), (130, 1, 256, 1300, 900, 101), (65, 1, 250, 1290, 1200, 200),
+    (300, 1, 48, 900, 0, 900),                                      # as many tokens as positions
+    (300, 1, 64, 800, 700, 200),                                    # and tokens past them
+    (128, 1, 64, 400_000, 350_000, 1), (128, 1, 256, 40_000, 33_000, 4),   # few rows, split many ways
+    (128, 1, 64, 400_000, 300_000, 1), (128, 1, 256, 40_000, 30_000, 4), (128, 1, 64, 400_000, 77, 1),
+    (128, 2, 128, 9000, 8000, 60),
+]
+
+
+def check_some(got, q, K, V, n_head, n_kv, hd, pos, n_ctx, rng, count=150):
+    """The first and last row and some between, of a pass too large for the plain one."""
+    M, group = q.shape[0], n_head // n_kv
+    K, V = np.float64(K), np.float64(V)
+    assert np.isfinite(got).all()
+    picks = [0, M * n_head - 1, *rng.integers(0, M * n_head, count)]
+    for t, h in (divmod(int(i), n_head) for i in picks):
+        at, kv = slice(h * hd, (h + 1) * hd), slice(h // group * hd, (h // group + 1) * hd)
+        want, sizes = kr.attention(q[t:t + 1, at], K[:, kv], V[:, kv], 1, 1, hd, min(pos + t, n_ctx - 1), n_ctx)
+        off, bound = np.abs(got[t:t + 1, at] - want), kr.attention_bound(sizes, min(pos + t + 1, n_ctx), hd)
+        assert np.all(off <= bound), (t, h, (off / bound).max())
+
+
+@pytest.mark.parametrize("case", LONG_WORK, ids=str)
+@pytest.mark.parametrize("bits", BITS)
+def test_long_work(gpu, bits, case):
+    n_head, n_kv, hd, n_ctx, pos, M = case
+    rng = np.random.default_rng(pos + M)
+    n = min(pos + M, n_ctx)
+    K, V = (rng.standard_normal((n, n_kv * hd), np.float32) for _ in range(2))
+    q = (1.5 * rng.standard_normal((M, n_head * hd), np.float32)).astype(np.float32)
+    c = fill(gpu, bits, n_ctx, n_kv, hd, K, V)               # (rows past n stay poisoned)
+    got = attend(gpu, bits, c, q, n_head, n_kv, hd, n_ctx, pos, pad=3 if M % 2 else 0)
+    check_some(got, q, kr.held(K, bits, hd), kr.held(V, bits, hd), n_head, n_kv, hd, pos, n_ctx, rng,
+               150 if n < 20000 else 20)
+
+
+@pytest.mark.parametrize("n_head,hd,pos", [(640, 64, 300), (260, 256, 300)])
+@pytest.mark.parametrize("side", ["k", "v", "q"])
+@pytest.mark.parametrize("bits", BITS)
+def test_a_nan_in_long_work(gpu, bits, side, n_head, hd, pos):
+    """As in the short passes: a key's NaN takes the rows that see it, a value's its group's columns
+    of them, a query's or its infinity its own row."""
+    M, j = 150, 90
+    n = n_ctx = pos + M
+    rng = np.random.default_rng(hd)
+    K, V = rows(rng, n, hd), rows(rng, n, hd)
+    q = rng.standard_normal((M, n_head * hd)).astype(np.float32)
+    hit = np.zeros((M, n_head, hd), bool)
+    if side == "q":
+        q[j, 7 * hd + 3], q[j, 30 * hd] = np.nan, np.inf
+        hit[j, 7] = hit[j, 30] = True
+    else:
+        (K if side == "k" else V)[pos + j, 40] = np.nan      # the second group
+        hit[j:, :, slice(None) if side == "k" else slice(32, 64)] = True
+    c = fill(gpu, bits, n_ctx, 1, hd, K, V)
+    got = attend(gpu, bits, c, q, n_head, 1, hd, n_ctx, pos)
+    assert np.array_equal(np.isnan(got), hit.reshape(M, -1))
+
+
+def test_long_work_captured(gpu):
+    """One capture serves positions on both sides of where long work begins: each replay against the
+    eager call, bit for bit, and against the plain one."""
+    n_head, n_kv, hd, n_ctx, M = 512, 1, 64, 900, 100
+    rng = np.random.default_rng(5)
+    K, V = rows(rng, n_ctx, hd), rows(rng, n_ctx, hd)
+    Kh, Vh = kr.held(K, 4, hd), kr.held(V, 4, hd)
+    c = fill(gpu, 4, n_ctx, n_kv, hd, K, V)
+    q = rng.standard_normal((M, n_head * hd)).astype(np.float32)
+    dq, pos = gpu.array(q), u32(gpu, 0)
+    out, other = (gpu.empty((M, n_head * hd), np.float32) for _ in range(2))
+    gpu.kvq_attention(out, dq, 4, c, n_head, n_kv, hd, M, pos, n_ctx)        # (any workspace is taken here)
+    g = C.c_void_p()
+    assert gpu.lib.fox_gpu_graph_begin(gpu.ctx) == 0
+    gpu.kvq_attention(out, dq, 4, c, n_head, n_kv, hd, M, pos, n_ctx)
+    assert gpu.lib.fox_gpu_graph_end(gpu.ctx, C.byref(g)) == 0
+    for p in (790, 0, 730, 710, 720, 800, 30):
+        pos.upload(np.array([p], np.uint32))
+        out.fill(0xFF)
+        assert gpu.lib.fox_gpu_graph_launch(gpu.ctx, g) == 0
+        got = out.numpy()
+        gpu.kvq_attention(other, dq, 4, c, n_head, n_kv, hd, M, pos, n_ctx)
+        assert np.array_equal(other.numpy(), got)
+        check_some(got, q, Kh, Vh, n_head, n_kv, hd, p, n_ctx, rng, 40)
+    gpu.lib.fox_gpu_graph_free(g)
+
+
 # ----------------------------------------------------------- as they are used
 
 @pytest.mark.parametrize("bits", BITS)
