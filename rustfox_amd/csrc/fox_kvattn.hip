@@ -329,7 +329,7 @@ __global__ __launch_bounds__(64 * KA_WAVES, NG > 4 ? 1 : 2) void kv_attn_few(con
     __shared__ float tops[KA_WAVES][T][16], sm[KA_WAVES][T][16], sl[KA_WAVES][T][16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, c = lane >> 4;
-    const int split = blockIdx.x, kvh = blockIdx.y, row0 = blockIdx.z * ROWS;
+    const int split = blockIdx.x, kvh = blockIdx.y, row0 = (gridDim.z - 1 - blockIdx.z) * ROWS;   // (longest rows first)
     const int rows = A.M * A.G;
     // queries: lane (r, c) has row r's dimensions of chunk c, product step j the
     // eight from 8 (NG c + j) on; a wave prepares some steps for all
