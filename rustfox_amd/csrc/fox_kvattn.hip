@@ -255,10 +255,15 @@ __device__ __forceinline__ void put_sums(const AttnArgs &A, int kvh, int row, in
                                          float l, bool whole, int split, int width)
 {
     if (whole) {
-        float *dst = out_row(A, kvh, row);
+        float *dst = out_row(A, kvh, row) + dim;
+        v *= 0.25f / l;
+        if (A.out_wide) {
+            if (dim < A.hd) *(f4v *)dst = v;
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; e++)
-            if (dim + e < A.hd) dst[dim + e] = v[e] * 0.25f / l;
+            for (int e = 0; e < 4; e++)
+                if (dim + e < A.hd) dst[e] = v[e];
+        }
     } else {
         float *dst = A.part + (((size_t)kvh * A.M * A.G + row) * A.splits + split) * (4 + width);
         if (dim == 0) {
