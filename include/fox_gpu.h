@@ -453,7 +453,8 @@ fox_gpu_status fox_gpu_kvq_norm_rope_store(
 
 /* Causal GQA attention of M <= FOX_GPU_BATCH_TOKENS tokens at positions
  * pos[0] + t over positions 0 .. pos[0] + t of a quantised cache:
- * softmax(q.k / sqrt(hd)) v, for any number of query heads per kv head.  The
+ * softmax(q.k / sqrt(hd)) v, for any number of query heads per kv head (M
+ * n_head / n_head_kv at most 2097120 where head_dim is 130 .. 192).  The
  * cache's values are multiplied as they are; sums, maxima and the softmax are in
  * 32 bits.  out must not overlap q. */
 fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, size_t out_stride,

@@ -250,20 +250,25 @@ __device__ __forceinline__ f16v mfma(h8v a, h8v b, f16v c)
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
+// four results of a row from dimension `dim` on
+__device__ __forceinline__ void put_row(const AttnArgs &A, int kvh, int row, int dim, f4v v)
+{
+    float *dst = out_row(A, kvh, row) + dim;
+    if (A.out_wide) {
+        if (dim < A.hd) *(f4v *)dst = v;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (dim + e < A.hd) dst[e] = v[e];
+    }
+}
+
 // Four sums of one row at dimension `dim` of kv head kvh: the result, or a split's record.
 __device__ __forceinline__ void put_sums(const AttnArgs &A, int kvh, int row, int dim, f4v v, float m,
                                          float l, bool whole, int split, int width)
 {
     if (whole) {
-        float *dst = out_row(A, kvh, row) + dim;
-        v *= 0.25f / l;
-        if (A.out_wide) {
-            if (dim < A.hd) *(f4v *)dst = v;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (dim + e < A.hd) dst[e] = v[e];
-        }
+        put_row(A, kvh, row, dim, v * (0.25f / l));
     } else {
         float *dst = A.part + (((size_t)kvh * A.M * A.G + row) * A.splits + split) * (4 + width);
         if (dim == 0) {
@@ -322,6 +327,13 @@ struct Tile {
 // ROWS 8: the columns of one product hold the rows' upper halves and their
 // lower ones, so a tile takes half the products; the two columns of a row are
 // added where a score is used and at the end.
+// What bounds it is unpacking, then the read: one row of 32 heads over 8 of 128
+// dimensions, 4 bits, at 131,071 positions (143 MB) takes 32.5 us, 4.4 TB/s with
+// the vector units busy 57% and the matrix cores 10% of the time; 8 bits, fewer
+// instructions a value, reads 4.9 TB/s (60,000 positions, 29.4 us with both launches).
+// Reading two tiles ahead is slower (39.4 us for 36.5), as is one copy of the loop's
+// body that reads past its last tile (8.4 -> 8.8 us at 1500 positions).
+// Short contexts are a launch and 2 to 4 us: 34 positions of 6 heads 4.4 us in all.
 template <int BITS, int NG, int ROWS>
 __global__ __launch_bounds__(64 * KA_WAVES, NG > 4 ? 1 : 2) void kv_attn_few(const uint32_t *pos, AttnArgs A)
 {
@@ -545,22 +557,24 @@ __global__ __launch_bounds__(64 * KA_WAVES, NG > 4 ? 1 : 2) void kv_attn_few(con
     }
 }
 
-// Many rows: RW waves of 32 rows each share a tile's unpacked halves in LDS, a
-// piece unpacked by each of them, and PW such groups of a workgroup take tiles in
-// turn, merged at the end.  Products are 32x32x16: at the 16x16x32 form's
+// Many rows: four waves of 32 rows each share a tile's unpacked halves in LDS, a
+// quarter unpacked by each of them, and PW such groups of a workgroup take tiles in
+// turn, added at the end.  Products are 32x32x16: at the 16x16x32 form's
 // back-to-back rate the matrix cores idle half the time (32 cycles an
 // instruction against 16, measured; with vector instructions between, 19 to 23
 // against 17 to 19).  A tile's weights are formed beside the next one's scores; a tile is
 // unpacked while the one before it is multiplied, its words read a step
-// earlier still.
+// earlier still.  777 tokens on 8000 positions of 32 heads over 8 of 128 take 215 us, 1000
+// TFLOP/s of half products (two a product, see above) where a large library product
+// of halves reaches 1136: matrix cores busy 41%, vector units 37% of the time.
 template <int BITS, int NG, int PW>
 __global__ __launch_bounds__(256 * PW, NG > 4 ? 1 : 2) void kv_attn_many(const uint32_t *pos, AttnArgs A)
 {
-    constexpr int WIDTH = 32 * NG, NF = 2 * NG, RW = 4;
-    constexpr int FW = (NF + RW - 1) / RW;                       // fragments a wave unpacks, of K and V each
+    constexpr int WIDTH = 32 * NG, NF = 2 * NG;
+    constexpr int FW = (NF + 3) / 4;                             // fragments a wave unpacks, of K and V each
     constexpr int CODES = KVQ_TILE * WIDTH * BITS / 8, REC = 2 * (CODES + KVQ_TILE * NG);
     static_assert(2 * PW * 2 * NF * 1024 + 4096 <= 160 * 1024 &&
-                  32 * RW * PW * (WIDTH + 4) * 4 + 4096 <= 160 * 1024, "LDS");
+                  128 * PW * (WIDTH + 4) * 4 + 4096 <= 160 * 1024, "LDS");
     // [buffer][group][K fragments, V fragments][lane]: a fragment is an MFMA
     // operand; f of K holds 8 dimensions of each half of the 32 positions' rows, from
     // 8 f and from WIDTH / 2 + 8 f on; f of V dimensions 32 (f / 2) + 0..31 of
@@ -568,17 +582,17 @@ __global__ __launch_bounds__(256 * PW, NG > 4 ? 1 : 2) void kv_attn_many(const u
     extern __shared__ h8v frag[];
     constexpr int ROW = WIDTH + 4;                               // floats of a row in LDS, when rows pass through it
     __shared__ int nan_at[2][PW][NG];
-    __shared__ float sm[PW][RW][32], sl[PW][RW][32];
+    __shared__ float sm[PW][4][32], sl[PW][4][32];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int r = lane & 31, c = lane >> 5, rw = wave % RW, pw = wave / RW;
+    const int r = lane & 31, c = lane >> 5, rw = wave % 4, pw = wave / 4;
     // workgroups that share a kv head's cache get the same blockIdx % n_head_kv; the
     // longest rows first
-    const int rows = A.M * A.G, blocks = (rows + 32 * RW - 1) / (32 * RW);
+    const int rows = A.M * A.G, blocks = (rows + 127) / 128;
     const int kvh = blockIdx.x % A.n_head_kv, item = blockIdx.x / A.n_head_kv;
-    const int split = item % A.splits, row0 = (blocks - 1 - item / A.splits) * 32 * RW;
+    const int split = item % A.splits, row0 = (blocks - 1 - item / A.splits) * 128;
     const size_t p0 = pos[0];
     auto end_of = [&](int row) { return (int)min(p0 + (size_t)token_of(A, row) + 1, (size_t)A.n_ctx); };
-    const int last = end_of(min(row0 + 32 * RW, rows) - 1), first = end_of(row0);
+    const int last = end_of(min(row0 + 128, rows) - 1), first = end_of(row0);
     const int n_tiles = (last + KVQ_TILE - 1) / KVQ_TILE, step = A.splits * PW;
     if (split * PW >= n_tiles || seen_of(A, p0) < A.from) return;   // (uniform)
     const int used = min(A.splits, (n_tiles + PW - 1) / PW);
@@ -623,7 +637,7 @@ __global__ __launch_bounds__(256 * PW, NG > 4 ? 1 : 2) void kv_attn_many(const u
 #pragma unroll
         for (int u = 0; u < FW; u++) {
             const int f = rw * FW + u;
-            if (FW * RW > NF && f >= NF) break;
+            if (4 * FW > NF && f >= NF) break;
             place(buf)[f * 64] = unpack_k<BITS>(kw[u], ks[u], 0);
         }
     };
@@ -631,7 +645,7 @@ __global__ __launch_bounds__(256 * PW, NG > 4 ? 1 : 2) void kv_attn_many(const u
 #pragma unroll
         for (int u = 0; u < FW; u++) {
             const int f = rw * FW + u;
-            if (FW * RW > NF && f >= NF) break;
+            if (4 * FW > NF && f >= NF) break;
             h2v d[4], mm[4];
             v_scales(vs[u], d, mm);
             place(buf)[(NF + f) * 64] = unpack<BITS>(vw[u], d, mm);
@@ -657,17 +671,17 @@ __global__ __launch_bounds__(256 * PW, NG > 4 ? 1 : 2) void kv_attn_many(const u
     // queries, through LDS: a row's pieces side by side from memory (a lane a
     // row touches 64 lines with every load)
     float *rowbuf = (float *)frag;
-    constexpr int QUADS = WIDTH / 4, AT_ONCE = 64 * RW * PW / QUADS;   // rows that the threads cover at once
+    constexpr int QUADS = WIDTH / 4, AT_ONCE = 256 * PW / QUADS;   // rows that the threads cover at once
     const int rr0 = threadIdx.x / QUADS, d0 = threadIdx.x % QUADS * 4;
     if (rr0 < AT_ONCE) {
         if (A.q_wide) {
 #pragma unroll 8
-            for (int rr = rr0; rr < 32 * RW; rr += AT_ONCE)
+            for (int rr = rr0; rr < 128; rr += AT_ONCE)
                 *(f4v *)(rowbuf + rr * ROW + d0) =
                     d0 < A.hd ? *(const f4v *)(query_row(A, kvh, min(row0 + rr, rows - 1)) + d0) : f4v{0, 0, 0, 0};
         } else {
 #pragma unroll 1
-            for (int rr = rr0; rr < 32 * RW; rr += AT_ONCE)
+            for (int rr = rr0; rr < 128; rr += AT_ONCE)
                 *(float4 *)(rowbuf + rr * ROW + d0) =
                     query_quad(query_row(A, kvh, min(row0 + rr, rows - 1)), d0, A);
         }
@@ -762,7 +776,7 @@ __global__ __launch_bounds__(256 * PW, NG > 4 ? 1 : 2) void kv_attn_many(const u
         sm[pw][rw][r] = m;
         sl[pw][rw][r] = l;
     }
-    float *mine = rowbuf + ((pw * RW + rw) * 32 + r) * ROW + 4 * c;
+    float *mine = rowbuf + ((pw * 4 + rw) * 32 + r) * ROW + 4 * c;
 #pragma unroll
     for (int k = 0; k < 4 * NG; k++)
         *(f4v *)(mine + 8 * k) = f4v{o[k >> 2][4 * (k & 3)], o[k >> 2][4 * (k & 3) + 1],
@@ -773,7 +787,7 @@ __global__ __launch_bounds__(256 * PW, NG > 4 ? 1 : 2) void kv_attn_many(const u
     const int d1 = thread % QUADS * 4;
     if (thread / QUADS >= AT_ONCE) return;
 #pragma unroll 2
-    for (int rr = thread / QUADS; rr < 32 * RW; rr += AT_ONCE) {
+    for (int rr = thread / QUADS; rr < 128; rr += AT_ONCE) {
         const int at = row0 + rr;
         if (at >= rows) break;
         float mx = sm[0][0][rr], sum = 0.0f;
@@ -784,7 +798,7 @@ __global__ __launch_bounds__(256 * PW, NG > 4 ? 1 : 2) void kv_attn_many(const u
         for (int w = 0; w < PW; w++) {
             const float f = __builtin_amdgcn_exp2f(sm[w][0][rr] - mx);
             sum += sl[w][0][rr] * f;
-            v += *(const f4v *)(rowbuf + (w * 32 * RW + rr) * ROW + d1) * f;
+            v += *(const f4v *)(rowbuf + (w * 128 + rr) * ROW + d1) * f;
         }
         if (used > 1) {
             float *dst = A.part + (((size_t)kvh * rows + at) * A.splits + split) * (4 + WIDTH);
@@ -794,15 +808,7 @@ __global__ __launch_bounds__(256 * PW, NG > 4 ? 1 : 2) void kv_attn_many(const u
                 dst[1] = sum;
             }
         } else {
-            float *dst = out_row(A, kvh, at) + d1;
-            v *= 0.25f / sum;
-            if (A.out_wide) {
-                if (d1 < A.hd) *(f4v *)dst = v;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (d1 + e < A.hd) dst[e] = v[e];
-            }
+            put_row(A, kvh, at, d1, v * (0.25f / sum));
         }
     }
 }
@@ -873,9 +879,7 @@ __global__ __launch_bounds__(256) void kv_merge_k(const uint32_t *pos, AttnArgs 
                 sum += sl[g] * f;
                 v += so[g][cq] * f;
             }
-            float *dst = out_row(A, kvh, row);
-            for (int e = 0; e < 4; e++)
-                if (4 * c4 + e < A.hd) dst[4 * c4 + e] = v[e] * 0.25f / sum;
+            put_row(A, kvh, row, 4 * c4, v * (0.25f / sum));
         }
         __syncthreads();
     }
@@ -896,7 +900,6 @@ __global__ __launch_bounds__(256) void kv_merge_rows_k(const uint32_t *pos, Attn
     if (used == 1) return;
     const size_t rec = 4 + (size_t)width;
     const float *base = A.part + ((size_t)kvh * rows + row) * P.splits * rec;
-    float *dst = out_row(A, kvh, row);
     for (int c4 = threadIdx.x & 31; c4 < width / 4; c4 += 32) {
         float m = -FLT_MAX, l = 0.0f;
         f4v o = {0, 0, 0, 0};
@@ -924,8 +927,7 @@ __global__ __launch_bounds__(256) void kv_merge_rows_k(const uint32_t *pos, Attn
             }
             m = mn;
         }
-        for (int e = 0; e < 4; e++)
-            if (4 * c4 + e < A.hd) dst[4 * c4 + e] = o[e] * 0.25f / l;
+        put_row(A, kvh, row, 4 * c4, o * (0.25f / l));
     }
 }
 
@@ -964,7 +966,7 @@ static const void *many_kernel(int ng)
 // two at a time at 1.7 times one's time; tried are the fewest splits
 // that give the steps that w = 1..4 workgroups each can have.
 static int split_count(size_t items, size_t most, int n_cu, bool pairs, double way, double step, double merge,
-                          double records)
+                       double records)
 {
     size_t best = 1;
     double least = 0.0;
@@ -1000,6 +1002,9 @@ extern "C" fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, si
         return fox_fail(FOX_GPU_ERR_ARG, "kvq_attention: %zu heads over %zu kv heads", n_head,
                         n_head_kv);
     if (M > FOX_GPU_BATCH_TOKENS) return fox_fail(FOX_GPU_ERR_ARG, "kvq_attention: too many tokens");
+    // (65535 blocks of 32 rows in a launch; other widths go to kv_attn_many long before)
+    if (kvq_width((int)head_dim) == 192 && M * (n_head / n_head_kv) > 65535 * 32)
+        return fox_fail(FOX_GPU_ERR_ARG, "kvq_attention: %zu query rows a kv head", M * (n_head / n_head_kv));
     if (M > 1 && (q_stride < n_head * head_dim || out_stride < n_head * head_dim))
         return fox_fail(FOX_GPU_ERR_ARG, "kvq_attention: a stride below the row's width");
     if ((uintptr_t)cache % 16)
@@ -1026,7 +1031,7 @@ extern "C" fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, si
     const bool q4 = kv_type == FOX_GPU_KV_Q4;
     // Unpacking a tile once for 128 rows costs a long way in and out (a workgroup of
     // one tile 9 us against 4), so only long work pays for it: from 4.2e7 pairs of
-    // a row and a position on, and where the last 128 rows are not mostly empty.
+    // a row and a position on (1.6e7 of 256 dimensions), and where the last 128 rows are not mostly empty.
     // Heads of 128 dimensions, kv heads x rows x positions, in tiles by the wave and
     // unpacked once: 8 x 64 x 128 8.3 / 12.7 us, 8 x 4000 x 1024 38.1 / 38.2,
     // 8 x 4000 x 2500 88 / 79, 8 x 192 x 40000 79 / 88, 8 x 256 x 40000 97 / 91.

@@ -69,7 +69,8 @@ CALLS = {
     "attention": ("fox_gpu_kvq_attention", ATTN, SHAPE + [
         (dict(ctx=None), ARG), (dict(o=None), ARG), (dict(q=None), ARG), (dict(cache=None), ARG),
         (dict(pos=None), ARG), (dict(nh=0), ARG), (dict(nh=5), ARG), (dict(M=0), ARG),
-        (dict(M=1025), ARG), (dict(qs=255), ARG), (dict(os=255), ARG), (dict(cache=P + 8), ARG)]),
+        (dict(M=1025), ARG), (dict(qs=255), ARG), (dict(os=255), ARG), (dict(cache=P + 8), ARG),
+        (dict(hd=192, nkv=1, nh=65535, M=33, qs=1 << 24, os=1 << 24), ARG)]),
 }
 
 
