@@ -333,8 +333,11 @@ struct Tile {
 // instructions a value, reads 4.9 TB/s (60,000 positions, 29.4 us with both launches).
 // Reading two tiles ahead is slower (39.4 us for 36.5), as is one copy of the loop's
 // body that reads past its last tile (8.4 -> 8.8 us at 1500 positions).
-// Short contexts are a launch and 2 to 4 us: 34 positions of 6 heads 4.4 us in all.
-template <int BITS, int NG, int ROWS>
+// Short contexts are a launch and 2 to 4 us: 34 positions of 6 heads 3.8 to 4.5 us in all.
+// ONE: a single split, whose first tiles are read before the position is known (that row
+// at 300 positions 6.7 -> 6.3 us; with more splits most such reads would be for nothing
+// where a long cache is not full: 8.1 -> 8.7 us at 1000 of 32768 positions).
+template <int BITS, int NG, int ROWS, bool ONE>
 __global__ __launch_bounds__(64 * KA_WAVES, NG > 4 ? 1 : 2) void kv_attn_few(const uint32_t *pos, AttnArgs A)
 {
     constexpr bool PACK = ROWS == 8;
@@ -362,6 +365,15 @@ __global__ __launch_bounds__(64 * KA_WAVES, NG > 4 ? 1 : 2) void kv_attn_few(con
             *(float4 *)(x[t][u] + 4) = query_quad(qr, 8 * (NG * c + j) + 4, A);
         }
     }
+    const int recs = (A.n_ctx + KVQ_TILE - 1) / KVQ_TILE;
+    constexpr int REC = 2 * (KVQ_TILE * WIDTH * BITS / 8 + KVQ_TILE * NG);
+    const uint8_t *base = A.cache + (size_t)kvh * recs * REC;
+    int tile = split * KA_WAVES + wave;
+    Tile<BITS, NG> cur;
+    if (ONE) {
+        cur.load_k(base + (size_t)min(tile, recs - 1) * REC, lane);
+        cur.load_v(base + (size_t)min(tile, recs - 1) * REC, lane);
+    }
     const size_t p0 = pos[0];
     auto end_of = [&](int row) { return (int)min(p0 + (size_t)token_of(A, row) + 1, (size_t)A.n_ctx); };
     const int last = end_of(min(row0 + ROWS, rows) - 1);         // positions any row sees
@@ -369,13 +381,7 @@ __global__ __launch_bounds__(64 * KA_WAVES, NG > 4 ? 1 : 2) void kv_attn_few(con
     const int n_tiles = (last + KVQ_TILE - 1) / KVQ_TILE, step = A.splits * KA_WAVES;
     if (split * KA_WAVES >= n_tiles || seen_of(A, p0) >= A.from) return;   // (uniform)
     const int used = min(A.splits, (n_tiles + KA_WAVES - 1) / KA_WAVES);
-    const size_t recs = (A.n_ctx + KVQ_TILE - 1) / KVQ_TILE;
-    constexpr int REC = 2 * (KVQ_TILE * WIDTH * BITS / 8 + KVQ_TILE * NG);
-    const uint8_t *base = A.cache + (size_t)kvh * recs * REC;
-
-    int tile = split * KA_WAVES + wave;
-    Tile<BITS, NG> cur;
-    if (tile < n_tiles) {
+    if (!ONE && tile < n_tiles) {
         cur.load_k(base + (size_t)tile * REC, lane);
         cur.load_v(base + (size_t)tile * REC, lane);
     }
@@ -931,19 +937,19 @@ __global__ __launch_bounds__(256) void kv_merge_rows_k(const uint32_t *pos, Attn
     }
 }
 
-template <int BITS>
+template <int BITS, bool ONE>
 static const void *few_kernel(int ng, int per)
 {
 #define FOX_FEW(n)                                                                     \
-    (per == 8 ? (const void *)kv_attn_few<BITS, n, 8>                                  \
-              : per == 16 ? (const void *)kv_attn_few<BITS, n, 16> : (const void *)kv_attn_few<BITS, n, 32>)
+    (per == 8 ? (const void *)kv_attn_few<BITS, n, 8, ONE>                                  \
+              : per == 16 ? (const void *)kv_attn_few<BITS, n, 16, ONE> : (const void *)kv_attn_few<BITS, n, 32, ONE>)
     switch (ng) {
     case 1: return FOX_FEW(1);
     case 2: return FOX_FEW(2);
     case 3: return FOX_FEW(3);
     case 4: return FOX_FEW(4);
     case 6: return FOX_FEW(6);
-    default: return per == 8 ? (const void *)kv_attn_few<BITS, 8, 8> : (const void *)kv_attn_few<BITS, 8, 16>;
+    default: return per == 8 ? (const void *)kv_attn_few<BITS, 8, 8, ONE> : (const void *)kv_attn_few<BITS, 8, 16, ONE>;
     }
 #undef FOX_FEW
 }
@@ -1065,10 +1071,12 @@ extern "C" fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, si
     }
     void *args[] = {(void *)&pos, &A};
     A.splits = few_parts.splits;
-    if (few)
-        FOX_HIP(hipLaunchKernel(q4 ? few_kernel<4>(ng, (int)per) : few_kernel<8>(ng, (int)per),
-                                dim3((unsigned)few_parts.splits, (unsigned)n_head_kv, (unsigned)few_blocks),
+    if (few) {
+        const void *k = A.splits == 1 ? q4 ? few_kernel<4, true>(ng, (int)per) : few_kernel<8, true>(ng, (int)per)
+                                      : q4 ? few_kernel<4, false>(ng, (int)per) : few_kernel<8, false>(ng, (int)per);
+        FOX_HIP(hipLaunchKernel(k, dim3((unsigned)few_parts.splits, (unsigned)n_head_kv, (unsigned)few_blocks),
                                 dim3(64 * KA_WAVES), args, 0, ctx->stream));
+    }
     if (many) {
         A.splits = many_parts.splits;
         const void *k = q4 ? many_kernel<4>(ng) : many_kernel<8>(ng);
