@@ -966,16 +966,21 @@ static const void *many_kernel(int ng)
     }
 }
 
-// Into how many splits of `most` side-by-side steps at most each item's positions go, by the
-// microseconds (as measured) of a workgroup's way in and out, of a step of it, of the
-// merge and of a split's records.  A compute unit takes w workgroups one after another, or
-// two at a time at 1.7 times one's time; tried are the fewest splits
-// that give the steps that w = 1..4 workgroups each can have.
-static int split_count(size_t items, size_t most, int n_cu, bool pairs, double way, double step, double merge,
-                       double records)
+// What a workgroup costs, in microseconds as measured: its way in and out, a step
+// (its waves' next tiles), the merge behind it and a split's records; pairs: two share a
+// compute unit, in 1.2 times one's way and 1.7 times its steps.
+struct Cost {
+    double way, step, merge, record;
+    bool pairs;
+};
+
+// Into how many splits of `most` steps at most each item's positions go: the
+// fewest that give the steps that 1..4 workgroups a compute unit can have, or one.  A
+// call's time is its longest workgroup's or a compute unit's share, whose
+// rows see `share` of the positions on average.
+static int split_count(size_t items, size_t most, int n_cu, double share, const Cost &c, double &least)
 {
     size_t best = 1;
-    double least = 0.0;
     for (int w = 0; w <= 4; w++) {                               // (w = 0: one split)
         size_t s = w ? w * (size_t)n_cu / items : 1;
         if (s > most) s = most;
@@ -983,9 +988,11 @@ static int split_count(size_t items, size_t most, int n_cu, bool pairs, double w
         const size_t steps = (most + s - 1) / s;
         s = (most + steps - 1) / steps;
         const size_t load = (items * s + n_cu - 1) / n_cu;
-        const double us = (pairs ? 1.7 * (double)(load / 2) + (double)(load % 2) : (double)load) *
-                              (way + step * (double)steps) +
-                          (s > 1 ? merge + records * (double)s : 0.0);
+        const double longest = c.step * (double)steps, mean = longest * share;
+        double us = c.pairs ? (double)(load / 2) * (1.2 * c.way + 1.7 * mean) + (double)(load % 2) * (c.way + mean)
+                            : (double)load * (c.way + mean);
+        if (us < c.way + longest) us = c.way + longest;
+        if (s > 1) us += c.merge + c.record * (double)s;
         if (w == 0 || us < least) {
             least = us;
             best = s;
@@ -1045,24 +1052,41 @@ extern "C" fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, si
     // 2500 57 / 60, 16 x 96 x 16000 110 / 107, 4 x 768 x 16000 254 / 143.  Of 192, never
     // (4 x 6000 x 16000 675 / 716).  Where the position decides, both are launched
     // and the one that it is not for ends at once (2 us).
-    const size_t per = rows <= 8 ? 8 : rows <= 16 || ng > 6 ? 16 : 32, turns = ng > 4 ? 1 : 2;
-    const bool wide = ng != 6 && 2 * ((rows + per - 1) / per) > (ng > 6 ? 10 : 7) * ((rows + 127) / 128);
+    const size_t most_per = ng > 6 ? 16 : 32, turns = ng > 4 ? 1 : 2, many_blocks = (rows + 127) / 128;
+    const bool wide = ng != 6 && 2 * ((rows + most_per - 1) / most_per) > (ng > 6 ? 10 : 7) * many_blocks;
     const double from = (ng > 6 ? 1.6e7 : 4.2e7) / ((double)rows * (double)n_head_kv);
     A.from = wide && from < (double)n_ctx ? (int)from + 1 : INT_MAX;
     const bool many = A.from <= (int64_t)n_ctx, few = A.from > (int64_t)M;   // (a call has M positions at least)
     Parts few_parts = {}, many_parts = {};
     const double record = 1e-6 * (double)(rows * n_head_kv) * (4 + width) * sizeof(float);   // MB of a split's
-    const size_t few_blocks = (rows + per - 1) / per, many_blocks = (rows + 127) / 128;
+    double us, least = 0.0;
+    size_t few_blocks = 0;
     if (few) {
+        // Rows of a workgroup, 8, 16 or 32: more of them share a tile's unpacking, but a
+        // short call waits longer for one.  Whole calls, 16 / 32 rows (heads of
+        // 128): 12 tokens of 32 heads over 8 at 100 positions 4.9 / 7.0 us, 31 at 1000
+        // 11.1 / 13.5, at 9000 24.4 / 22.6, a prompt of 200 7.4 / 9.0, of 500 16.6 / 14.0.
         const size_t n = A.from < (int64_t)n_ctx ? (size_t)A.from : n_ctx;
-        few_parts = {split_count(n_head_kv * few_blocks, (n + KVQ_TILE * KA_WAVES - 1) / (KVQ_TILE * KA_WAVES), ctx->n_cu,
-                             ng <= 4, 0.45 * ng, per == 32 ? 0.35 + 0.19 * ng : 0.2 + 0.18 * ng, 1.9, 0.5 * record),
-                 (int)per, KA_WAVES};
+        const double share = M < n ? 1.0 - 0.5 * (double)M / (double)n : 0.5;
+        for (size_t per = 8; per <= most_per && (per == 8 || rows > per / 2); per *= 2) {
+            const Cost c = {per == 32 ? 0.3 + 0.9 * ng : per == 16 ? 0.4 + 0.42 * ng : 0.2 + 0.4 * ng,
+                            per == 32 ? 0.35 + 0.19 * ng : 0.2 + 0.18 * ng, 1.9, 0.5 * record, ng <= 4};
+            const size_t blocks = (rows + per - 1) / per;
+            if (blocks > 65535) continue;                        // (a launch's third dimension)
+            const int s = split_count(n_head_kv * blocks, (n + KVQ_TILE * KA_WAVES - 1) / (KVQ_TILE * KA_WAVES),
+                                      ctx->n_cu, share, c, us);
+            if (few_blocks && us >= least) continue;
+            least = us;
+            few_blocks = blocks;
+            few_parts = {s, (int)per, KA_WAVES};
+        }
     }
-    if (many)
-        many_parts = {split_count(n_head_kv * many_blocks, (n_ctx + KVQ_TILE * turns - 1) / (KVQ_TILE * turns), ctx->n_cu,
-                              false, 8.0, 1.65, 5.0, record),
-                  128, (int)turns};
+    if (many) {
+        const Cost c = {8.0, 1.65, 5.0, record, false};
+        many_parts = {split_count(n_head_kv * many_blocks, (n_ctx + KVQ_TILE * turns - 1) / (KVQ_TILE * turns),
+                                  ctx->n_cu, 1.0, c, us),
+                      128, (int)turns};
+    }
     const int splits = few_parts.splits > many_parts.splits ? few_parts.splits : many_parts.splits;
     if (splits > 1) {
         st = fox_ws_reserve(ctx, n_head_kv * rows * splits * (4 + (size_t)width) * sizeof(float));
@@ -1072,8 +1096,8 @@ extern "C" fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, si
     void *args[] = {(void *)&pos, &A};
     A.splits = few_parts.splits;
     if (few) {
-        const void *k = A.splits == 1 ? q4 ? few_kernel<4, true>(ng, (int)per) : few_kernel<8, true>(ng, (int)per)
-                                      : q4 ? few_kernel<4, false>(ng, (int)per) : few_kernel<8, false>(ng, (int)per);
+        const void *k = A.splits == 1 ? q4 ? few_kernel<4, true>(ng, few_parts.rows) : few_kernel<8, true>(ng, few_parts.rows)
+                                      : q4 ? few_kernel<4, false>(ng, few_parts.rows) : few_kernel<8, false>(ng, few_parts.rows);
         FOX_HIP(hipLaunchKernel(k, dim3((unsigned)few_parts.splits, (unsigned)n_head_kv, (unsigned)few_blocks),
                                 dim3(64 * KA_WAVES), args, 0, ctx->stream));
     }
@@ -1087,7 +1111,9 @@ extern "C" fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, si
                                 lds, ctx->stream));
     }
     if (splits > 1) {
-        const bool by_rows = splits <= 16 && rows * n_head_kv >= 1024, either = few && many;
+        // a workgroup a row or eight rows: whole calls of 512 rows 18.2 / 19.9 us, of
+        // 992 14.0 / 13.5 and 23.0 / 22.5
+        const bool by_rows = splits <= 16 && rows * n_head_kv >= 800, either = few && many;
         if (!few) few_parts = many_parts;
         const void *k = by_rows ? either ? (const void *)kv_merge_rows_k<true> : (const void *)kv_merge_rows_k<false>
                                 : either ? (const void *)kv_merge_k<true> : (const void *)kv_merge_k<false>;

@@ -419,7 +419,34 @@ def test_long_work(gpu, bits, case):
                150 if n < 20000 else 20)
 
 
-@pytest.mark.parametrize("n_head,hd,pos", [(640, 64, 300), (260, 256, 300)])
+DIVISIONS = [  # n_head, n_kv, hd, n_ctx, pos, M: 8, 16 or 32 rows of a workgroup, or 128, in one or several splits, by width
+    (1, 1, 24, 776, 775, 1), (66, 2, 24, 74, 11, 33), (5, 1, 24, 828, 766, 61), (64, 1, 24, 1956, 1909, 17),
+    (64, 1, 32, 2671, 2420, 250), (64, 1, 48, 54, 14, 33), (64, 1, 64, 180, 30, 150), (2, 1, 80, 390, 355, 5),
+    (128, 2, 80, 50, 26, 17), (500, 1, 80, 1603, 1599, 3), (500, 1, 96, 5022, 5004, 17),
+    (64, 1, 112, 44, 10, 33), (16, 1, 126, 1289, 1159, 130), (16, 1, 128, 350, 200, 150),
+    (64, 1, 128, 250, 100, 150), (64, 1, 150, 50, 10, 33), (16, 1, 160, 392, 359, 33),
+    (128, 2, 192, 43, 10, 33), (8, 1, 150, 2337, 2177, 130), (1, 1, 200, 70, 39, 1), (16, 1, 256, 350, 200, 150),
+    (120, 1, 200, 1036, 876, 130),
+]
+
+
+@pytest.mark.parametrize("case", DIVISIONS, ids=str)
+@pytest.mark.parametrize("pad", [0, 3])
+@pytest.mark.parametrize("bits", BITS)
+def test_rows_divided(gpu, bits, pad, case):
+    n_head, n_kv, hd, n_ctx, pos, M = case
+    rng = np.random.default_rng(pos + hd)
+    n = pos + M
+    K, V = (rng.standard_normal((n, n_kv * hd), np.float32) for _ in range(2))
+    q = (1.5 * rng.standard_normal((M, n_head * hd), np.float32)).astype(np.float32)
+    c = fill(gpu, bits, n_ctx, n_kv, hd, K, V)               # (rows past n stay poisoned)
+    got = attend(gpu, bits, c, q, n_head, n_kv, hd, n_ctx, pos, pad=pad)
+    check_some(got, q, kr.held(K, bits, hd), kr.held(V, bits, hd), n_head, n_kv, hd, pos, n_ctx, rng, 60)
+
+
+@pytest.mark.parametrize("n_head,hd,pos", [(640, 64, 300), (260, 256, 300), (16, 64, 100), (64, 64, 30),
+                                           (16, 128, 200), (64, 128, 100), (16, 192, 100), (32, 192, 200),
+                                           (16, 256, 200)])
 @pytest.mark.parametrize("side", ["k", "v", "q"])
 @pytest.mark.parametrize("bits", BITS)
 def test_a_nan_in_long_work(gpu, bits, side, n_head, hd, pos):
@@ -432,8 +459,8 @@ def test_a_nan_in_long_work(gpu, bits, side, n_head, hd, pos):
     q = rng.standard_normal((M, n_head * hd)).astype(np.float32)
     hit = np.zeros((M, n_head, hd), bool)
     if side == "q":
-        q[j, 7 * hd + 3], q[j, 30 * hd] = np.nan, np.inf
-        hit[j, 7] = hit[j, 30] = True
+        q[j, 7 * hd + 3], q[j, 11 * hd] = np.nan, np.inf
+        hit[j, 7] = hit[j, 11] = True
     else:
         (K if side == "k" else V)[pos + j, 40] = np.nan      # the second group
         hit[j:, :, slice(None) if side == "k" else slice(32, 64)] = True
