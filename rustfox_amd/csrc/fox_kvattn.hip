@@ -1043,18 +1043,19 @@ extern "C" fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, si
     const size_t rows = M * (size_t)A.G;
     const bool q4 = kv_type == FOX_GPU_KV_Q4;
     // Unpacking a tile once for 128 rows costs a long way in and out (a workgroup of
-    // one tile 9 us against 4), so only long work pays for it: from 4.2e7 pairs of
-    // a row and a position on (1.6e7 of 256 dimensions), and where the last 128 rows are not mostly empty.
-    // Heads of 128 dimensions, kv heads x rows x positions, in tiles by the wave and
-    // unpacked once: 8 x 64 x 128 8.3 / 12.7 us, 8 x 4000 x 1024 38.1 / 38.2,
-    // 8 x 4000 x 2500 88 / 79, 8 x 192 x 40000 79 / 88, 8 x 256 x 40000 97 / 91.
-    // Heads of 256, where a wave holds 16 rows: 4 x 192 x 2500 30 / 47, 4 x 768 x
-    // 2500 57 / 60, 16 x 96 x 16000 110 / 107, 4 x 768 x 16000 254 / 143.  Of 192, never
-    // (4 x 6000 x 16000 675 / 716).  Where the position decides, both are launched
-    // and the one that it is not for ends at once (2 us).
+    // one tile 9 us against 2 to 6), so only long work pays for it: from 9e7 pairs
+    // of a row and a position on (2e7 of 256 dimensions, where a wave holds 16 rows), and
+    // where the last 128 rows are not mostly empty.  In tiles by the wave and unpacked
+    // once, kv heads x rows x positions, of 128 dimensions: 8 x 4000 x 1500 47 / 52 us,
+    // 8 x 4000 x 2500 80 / 80, 8 x 4000 x 6000 197 / 183, 8 x 3108 x 8777 279 / 224,
+    // 8 x 192 x 40000 79 / 88, 8 x 512 x 40000 181 / 164; of 64: 2 x 4000 x 6000 38 / 38,
+    // 2 x 4096 x 16000 87 / 79; of 256: 16 x 1024 x 1024 76 / 97, 16 x 512 x 2500
+    // 87 / 80, 4 x 384 x 16000 114 / 89.  Of 192, never (4 x 6000 x 16000 675 / 716).
+    // Where the position decides, both are launched and the one that it is not for
+    // ends at once (2 us).
     const size_t most_per = ng > 6 ? 16 : 32, turns = ng > 4 ? 1 : 2, many_blocks = (rows + 127) / 128;
     const bool wide = ng != 6 && 2 * ((rows + most_per - 1) / most_per) > (ng > 6 ? 10 : 7) * many_blocks;
-    const double from = (ng > 6 ? 1.6e7 : 4.2e7) / ((double)rows * (double)n_head_kv);
+    const double from = (ng > 6 ? 2e7 : 9e7) / ((double)rows * (double)n_head_kv);
     A.from = wide && from < (double)n_ctx ? (int)from + 1 : INT_MAX;
     const bool many = A.from <= (int64_t)n_ctx, few = A.from > (int64_t)M;   // (a call has M positions at least)
     Parts few_parts = {}, many_parts = {};

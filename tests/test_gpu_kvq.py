@@ -380,15 +380,17 @@ def test_small_and_large_values(gpu):
             check(got, q, kr.held(K, bits, hd), kr.held(V, bits, hd), n_head, n_kv, hd, n_ctx - 1, n_ctx)
 
 
-LONG_WORK = [  # n_head, n_kv, hd, n_ctx, pos, M: 4.2e7 pairs of a row and a position (1.6e7 of 256 dimensions)
-    (1100, 1, 32, 520, 310, 100), (1100, 1, 32, 520, 100, 100),     # past them, and below in the same cache
-    (512, 1, 64, 700, 500, 192), (520, 1, 90, 930, 800, 101), (512, 2, 128, 1200, 1000, 100),
-    (130, 1, 256, 1300, 1200, 101), (130, 1, 256, 1300, 900, 101), (65, 1, 250, 1290, 1200, 200),
+LONG_WORK = [  # n_head, n_kv, hd, n_ctx, pos, M: 9e7 pairs of a row and a position (2e7 of 256 dimensions)
+    (2200, 1, 32, 520, 310, 100), (2200, 1, 32, 520, 100, 100),     # past them, and below in the same cache
+    (512, 1, 64, 1100, 900, 192), (1000, 1, 90, 930, 800, 101), (512, 1, 128, 1850, 1750, 100),
+    (170, 1, 256, 1300, 1200, 101), (170, 1, 256, 1300, 900, 101), (90, 1, 250, 1290, 1200, 200),
     (300, 1, 48, 900, 0, 900),                                      # as many tokens as positions
-    (300, 1, 64, 800, 700, 200),                                    # and tokens past them
-    (128, 1, 64, 400_000, 350_000, 1), (128, 1, 256, 40_000, 33_000, 4),   # few rows, split many ways
-    (128, 1, 64, 400_000, 300_000, 1), (128, 1, 256, 40_000, 30_000, 4), (128, 1, 64, 400_000, 77, 1),
-    (128, 2, 128, 9000, 8000, 60),
+    (600, 1, 64, 800, 700, 200),                                    # and tokens past them
+    (256, 1, 64, 400_000, 360_000, 1), (128, 1, 256, 40_000, 39_500, 4),   # few rows, split many ways
+    (256, 1, 64, 400_000, 300_000, 1), (128, 1, 256, 40_000, 30_000, 4), (256, 1, 64, 400_000, 77, 1),
+    (128, 2, 128, 13000, 12000, 60), (500, 1, 96, 10700, 10640, 17), (64, 1, 32, 5700, 5450, 250),
+    (1100, 1, 32, 520, 310, 100), (520, 1, 90, 930, 800, 101), (300, 1, 64, 800, 700, 200),
+    (130, 1, 256, 1300, 1200, 101), (128, 1, 64, 400_000, 350_000, 1), (128, 2, 128, 9000, 8000, 60),
 ]
 
 
@@ -426,7 +428,7 @@ DIVISIONS = [  # n_head, n_kv, hd, n_ctx, pos, M: 8, 16 or 32 rows of a workgrou
     (64, 1, 112, 44, 10, 33), (16, 1, 126, 1289, 1159, 130), (16, 1, 128, 350, 200, 150),
     (64, 1, 128, 250, 100, 150), (64, 1, 150, 50, 10, 33), (16, 1, 160, 392, 359, 33),
     (128, 2, 192, 43, 10, 33), (8, 1, 150, 2337, 2177, 130), (1, 1, 200, 70, 39, 1), (16, 1, 256, 350, 200, 150),
-    (120, 1, 200, 1036, 876, 130),
+    (120, 1, 200, 1036, 876, 130), (160, 1, 200, 1036, 876, 130),
 ]
 
 
@@ -444,7 +446,7 @@ def test_rows_divided(gpu, bits, pad, case):
     check_some(got, q, kr.held(K, bits, hd), kr.held(V, bits, hd), n_head, n_kv, hd, pos, n_ctx, rng, 60)
 
 
-@pytest.mark.parametrize("n_head,hd,pos", [(640, 64, 300), (260, 256, 300), (16, 64, 100), (64, 64, 30),
+@pytest.mark.parametrize("n_head,hd,pos", [(1340, 64, 300), (330, 256, 300), (640, 64, 300), (260, 256, 300), (16, 64, 100), (64, 64, 30),
                                            (16, 128, 200), (64, 128, 100), (16, 192, 100), (32, 192, 200),
                                            (16, 256, 200)])
 @pytest.mark.parametrize("side", ["k", "v", "q"])
@@ -472,7 +474,7 @@ def test_a_nan_in_long_work(gpu, bits, side, n_head, hd, pos):
 def test_long_work_captured(gpu):
     """One capture serves positions on both sides of where long work begins: each replay against the
     eager call, bit for bit, and against the plain one."""
-    n_head, n_kv, hd, n_ctx, M = 512, 1, 64, 900, 100
+    n_head, n_kv, hd, n_ctx, M = 1100, 1, 64, 900, 100      # (from 819 positions on)
     rng = np.random.default_rng(5)
     K, V = rows(rng, n_ctx, hd), rows(rng, n_ctx, hd)
     Kh, Vh = kr.held(K, 4, hd), kr.held(V, 4, hd)
