@@ -1067,11 +1067,16 @@ extern "C" fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, si
         // short call waits longer for one.  Whole calls, 16 / 32 rows (heads of
         // 128): 12 tokens of 32 heads over 8 at 100 positions 4.9 / 7.0 us, 31 at 1000
         // 11.1 / 13.5, at 9000 24.4 / 22.6, a prompt of 200 7.4 / 9.0, of 500 16.6 / 14.0.
+        // Records cost 0.5 us a MB, at any position, where a split gains at long ones only, so
+        // they count four times: 200 tokens at 700 of 32768 positions 29.9 -> 22.1 us,
+        // of 5000 20.4 -> 16.9; at 9000 of 9100, 100 tokens, 47.0 -> 50.5.  (Not of more
+        // dimensions, where a step is longer: 200 at 2000 of 2200 68.7 -> 76.3.)
         const size_t n = A.from < (int64_t)n_ctx ? (size_t)A.from : n_ctx;
         const double share = M < n ? 1.0 - 0.5 * (double)M / (double)n : 0.5;
         for (size_t per = 8; per <= most_per && (per == 8 || rows > per / 2); per *= 2) {
             const Cost c = {per == 32 ? 0.3 + 0.9 * ng : per == 16 ? 0.4 + 0.42 * ng : 0.2 + 0.4 * ng,
-                            per == 32 ? 0.35 + 0.19 * ng : 0.2 + 0.18 * ng, 1.9, 0.5 * record, ng <= 4};
+                            per == 32 ? 0.35 + 0.19 * ng : 0.2 + 0.18 * ng, 1.9,
+                            (ng > 4 ? 0.5 : 2.0) * record, ng <= 4};
             const size_t blocks = (rows + per - 1) / per;
             if (blocks > 65535) continue;                        // (a launch's third dimension)
             const int s = split_count(n_head_kv * blocks, (n + KVQ_TILE * KA_WAVES - 1) / (KVQ_TILE * KA_WAVES),
