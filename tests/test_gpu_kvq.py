@@ -428,7 +428,7 @@ DIVISIONS = [  # n_head, n_kv, hd, n_ctx, pos, M: 8, 16 or 32 rows of a workgrou
     (64, 1, 112, 44, 10, 33), (16, 1, 126, 1289, 1159, 130), (16, 1, 128, 350, 200, 150),
     (64, 1, 128, 250, 100, 150), (64, 1, 150, 50, 10, 33), (16, 1, 160, 392, 359, 33),
     (128, 2, 192, 43, 10, 33), (8, 1, 150, 2337, 2177, 130), (1, 1, 200, 70, 39, 1), (16, 1, 256, 350, 200, 150),
-    (120, 1, 200, 1036, 876, 130), (160, 1, 200, 1036, 876, 130),
+    (120, 1, 200, 1036, 876, 130), (160, 1, 200, 1036, 876, 130),    (6, 2, 24, 2831, 2581, 250), (33, 1, 80, 926, 879, 17), (16, 1, 112, 2485, 2354, 130),
 ]
 
 
