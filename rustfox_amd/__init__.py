@@ -58,6 +58,8 @@ def probe_lib() -> C.CDLL:
         L.fox_gpu_read_probe.argtypes = [vp, vp, sz, C.c_int, C.c_int, vp]
         L.fox_gpu_empty_probe.argtypes = [vp, C.c_int, vp]
         L.fox_gpu_sum_probe.argtypes = [vp, vp, C.c_int, C.c_float, vp]
+        L.fox_gpu_kvq_plan_probe.argtypes = [sz, sz, sz, sz, sz, C.c_int, vp]
+        L.fox_gpu_kvq_plan_probe.restype = None
         _probe = L
     return _probe
 

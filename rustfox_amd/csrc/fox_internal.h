@@ -200,3 +200,16 @@ fox_gpu_status fox_few_gemv(fox_gpu_ctx *ctx, size_t n, const fox_gpu_tensor *co
 // the shapes quantised caches take (fox_kvq.hip); `what` names the caller in the message
 fox_gpu_status fox_kvq_shape(const char *what, int kv_type, size_t n_ctx, size_t n_head_kv,
                              size_t head_dim);
+
+// How attention over a quantised cache is launched (fox_kvattn.hip): a kernel's
+// rows and positions as they are divided, and which of the two kernels run.
+struct KvqParts {
+    int splits, rows, tiles;      // splits of the positions; rows of a workgroup, tiles it takes side by side
+};
+struct KvqPlan {
+    int from;                     // positions from which kv_attn_many takes the call, kv_attn_few below
+    bool few, many;               // the kernels that are launched
+    size_t few_blocks, many_blocks;   // of rows
+    KvqParts few_parts, many_parts;
+};
+KvqPlan fox_kvq_plan(size_t head_dim, size_t n_head, size_t n_head_kv, size_t M, size_t n_ctx, int n_cu);

@@ -34,11 +34,6 @@ typedef uint32_t u4v __attribute__((ext_vector_type(4)));
 #define KA_ROOM 8.0f            // how far scores may pass the running maximum
 #define KA_LIFT 7.0f            // weights are scaled by 2^7: 2^(8 + 7) is within a half
 
-// how a kernel's rows and positions are divided
-struct Parts {
-    int splits, rows, tiles;      // splits of the positions; rows of a workgroup, tiles it takes side by side
-};
-
 struct AttnArgs {
     float *out, *part;
     size_t out_stride, q_stride;
@@ -823,7 +818,7 @@ __global__ __launch_bounds__(256 * PW, NG > 4 ? 1 : 2) void kv_attn_many(const u
 // maximum.  32 threads to a column quad's splits, eight split groups.  (EITHER: both
 // kernels were launched; otherwise the position is not waited for.)
 template <bool EITHER>
-__global__ __launch_bounds__(256) void kv_merge_k(const uint32_t *pos, AttnArgs A, int width, Parts few, Parts many)
+__global__ __launch_bounds__(256) void kv_merge_k(const uint32_t *pos, AttnArgs A, int width, KvqParts few, KvqParts many)
 {
     __shared__ float sm[8], sl[8];
     __shared__ f4v so[8][32];
@@ -832,7 +827,7 @@ __global__ __launch_bounds__(256) void kv_merge_k(const uint32_t *pos, AttnArgs 
     const size_t rec = 4 + (size_t)width;
     // the splits that hold this row: of its block of P.rows rows, P.tiles tiles
     // of a split at a time
-    const Parts P = EITHER && seen_of(A, pos[0]) >= A.from ? many : few;
+    const KvqParts P = EITHER && seen_of(A, pos[0]) >= A.from ? many : few;
     const float *base = A.part + ((size_t)kvh * rows + row) * P.splits * rec;
     const int row_last = min(row / P.rows * P.rows + P.rows, rows) - 1;
     const int last = (int)min((size_t)pos[0] + (size_t)token_of(A, row_last) + 1, (size_t)A.n_ctx);
@@ -894,11 +889,11 @@ __global__ __launch_bounds__(256) void kv_merge_k(const uint32_t *pos, AttnArgs 
 // The same for up to 16 splits: 32 threads to a row, eight rows to a workgroup,
 // a column quad's records read together.
 template <bool EITHER>
-__global__ __launch_bounds__(256) void kv_merge_rows_k(const uint32_t *pos, AttnArgs A, int width, Parts few, Parts many)
+__global__ __launch_bounds__(256) void kv_merge_rows_k(const uint32_t *pos, AttnArgs A, int width, KvqParts few, KvqParts many)
 {
     const int rows = A.M * A.G, row = blockIdx.x * 8 + (threadIdx.x >> 5), kvh = blockIdx.y;
     if (row >= rows) return;
-    const Parts P = EITHER && seen_of(A, pos[0]) >= A.from ? many : few;
+    const KvqParts P = EITHER && seen_of(A, pos[0]) >= A.from ? many : few;
     const int row_last = min(row / P.rows * P.rows + P.rows, rows) - 1;
     const int last = (int)min((size_t)pos[0] + (size_t)token_of(A, row_last) + 1, (size_t)A.n_ctx);
     const int n_tiles = (last + KVQ_TILE - 1) / KVQ_TILE;
@@ -1001,6 +996,68 @@ static int split_count(size_t items, size_t most, int n_cu, double share, const 
     return (int)best;
 }
 
+// Which kernels a call launches, and how it is divided: a choice by sizes alone.
+KvqPlan fox_kvq_plan(size_t head_dim, size_t n_head, size_t n_head_kv, size_t M, size_t n_ctx, int n_cu)
+{
+    KvqPlan p = {};
+    const int width = kvq_width((int)head_dim), ng = width / 32;
+    const size_t rows = M * (n_head / n_head_kv);
+    // Unpacking a tile once for 128 rows costs a long way in and out (a workgroup of
+    // one tile 9 us against 2 to 6), so only long work pays for it: from 9e7 pairs
+    // of a row and a position on (2e7 of 256 dimensions, where a wave holds 16 rows), and
+    // where the last 128 rows are not mostly empty.  In tiles by the wave and unpacked
+    // once, kv heads x rows x positions, of 128 dimensions: 8 x 4000 x 1500 47 / 52 us,
+    // 8 x 4000 x 2500 80 / 80, 8 x 4000 x 6000 197 / 183, 8 x 3108 x 8777 279 / 224,
+    // 8 x 192 x 40000 79 / 88, 8 x 512 x 40000 181 / 164; of 64: 2 x 4000 x 6000 38 / 38,
+    // 2 x 4096 x 16000 87 / 79; of 256: 16 x 1024 x 1024 76 / 97, 16 x 512 x 2500
+    // 87 / 80, 4 x 384 x 16000 114 / 89.  Of 192, never (4 x 6000 x 16000 675 / 716).
+    // Where the position decides, both are launched and the one that it is not for
+    // ends at once (2 us).  More rows than 65535 blocks of a wave's (a launch's third
+    // dimension) go to kv_attn_many at any position.
+    const size_t most_per = ng > 6 ? 16 : 32, turns = ng > 4 ? 1 : 2, many_blocks = (rows + 127) / 128;
+    const bool wide = ng != 6 && 2 * ((rows + most_per - 1) / most_per) > (ng > 6 ? 10 : 7) * many_blocks;
+    const double from = (ng > 6 ? 2e7 : 9e7) / ((double)rows * (double)n_head_kv);
+    const bool fits = (rows + most_per - 1) / most_per <= 65535;
+    p.from = !fits ? 0 : wide && from < (double)n_ctx ? (int)from + 1 : INT_MAX;
+    p.many = p.from <= (int64_t)n_ctx;
+    p.few = p.from > (int64_t)M;                                  // (a call has M positions at least)
+    const double record = 1e-6 * (double)(rows * n_head_kv) * (4 + width) * sizeof(float);   // MB of a split's
+    double us, least = 0.0;
+    if (p.few) {
+        // Rows of a workgroup, 8, 16 or 32: more of them share a tile's unpacking, but a
+        // short call waits longer for one.  Whole calls, 16 / 32 rows (heads of
+        // 128): 12 tokens of 32 heads over 8 at 100 positions 4.9 / 7.0 us, 31 at 1000
+        // 11.1 / 13.5, at 9000 24.4 / 22.6, a prompt of 200 7.4 / 9.0, of 500 16.6 / 14.0.
+        // Records cost 0.5 us a MB, at any position, where a split gains at long ones only, so
+        // they count four times: 200 tokens at 700 of 32768 positions 29.9 -> 22.1 us,
+        // of 5000 20.4 -> 16.9; at 9000 of 9100, 100 tokens, 47.0 -> 50.5.  (Not of more
+        // dimensions, where a step is longer: 200 at 2000 of 2200 68.7 -> 76.3.)
+        const size_t n = p.from < (int64_t)n_ctx ? (size_t)p.from : n_ctx;
+        const double share = M < n ? 1.0 - 0.5 * (double)M / (double)n : 0.5;
+        for (size_t per = 8; per <= most_per && (per == 8 || rows > per / 2); per *= 2) {
+            const Cost c = {per == 32 ? 0.3 + 0.9 * ng : per == 16 ? 0.4 + 0.42 * ng : 0.2 + 0.4 * ng,
+                            per == 32 ? 0.35 + 0.19 * ng : 0.2 + 0.18 * ng, 1.9,
+                            (ng > 4 ? 0.5 : 2.0) * record, ng <= 4};
+            const size_t blocks = (rows + per - 1) / per;
+            if (blocks > 65535) continue;                        // (more rows a workgroup fit)
+            const int s = split_count(n_head_kv * blocks, (n + KVQ_TILE * KA_WAVES - 1) / (KVQ_TILE * KA_WAVES),
+                                      n_cu, share, c, us);
+            if (p.few_blocks && us >= least) continue;
+            least = us;
+            p.few_blocks = blocks;
+            p.few_parts = {s, (int)per, KA_WAVES};
+        }
+    }
+    if (p.many) {
+        const Cost c = {8.0, 1.65, 5.0, record, false};
+        p.many_blocks = many_blocks;
+        p.many_parts = {split_count(n_head_kv * many_blocks, (n_ctx + KVQ_TILE * turns - 1) / (KVQ_TILE * turns),
+                                    n_cu, 1.0, c, us),
+                        128, (int)turns};
+    }
+    return p;
+}
+
 extern "C" fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, size_t out_stride,
                                                 const float *q, size_t q_stride, int kv_type,
                                                 const void *cache, size_t n_head, size_t n_head_kv,
@@ -1015,7 +1072,7 @@ extern "C" fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, si
         return fox_fail(FOX_GPU_ERR_ARG, "kvq_attention: %zu heads over %zu kv heads", n_head,
                         n_head_kv);
     if (M > FOX_GPU_BATCH_TOKENS) return fox_fail(FOX_GPU_ERR_ARG, "kvq_attention: too many tokens");
-    // (65535 blocks of 32 rows in a launch; other widths go to kv_attn_many long before)
+    // (65535 blocks of 32 rows in a launch; of other widths kv_attn_many takes them)
     if (kvq_width((int)head_dim) == 192 && M * (n_head / n_head_kv) > 65535 * 32)
         return fox_fail(FOX_GPU_ERR_ARG, "kvq_attention: %zu query rows a kv head", M * (n_head / n_head_kv));
     if (M > 1 && (q_stride < n_head * head_dim || out_stride < n_head * head_dim))
@@ -1042,88 +1099,40 @@ extern "C" fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, si
     const int width = kvq_width((int)head_dim), ng = width / 32;
     const size_t rows = M * (size_t)A.G;
     const bool q4 = kv_type == FOX_GPU_KV_Q4;
-    // Unpacking a tile once for 128 rows costs a long way in and out (a workgroup of
-    // one tile 9 us against 2 to 6), so only long work pays for it: from 9e7 pairs
-    // of a row and a position on (2e7 of 256 dimensions, where a wave holds 16 rows), and
-    // where the last 128 rows are not mostly empty.  In tiles by the wave and unpacked
-    // once, kv heads x rows x positions, of 128 dimensions: 8 x 4000 x 1500 47 / 52 us,
-    // 8 x 4000 x 2500 80 / 80, 8 x 4000 x 6000 197 / 183, 8 x 3108 x 8777 279 / 224,
-    // 8 x 192 x 40000 79 / 88, 8 x 512 x 40000 181 / 164; of 64: 2 x 4000 x 6000 38 / 38,
-    // 2 x 4096 x 16000 87 / 79; of 256: 16 x 1024 x 1024 76 / 97, 16 x 512 x 2500
-    // 87 / 80, 4 x 384 x 16000 114 / 89.  Of 192, never (4 x 6000 x 16000 675 / 716).
-    // Where the position decides, both are launched and the one that it is not for
-    // ends at once (2 us).
-    const size_t most_per = ng > 6 ? 16 : 32, turns = ng > 4 ? 1 : 2, many_blocks = (rows + 127) / 128;
-    const bool wide = ng != 6 && 2 * ((rows + most_per - 1) / most_per) > (ng > 6 ? 10 : 7) * many_blocks;
-    const double from = (ng > 6 ? 2e7 : 9e7) / ((double)rows * (double)n_head_kv);
-    A.from = wide && from < (double)n_ctx ? (int)from + 1 : INT_MAX;
-    const bool many = A.from <= (int64_t)n_ctx, few = A.from > (int64_t)M;   // (a call has M positions at least)
-    Parts few_parts = {}, many_parts = {};
-    const double record = 1e-6 * (double)(rows * n_head_kv) * (4 + width) * sizeof(float);   // MB of a split's
-    double us, least = 0.0;
-    size_t few_blocks = 0;
-    if (few) {
-        // Rows of a workgroup, 8, 16 or 32: more of them share a tile's unpacking, but a
-        // short call waits longer for one.  Whole calls, 16 / 32 rows (heads of
-        // 128): 12 tokens of 32 heads over 8 at 100 positions 4.9 / 7.0 us, 31 at 1000
-        // 11.1 / 13.5, at 9000 24.4 / 22.6, a prompt of 200 7.4 / 9.0, of 500 16.6 / 14.0.
-        // Records cost 0.5 us a MB, at any position, where a split gains at long ones only, so
-        // they count four times: 200 tokens at 700 of 32768 positions 29.9 -> 22.1 us,
-        // of 5000 20.4 -> 16.9; at 9000 of 9100, 100 tokens, 47.0 -> 50.5.  (Not of more
-        // dimensions, where a step is longer: 200 at 2000 of 2200 68.7 -> 76.3.)
-        const size_t n = A.from < (int64_t)n_ctx ? (size_t)A.from : n_ctx;
-        const double share = M < n ? 1.0 - 0.5 * (double)M / (double)n : 0.5;
-        for (size_t per = 8; per <= most_per && (per == 8 || rows > per / 2); per *= 2) {
-            const Cost c = {per == 32 ? 0.3 + 0.9 * ng : per == 16 ? 0.4 + 0.42 * ng : 0.2 + 0.4 * ng,
-                            per == 32 ? 0.35 + 0.19 * ng : 0.2 + 0.18 * ng, 1.9,
-                            (ng > 4 ? 0.5 : 2.0) * record, ng <= 4};
-            const size_t blocks = (rows + per - 1) / per;
-            if (blocks > 65535) continue;                        // (a launch's third dimension)
-            const int s = split_count(n_head_kv * blocks, (n + KVQ_TILE * KA_WAVES - 1) / (KVQ_TILE * KA_WAVES),
-                                      ctx->n_cu, share, c, us);
-            if (few_blocks && us >= least) continue;
-            least = us;
-            few_blocks = blocks;
-            few_parts = {s, (int)per, KA_WAVES};
-        }
-    }
-    if (many) {
-        const Cost c = {8.0, 1.65, 5.0, record, false};
-        many_parts = {split_count(n_head_kv * many_blocks, (n_ctx + KVQ_TILE * turns - 1) / (KVQ_TILE * turns),
-                                  ctx->n_cu, 1.0, c, us),
-                      128, (int)turns};
-    }
-    const int splits = few_parts.splits > many_parts.splits ? few_parts.splits : many_parts.splits;
+    const KvqPlan p = fox_kvq_plan(head_dim, n_head, n_head_kv, M, n_ctx, ctx->n_cu);
+    A.from = p.from;
+    const int splits = p.few_parts.splits > p.many_parts.splits ? p.few_parts.splits : p.many_parts.splits;
     if (splits > 1) {
         st = fox_ws_reserve(ctx, n_head_kv * rows * splits * (4 + (size_t)width) * sizeof(float));
         if (st) return st;
         A.part = (float *)ctx->ws;
     }
     void *args[] = {(void *)&pos, &A};
-    A.splits = few_parts.splits;
-    if (few) {
-        const void *k = A.splits == 1 ? q4 ? few_kernel<4, true>(ng, few_parts.rows) : few_kernel<8, true>(ng, few_parts.rows)
-                                      : q4 ? few_kernel<4, false>(ng, few_parts.rows) : few_kernel<8, false>(ng, few_parts.rows);
-        FOX_HIP(hipLaunchKernel(k, dim3((unsigned)few_parts.splits, (unsigned)n_head_kv, (unsigned)few_blocks),
+    A.splits = p.few_parts.splits;
+    if (p.few) {
+        const void *k = A.splits == 1 ? q4 ? few_kernel<4, true>(ng, p.few_parts.rows) : few_kernel<8, true>(ng, p.few_parts.rows)
+                                      : q4 ? few_kernel<4, false>(ng, p.few_parts.rows) : few_kernel<8, false>(ng, p.few_parts.rows);
+        FOX_HIP(hipLaunchKernel(k, dim3((unsigned)p.few_parts.splits, (unsigned)n_head_kv, (unsigned)p.few_blocks),
                                 dim3(64 * KA_WAVES), args, 0, ctx->stream));
     }
-    if (many) {
-        A.splits = many_parts.splits;
+    if (p.many) {
+        A.splits = p.many_parts.splits;
         const void *k = q4 ? many_kernel<4>(ng) : many_kernel<8>(ng);
+        const size_t turns = p.many_parts.tiles;
         const size_t tiles_lds = 2 * turns * 4 * ng * 1024, rows_lds = 128 * turns * (width + 4) * sizeof(float);
         const size_t lds = tiles_lds > rows_lds ? tiles_lds : rows_lds;
         FOX_HIP(hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-        FOX_HIP(hipLaunchKernel(k, dim3((unsigned)(n_head_kv * many_blocks * many_parts.splits)), dim3(256 * turns), args,
-                                lds, ctx->stream));
+        FOX_HIP(hipLaunchKernel(k, dim3((unsigned)(n_head_kv * p.many_blocks * p.many_parts.splits)), dim3(256 * turns),
+                                args, lds, ctx->stream));
     }
     if (splits > 1) {
         // a workgroup a row or eight rows: whole calls of 512 rows 18.2 / 19.9 us, of
         // 992 14.0 / 13.5 and 23.0 / 22.5
-        const bool by_rows = splits <= 16 && rows * n_head_kv >= 800, either = few && many;
-        if (!few) few_parts = many_parts;
+        const bool by_rows = splits <= 16 && rows * n_head_kv >= 800, either = p.few && p.many;
+        KvqParts few = p.few ? p.few_parts : p.many_parts, many = p.many_parts;
         const void *k = by_rows ? either ? (const void *)kv_merge_rows_k<true> : (const void *)kv_merge_rows_k<false>
                                 : either ? (const void *)kv_merge_k<true> : (const void *)kv_merge_k<false>;
-        void *merge_args[] = {(void *)&pos, &A, (void *)&width, &few_parts, &many_parts};
+        void *merge_args[] = {(void *)&pos, &A, (void *)&width, &few, &many};
         FOX_HIP(hipLaunchKernel(k, dim3((unsigned)(by_rows ? (rows + 7) / 8 : rows), (unsigned)n_head_kv), dim3(256),
                                 merge_args, 0, ctx->stream));
     }

@@ -15,7 +15,11 @@
 //       floats from acc, by one wave, into out[0], and the one-add-at-a-time
 //       chain's into out[2] (out[1], out[3]: their shader clocks): its tests
 //       compare them with the sum in order on inputs chosen to hit its
-//       events.
+//       events;
+//   fox_gpu_kvq_plan_probe(hd, n_head, n_head_kv, M, n_ctx, n_cu, out)
+//       how attention over a quantised cache would be launched (no GPU is
+//       asked): from, few, many, few's blocks, splits and rows of a
+//       workgroup, many's blocks and splits, into the host's out[8].
 //
 // sink (device memory, 4 bytes) is written only if the folded data hit a
 // fixed constant, so the loads cannot be dropped and nothing is written in
@@ -130,4 +134,15 @@ extern "C" fox_gpu_status fox_gpu_sum_probe(fox_gpu_ctx *ctx, const float *e, in
     hipLaunchKernelGGL(sum_probe_k, dim3(1), dim3(64), lds, ctx->stream, e, n, acc, out);
     FOX_LAUNCHED("sum_probe");
     return FOX_GPU_OK;
+}
+
+// ------------------------------------------------------- plan probe
+
+extern "C" void fox_gpu_kvq_plan_probe(size_t hd, size_t n_head, size_t n_head_kv, size_t M, size_t n_ctx,
+                                       int n_cu, int64_t *out)
+{
+    const KvqPlan p = fox_kvq_plan(hd, n_head, n_head_kv, M, n_ctx, n_cu);
+    const int64_t v[8] = {p.from, p.few, p.many, (int64_t)p.few_blocks, p.few_parts.splits, p.few_parts.rows,
+                          (int64_t)p.many_blocks, p.many_parts.splits};
+    for (int i = 0; i < 8; i++) out[i] = v[i];
 }
