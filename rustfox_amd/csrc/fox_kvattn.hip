@@ -145,11 +145,12 @@ __device__ __forceinline__ float less(float a, _Float16 h)
     return __builtin_fmaf((float)h, minus, a);
 }
 
-// 2^(14 - exponent of a row's largest value), the exponent kept within range;
-// back turns a score of the scaled row into powers of two
+// 2^(14 - exponent of a row's largest value), the exponent kept at -100 or above
+// and at 127, a float's largest, for rows with an infinity or a NaN: both
+// powers are normal floats.  back turns a score of the scaled row into powers of two
 __device__ __forceinline__ float query_scale(float top, float score, float &back)
 {
-    const int ex = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 113);
+    const int ex = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 127);
     back = score * __uint_as_float((uint32_t)(127 - 14 + ex) << 23);
     return __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
 }

@@ -21,3 +21,28 @@ def test_the_most_rows(gpu, bits, n_head, hd, n_ctx, pos, M):
     c = fill(gpu, bits, n_ctx, 1, hd, K, V)
     got = attend(gpu, bits, c, q, n_head, 1, hd, n_ctx, pos)
     check_some(got, q, kr.held(K, bits, hd), kr.held(V, bits, hd), n_head, 1, hd, pos, n_ctx, rng)
+
+
+# one row, rows of several sizes a workgroup, several splits, and the kernel of long work
+LARGE = [(4, 1, 128, 300, 200, 1), (8, 2, 64, 300, 200, 40), (32, 8, 128, 300, 10, 70), (16, 2, 256, 90, 30, 9),
+         (32, 8, 128, 5000, 4990, 1), (8, 1, 96, 6000, 5900, 33), (2200, 1, 32, 520, 310, 100)]
+
+
+@pytest.mark.parametrize("case", LARGE, ids=str)
+@pytest.mark.parametrize("bits", BITS)
+def test_the_largest_queries(gpu, bits, case):
+    """Finite queries of any size, on dimensions where every key is zero: all scores are zero, so
+    results are the values' means."""
+    n_head, n_kv, hd, n_ctx, pos, M = case
+    rng = np.random.default_rng(hd + M)
+    n = pos + M
+    K, V = rows(rng, n, n_kv * hd), rows(rng, n, n_kv * hd)
+    K[:, 5::hd], K[:, 9::hd] = 0.0, -0.0
+    q = np.zeros((M, n_head * hd), np.float32)
+    sizes = np.array([1e20, 4.1e34, 4.2e34, 8.4e34, -1e37, -1.7e38, 3.4028235e38], np.float32)
+    q[:, 5::hd] = np.resize(sizes, M * n_head).reshape(M, n_head)
+    q[:, 9::hd] = -q[:, 5::hd]
+    c = fill(gpu, bits, n_ctx, n_kv, hd, K, V)
+    got = attend(gpu, bits, c, q, n_head, n_kv, hd, n_ctx, pos)
+    # (the plain form of these queries: a row of zeros)
+    check_some(got, np.zeros_like(q), kr.held(K, bits, hd), kr.held(V, bits, hd), n_head, n_kv, hd, pos, n_ctx, rng)
