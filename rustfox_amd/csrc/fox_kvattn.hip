@@ -4,8 +4,12 @@
 // Arithmetic.  The cache's values are exactly halves (fox_kvq_dev.h), so an
 // f16 MFMA multiplies them without rounding; the other operand, the query or the
 // softmax's weight, is the sum of two halves (22 bits of it), each its own MFMA into
-// the same float sums.  A query head's row is scaled by a power of two first, its
-// largest value to 2^14, so that the lower half is not lost below the half's range.
+// the same float sums.  A query head's row is multiplied by log2(e) / sqrt(hd) and a
+// power of two first, its largest value to 2^14, so that the lower half is not lost
+// below the half's range.  Scores are then a power of two away from exponents: the
+// largest one's product with it, the maximum, is exact, and that score's weight, 2^7
+// (1 to 2^8 from 2^24 on, where the 7 is rounded to the maximum's last bit), stays a
+// half however large the score is.
 //
 // A step is 32 positions (a tile) of one kv head by 16 or 32 query rows (row =
 // token * G + head in the group of G = n_head / n_head_kv that share it):
@@ -41,7 +45,7 @@ struct AttnArgs {
     const uint8_t *cache;
     int n_ctx, n_head_kv, G, splits;
     uint32_t by_g;                // row / G: see token_of
-    float score;                  // log2(e) / sqrt(hd) / 4 (the halves are 4 times the values)
+    float score;                  // log2(e) / sqrt(hd)
     int from;                     // positions from which kv_attn_many takes the call, kv_attn_few below
     uint16_t hd, M;
     uint8_t g_shift;
@@ -145,14 +149,15 @@ __device__ __forceinline__ float less(float a, _Float16 h)
     return __builtin_fmaf((float)h, minus, a);
 }
 
-// 2^(14 - exponent of a row's largest value), the exponent kept at -100 or above
-// and at 127, a float's largest, for rows with an infinity or a NaN: both
-// powers are normal floats.  back turns a score of the scaled row into powers of two
+// score 2^(14 - exponent of a row's largest value times score), the exponent kept
+// at -100 or above and at 127, a float's largest, for rows with an infinity or a NaN:
+// both powers are normal floats.  back turns a score of the scaled row into powers of
+// two (the cache's halves are 4 times its values); it is one itself, see above
 __device__ __forceinline__ float query_scale(float top, float score, float &back)
 {
-    const int ex = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 127);
-    back = score * __uint_as_float((uint32_t)(127 - 14 + ex) << 23);
-    return __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
+    const int ex = min(max((int)(__float_as_uint(top * score) >> 23) - 127, -100), 127);
+    back = __uint_as_float((uint32_t)(127 - 16 + ex) << 23);
+    return score * __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
 }
 
 // eight scaled values as two halves each
@@ -162,7 +167,11 @@ __device__ __forceinline__ void split_8(const float x[8], float up, h8v &hi, h8v
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const float a = x[2 * i] * up, b = x[2 * i + 1] * up;
-        h[i] = h2v{(_Float16)a, (_Float16)b};
+        // (one value of the upper halves: the compiler forms them from the product and from
+        // its float, whose roundings differ now and then, and would subtract the other one)
+        uint32_t hw = as_u(h2v{(_Float16)a, (_Float16)b});
+        asm("" : "+v"(hw));
+        h[i] = as_h2(hw);
         d[i] = h2v{(_Float16)less(a, h[i][0]), (_Float16)less(b, h[i][1])};
     }
     hi = __builtin_bit_cast(h8v, *(u4v *)h);
@@ -1093,7 +1102,7 @@ extern "C" fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, si
     A.hd = (uint16_t)head_dim;
     while (((uint32_t)1 << A.g_shift) < (uint32_t)A.G) A.g_shift++;
     A.by_g = (uint32_t)((((uint64_t)1 << (30 + A.g_shift)) + (uint32_t)A.G - 1) / (uint32_t)A.G);
-    A.score = (float)(1.4426950408889634 / std::sqrt((double)head_dim) / 4);
+    A.score = (float)(1.4426950408889634 / std::sqrt((double)head_dim));
     A.M = (uint16_t)M;
     A.q_wide = head_dim % 4 == 0 && (uintptr_t)q % 16 == 0 && (M == 1 || q_stride % 4 == 0);
     A.out_wide = head_dim % 4 == 0 && (uintptr_t)out % 16 == 0 && (M == 1 || out_stride % 4 == 0);

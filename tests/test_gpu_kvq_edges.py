@@ -46,3 +46,45 @@ def test_the_largest_queries(gpu, bits, case):
     got = attend(gpu, bits, c, q, n_head, n_kv, hd, n_ctx, pos)
     # (the plain form of these queries: a row of zeros)
     check_some(got, np.zeros_like(q), kr.held(K, bits, hd), kr.held(V, bits, hd), n_head, n_kv, hd, pos, n_ctx, rng)
+
+
+@pytest.mark.parametrize("alike", [True, False], ids=["alike", "apart"])
+@pytest.mark.parametrize("case", LARGE, ids=str)
+@pytest.mark.parametrize("bits", BITS)
+def test_the_largest_scores(gpu, bits, case, alike):
+    """Scores up to a float's range, where their own last bit is many powers of two.  Keys alike at
+    every position: results are the values' means.  Keys apart, by far more than the scores may be
+    off: results are the value of the largest score."""
+    n_head, n_kv, hd, n_ctx, pos, M = case
+    rng = np.random.default_rng(hd * M)
+    n = pos + M
+    K, V = rows(rng, n, n_kv * hd), rows(rng, n, n_kv * hd)
+    if alike:
+        K[:] = K[1]
+    c = fill(gpu, bits, n_ctx, n_kv, hd, K, V)
+    Kh, Vh = (np.float64(kr.held(x, bits, hd)) for x in (K, V))
+    # (a score's size is at most hd max|k| max|q| / sqrt(hd))
+    limit = 1e38 / (np.sqrt(hd) * np.abs(Kh).max() * 6)
+    for size in (1e6, 1e8, 3e8, 1e9, 1e12, 1e20, 1e30, limit):
+        q = rng.standard_normal((M, n_head * hd)).clip(-6, 6).astype(np.float32) * np.float32(size)
+        got = attend(gpu, bits, c, q, n_head, n_kv, hd, n_ctx, pos)
+        assert np.isfinite(got).all(), size
+        if alike:
+            check_some(got, np.zeros_like(q), Kh, Vh, n_head, n_kv, hd, pos, n_ctx, rng, 60)
+            continue
+        clear = 0
+        for t, h in (divmod(int(i), n_head) for i in rng.integers(0, M * n_head, 60)):
+            at, g = slice(h * hd, (h + 1) * hd), h // (n_head // n_kv)
+            k, v = (x[:pos + t + 1, g * hd:(g + 1) * hd] for x in (Kh, Vh))
+            s = k @ np.float64(q[t, at]) / np.sqrt(hd)
+            top = (np.abs(k) @ np.abs(np.float64(q[t, at]))).max() / np.sqrt(hd)
+            best = int(s.argmax())
+            gap = s[best] - np.delete(s, best).max(initial=-np.inf)
+            # each of two scores is off by at most (hd + 16) 2^-23 of top, as in attention_bound; 40
+            # more leaves the others e^-40 together
+            if gap < 2 * top * (hd + 16) * 2.0 ** -23 + 40 + np.log(n):
+                continue
+            clear += 1
+            assert np.all(np.abs(got[t, at] - v[best]) <= 2.0 ** -20 * np.abs(v[best]) +
+                          2.0 ** -31 * np.abs(v).sum(0)), (size, t, h)
+        assert clear > 10, (size, clear)
