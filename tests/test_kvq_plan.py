@@ -7,6 +7,7 @@ import pytest
 
 import rustfox_amd as rf
 import test_gpu_kvq as shapes
+import test_gpu_kvq_rounding as rounding
 
 N_CU = 256
 
@@ -59,3 +60,19 @@ def test_every_shape_has_a_launch(hd):
         if g * n_kv > 65535 or (width(hd) == 192 and M * g > 65535 * 32):
             continue                                         # (refused)
         check(hd, g * n_kv, n_kv, M, n_ctx)
+
+
+def test_the_gpu_tests_reach_every_kernel():
+    """Each width's kernels of 8, 16 and 32 rows, in one split and in several, and the one of 128
+    rows, at the sizes that test_gpu_kvq_rounding runs."""
+    met = set()
+    for n_head, n_kv, hd, n_ctx, pos, M in rounding.MORE + shapes.ATTN_CASES + shapes.LONG_WORK + shapes.DIVISIONS:
+        p, seen = plan(hd, n_head, n_kv, M, n_ctx), min(pos + M, n_ctx)
+        if seen >= p["from_"]:
+            met.add((width(hd), 128, p["many_splits"] > 1))
+        else:
+            met.add((width(hd), p["few_rows"], p["few_splits"] > 1))
+    missing = [(w, per, several) for w in (32, 64, 96, 128, 192, 256) for per in (8, 16, 32, 128)
+               for several in (False, True)
+               if (w, per) not in ((256, 32), (192, 128)) and (w, per, several) not in met]
+    assert not missing
