@@ -632,7 +632,7 @@ static fox_gpu_status rope_args(const char *what, fox_gpu_ctx *ctx, const float 
     if (pairs != FOX_GPU_PAIRS_ADJACENT && pairs != FOX_GPU_PAIRS_HALVES)
         return fox_fail(FOX_GPU_ERR_ARG, "%s: unknown pairing %d", what, pairs);
     if (M > FOX_GPU_BATCH_TOKENS) return fox_fail(FOX_GPU_ERR_ARG, "%s: too many tokens", what);
-    if (n_head + 2 * n_head_kv > 65535)                      // (rows of the grid)
+    if (n_head > 65535 || n_head + 2 * n_head_kv > 65535)    // (rows of the grid; the sum may wrap)
         return fox_fail(FOX_GPU_ERR_ARG, "%s: %zu heads beside %zu kv heads are too many", what, n_head,
                         n_head_kv);
     if (M > 1 && (q_stride < nq || qo_stride < nq || k_stride < nkv || v_stride < nkv))
