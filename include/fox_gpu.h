@@ -409,7 +409,10 @@ fox_gpu_status fox_gpu_batch_attention(fox_gpu_ctx *ctx, float *out, size_t out_
  * most 2^30.  Strides are in floats, used when there is more than one row,
  * and at least the row's width.  pos[0] is the position of the first row,
  * read on the device (one graph serves every step); rows whose position is
- * not below n_ctx are not stored. */
+ * not below n_ctx are not stored.  Every call on a cache gives the kv_type, n_ctx,
+ * n_head_kv and head_dim that it was written with.  Calls on several contexts may run
+ * at once on one cache where one of them at most writes it, and the others read
+ * positions that it does not write. */
 enum { FOX_GPU_KV_Q4 = 4, FOX_GPU_KV_Q8 = 8 };
 
 /* bytes of a layer's cache; 0 for a shape that is not taken */
@@ -455,8 +458,10 @@ fox_gpu_status fox_gpu_kvq_norm_rope_store(
  * pos[0] + t over positions 0 .. pos[0] + t of a quantised cache:
  * softmax(q.k / sqrt(hd)) v, for any number of query heads per kv head (M
  * n_head / n_head_kv at most 2097120 where head_dim is 130 .. 192).  The
- * cache's values are multiplied as they are; sums, maxima and the softmax are in
- * 32 bits.  out must not overlap q. */
+ * cache's values are multiplied as they are; scores, maxima, exponents and sums are in
+ * 32 bits.  The other factors are held in fewer: a query's value to 2^-22 of it
+ * and 2^-38 of its head's largest, a softmax weight to 2^-21 of it and 2^-31 of its row's
+ * largest.  A score past a float's range gives NaN.  out must not overlap q. */
 fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, size_t out_stride,
                                      const float *q, size_t q_stride, int kv_type,
                                      const void *cache, size_t n_head, size_t n_head_kv,

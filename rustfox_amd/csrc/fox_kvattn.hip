@@ -225,7 +225,10 @@ __device__ __forceinline__ void exponents(float x[N], const float s[N], float sc
     }
 }
 
-// The weights of eight positions, as two halves each, and their sum.
+// The weights of eight positions, as two halves each, and their sum.  Both halves are
+// truncated, which leaves up to 2^-21 of a weight out of the products, not of the sum.  Rounded
+// to the nearest, whole passes are off by as much (777 tokens at 8000 positions 1.01e-6 / 1.00e-6 of the
+// result, 512 at none 3.6e-7 / 3.5e-7: scores' errors count more) and take 1 to 5% longer.
 __device__ __forceinline__ void weigh(const float x[8], float &l, h8v &ph, h8v &pl)
 {
     h2v hi[4], lo[4];
@@ -333,12 +336,11 @@ struct Tile {
 // lower ones, so a tile takes half the products; the two columns of a row are
 // added where a score is used and at the end.
 // What bounds it is unpacking, then the read: one row of 32 heads over 8 of 128
-// dimensions, 4 bits, at 131,071 positions (143 MB) takes 32.5 us, 4.4 TB/s with
-// the vector units busy 57% and the matrix cores 10% of the time; 8 bits, fewer
-// instructions a value, reads 4.9 TB/s (60,000 positions, 29.4 us with both launches).
+// dimensions, 4 bits, at 131,071 positions (143 MB) takes 36 to 37 us a call with its
+// merge, 3.9 TB/s, the vector units busy 52% and the matrix cores 9% of the time.
 // Reading two tiles ahead is slower (39.4 us for 36.5), as is one copy of the loop's
 // body that reads past its last tile (8.4 -> 8.8 us at 1500 positions).
-// Short contexts are a launch and 2 to 4 us: 34 positions of 6 heads 3.8 to 4.5 us in all.
+// Short contexts are a launch and 2 to 4 us: 34 positions of 6 heads 3.8 to 4.8 us in all.
 // ONE: a single split, whose first tiles are read before the position is known (that row
 // at 300 positions 6.7 -> 6.3 us; with more splits most such reads would be for nothing
 // where a long cache is not full: 8.1 -> 8.7 us at 1000 of 32768 positions).
@@ -575,9 +577,9 @@ __global__ __launch_bounds__(64 * KA_WAVES, NG > 4 ? 1 : 2) void kv_attn_few(con
 // instruction against 16, measured; with vector instructions between, 19 to 23
 // against 17 to 19).  A tile's weights are formed beside the next one's scores; a tile is
 // unpacked while the one before it is multiplied, its words read a step
-// earlier still.  777 tokens on 8000 positions of 32 heads over 8 of 128 take 215 us, 1000
-// TFLOP/s of half products (two a product, see above) where a large library product
-// of halves reaches 1136: matrix cores busy 41%, vector units 37% of the time.
+// earlier still.  777 tokens on 8000 positions of 32 heads over 8 of 128 take 217 to 226 us a
+// call, 945 to 985 TFLOP/s of half products (two a product, see above) where a large library
+// product of halves reaches 1136 to 1167: matrix cores busy 41%, vector units 38% of the time.
 template <int BITS, int NG, int PW>
 __global__ __launch_bounds__(256 * PW, NG > 4 ? 1 : 2) void kv_attn_many(const uint32_t *pos, AttnArgs A)
 {

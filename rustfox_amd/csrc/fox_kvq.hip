@@ -430,7 +430,8 @@ __device__ __forceinline__ int code_of(const uint32_t *w, int e)
 __device__ __forceinline__ void put_quad(float *dst, const float x[4], int d, int hd, bool wide)
 {
     if (wide) {
-        // (past the caches: 16077 rows of 8 heads of 128 then take 30 us instead of 42)
+        // (past the caches: 16077 rows of 8 heads of 128, into three outputs in turn, take 34.8 us
+        // instead of 44.8; into one output alone both ways 26.5)
         __builtin_nontemporal_store(*(const f4v *)x, (f4v *)(dst + d));
         return;
     }

@@ -8,8 +8,8 @@
 // stored as bits 14..7 of the half d * 4, and a code per value,
 //   x ~ d * c,  c = round_half_even(x / d) in [-h, h - 1],  h = 2^(BITS - 1),
 // where d is the least scale with max(x) <= (h - 1/2) d and
-// -min(x) <= (h + 1/2) d, so no code is clamped and |x - d c| <= d / 2 (up to
-// the largest scale, KVQ_CAP; larger values saturate).  A group holding a NaN
+// -min(x) <= (h + 1/2) d, so |x - d c| <= d / 2 (up to the largest scale, KVQ_CAP;
+// larger values saturate; x = (h - 1/2) d alone, a tie, is clamped to h - 1).  A group holding a NaN
 // or an infinity gets the scale byte 0xFF, a NaN half: it reads as NaN.
 //
 // Why four significant bits: times a 4-bit code that is at most 8 of them,

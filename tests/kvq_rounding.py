@@ -5,11 +5,11 @@ row is off by far less, and a product that went missing would hide below that bo
 row's error is held, as a length over its head_dim results, to a small multiple of what
 independent roundings add up to as the root of their squares, in units of 2^-24:
 
-  scores   A query's value is held to 2^-24 of it in two halves (11 bits, and 11 of what is left: 2^-12
-           of at most 2^-12) after one rounding to a float, 2; its products with the cache's values
-           are exact and their sums rounded a few times, 2.  Position i's exponent
+  scores   A query's value is rounded to a float once, 1, and held in two halves, 2 (11 bits, and 11 of
+           the 2^-11 that is left at most); its products with the cache's values are exact and
+           their sums rounded a few times, 2.  Position i's exponent
            x = (s - largest s) log2(e) + at most 15 is rounded once.  So a weight is off,
-           relatively, by 4 r + |x| with r = sqrt(sum_d (q_d k_d)^2 / head_dim), and the row by
+           relatively, by 5 r + |x| with r = sqrt(sum_d (q_d k_d)^2 / head_dim), and the row by
            weight * |v - result| of that.
   weights  exp2 is off by 2 and the weight's two halves, truncated, by at most 8 of it: with the quotient's
            roundings 12 of a product's size, root of squares over the positions, and of the
@@ -49,7 +49,7 @@ def rows_of(q, K, V, upto):
         r2 = (a * a) @ (k * k).T / hd
         p2 = p * p
         away = np.maximum(w[None, :] - 2 * (o @ v.T) + (o * o).sum(1)[:, None], 0.0)
-        score2 = (p2 * (4 * np.sqrt(r2) + x) ** 2 * away).sum(1)
+        score2 = (p2 * (5 * np.sqrt(r2) + x) ** 2 * away).sum(1)
         size2 = p2 @ w + (o * o).sum(1)
         ends2 = (2.0 ** -7 * p.max(1)) ** 2 * np.cumsum(w)[n - 1]
         out[i:i + step] = o
