@@ -335,12 +335,12 @@ def read_probe():
     # one launch at the sizes of a decode step's kernels (2 loads in flight,
     # 1024 workgroups): a new region of the buffer each launch (cold), or
     # the same region every time (warm: the infinity cache and L2 hold it)
+    probe = rf.probe_lib().fox_gpu_read_probe
     for n in (3 << 20, 15138816 // 4096 * 4096, 27 << 20, 64 << 20):
         nreg = READ_PROBE_BYTES // n
         for mode in ("cold", "warm"):
             offs = [(i % nreg) * n if mode == "cold" else 0 for i in range(64)]
-            run = lambda o: rf._check(gpu.lib.fox_gpu_read_probe(gpu.ctx, src.ptr + o, n, 2,
-                                                                  1024, sink.ptr))
+            run = lambda o: rf._check(probe(gpu.ctx, src.ptr + o, n, 2, 1024, sink.ptr))
             for o in offs[:4]:
                 run(o)
             gpu.record(e0)
