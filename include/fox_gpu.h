@@ -45,11 +45,11 @@ typedef enum {
 } fox_gpu_status;
 
 /* ggml type ids (include/fox/fox.h:213-224) understood by the device path
- * (Q4_0, Q8_0 and Q5_K by fox_gpu_dequant only) */
+ * (Q4_0, Q8_0 and Q5_K by fox_gpu_dequant only, BF16 by paged caches only) */
 enum {
     FOX_GPU_F32 = 0, FOX_GPU_F16 = 1, FOX_GPU_Q4_0 = 2, FOX_GPU_Q8_0 = 8,
     FOX_GPU_Q4_K = 12, FOX_GPU_Q5_K = 13, FOX_GPU_Q6_K = 14,
-    FOX_GPU_TQ1_0 = 34, FOX_GPU_TQ2_0 = 35
+    FOX_GPU_BF16 = 30, FOX_GPU_TQ1_0 = 34, FOX_GPU_TQ2_0 = 35
 };
 
 /* largest token count of one multi-token gemv / forward call */
@@ -466,6 +466,106 @@ fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, size_t out_st
                                      const float *q, size_t q_stride, int kv_type,
                                      const void *cache, size_t n_head, size_t n_head_kv,
                                      size_t head_dim, size_t M, const uint32_t *pos, size_t n_ctx);
+
+/* -------------------------------------------------------- paged caches */
+
+/* Keys and values of many sequences in one pool of pages of 16-bit rows, for a
+ * server that decodes them together (no counterpart in RustFox: one sequence,
+ * one float cache).  Pools, table and the arrays beside them are the caller's
+ * device memory, laid out plainly:
+ *   k, v      [n_pages][n_head_kv][page_size][head_dim] of `type`, 16-byte aligned
+ *   table     [n_seqs][max_pages] pages of each sequence, in order
+ *   weight    [n_seqs][n_head_kv][max_pages * page_size] attention that each row
+ *             has got so far, or NULL
+ *   position  the same shape: each row's token's position, or NULL (both or none)
+ * Row r of a sequence is row r % page_size of page table[seq][r / page_size].
+ * Pages may come in any order and be shared by sequences that only read them;
+ * a page number not below n_pages is no page: its rows are not stored, and
+ * hidden from attention.
+ *
+ * type is FOX_GPU_F16 or FOX_GPU_BF16; page_size a power of two, 16 to 4096;
+ * head_dim a multiple of 8 up to 256 (else FOX_GPU_ERR_UNSUPPORTED); at most
+ * 2^30 rows a sequence, 65535 sequences, 4096 kv heads (2^20 of all sequences),
+ * 2^31 pages.  Lengths, positions and sequences are read on the device, so one
+ * graph serves every step.  The
+ * struct itself is read during the call only.  Calls on several contexts may
+ * run at once on one cache where they write no row or array that another reads. */
+typedef struct {
+    int             type;
+    void           *k, *v;
+    size_t          n_pages, page_size, n_head_kv, head_dim;
+    const uint32_t *table;
+    size_t          n_seqs, max_pages;
+    float          *weight;
+    uint32_t       *position;
+} fox_gpu_paged;
+
+/* Cosines and sines of positions p0 .. p0+n-1, n rows of n_rot/2 (n_rot even, at
+ * most 256; p0 + n at most 2^30), for every call here that takes tables:
+ *   f_j = base^(-2j / n_rot) / factors[j]             (factors NULL: all one)
+ *   w_j = f_j (scale (1 - mix_j) + mix_j),  mix_j = ext (1 - clamp((j - lo) / max(hi - lo, 0.001), 0, 1))
+ *   cos[p][j] = magnitude cos(p w_j), and sin likewise,
+ * with lo = max(0, floor(at(beta_fast))) and hi = min(n_rot - 1, ceil(at(beta_slow))),
+ * at(b) = n_rot ln(orig_ctx / (2 pi b)) / (2 ln base).  So `scale` alone (1 /
+ * the stretch) slows every pair alike; with ext = 1, pairs that turn more than
+ * beta_fast times within orig_ctx positions keep their speed and those of less
+ * than beta_slow turns are slowed; with ext = 0 the last three are not looked at.  `factors`
+ * (device memory) divides each pair's speed by its own.  Computed in double and rounded
+ * once. */
+typedef struct {
+    double       base, scale, ext, beta_fast, beta_slow, orig_ctx, magnitude;
+    const float *factors;
+} fox_gpu_rope_freq;
+fox_gpu_status fox_gpu_rope_tables(fox_gpu_ctx *ctx, float *cos_t, float *sin_t, size_t p0,
+                                   size_t n, size_t n_rot, const fox_gpu_rope_freq *freq);
+
+/* Queries and keys of M <= FOX_GPU_BATCH_TOKENS tokens normed head by head
+ * (q_norm, k_norm; NULL: not, and then eps is not looked at), the first n_rot dimensions of each head
+ * rotated (n_rot even, 2 to head_dim: pairs (2j, 2j+1) or (j, j + n_rot/2); the others as they are),
+ * and keys and values stored.  Token i belongs to sequence seq[i] (seq NULL: i), stands
+ * at position pos[i] (a row of the tables, n_table rows of n_rot/2) and
+ * becomes row row[i] of the sequence (row NULL: pos[i]; after an eviction
+ * the two differ).  As fox_gpu_norm_rope_store, in double, rounded to float once: queries
+ * to q_out (which may be q, with its stride), keys and values then to the cache's type, to the
+ * nearest, ties to even (halves end at 65504, also where a value is infinite; a NaN stays one).
+ * Where the cache has weight and position, the row's become 0 and pos[i].  A token whose sequence is not
+ * below n_seqs or whose position is not below n_table is neither turned nor stored; one whose row
+ * has no page is turned only.  Two tokens of a call must not share a row. */
+fox_gpu_status fox_gpu_paged_rope_store(
+    fox_gpu_ctx *ctx, const fox_gpu_paged *cache, const float *q, size_t q_stride, float *q_out,
+    size_t q_out_stride, size_t n_head, const float *k, size_t k_stride, const float *v,
+    size_t v_stride, size_t M, const float *q_norm, const float *k_norm, float eps, int pairs,
+    size_t n_rot, const float *cos_t, const float *sin_t, size_t n_table, const uint32_t *pos,
+    const uint32_t *seq, const uint32_t *row);
+
+/* GQA attention of M <= FOX_GPU_BATCH_TOKENS tokens, each over the first
+ * length[i] rows of sequence seq[i] (NULL: i): softmax(q.k / sqrt(hd)) v.  A
+ * step gives one token of every sequence; tokens of one sequence may also stand in a
+ * call, each with its own length.  A length past the table's rows means all of them;
+ * a token that sees no row (length 0, no page, a sequence not below n_seqs) gets
+ * zeros.  Hidden rows may hold anything.  weigh != 0 (seq NULL, the cache has weight): every
+ * row's softmax weights, summed over the query heads of its kv head, are
+ * added to cache->weight.  The cache's values are multiplied as they are; scores, maxima, weights
+ * and sums are in 32 bits.  A query's value is held to 2^-22 of it (and
+ * halves' to 2^-38 of its head's largest).  A score past a float's range gives NaN.
+ * n_head is a multiple of n_head_kv, at most 65535.  out must not overlap q. */
+fox_gpu_status fox_gpu_paged_attention(fox_gpu_ctx *ctx, const fox_gpu_paged *cache, float *out,
+                                       size_t out_stride, const float *q, size_t q_stride,
+                                       size_t n_head, size_t M, const uint32_t *length,
+                                       const uint32_t *seq, int weigh);
+
+/* Of every sequence with more than `keep` rows (length[i], i < n_seqs), each kv
+ * head keeps `keep` of them: first those whose position is greater than the
+ * head's greatest less `recent` (0: none), then those of the greatest weight (a weight that is not
+ * greater than 0, a NaN too, counts as 0), of equal ones the lower row.  Kept rows from `keep` on, in
+ * order, take the places of the rows that are not kept below `keep`, in order:
+ * keys, values, weights and positions; the others stay where they are, so few rows move.
+ * kept[i] = min(length[i], keep), rows from there on are free.  Sequences that are cut
+ * must not share pages.  keep >= 1, recent <= keep; the cache has weight
+ * and position; kept is another array than length. */
+fox_gpu_status fox_gpu_paged_evict(fox_gpu_ctx *ctx, const fox_gpu_paged *cache,
+                                   const uint32_t *length, uint32_t *kept, size_t keep,
+                                   size_t recent);
 
 /* ------------------------------------------------------------- graphs */
 

@@ -21,7 +21,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 GPU_LIB = os.path.join(HERE, "lib", "librustfox_amd.so")
 HOST_LIB = os.path.join(HERE, "lib", "libfox.so")
 
-F32, F16, Q4_K, Q6_K, TQ1_0, TQ2_0 = 0, 1, 12, 14, 34, 35
+F32, F16, Q4_K, Q6_K, BF16, TQ1_0, TQ2_0 = 0, 1, 12, 14, 30, 34, 35
 ACT_PER_VECTOR, ACT_PER_BLOCK = 0, 1
 GEMV_ACCUMULATE = 1
 ATTN_SPLIT, ATTN_EXACT = 0, 1
@@ -129,6 +129,11 @@ def gpu_lib() -> C.CDLL:
         "fox_gpu_kvq_norm_rope_store": [vp, vp, sz, vp, sz, vp, sz, vp, sz, sz, sz, sz, sz, vp, vp,
                                         C.c_float, C.c_int, vp, vp, vp, C.c_int, vp, sz],
         "fox_gpu_kvq_attention": [vp, vp, sz, vp, sz, C.c_int, vp, sz, sz, sz, sz, vp, sz],
+        "fox_gpu_rope_tables": [vp, vp, vp, sz, sz, sz, C.POINTER(RopeFreq)],
+        "fox_gpu_paged_rope_store": [vp, C.POINTER(Paged), vp, sz, vp, sz, sz, vp, sz, vp, sz, sz, vp, vp,
+                                     C.c_float, C.c_int, sz, vp, vp, sz, vp, vp, vp],
+        "fox_gpu_paged_attention": [vp, C.POINTER(Paged), vp, sz, vp, sz, sz, sz, vp, vp, C.c_int],
+        "fox_gpu_paged_evict": [vp, C.POINTER(Paged), vp, vp, sz, sz],
         "fox_gpu_silu_mul": [vp, vp, vp, sz, sz, sz],
         "fox_gpu_add": [vp, vp, vp, sz, sz, sz],
         "fox_gpu_argmax": [vp, vp, sz, vp, vp, C.c_uint32, vp],
@@ -160,6 +165,33 @@ def _check(st: int):
     if st != 0:
         msg = gpu_lib().fox_gpu_last_error()
         raise FoxError(st, msg.decode() if msg else "")
+
+
+class Paged(C.Structure):
+    """fox_gpu_paged (include/fox_gpu.h)."""
+    _fields_ = [("type", C.c_int), ("k", C.c_void_p), ("v", C.c_void_p), ("n_pages", C.c_size_t),
+                ("page_size", C.c_size_t), ("n_head_kv", C.c_size_t), ("head_dim", C.c_size_t),
+                ("table", C.c_void_p), ("n_seqs", C.c_size_t), ("max_pages", C.c_size_t),
+                ("weight", C.c_void_p), ("position", C.c_void_p)]
+
+
+class RopeFreq(C.Structure):
+    """fox_gpu_rope_freq (include/fox_gpu.h)."""
+    _fields_ = [(f, C.c_double) for f in ("base", "scale", "ext", "beta_fast", "beta_slow", "orig_ctx",
+                                          "magnitude")] + [("factors", C.c_void_p)]
+
+
+class PagedCache:
+    """Pools, page table and the arrays beside them of many sequences' caches (fox_gpu_paged); the
+    device arrays are the caller's and are kept alive with it.  kv_type F16 or BF16."""
+
+    def __init__(self, kv_type, k: DeviceArray, v: DeviceArray, n_pages, page_size, n_head_kv, head_dim,
+                 table: DeviceArray, n_seqs, max_pages, weight: DeviceArray = None,
+                 position: DeviceArray = None):
+        self.arrays = (k, v, table, weight, position)
+        self.n_head_kv, self.head_dim = n_head_kv, head_dim
+        self.c = Paged(kv_type, k.ptr, v.ptr, n_pages, page_size, n_head_kv, head_dim, table.ptr, n_seqs,
+                       max_pages, weight.ptr if weight else None, position.ptr if position else None)
 
 
 class DeviceArray:
@@ -472,6 +504,43 @@ class Gpu:
         _check(self.lib.fox_gpu_kvq_attention(self.ctx, out.ptr, out_stride or w, q.ptr,
                                               q_stride or w, kv_type, cache.ptr, n_head, n_head_kv,
                                               head_dim, M, pos.ptr, n_ctx))
+
+    # -- paged caches (many sequences; strides default to the row's width)
+    def rope_tables(self, cos_t: DeviceArray, sin_t: DeviceArray, n, n_rot, p0=0, base=10000.0, scale=1.0,
+                    ext=0.0, beta_fast=32.0, beta_slow=1.0, orig_ctx=0.0, magnitude=1.0,
+                    factors: DeviceArray = None):
+        """Cosines and sines of positions p0 .. p0 + n - 1, scaled for long contexts if asked."""
+        f = RopeFreq(base, scale, ext, beta_fast, beta_slow, orig_ctx, magnitude,
+                     factors.ptr if factors else None)
+        _check(self.lib.fox_gpu_rope_tables(self.ctx, cos_t.ptr, sin_t.ptr, p0, n, n_rot, C.byref(f)))
+
+    def paged_rope_store(self, cache: PagedCache, q: DeviceArray, q_out: DeviceArray, n_head,
+                         k: DeviceArray, v: DeviceArray, M, pos: DeviceArray, n_rot, pairs,
+                         cos_t: DeviceArray, sin_t: DeviceArray, n_table, q_norm: DeviceArray = None,
+                         k_norm: DeviceArray = None, eps=0.0, seq: DeviceArray = None,
+                         row: DeviceArray = None, q_stride=None, q_out_stride=None, k_stride=None,
+                         v_stride=None):
+        """Head norms (None: none), rotation of the first n_rot dimensions and the store of M tokens
+        of any sequences into their pages."""
+        nq, nk = n_head * cache.head_dim, cache.n_head_kv * cache.head_dim
+        _check(self.lib.fox_gpu_paged_rope_store(
+            self.ctx, C.byref(cache.c), q.ptr, q_stride or nq, q_out.ptr, q_out_stride or nq, n_head, k.ptr,
+            k_stride or nk, v.ptr, v_stride or nk, M, q_norm.ptr if q_norm else None,
+            k_norm.ptr if k_norm else None, eps, pairs, n_rot, cos_t.ptr, sin_t.ptr, n_table, pos.ptr,
+            seq.ptr if seq else None, row.ptr if row else None))
+
+    def paged_attention(self, cache: PagedCache, out: DeviceArray, q: DeviceArray, n_head, M,
+                        length: DeviceArray, seq: DeviceArray = None, weigh=False, out_stride=None,
+                        q_stride=None):
+        """Attention of M tokens over the first length[i] rows of their sequences."""
+        w = n_head * cache.head_dim
+        _check(self.lib.fox_gpu_paged_attention(self.ctx, C.byref(cache.c), out.ptr, out_stride or w, q.ptr,
+                                                q_stride or w, n_head, M, length.ptr,
+                                                seq.ptr if seq else None, int(weigh)))
+
+    def paged_evict(self, cache: PagedCache, length: DeviceArray, kept: DeviceArray, keep, recent=0):
+        """Every sequence of more than `keep` rows cut back to those, the least weighed given up."""
+        _check(self.lib.fox_gpu_paged_evict(self.ctx, C.byref(cache.c), length.ptr, kept.ptr, keep, recent))
 
     def event(self):
         e = C.c_void_p()

@@ -201,6 +201,17 @@ fox_gpu_status fox_few_gemv(fox_gpu_ctx *ctx, size_t n, const fox_gpu_tensor *co
 fox_gpu_status fox_kvq_shape(const char *what, int kv_type, size_t n_ctx, size_t n_head_kv,
                              size_t head_dim);
 
+// a paged cache as the kernels take it, checked (fox_paged.hip); `track`: weight and position are needed
+struct PagedDev {
+    void *k, *v;
+    const uint32_t *table;
+    float *weight;
+    uint32_t *position;
+    uint32_t n_pages, n_seqs, max_pages, n_kv, hd, shift;   // page_size = 1 << shift
+    uint32_t cap;                                           // rows of a sequence
+};
+fox_gpu_status fox_paged_check(const char *what, const fox_gpu_paged *cache, bool track, PagedDev *out);
+
 // How attention over a quantised cache is launched (fox_kvattn.hip): a kernel's
 // rows and positions as they are divided, and which of the two kernels run.
 struct KvqParts {

@@ -1,0 +1,408 @@
+// fox_paged.hip -- paged caches of many sequences: tables of the rotation,
+// a pass's queries, keys and values normed, rotated and stored into pages, and
+// eviction of the rows that got the least attention.
+#include "fox_paged_dev.h"
+
+#include <cmath>
+#include <cstring>
+
+#define PG_THREADS 256
+
+// ------------------------------------------------------------------ shapes
+
+fox_gpu_status fox_paged_check(const char *what, const fox_gpu_paged *c, bool track, PagedDev *out)
+{
+    if (!c) return fox_fail(FOX_GPU_ERR_ARG, "%s: no cache", what);
+    if (!c->k || !c->v || !c->table || c->n_pages == 0 || c->page_size == 0 || c->n_head_kv == 0 ||
+        c->head_dim == 0 || c->n_seqs == 0 || c->max_pages == 0)
+        return fox_fail(FOX_GPU_ERR_ARG, "%s: the cache has a null pointer or a zero size", what);
+    if (c->type != FOX_GPU_F16 && c->type != FOX_GPU_BF16)
+        return fox_fail(FOX_GPU_ERR_UNSUPPORTED, "%s: a paged cache is F16 or BF16, not type %d", what, c->type);
+    if (c->head_dim % 8 || c->head_dim > 256)
+        return fox_fail(FOX_GPU_ERR_UNSUPPORTED, "%s: head_dim is a multiple of 8 up to 256, not %zu", what,
+                        c->head_dim);
+    if (c->page_size & (c->page_size - 1) || c->page_size < 16 || c->page_size > 4096)
+        return fox_fail(FOX_GPU_ERR_UNSUPPORTED, "%s: page_size is a power of two from 16 to 4096, not %zu", what,
+                        c->page_size);
+    if (c->n_pages > (1u << 31) || c->n_seqs > 65535 || c->n_head_kv > 4096 ||
+        c->n_seqs * c->n_head_kv > (1u << 20) || c->max_pages > (1u << 30) / c->page_size)
+        return fox_fail(FOX_GPU_ERR_ARG, "%s: %zu pages, %zu sequences of %zu pages, %zu kv heads are too many",
+                        what, c->n_pages, c->n_seqs, c->max_pages, c->n_head_kv);
+    if ((uintptr_t)c->k % 16 || (uintptr_t)c->v % 16)
+        return fox_fail(FOX_GPU_ERR_ARG, "%s: the pools must be 16-byte aligned", what);
+    if ((c->weight == nullptr) != (c->position == nullptr))
+        return fox_fail(FOX_GPU_ERR_ARG, "%s: the cache has one of weight and position", what);
+    if (track && !c->weight)
+        return fox_fail(FOX_GPU_ERR_ARG, "%s: the cache has no weight and position", what);
+    *out = {};
+    out->k = c->k;
+    out->v = c->v;
+    out->table = c->table;
+    out->weight = c->weight;
+    out->position = c->position;
+    out->n_pages = (uint32_t)c->n_pages;
+    out->n_seqs = (uint32_t)c->n_seqs;
+    out->max_pages = (uint32_t)c->max_pages;
+    out->n_kv = (uint32_t)c->n_head_kv;
+    out->hd = (uint32_t)c->head_dim;
+    while (((size_t)1 << out->shift) < c->page_size) out->shift++;
+    out->cap = (uint32_t)(c->max_pages * c->page_size);
+    return FOX_GPU_OK;
+}
+
+// ------------------------------------------------------------------ tables
+
+struct FreqArgs {
+    double turn[128];             // turns a position, pair by pair
+    double magnitude;
+    const float *factors;
+    float *cos_t, *sin_t;
+    uint32_t half, p0;
+    uint64_t total;               // n half
+};
+
+// Angles are counted in turns: what is left of p turn[j] after the nearest quarter is exact,
+// and within an eighth of a turn twelve terms of sine and cosine are good to 2^-36.
+// (Angles in floats would be off by 2^-24 of all the turns made.)
+__global__ __launch_bounds__(PG_THREADS) void rope_tables_k(FreqArgs A)
+{
+    const uint64_t at = (uint64_t)blockIdx.x * PG_THREADS + threadIdx.x;
+    if (at >= A.total) return;
+    const uint32_t j = (uint32_t)(at % A.half);
+    double w = A.turn[j];
+    if (A.factors) w = w / (double)A.factors[j];
+    const double a = (double)(A.p0 + at / A.half) * w, n = rint(4.0 * a);
+    const double x = __builtin_fma(-0.25, n, a) * 6.283185307179586;
+    const double s = sin(x), c = cos(x);
+    const int quarter = (int)((int64_t)n & 3);
+    const double cs = quarter == 0 ? c : quarter == 1 ? -s : quarter == 2 ? -c : s;
+    const double sn = quarter == 0 ? s : quarter == 1 ? c : quarter == 2 ? -s : -c;
+    A.cos_t[at] = (float)(A.magnitude * cs);
+    A.sin_t[at] = (float)(A.magnitude * sn);
+}
+
+extern "C" fox_gpu_status fox_gpu_rope_tables(fox_gpu_ctx *ctx, float *cos_t, float *sin_t, size_t p0, size_t n,
+                                              size_t n_rot, const fox_gpu_rope_freq *f)
+{
+    if (!ctx || !cos_t || !sin_t || !f || n == 0 || n_rot == 0)
+        return fox_fail(FOX_GPU_ERR_ARG, "rope_tables: bad argument");
+    if (n_rot % 2 || n_rot > 256)
+        return fox_fail(FOX_GPU_ERR_UNSUPPORTED, "rope_tables: n_rot is even and at most 256, not %zu", n_rot);
+    if (p0 > (1u << 30) || n > (1u << 30) - p0)
+        return fox_fail(FOX_GPU_ERR_ARG, "rope_tables: %zu positions from %zu on are too many", n, p0);
+    // (a NaN fails every comparison)
+    if (!(f->base > 0.0 && std::isfinite(f->base) && std::isfinite(f->scale) && std::isfinite(f->ext) &&
+          std::isfinite(f->magnitude)))
+        return fox_fail(FOX_GPU_ERR_ARG, "rope_tables: base must be above 0 and every figure finite");
+    double lo = 0.0, hi = 0.0;
+    if (f->ext != 0.0) {
+        if (!(f->base > 1.0 && f->beta_fast > 0.0 && f->beta_slow > 0.0 && f->orig_ctx > 0.0 &&
+              std::isfinite(f->beta_fast) && std::isfinite(f->beta_slow) && std::isfinite(f->orig_ctx)))
+            return fox_fail(FOX_GPU_ERR_ARG, "rope_tables: with ext, base must be above 1, beta_fast, beta_slow "
+                            "and orig_ctx above 0");
+        const double by = (double)n_rot / (2.0 * std::log(f->base));
+        lo = std::fmax(0.0, std::floor(by * std::log(f->orig_ctx / (2.0 * M_PI * f->beta_fast))));
+        hi = std::fmin((double)n_rot - 1.0, std::ceil(by * std::log(f->orig_ctx / (2.0 * M_PI * f->beta_slow))));
+    }
+    FreqArgs A = {};
+    A.half = (uint32_t)(n_rot / 2);
+    for (uint32_t j = 0; j < A.half; j++) {
+        double mix = 0.0;
+        if (f->ext != 0.0) {
+            const double ramp = ((double)j - lo) / std::fmax(hi - lo, 0.001);
+            mix = f->ext * (1.0 - std::fmin(std::fmax(ramp, 0.0), 1.0));
+        }
+        A.turn[j] = std::pow(f->base, -2.0 * j / (double)n_rot) * (f->scale * (1.0 - mix) + mix) / (2.0 * M_PI);
+    }
+    A.magnitude = f->magnitude;
+    A.factors = f->factors;
+    A.cos_t = cos_t;
+    A.sin_t = sin_t;
+    A.p0 = (uint32_t)p0;
+    A.total = (uint64_t)n * A.half;
+    FOX_HIP(hipSetDevice(ctx->device));
+    rope_tables_k<<<dim3((unsigned)((A.total + PG_THREADS - 1) / PG_THREADS)), dim3(PG_THREADS), 0, ctx->stream>>>(A);
+    FOX_LAUNCHED("rope_tables");
+    return FOX_GPU_OK;
+}
+
+// ----------------------------------------------------------------- storing
+
+struct PagedStoreArgs {
+    PagedDev C;
+    const float *q, *k, *v, *q_norm, *k_norm, *cos_t, *sin_t;
+    float *q_out;
+    size_t q_stride, qo_stride, k_stride, v_stride;
+    const uint32_t *pos, *seq, *row;
+    uint32_t n_head, M, n_rot, n_table;
+    float eps;
+    int halves;
+};
+
+// One wave per (token, head): keys first, then values, then queries.
+template <bool BF>
+__global__ __launch_bounds__(PG_THREADS) void paged_store_k(PagedStoreArgs A)
+{
+    __shared__ double lds[PG_THREADS / 64][256];
+    const uint32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6, hd = A.C.hd;
+    const uint32_t heads = A.n_head + 2 * A.C.n_kv;
+    const uint32_t at = blockIdx.y * (PG_THREADS / 64) + w, t = blockIdx.x;
+    const bool on = at < heads;
+    const uint32_t part = at < A.C.n_kv ? 0 : at < 2 * A.C.n_kv ? 1 : 2;
+    const uint32_t h = on ? at - part * A.C.n_kv : 0;
+    const uint32_t s = A.seq ? A.seq[t] : t, p = A.pos[t];
+    if (s >= A.C.n_seqs || p >= A.n_table) return;       // (uniform)
+    const float *src = part == 0 ? A.k + t * A.k_stride : part == 1 ? A.v + t * A.v_stride : A.q + t * A.q_stride;
+    const float *nw = part == 0 ? A.k_norm : part == 1 ? nullptr : A.q_norm;
+    double *x = lds[w];
+    double ss = 0.0;
+    if (on)
+        for (uint32_t d = lane; d < hd; d += 64) {
+            x[d] = (double)src[(size_t)h * hd + d];
+            ss += x[d] * x[d];
+        }
+    for (int m = 32; m; m >>= 1) ss += __shfl_xor(ss, m);
+    __syncthreads();
+    if (!on) return;
+    const double inv = nw ? 1.0 / sqrt(ss / (double)hd + (double)A.eps) : 1.0;
+    const uint32_t r = A.row ? A.row[t] : p, half = A.n_rot / 2;
+    const size_t to = part == 2 || r >= A.C.cap ? ~(size_t)0 : paged_row(A.C, s, h, r);
+    if (part != 2 && to == ~(size_t)0) return;
+    for (uint32_t d = lane; d < hd; d += 64) {
+        double y = x[d] * inv;
+        if (nw) y *= (double)nw[d];
+        if (part != 1 && d < A.n_rot) {
+            const bool second = A.halves ? d >= half : d & 1;
+            const uint32_t o = A.halves ? (second ? d - half : d + half) : d ^ 1;
+            const uint32_t j = A.halves ? (second ? d - half : d) : d / 2;
+            double z = x[o] * inv;
+            if (nw) z *= (double)nw[o];
+            const double c = (double)A.cos_t[(size_t)p * half + j], sn = (double)A.sin_t[(size_t)p * half + j];
+            y = second ? z * sn + y * c : y * c - z * sn;
+        }
+        if (part == 2) A.q_out[t * A.qo_stride + (size_t)h * hd + d] = (float)y;
+        else ((uint16_t *)(part ? A.C.v : A.C.k))[to + d] = paged_round<BF>((float)y);
+    }
+    if (part == 0 && lane == 0 && A.C.weight) {
+        const size_t i = ((size_t)s * A.C.n_kv + h) * A.C.cap + r;
+        A.C.weight[i] = 0.0f;
+        A.C.position[i] = p;
+    }
+}
+
+extern "C" fox_gpu_status fox_gpu_paged_rope_store(
+    fox_gpu_ctx *ctx, const fox_gpu_paged *cache, const float *q, size_t q_stride, float *q_out,
+    size_t q_out_stride, size_t n_head, const float *k, size_t k_stride, const float *v,
+    size_t v_stride, size_t M, const float *q_norm, const float *k_norm, float eps, int pairs,
+    size_t n_rot, const float *cos_t, const float *sin_t, size_t n_table, const uint32_t *pos,
+    const uint32_t *seq, const uint32_t *row)
+{
+    if (!ctx || !q || !q_out || !k || !v || !cos_t || !sin_t || !pos || n_head == 0 || M == 0 || n_table == 0)
+        return fox_fail(FOX_GPU_ERR_ARG, "paged_rope_store: bad argument");
+    PagedStoreArgs A = {};
+    fox_gpu_status st = fox_paged_check("paged_rope_store", cache, false, &A.C);
+    if (st) return st;
+    const size_t nq = n_head * cache->head_dim, nkv = cache->n_head_kv * cache->head_dim;
+    if (pairs != FOX_GPU_PAIRS_ADJACENT && pairs != FOX_GPU_PAIRS_HALVES)
+        return fox_fail(FOX_GPU_ERR_ARG, "paged_rope_store: unknown pairing %d", pairs);
+    if (n_rot == 0 || n_rot % 2 || n_rot > cache->head_dim)
+        return fox_fail(FOX_GPU_ERR_ARG, "paged_rope_store: n_rot is even and at most head_dim, not %zu", n_rot);
+    if (M > FOX_GPU_BATCH_TOKENS) return fox_fail(FOX_GPU_ERR_ARG, "paged_rope_store: too many tokens");
+    if (n_head > 65535) return fox_fail(FOX_GPU_ERR_ARG, "paged_rope_store: %zu heads are too many", n_head);
+    if (n_table > (1u << 30))
+        return fox_fail(FOX_GPU_ERR_ARG, "paged_rope_store: tables of %zu positions are too long", n_table);
+    if (M > 1 && (q_stride < nq || q_out_stride < nq || k_stride < nkv || v_stride < nkv))
+        return fox_fail(FOX_GPU_ERR_ARG, "paged_rope_store: a stride below the row's width");
+    if (!seq && M > cache->n_seqs)
+        return fox_fail(FOX_GPU_ERR_ARG, "paged_rope_store: %zu tokens for %zu sequences", M, cache->n_seqs);
+    A.q = q;
+    A.k = k;
+    A.v = v;
+    A.q_norm = q_norm;
+    A.k_norm = k_norm;
+    A.cos_t = cos_t;
+    A.sin_t = sin_t;
+    A.q_out = q_out;
+    A.q_stride = q_stride;
+    A.qo_stride = q_out_stride;
+    A.k_stride = k_stride;
+    A.v_stride = v_stride;
+    A.pos = pos;
+    A.seq = seq;
+    A.row = row;
+    A.n_head = (uint32_t)n_head;
+    A.M = (uint32_t)M;
+    A.n_rot = (uint32_t)n_rot;
+    A.n_table = (uint32_t)n_table;
+    A.eps = eps;
+    A.halves = pairs == FOX_GPU_PAIRS_HALVES;
+    FOX_HIP(hipSetDevice(ctx->device));
+    const dim3 grid((unsigned)M, (unsigned)((n_head + 2 * cache->n_head_kv + 3) / 4));
+    if (cache->type == FOX_GPU_BF16)
+        paged_store_k<true><<<grid, dim3(PG_THREADS), 0, ctx->stream>>>(A);
+    else
+        paged_store_k<false><<<grid, dim3(PG_THREADS), 0, ctx->stream>>>(A);
+    FOX_LAUNCHED("paged_rope_store");
+    return FOX_GPU_OK;
+}
+
+// ---------------------------------------------------------------- eviction
+
+#define EV_THREADS 1024
+#define EV_MOVERS 8              // workgroups that move a kv head's rows
+
+struct EvictArgs {
+    PagedDev C;
+    const uint32_t *length;
+    uint32_t *kept, *list;        // places, then rows to move, of every kv head: 2 room each
+    uint32_t *count;              // rows to move of every kv head
+    uint32_t keep, recent, room;
+};
+
+// a row's rank: the newest before all, then by weight (0 and above)
+__device__ __forceinline__ uint32_t evict_key(float w, uint32_t p, uint32_t newest, uint32_t recent)
+{
+    if (newest - p < recent) return 0xFFFFFFFFu;
+    return w > 0.0f ? __float_as_uint(w) : 0u;
+}
+
+// sum of every thread's v (exclusive of its own, in thread order), and the total
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *lds, uint32_t &total)
+{
+    const uint32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    uint32_t x = v;
+    for (uint32_t m = 1; m < 64; m <<= 1) {
+        const uint32_t y = __shfl_up(x, m);
+        if (lane >= m) x += y;
+    }
+    if (lane == 63) lds[w] = x;
+    __syncthreads();
+    uint32_t before = 0;
+    total = 0;
+    for (uint32_t i = 0; i < EV_THREADS / 64; i++) {
+        if (i < w) before += lds[i];
+        total += lds[i];
+    }
+    __syncthreads();
+    return before + x - v;
+}
+
+// One workgroup per (kv head, sequence) finds the least key that is kept, by its
+// bytes from the top: a histogram of the keys that share the bytes found so
+// far says which next byte holds the keep-th key.  Rows above it and the first
+// of those equal to it are kept; the places and the rows that fill them are listed in order.
+__global__ __launch_bounds__(EV_THREADS) void evict_select_k(EvictArgs A)
+{
+    __shared__ uint32_t hist[256], lds[EV_THREADS / 64], found[2];
+    const uint32_t h = blockIdx.x, s = blockIdx.y, tid = threadIdx.x;
+    const size_t head = (size_t)s * A.C.n_kv + h;
+    const uint32_t n = min(A.length[s], A.C.cap);
+    if (h == 0 && tid == 0) A.kept[s] = min(n, A.keep);
+    if (n <= A.keep) {
+        if (tid == 0) A.count[head] = 0;
+        return;
+    }
+    const float *weight = A.C.weight + head * A.C.cap;
+    const uint32_t *position = A.C.position + head * A.C.cap;
+    uint32_t newest = 0;
+    for (uint32_t i = tid; i < n; i += EV_THREADS) newest = max(newest, position[i]);
+    for (int m = 32; m; m >>= 1) newest = max(newest, (uint32_t)__shfl_xor((int)newest, m));
+    if ((tid & 63) == 0) lds[tid >> 6] = newest;
+    __syncthreads();
+    for (uint32_t i = 0; i < EV_THREADS / 64; i++) newest = max(newest, lds[i]);
+    uint32_t least = 0, want = A.keep;       // the bytes found; rows still to take among those that share them
+    for (int at = 24; at >= 0; at -= 8) {
+        const uint32_t mask = at == 24 ? 0u : 0xFFFFFFFFu << (at + 8);
+        if (tid < 256) hist[tid] = 0;
+        __syncthreads();
+        for (uint32_t i = tid; i < n; i += EV_THREADS) {
+            const uint32_t key = evict_key(weight[i], position[i], newest, A.recent);
+            if ((key & mask) == least) atomicAdd(&hist[key >> at & 255u], 1u);
+        }
+        __syncthreads();
+        if (tid == 0) {
+            uint32_t left = want, b = 255;
+            for (;; b--) {
+                if (hist[b] >= left || b == 0) break;
+                left -= hist[b];
+            }
+            found[0] = least | b << at;
+            found[1] = left;
+        }
+        __syncthreads();
+        least = found[0];
+        want = found[1];
+        __syncthreads();
+    }
+    uint32_t *to = A.list + head * 2 * A.room, *from = to + A.room;
+    uint32_t ties = 0, places = 0, movers = 0, total;
+    for (uint32_t base = 0; base < n; base += EV_THREADS) {
+        const uint32_t i = base + tid;
+        const uint32_t key = i < n ? evict_key(weight[i], position[i], newest, A.recent) : 0u;
+        const bool tie = i < n && key == least;
+        const uint32_t mine = ties + block_scan(tie, lds, total);
+        ties += total;
+        const bool stays = i < n && (key > least || (tie && mine < want));
+        const bool place = i < A.keep && !stays, mover = i >= A.keep && stays;
+        const uint32_t a = places + block_scan(place, lds, total);
+        places += total;
+        const uint32_t b = movers + block_scan(mover, lds, total);
+        movers += total;
+        if (place && a < A.room) to[a] = i;
+        if (mover && b < A.room) from[b] = i;
+    }
+    if (tid == 0) A.count[head] = min(places, movers);   // (equal)
+}
+
+// rows to their places: no place is another's row, so in any order
+__global__ __launch_bounds__(PG_THREADS) void evict_move_k(EvictArgs A)
+{
+    const uint32_t head = blockIdx.x / EV_MOVERS, h = head % A.C.n_kv, s = head / A.C.n_kv;
+    const uint32_t n = min(A.count[head], A.room), pieces = A.C.hd / 8;
+    const uint32_t *to = A.list + (size_t)head * 2 * A.room, *from = to + A.room;
+    const uint64_t total = (uint64_t)n * pieces * 2;
+    for (uint64_t i = blockIdx.x % EV_MOVERS * PG_THREADS + threadIdx.x; i < total; i += EV_MOVERS * PG_THREADS) {
+        const uint32_t piece = (uint32_t)(i % (2 * pieces)), m = (uint32_t)(i / (2 * pieces));
+        const size_t a = paged_row(A.C, s, h, to[m]), b = paged_row(A.C, s, h, from[m]);
+        uint16_t *pool = (uint16_t *)(piece < pieces ? A.C.k : A.C.v);
+        const uint32_t d = piece % pieces * 8;
+        if (a != ~(size_t)0 && b != ~(size_t)0) *(uint4 *)(pool + a + d) = *(const uint4 *)(pool + b + d);
+        if (piece == 0) {
+            const size_t base = (size_t)head * A.C.cap;
+            A.C.weight[base + to[m]] = A.C.weight[base + from[m]];
+            A.C.position[base + to[m]] = A.C.position[base + from[m]];
+        }
+    }
+}
+
+extern "C" fox_gpu_status fox_gpu_paged_evict(fox_gpu_ctx *ctx, const fox_gpu_paged *cache, const uint32_t *length,
+                                              uint32_t *kept, size_t keep, size_t recent)
+{
+    if (!ctx || !length || !kept || keep == 0) return fox_fail(FOX_GPU_ERR_ARG, "paged_evict: bad argument");
+    EvictArgs A = {};
+    fox_gpu_status st = fox_paged_check("paged_evict", cache, true, &A.C);
+    if (st) return st;
+    if (recent > keep)
+        return fox_fail(FOX_GPU_ERR_ARG, "paged_evict: the %zu newest rows are more than the %zu kept", recent, keep);
+    const uintptr_t la = (uintptr_t)length, ka = (uintptr_t)kept, size = cache->n_seqs * sizeof(uint32_t);
+    if (la < ka + size && ka < la + size)
+        return fox_fail(FOX_GPU_ERR_ARG, "paged_evict: kept must be another array than length");
+    A.length = length;
+    A.kept = kept;
+    A.keep = (uint32_t)(keep < A.C.cap ? keep : A.C.cap);
+    A.recent = (uint32_t)(recent < A.C.cap ? recent : A.C.cap);
+    // at most so many rows can move
+    A.room = A.C.cap - A.keep < A.keep ? A.C.cap - A.keep : A.keep;
+    const size_t heads = cache->n_seqs * cache->n_head_kv;
+    if ((st = fox_ws_reserve(ctx, (heads + heads * 2 * A.room) * sizeof(uint32_t)))) return st;
+    A.count = (uint32_t *)ctx->ws;
+    A.list = A.count + heads;
+    FOX_HIP(hipSetDevice(ctx->device));
+    evict_select_k<<<dim3((unsigned)cache->n_head_kv, (unsigned)cache->n_seqs), dim3(EV_THREADS), 0, ctx->stream>>>(A);
+    FOX_LAUNCHED("paged_evict");
+    if (A.room) {
+        evict_move_k<<<dim3((unsigned)(heads * EV_MOVERS)), dim3(PG_THREADS), 0, ctx->stream>>>(A);
+        FOX_LAUNCHED("paged_evict");
+    }
+    return FOX_GPU_OK;
+}
