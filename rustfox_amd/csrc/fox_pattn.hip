@@ -55,12 +55,6 @@ struct PagedAttnArgs {
 
 // ---------------------------------------------------------------- division
 
-// Units of a call: rows' heads (items) in order, each as many as its row has.
-struct PagedWork {
-    uint64_t run;                // units of a worker
-    uint64_t total;
-};
-
 __device__ __forceinline__ uint32_t row_length(const PagedAttnArgs &A, uint32_t t)
 {
     const uint32_t s = A.seq ? A.seq[t] : t;
@@ -69,38 +63,102 @@ __device__ __forceinline__ uint32_t row_length(const PagedAttnArgs &A, uint32_t 
 
 __device__ __forceinline__ uint32_t units_of(uint32_t n) { return (n + PA_UNIT - 1) / PA_UNIT; }
 
-// start[t] = units of one item of each row before t, t = 0 .. M, by the workgroup
+// Where the units of each row begin, counted for one of its heads (an item): up to 64
+// rows by every wave for itself, lane t row t, without LDS or a barrier; more by the
+// workgroup, in LDS.
+struct PagedWork {
+    const uint64_t *start;        // [M + 1], past 64 rows
+    uint64_t run, total;          // units of a worker; of the call
+    uint32_t items, M, before, units;
+
+    // the row that holds unit u of the call, and its first unit of one item
+    __device__ __forceinline__ uint32_t row_of(uint64_t u, uint64_t &first, uint32_t &n) const
+    {
+        uint32_t t;
+        if (M <= 64) {
+            const uint32_t lane = threadIdx.x & 63;
+            t = 63 - __builtin_clzll(__ballot(lane < M && (uint64_t)before * items <= u));
+        } else {
+            uint32_t lo = 0, hi = M;                        // the last with start items <= u
+            while (hi - lo > 1) {
+                const uint32_t mid = (lo + hi) / 2;
+                if (start[mid] * items <= u) lo = mid;
+                else hi = mid;
+            }
+            t = __builtin_amdgcn_readfirstlane(lo);
+        }
+        row(t, first, n);
+        return t;
+    }
+    __device__ __forceinline__ void row(uint32_t t, uint64_t &first, uint32_t &n) const
+    {
+        if (M <= 64) {
+            first = (uint32_t)__builtin_amdgcn_readlane((int)before, t);
+            n = (uint32_t)__builtin_amdgcn_readlane((int)units, t);
+        } else {
+            first = start[t];
+            n = (uint32_t)(start[t + 1] - first);
+        }
+    }
+    // the workers whose runs hold an item's units: first and last
+    __device__ __forceinline__ void runs(uint32_t t, uint32_t item, uint32_t &a, uint32_t &b) const
+    {
+        uint64_t first;
+        uint32_t n;
+        row(t, first, n);
+        const uint64_t u = first * items + (uint64_t)item * n;
+        a = (uint32_t)(u / run);
+        b = (uint32_t)((u + n - 1) / run);
+    }
+};
+
 __device__ __forceinline__ PagedWork divide(const PagedAttnArgs &A, uint64_t *start)
 {
     __shared__ uint64_t sums[PA_WAVES];
     const uint32_t tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    const uint32_t each = (A.M + PA_THREADS - 1) / PA_THREADS;      // (at most 4)
-    uint64_t mine = 0;
-    for (uint32_t i = 0; i < each; i++) {
-        const uint32_t t = tid * each + i;
-        if (t < A.M) mine += units_of(row_length(A, t));
+    PagedWork D;
+    D.start = start;
+    D.M = A.M;
+    D.items = A.C.n_kv * A.tiles;
+    if (A.M <= 64) {
+        D.units = lane < A.M ? units_of(row_length(A, lane)) : 0;   // (64 of at most 2^24)
+        uint32_t x = D.units;
+        if (A.M > 1)
+#pragma unroll
+            for (uint32_t m = 1; m < 64; m <<= 1) {
+                const uint32_t y = __shfl_up(x, m);
+                if (lane >= m) x += y;
+            }
+        D.before = x - D.units;
+        D.total = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)x, (int)A.M - 1) * D.items;
+    } else {
+        const uint32_t each = (A.M + PA_THREADS - 1) / PA_THREADS;  // (at most 4)
+        uint64_t mine = 0;
+        for (uint32_t i = 0; i < each; i++) {
+            const uint32_t t = tid * each + i;
+            if (t < A.M) mine += units_of(row_length(A, t));
+        }
+        uint64_t x = mine;
+        for (uint32_t m = 1; m < 64; m <<= 1) {
+            const uint64_t y = __shfl_up((unsigned long long)x, m);
+            if (lane >= m) x += y;
+        }
+        if (lane == 63) sums[w] = x;
+        __syncthreads();
+        uint64_t before = x - mine;
+        for (uint32_t i = 0; i < w; i++) before += sums[i];
+        for (uint32_t i = 0; i < each; i++) {
+            const uint32_t t = tid * each + i;
+            if (t >= A.M) break;
+            start[t] = before;
+            before += units_of(row_length(A, t));
+        }
+        if (tid == PA_THREADS - 1) start[A.M] = before;
+        __syncthreads();
+        D.total = start[A.M] * D.items;
     }
-    uint64_t x = mine;
-    for (uint32_t m = 1; m < 64; m <<= 1) {
-        const uint64_t y = __shfl_up((unsigned long long)x, m);
-        if (lane >= m) x += y;
-    }
-    if (lane == 63) sums[w] = x;
-    __syncthreads();
-    uint64_t before = x - mine;
-    for (uint32_t i = 0; i < w; i++) before += sums[i];
-    for (uint32_t i = 0; i < each; i++) {
-        const uint32_t t = tid * each + i;
-        if (t > A.M) break;
-        start[t] = before;
-        if (t < A.M) before += units_of(row_length(A, t));
-    }
-    if (tid == PA_THREADS - 1) start[A.M] = before;
-    __syncthreads();
-    PagedWork d;
-    d.total = start[A.M] * A.C.n_kv * A.tiles;
-    d.run = (d.total + A.workers - 1) / A.workers;
-    return d;
+    D.run = (D.total + A.workers - 1) / A.workers;
+    return D;
 }
 
 // ------------------------------------------------------------------- tiles
@@ -221,42 +279,55 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_k(PagedAttnArgs A)
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t hd = FULL ? W : A.C.hd, width = A.C.n_kv * A.G * hd;
     const PagedWork D = divide(A, start);
-    for (uint32_t t = blockIdx.x; t < A.M; t += gridDim.x)
-        if (start[t] == start[t + 1])
+    for (uint32_t t = blockIdx.x; t < A.M; t += gridDim.x) {
+        uint64_t first;
+        uint32_t n;
+        D.row(t, first, n);
+        if (n == 0)
             for (uint32_t d = tid; d < width; d += PA_THREADS) A.out[t * A.out_stride + d] = 0.0f;
+    }
     uint64_t u = blockIdx.x * D.run;
     const uint64_t end = min(u + D.run, D.total);
-    const uint32_t items = A.C.n_kv * A.tiles;
     while (u < end) {                                       // (uniform)
-        uint32_t lo = 0, hi = A.M;                          // row: the last with start items <= u
-        while (hi - lo > 1) {
-            const uint32_t mid = (lo + hi) / 2;
-            if (start[mid] * items <= u) lo = mid;
-            else hi = mid;
-        }
-        const uint32_t t = __builtin_amdgcn_readfirstlane(lo);
-        const uint32_t units = (uint32_t)(start[t + 1] - start[t]);
-        const uint64_t in_row = u - start[t] * items;
+        uint64_t first;
+        uint32_t units;
+        const uint32_t t = D.row_of(u, first, units);
+        const uint64_t in_row = u - first * D.items;
         const uint32_t item = __builtin_amdgcn_readfirstlane((uint32_t)(in_row / units));
-        const uint32_t k0 = __builtin_amdgcn_readfirstlane((uint32_t)(in_row % units));
+        const uint32_t k0 = __builtin_amdgcn_readfirstlane((uint32_t)(in_row - (uint64_t)item * units));
         const uint32_t k1 = __builtin_amdgcn_readfirstlane((uint32_t)min((uint64_t)units, k0 + (end - u)));
         const uint32_t h = item / A.tiles, h0 = item % A.tiles * A.per, heads = min(A.per, A.G - h0);
         const uint32_t n = __builtin_amdgcn_readfirstlane(row_length(A, t));
         const uint32_t s = A.seq ? A.seq[t] : t;
         const uint32_t *table = A.C.table + (size_t)s * A.C.max_pages;
 
-        // the queries
+        // the queries' rows and the first tile are asked for together
+        float x[NC][8], top = 0.0f;
+        {
+            const float *row = A.q + t * A.q_stride + (size_t)(h * A.G + h0 + (i < heads ? i : 0)) * hd;
+#pragma unroll
+            for (int c = 0; c < NC; c++) load_q(x[c], row, 32 * c + 8 * g, hd, i < heads, A.q_wide);
+        }
+        Tile<W> now, next;
+        const uint32_t in_page = (1u << A.C.shift) - 1;
+        auto load = [&](Tile<W> &T, uint32_t page, uint32_t p) {       // p: a tile's first position
+            const size_t at = ((((size_t)page * A.C.n_kv + h) << A.C.shift) + (p & in_page)) * hd;
+            load_tile<W, FULL>(T, A, (const uint16_t *)A.C.k + at, (const uint16_t *)A.C.v + at);
+        };
+        uint32_t p0 = k0 * PA_UNIT + wave * PA_TILE;
+        const uint32_t stop = min(n, k1 * PA_UNIT);
+        // pages of this tile and the next, read one tile before its rows are
+        uint32_t page = p0 < stop ? table[p0 >> A.C.shift] : ~0u;
+        uint32_t page_next = p0 + PA_UNIT < stop ? table[(p0 + PA_UNIT) >> A.C.shift] : ~0u;
+        if (page < A.C.n_pages) load(now, page, p0);
+
         uint4 q[QLDS ? 1 : NC][NP];
         float factor;
         {
-            const float *row = A.q + t * A.q_stride + (size_t)(h * A.G + h0 + (i < heads ? i : 0)) * hd;
-            float x[NC][8], top = 0.0f;
 #pragma unroll
-            for (int c = 0; c < NC; c++) {
-                load_q(x[c], row, 32 * c + 8 * g, hd, i < heads, A.q_wide);
+            for (int c = 0; c < NC; c++)
 #pragma unroll
                 for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(x[c][j]));
-            }
             int e = 0;
             if (!BF) {
                 top = max_of_groups(top);
@@ -281,29 +352,18 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_k(PagedAttnArgs A)
 #pragma unroll
         for (int a = 0; a < NA; a++) acc[a] = f4v{0, 0, 0, 0};
         float m = -INFINITY, l = 0.0f;
-        Tile<W> now, next;
-        const uint32_t in_page = (1u << A.C.shift) - 1;
-        auto load = [&](Tile<W> &T, uint32_t p0) -> bool {           // p0: a tile's first position
-            const uint32_t page = table[p0 >> A.C.shift];
-            if (page >= A.C.n_pages) return false;
-            const size_t at = ((((size_t)page * A.C.n_kv + h) << A.C.shift) + (p0 & in_page)) * hd;
-            load_tile<W, FULL>(T, A, (const uint16_t *)A.C.k + at, (const uint16_t *)A.C.v + at);
-            return true;
-        };
-        uint32_t p0 = k0 * PA_UNIT + wave * PA_TILE;
-        const uint32_t stop = min(n, k1 * PA_UNIT);
-        bool there = p0 < stop && load(now, p0);
         while (p0 < stop) {
-            const uint32_t p1 = p0 + PA_UNIT;
-            const bool then = p1 < stop && load(next, p1);
-            if (there) {
+            const uint32_t p1 = p0 + PA_UNIT, p2 = p1 + PA_UNIT;
+            const uint32_t page_after = p2 < stop ? table[p2 >> A.C.shift] : ~0u;
+            if (page_next < A.C.n_pages) load(next, page_next, p1);
+            if (page < A.C.n_pages) {
                 f4v S = {0, 0, 0, 0};
 #pragma unroll
                 for (int c = 0; c < NC; c++)
 #pragma unroll
                     for (int k = 0; k < NP; k++)
                         S = mfma_16<BF>(now.k[c], QLDS ? qlds[(c * NP + k) * 64 + lane] : q[QLDS ? 0 : c][k], S);
-                float sc[4], top;
+                float sc[4];
                 const uint32_t p = p0 + 4 * g;
 #pragma unroll
                 for (int r = 0; r < 4; r++) sc[r] = S[r] * factor;
@@ -320,7 +380,7 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_k(PagedAttnArgs A)
                 }
                 if (WEIGH && i < heads)
                     *(f4v *)(A.scores + ((size_t)t * A.C.n_kv * A.G + h * A.G + h0 + i) * A.C.cap + p) = *(f4v *)sc;
-                top = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
+                const float top = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
                 if (__any(top > m + PA_ROOM)) {
                     const float mx = fmaxf(m, max_of_groups(top));
                     const float f = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mx);
@@ -352,7 +412,8 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_k(PagedAttnArgs A)
                 }
             }
             now = next;
-            there = then;
+            page = page_next;
+            page_next = page_after;
             p0 = p1;
         }
 
@@ -380,7 +441,7 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_k(PagedAttnArgs A)
         }
         __syncthreads();
         const bool whole = k0 == 0 && k1 == units;
-        const size_t slot = (size_t)blockIdx.x + (size_t)t * items + item;
+        const size_t slot = (size_t)blockIdx.x + (size_t)t * D.items + item;
         for (uint32_t x = tid; x < heads * hd; x += PA_THREADS) {
             const uint32_t j = x / hd, d = x % hd;
             float y = sums[x];
@@ -408,37 +469,66 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_k(PagedAttnArgs A)
 
 // ------------------------------------------------------------------- merge
 
-// the workers whose runs hold an item's units: first and last
-__device__ __forceinline__ void runs_of(const PagedWork &D, const uint64_t *start, uint32_t items, uint32_t t,
-                                        uint32_t item, uint32_t &first, uint32_t &last)
+// A head's maximum and sum over its parts, first .. last, by a wave: a lane a part.
+// `stats` of the head in part 0.
+__device__ __forceinline__ void all_parts(const float *stats, size_t stride, uint32_t first, uint32_t last, float &top,
+                                          float &all)
 {
-    const uint64_t units = start[t + 1] - start[t], u = start[t] * items + item * units;
-    first = (uint32_t)(u / D.run);
-    last = (uint32_t)((u + units - 1) / D.run);
+    const uint32_t lane = threadIdx.x & 63;
+    top = -INFINITY;
+    all = 0.0f;
+    for (uint32_t w = first + lane; w <= last; w += 64) {
+        const float m = stats[w * stride], l = stats[w * stride + 1], mx = fmaxf(top, m);
+        all = (top == -INFINITY ? all : all * __builtin_amdgcn_exp2f(top - mx)) +
+              (m == -INFINITY ? l : l * __builtin_amdgcn_exp2f(m - mx));
+        top = mx;
+    }
+    float mx = top;
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
+    if (top != -INFINITY) all *= __builtin_amdgcn_exp2f(top - mx);
+    top = mx;
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) all += __shfl_xor(all, x);
 }
 
-// A workgroup a query head: its parts at one maximum, added in order.
+// A workgroup a query head: its parts at one maximum, added.  A wave takes every
+// fourth part, a lane four dimensions.
 __global__ __launch_bounds__(PA_THREADS) void paged_merge_k(PagedAttnArgs A)
 {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    uint64_t *start = (uint64_t *)lds;
-    const PagedWork D = divide(A, start);
+    __shared__ __attribute__((aligned(16))) float sums[PA_WAVES][256];
+    const PagedWork D = divide(A, (uint64_t *)lds);
     const uint32_t t = blockIdx.y, head = blockIdx.x, h = head / A.G, j = head % A.G, tid = threadIdx.x;
-    const uint32_t items = A.C.n_kv * A.tiles, item = h * A.tiles + j / A.per;
-    if (start[t] == start[t + 1]) return;
-    uint32_t first, last;
-    runs_of(D, start, items, t, item, first, last);
+    const uint32_t wave = tid >> 6, d = (tid & 63) * 4, hd = A.C.hd;
+    const uint32_t item = h * A.tiles + j / A.per;
+    uint64_t at;
+    uint32_t units, first, last;
+    D.row(t, at, units);
+    if (units == 0) return;
+    D.runs(t, item, first, last);
     if (first == last) return;
-    const size_t slot = (size_t)t * items + item;
-    const float *stats = A.stats + j % A.per * 2, *part = A.part + j % A.per * (size_t)A.C.hd;
-    float top = -INFINITY, all = 0.0f, y = 0.0f;
-    for (uint32_t w = first; w <= last; w++) top = fmaxf(top, stats[(slot + w) * A.per * 2]);
-    for (uint32_t w = first; w <= last; w++) {
-        const float m = stats[(slot + w) * A.per * 2], f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - top);
-        all += stats[(slot + w) * A.per * 2 + 1] * f;
-        if (tid < A.C.hd) y += part[(slot + w) * A.per * A.C.hd + tid] * f;
-    }
-    if (tid < A.C.hd) A.out[t * A.out_stride + (size_t)head * A.C.hd + tid] = all == 0.0f ? 0.0f : y / all;
+    const size_t slot = (size_t)t * D.items + item;
+    const float *stats = A.stats + (slot * A.per + j % A.per) * 2;
+    const float *part = A.part + (slot * A.per + j % A.per) * hd + d;
+    float top, all;
+    all_parts(stats, A.per * 2, first, last, top, all);
+    float4 y = {0, 0, 0, 0};
+    if (d < hd)
+#pragma unroll 4
+        for (uint32_t w = first + wave; w <= last; w += PA_WAVES) {
+            const float m = stats[(size_t)w * A.per * 2], f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+            const float4 x = *(const float4 *)(part + (size_t)w * A.per * hd);
+            y.x += x.x * f;
+            y.y += x.y * f;
+            y.z += x.z * f;
+            y.w += x.w * f;
+        }
+    *(float4 *)(sums[wave] + d) = y;
+    __syncthreads();
+    if (tid < hd)
+        A.out[t * A.out_stride + (size_t)head * hd + tid] =
+            all == 0.0f ? 0.0f : (sums[0][tid] + sums[1][tid] + sums[2][tid] + sums[3][tid]) / all;
 }
 
 // A workgroup a kv head's PA_CHUNK positions: the group's weights of each, from the scores,
@@ -446,23 +536,17 @@ __global__ __launch_bounds__(PA_THREADS) void paged_merge_k(PagedAttnArgs A)
 __global__ __launch_bounds__(PA_THREADS) void paged_weigh_k(PagedAttnArgs A)
 {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    uint64_t *start = (uint64_t *)lds;
-    const PagedWork D = divide(A, start);
-    const uint32_t t = blockIdx.z, h = blockIdx.y, tid = threadIdx.x, items = A.C.n_kv * A.tiles;
+    const PagedWork D = divide(A, (uint64_t *)lds);
+    const uint32_t t = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
     const uint32_t n = row_length(A, t), p0 = blockIdx.x * PA_CHUNK;
     if (p0 >= n) return;
     float sum[PA_CHUNK / PA_THREADS] = {};
     for (uint32_t j = 0; j < A.G; j++) {
         const uint32_t item = h * A.tiles + j / A.per;
         uint32_t first, last;
-        runs_of(D, start, items, t, item, first, last);
-        const float *stats = A.stats + ((size_t)t * items + item) * A.per * 2 + j % A.per * 2;
-        float top = -INFINITY, all = 0.0f;
-        for (uint32_t w = first; w <= last; w++) top = fmaxf(top, stats[(size_t)w * A.per * 2]);
-        for (uint32_t w = first; w <= last; w++) {
-            const float m = stats[(size_t)w * A.per * 2];
-            all += stats[(size_t)w * A.per * 2 + 1] * (m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - top));
-        }
+        D.runs(t, item, first, last);
+        float top, all;
+        all_parts(A.stats + (((size_t)t * D.items + item) * A.per + j % A.per) * 2, A.per * 2, first, last, top, all);
         const float *sc = A.scores + ((size_t)t * A.C.n_kv * A.G + h * A.G + j) * A.C.cap;
         if (all == 0.0f) continue;
 #pragma unroll
