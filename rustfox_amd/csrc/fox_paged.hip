@@ -6,6 +6,8 @@
 #include <cmath>
 #include <cstring>
 
+typedef uint32_t u4v __attribute__((ext_vector_type(4)));
+
 #define PG_THREADS 256
 
 // ------------------------------------------------------------------ shapes
@@ -248,8 +250,9 @@ extern "C" fox_gpu_status fox_gpu_paged_rope_store(
 
 // ---------------------------------------------------------------- eviction
 
-#define EV_THREADS 1024
-#define EV_MOVERS 8              // workgroups that move a kv head's rows
+#define EV_COPIES 2              // of a histogram: lanes that meet in one place wait for each other
+#define EV_FEW 64                // so many rows are moved by the workgroup that finds them
+#define EV_DEEP 4                // rows that a thread of the mover has on the way
 
 struct EvictArgs {
     PagedDev C;
@@ -257,6 +260,7 @@ struct EvictArgs {
     uint32_t *kept, *list;        // places, then rows to move, of every kv head: 2 room each
     uint32_t *count;              // rows to move of every kv head
     uint32_t keep, recent, room;
+    uint32_t movers;              // workgroups that move a kv head's rows
 };
 
 // a row's rank: the newest before all, then by weight (0 and above)
@@ -266,112 +270,309 @@ __device__ __forceinline__ uint32_t evict_key(float w, uint32_t p, uint32_t newe
     return w > 0.0f ? __float_as_uint(w) : 0u;
 }
 
-// sum of every thread's v (exclusive of its own, in thread order), and the total
-__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *lds, uint32_t &total)
+// how many lanes below this one are in the mask
+__device__ __forceinline__ uint32_t lanes_below(uint64_t mask)
 {
-    const uint32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    uint32_t x = v;
-    for (uint32_t m = 1; m < 64; m <<= 1) {
-        const uint32_t y = __shfl_up(x, m);
-        if (lane >= m) x += y;
-    }
-    if (lane == 63) lds[w] = x;
-    __syncthreads();
-    uint32_t before = 0;
-    total = 0;
-    for (uint32_t i = 0; i < EV_THREADS / 64; i++) {
-        if (i < w) before += lds[i];
-        total += lds[i];
-    }
-    __syncthreads();
-    return before + x - v;
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
 }
 
-// One workgroup per (kv head, sequence) finds the least key that is kept, by its
-// bytes from the top: a histogram of the keys that share the bytes found so
-// far says which next byte holds the keep-th key.  Rows above it and the first
-// of those equal to it are kept; the places and the rows that fill them are listed in order.
-__global__ __launch_bounds__(EV_THREADS) void evict_select_k(EvictArgs A)
+// one 16-byte piece of a moved row, keys' pieces before values'; the first takes weight and position along
+__device__ __forceinline__ void move_piece(const EvictArgs &A, size_t head, uint32_t s, uint32_t h, const uint32_t *to,
+                                           const uint32_t *from, uint32_t piece, uint32_t pieces, bool on)
 {
-    __shared__ uint32_t hist[256], lds[EV_THREADS / 64], found[2];
-    const uint32_t h = blockIdx.x, s = blockIdx.y, tid = threadIdx.x;
+    u4v x[EV_DEEP];
+    size_t at[EV_DEEP];
+    float w[EV_DEEP];
+    uint32_t p[EV_DEEP];
+    uint16_t *pool = (uint16_t *)(piece < pieces ? A.C.k : A.C.v) + piece % pieces * 8;
+    const size_t base = head * A.C.cap;
+#pragma unroll
+    for (int i = 0; i < EV_DEEP; i++) {
+        at[i] = ~(size_t)0;
+        x[i] = u4v{0, 0, 0, 0};
+        w[i] = 0.0f;
+        p[i] = 0;
+        if (on && to[i] != ~0u) {
+            const size_t src = paged_row(A.C, s, h, from[i]);
+            if (src != ~(size_t)0) at[i] = paged_row(A.C, s, h, to[i]);
+            if (at[i] != ~(size_t)0) x[i] = *(const u4v *)(pool + src);
+            if (piece == 0) {
+                w[i] = A.C.weight[base + from[i]];
+                p[i] = A.C.position[base + from[i]];
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < EV_DEEP; i++) {
+        if (at[i] != ~(size_t)0) *(u4v *)(pool + at[i]) = x[i];
+        if (on && to[i] != ~0u && piece == 0) {
+            A.C.weight[base + to[i]] = w[i];
+            A.C.position[base + to[i]] = p[i];
+        }
+    }
+}
+
+// The bin of BINS that holds the want-th key from the top, its keys, and want less those
+// above it.  A wave sums its share of the bins, from the highest wave 0's; then
+// each finds the share, and in that the bin, for itself.  By the workgroup.
+template <int BINS, int WAVES>
+__device__ __forceinline__ uint32_t find_bin(const uint32_t (*hist)[BINS], uint32_t *shares, uint32_t &want, uint32_t &in)
+{
+    constexpr int SHARE = BINS / WAVES, EACH = SHARE / 64;
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    auto bins = [&](uint32_t share, uint32_t x[EACH]) -> uint32_t {      // a lane's bins, the highest first
+        uint32_t sum = 0;
+#pragma unroll
+        for (int i = 0; i < EACH; i++) {
+            x[i] = 0;
+#pragma unroll
+            for (int k = 0; k < EV_COPIES; k++) x[i] += hist[k][BINS - 1 - share * SHARE - lane * EACH - i];
+            sum += x[i];
+        }
+        return sum;
+    };
+    uint32_t x[EACH];
+    __syncthreads();
+    uint32_t above = wave_scan(bins(wave, x));
+    if (lane == 63) shares[wave] = above;
+    __syncthreads();
+    uint32_t sum = lane < WAVES ? shares[lane] : 0;
+    above = wave_scan(sum);
+    const uint32_t share = (uint32_t)__ffsll(__ballot(above >= want)) - 1;
+    want -= (uint32_t)__builtin_amdgcn_readlane((int)(above - sum), (int)share);
+    sum = bins(share, x);
+    above = wave_scan(sum);
+    const int owner = __ffsll(__ballot(above >= want)) - 1;
+    // (the first of the lane's bins that reaches it)
+    uint32_t before = above - sum, bin = EACH - 1;
+#pragma unroll
+    for (int i = 0; i < EACH - 1; i++)
+        if (bin == EACH - 1) {
+            if (before + x[i] >= want) bin = i;
+            else before += x[i];
+        }
+    in = x[EACH - 1];
+#pragma unroll
+    for (int i = 0; i < EACH - 1; i++)
+        if (bin == i) in = x[i];
+    want -= (uint32_t)__builtin_amdgcn_readlane((int)before, owner);
+    in = (uint32_t)__builtin_amdgcn_readlane((int)in, owner);
+    return BINS - 1 - share * SHARE - owner * EACH - (uint32_t)__builtin_amdgcn_readlane((int)bin, owner);
+}
+
+// Exclusive sums pre[0 .. N) of cnt, and the total, by every wave for itself: each writes the
+// same values and reads its own, so the workgroup need not wait.
+template <uint32_t N>
+__device__ __forceinline__ uint32_t scan_counts(const uint32_t *cnt, uint32_t *pre)
+{
+    constexpr uint32_t EACH = N / 64;
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t v[EACH], sum = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < EACH; i++) sum += v[i] = cnt[lane * EACH + i];
+    uint32_t x = wave_scan(sum);
+    const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+    x -= sum;
+#pragma unroll
+    for (uint32_t i = 0; i < EACH; i++) {
+        pre[lane * EACH + i] = x;
+        x += v[i];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    return total;
+}
+
+// One workgroup per (kv head, sequence) finds the least key that is kept, by its 12
+// highest bits (exponent and 3 bits more: most keys are told apart), then 10 and 10: a
+// histogram of the keys that share the bits found so far says which next ones
+// the keep-th key has, and a bin that is wholly kept ends the search.
+// Rows above it and the first of those equal to it are kept; the places and the rows that fill
+// them are listed in order: each wave's 64 rows are counted by a ballot, the counts
+// summed once.  Keys stay in registers, HELD a thread; of longer sequences
+// each turn reads weights and positions anew.  FEW: moves the rows, too.
+//
+// It waits, for loads, LDS and other waves, more than it works.
+template <bool FEW, int THREADS, int HELD>
+__global__ __launch_bounds__(THREADS) void evict_select_k(EvictArgs A)
+{
+    constexpr int WAVES = THREADS / 64, ROWS = THREADS * HELD;
+    static_assert(WAVES * HELD % 64 == 0, "scan_counts");
+    __shared__ uint32_t high[EV_COPIES][4096], low[2][EV_COPIES][1024], shares[3][WAVES], cnt[2][HELD * WAVES], pre[2][HELD * WAVES], red[WAVES];
+    __shared__ uint32_t few[FEW ? 2 * EV_FEW : 1];
+    const uint32_t h = blockIdx.x, s = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const size_t head = (size_t)s * A.C.n_kv + h;
     const uint32_t n = min(A.length[s], A.C.cap);
     if (h == 0 && tid == 0) A.kept[s] = min(n, A.keep);
     if (n <= A.keep) {
-        if (tid == 0) A.count[head] = 0;
+        if (!FEW && tid == 0) A.count[head] = 0;
         return;
     }
     const float *weight = A.C.weight + head * A.C.cap;
     const uint32_t *position = A.C.position + head * A.C.cap;
-    uint32_t newest = 0;
-    for (uint32_t i = tid; i < n; i += EV_THREADS) newest = max(newest, position[i]);
-    for (int m = 32; m; m >>= 1) newest = max(newest, (uint32_t)__shfl_xor((int)newest, m));
-    if ((tid & 63) == 0) lds[tid >> 6] = newest;
-    __syncthreads();
-    for (uint32_t i = 0; i < EV_THREADS / 64; i++) newest = max(newest, lds[i]);
-    uint32_t least = 0, want = A.keep;       // the bytes found; rows still to take among those that share them
-    for (int at = 24; at >= 0; at -= 8) {
-        const uint32_t mask = at == 24 ? 0u : 0xFFFFFFFFu << (at + 8);
-        if (tid < 256) hist[tid] = 0;
-        __syncthreads();
-        for (uint32_t i = tid; i < n; i += EV_THREADS) {
-            const uint32_t key = evict_key(weight[i], position[i], newest, A.recent);
-            if ((key & mask) == least) atomicAdd(&hist[key >> at & 255u], 1u);
-        }
-        __syncthreads();
-        if (tid == 0) {
-            uint32_t left = want, b = 255;
-            for (;; b--) {
-                if (hist[b] >= left || b == 0) break;
-                left -= hist[b];
+    const bool held = n <= ROWS;
+    uint32_t key[HELD], pos[HELD], newest = 0;
+
+    // the greatest position; of a short sequence the keys, too
+    for (uint32_t base = 0; base < n; base += ROWS) {
+#pragma unroll
+        for (int c = 0; c < HELD; c++) {
+            const uint32_t b = base + c * THREADS, i = min(b + tid, n - 1);
+            if (b < n) {                                     // (uniform)
+                pos[c] = position[i];
+                if (held) key[c] = __float_as_uint(weight[i]);
             }
-            found[0] = least | b << at;
-            found[1] = left;
+        }
+        if (base == 0) {
+            for (uint32_t i = tid; i < EV_COPIES * 4096; i += THREADS) (&high[0][0])[i] = 0;
+            for (uint32_t i = tid; i < EV_COPIES * 2048; i += THREADS) (&low[0][0][0])[i] = 0;
+        }
+#pragma unroll
+        for (int c = 0; c < HELD; c++)
+            if (base + c * THREADS < n) newest = max(newest, pos[c]);
+    }
+    newest = wave_max(newest);
+    if (lane == 0) red[wave] = newest;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < WAVES; i++) newest = max(newest, red[i]);
+    if (held) {
+#pragma unroll
+        for (int c = 0; c < HELD; c++)
+            if (c * THREADS < n) key[c] = evict_key(__uint_as_float(key[c]), pos[c], newest, A.recent);
+    }
+    auto read = [&](uint32_t base) {                         // keys of rows base .., where they are not held
+        if (held) return;
+#pragma unroll
+        for (int c = 0; c < HELD; c++) {
+            const uint32_t b = base + c * THREADS, i = min(b + tid, n - 1);
+            if (b < n) key[c] = evict_key(weight[i], position[i], newest, A.recent);
+        }
+    };
+
+    uint32_t least = 0, want = A.keep, in;   // the bits found; rows still to take among those that share them
+    const uint32_t copy = lane % EV_COPIES;
+    for (uint32_t base = 0; base < n; base += ROWS) {
+        read(base);
+#pragma unroll
+        for (int c = 0; c < HELD; c++)
+            if (base + c * THREADS < n && base + c * THREADS + tid < n) atomicAdd(&high[copy][key[c] >> 20], 1u);
+    }
+    least = find_bin<4096, WAVES>(high, shares[0], want, in) << 20;
+    bool every = in == want;                 // those are all taken
+#pragma unroll
+    for (int turn = 0; turn < 2; turn++) {
+        if (every) break;
+        const int at = turn ? 0 : 10;
+        for (uint32_t base = 0; base < n; base += ROWS) {
+            read(base);
+#pragma unroll
+            for (int c = 0; c < HELD; c++)
+                if (base + c * THREADS < n && base + c * THREADS + tid < n && (key[c] ^ least) >> (at + 10) == 0)
+                    atomicAdd(&low[turn][copy][key[c] >> at & 1023u], 1u);
+        }
+        least |= find_bin<1024, WAVES>(low[turn], shares[1 + turn], want, in) << at;
+        every = in == want;
+    }
+
+    uint32_t *to = FEW ? few : A.list + head * 2 * A.room, *from = FEW ? few + EV_FEW : to + A.room;
+    uint32_t ties = 0, places = 0, moves = 0;
+    for (uint32_t base = 0; base < n; base += ROWS) {
+        if (base) __syncthreads();
+        read(base);
+        uint32_t stays = 0;                                  // a bit a row
+        if (every) {
+#pragma unroll
+            for (int c = 0; c < HELD; c++)
+                if (base + c * THREADS < n && base + c * THREADS + tid < n && key[c] >= least) stays |= 1u << c;
+        } else {
+#pragma unroll
+            for (int c = 0; c < HELD; c++) {
+                const uint64_t tie = __ballot(base + c * THREADS < n && base + c * THREADS + tid < n && key[c] == least);
+                if (lane == 0) cnt[0][c * WAVES + wave] = __popcll(tie);
+            }
+            __syncthreads();
+            const uint32_t all = scan_counts<HELD * WAVES>(cnt[0], pre[0]);
+#pragma unroll
+            for (int c = 0; c < HELD; c++)
+                if (base + c * THREADS < n) {
+                    const bool in = base + c * THREADS + tid < n, tie = in && key[c] == least;
+                    const uint32_t rank = ties + pre[0][c * WAVES + wave] + lanes_below(__ballot(tie));
+                    if ((in && key[c] > least) || (tie && rank < want)) stays |= 1u << c;
+                }
+            ties += all;
+        }
+        // places in the low half, rows to move in the high half (a wave's 64 rows are mostly one or the other)
+#pragma unroll
+        for (int c = 0; c < HELD; c++) {
+            const uint32_t r0 = base + c * THREADS + wave * 64;
+            uint32_t x = 0;
+            if (r0 < n) {
+                const bool stay = stays >> c & 1;
+                if (r0 < A.keep) x = __popcll(__ballot(!stay && r0 + lane < A.keep));
+                if (r0 + 64 > A.keep) x |= __popcll(__ballot(stay && r0 + lane >= A.keep)) << 16;
+            }
+            if (lane == 0) cnt[1][c * WAVES + wave] = x;
         }
         __syncthreads();
-        least = found[0];
-        want = found[1];
-        __syncthreads();
+        const uint32_t all = scan_counts<HELD * WAVES>(cnt[1], pre[1]);
+#pragma unroll
+        for (int c = 0; c < HELD; c++) {
+            const uint32_t r0 = base + c * THREADS + wave * 64;
+            if (r0 < n) {
+                const bool stay = stays >> c & 1;
+                const uint32_t x = pre[1][c * WAVES + wave];
+                if (r0 < A.keep) {
+                    const bool place = !stay && r0 + lane < A.keep;
+                    const uint32_t a = places + (x & 0xFFFFu) + lanes_below(__ballot(place));
+                    if (place && a < A.room) to[a] = r0 + lane;
+                }
+                if (r0 + 64 > A.keep) {
+                    const bool mover = stay && r0 + lane >= A.keep;
+                    const uint32_t b = moves + (x >> 16) + lanes_below(__ballot(mover));
+                    if (mover && b < A.room) from[b] = r0 + lane;
+                }
+            }
+        }
+        places += all & 0xFFFFu;
+        moves += all >> 16;
     }
-    uint32_t *to = A.list + head * 2 * A.room, *from = to + A.room;
-    uint32_t ties = 0, places = 0, movers = 0, total;
-    for (uint32_t base = 0; base < n; base += EV_THREADS) {
-        const uint32_t i = base + tid;
-        const uint32_t key = i < n ? evict_key(weight[i], position[i], newest, A.recent) : 0u;
-        const bool tie = i < n && key == least;
-        const uint32_t mine = ties + block_scan(tie, lds, total);
-        ties += total;
-        const bool stays = i < n && (key > least || (tie && mine < want));
-        const bool place = i < A.keep && !stays, mover = i >= A.keep && stays;
-        const uint32_t a = places + block_scan(place, lds, total);
-        places += total;
-        const uint32_t b = movers + block_scan(mover, lds, total);
-        movers += total;
-        if (place && a < A.room) to[a] = i;
-        if (mover && b < A.room) from[b] = i;
+    const uint32_t rows = min(min(places, moves), A.room);   // (places and moves are equal)
+    if (!FEW) {
+        if (tid == 0) A.count[head] = rows;
+        return;
     }
-    if (tid == 0) A.count[head] = min(places, movers);   // (equal)
+    __syncthreads();
+    const uint32_t pieces = A.C.hd / 8, side = THREADS / (2 * pieces);
+    for (uint32_t m = tid / (2 * pieces); m < rows; m += side * EV_DEEP) {
+        uint32_t t[EV_DEEP], f[EV_DEEP];
+#pragma unroll
+        for (int i = 0; i < EV_DEEP; i++) {
+            const bool in = m + i * side < rows;
+            t[i] = in ? to[m + i * side] : ~0u;
+            f[i] = in ? from[m + i * side] : 0u;
+        }
+        move_piece(A, head, s, h, t, f, tid % (2 * pieces), pieces, tid < side * 2 * pieces);
+    }
 }
 
-// rows to their places: no place is another's row, so in any order
+// Rows to their places: no place is another's row, so in any order.  A thread has EV_DEEP
+// rows' pieces on the way, since each waits for the list, the table and the row in turn.
 __global__ __launch_bounds__(PG_THREADS) void evict_move_k(EvictArgs A)
 {
-    const uint32_t head = blockIdx.x / EV_MOVERS, h = head % A.C.n_kv, s = head / A.C.n_kv;
-    const uint32_t n = min(A.count[head], A.room), pieces = A.C.hd / 8;
+    const uint32_t head = blockIdx.x / A.movers, part = blockIdx.x % A.movers, h = head % A.C.n_kv, s = head / A.C.n_kv;
+    const uint32_t n = min(A.count[head], A.room), pieces = A.C.hd / 8, side = PG_THREADS / (2 * pieces);
     const uint32_t *to = A.list + (size_t)head * 2 * A.room, *from = to + A.room;
-    const uint64_t total = (uint64_t)n * pieces * 2;
-    for (uint64_t i = blockIdx.x % EV_MOVERS * PG_THREADS + threadIdx.x; i < total; i += EV_MOVERS * PG_THREADS) {
-        const uint32_t piece = (uint32_t)(i % (2 * pieces)), m = (uint32_t)(i / (2 * pieces));
-        const size_t a = paged_row(A.C, s, h, to[m]), b = paged_row(A.C, s, h, from[m]);
-        uint16_t *pool = (uint16_t *)(piece < pieces ? A.C.k : A.C.v);
-        const uint32_t d = piece % pieces * 8;
-        if (a != ~(size_t)0 && b != ~(size_t)0) *(uint4 *)(pool + a + d) = *(const uint4 *)(pool + b + d);
-        if (piece == 0) {
-            const size_t base = (size_t)head * A.C.cap;
-            A.C.weight[base + to[m]] = A.C.weight[base + from[m]];
-            A.C.position[base + to[m]] = A.C.position[base + from[m]];
+    for (uint64_t m = (uint64_t)part * side * EV_DEEP + threadIdx.x / (2 * pieces); m < n;
+         m += (uint64_t)A.movers * side * EV_DEEP) {
+        uint32_t t[EV_DEEP], f[EV_DEEP];
+#pragma unroll
+        for (int i = 0; i < EV_DEEP; i++) {
+            const bool in = m + i * side < n;
+            t[i] = in ? to[m + i * side] : ~0u;
+            f[i] = in ? from[m + i * side] : 0u;
         }
+        move_piece(A, head, s, h, t, f, threadIdx.x % (2 * pieces), pieces, threadIdx.x < side * 2 * pieces);
     }
 }
 
@@ -394,15 +595,27 @@ extern "C" fox_gpu_status fox_gpu_paged_evict(fox_gpu_ctx *ctx, const fox_gpu_pa
     // at most so many rows can move
     A.room = A.C.cap - A.keep < A.keep ? A.C.cap - A.keep : A.keep;
     const size_t heads = cache->n_seqs * cache->n_head_kv;
+    // Short sequences by 512 threads of 8 rows, long ones by 1024 of 24; the few rows that a step
+    // can give up are moved in the same launch.
+    const bool few = A.room <= EV_FEW, brief = A.C.cap <= 4096;
+    const void *k = few ? brief ? (const void *)evict_select_k<true, 512, 8> : (const void *)evict_select_k<true, 1024, 24>
+                        : brief ? (const void *)evict_select_k<false, 512, 8> : (const void *)evict_select_k<false, 1024, 24>;
+    const dim3 grid((unsigned)cache->n_head_kv, (unsigned)cache->n_seqs), block(brief ? 512 : 1024);
+    void *args[] = {&A};
+    FOX_HIP(hipSetDevice(ctx->device));
+    if (few) {
+        FOX_HIP(hipLaunchKernel(k, grid, block, args, 0, ctx->stream));
+        return FOX_GPU_OK;
+    }
     if ((st = fox_ws_reserve(ctx, (heads + heads * 2 * A.room) * sizeof(uint32_t)))) return st;
     A.count = (uint32_t *)ctx->ws;
     A.list = A.count + heads;
-    FOX_HIP(hipSetDevice(ctx->device));
-    evict_select_k<<<dim3((unsigned)cache->n_head_kv, (unsigned)cache->n_seqs), dim3(EV_THREADS), 0, ctx->stream>>>(A);
+    // one round of rows a workgroup, unless the heads alone are many
+    const size_t round = PG_THREADS / (cache->head_dim / 4) * EV_DEEP, rounds = (A.room + round - 1) / round;
+    const size_t most = (size_t)32 * ctx->n_cu / heads + 1;
+    A.movers = (uint32_t)(rounds < most ? rounds : most);
+    FOX_HIP(hipLaunchKernel(k, grid, block, args, 0, ctx->stream));
+    evict_move_k<<<dim3((unsigned)(heads * A.movers)), dim3(PG_THREADS), 0, ctx->stream>>>(A);
     FOX_LAUNCHED("paged_evict");
-    if (A.room) {
-        evict_move_k<<<dim3((unsigned)(heads * EV_MOVERS)), dim3(PG_THREADS), 0, ctx->stream>>>(A);
-        FOX_LAUNCHED("paged_evict");
-    }
     return FOX_GPU_OK;
 }

@@ -35,3 +35,32 @@ __device__ __forceinline__ float paged_float(uint16_t x)
 {
     return BF ? __uint_as_float((uint32_t)x << 16) : (float)__builtin_bit_cast(_Float16, x);
 }
+
+// Lane l gets the sum of x over lanes 0 .. l, in six adds between neighbours (row shifts, then a
+// row's last lane to the rows after it): a shuffle through LDS takes ten times an add.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x)
+{
+#define FOX_DPP(ctrl, rows) x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, rows, 0xF, false)
+    FOX_DPP(0x111, 0xF);
+    FOX_DPP(0x112, 0xF);
+    FOX_DPP(0x114, 0xF);
+    FOX_DPP(0x118, 0xF);
+    FOX_DPP(0x142, 0xA);
+    FOX_DPP(0x143, 0xC);
+#undef FOX_DPP
+    return x;
+}
+
+// the greatest x of all lanes
+__device__ __forceinline__ uint32_t wave_max(uint32_t x)
+{
+#define FOX_DPP(ctrl, rows) x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, rows, 0xF, false))
+    FOX_DPP(0x111, 0xF);
+    FOX_DPP(0x112, 0xF);
+    FOX_DPP(0x114, 0xF);
+    FOX_DPP(0x118, 0xF);
+    FOX_DPP(0x142, 0xA);
+    FOX_DPP(0x143, 0xC);
+#undef FOX_DPP
+    return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+}

@@ -122,13 +122,7 @@ __device__ __forceinline__ PagedWork divide(const PagedAttnArgs &A, uint64_t *st
     D.items = A.C.n_kv * A.tiles;
     if (A.M <= 64) {
         D.units = lane < A.M ? units_of(row_length(A, lane)) : 0;   // (64 of at most 2^24)
-        uint32_t x = D.units;
-        if (A.M > 1)
-#pragma unroll
-            for (uint32_t m = 1; m < 64; m <<= 1) {
-                const uint32_t y = __shfl_up(x, m);
-                if (lane >= m) x += y;
-            }
+        const uint32_t x = wave_scan(D.units);
         D.before = x - D.units;
         D.total = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)x, (int)A.M - 1) * D.items;
     } else {
