@@ -477,7 +477,8 @@ fox_gpu_status fox_gpu_kvq_attention(fox_gpu_ctx *ctx, float *out, size_t out_st
  *   table     [n_seqs][max_pages] pages of each sequence, in order
  *   weight    [n_seqs][n_head_kv][max_pages * page_size] attention that each row
  *             has got so far, or NULL
- *   position  the same shape: each row's token's position, or NULL (both or none)
+ *   position  the same shape: each row's token's position, or NULL (both or none;
+ *             16-byte aligned)
  * Row r of a sequence is row r % page_size of page table[seq][r / page_size].
  * Pages may come in any order and be shared by sequences that only read them;
  * a page number not below n_pages is no page: its rows are not stored, and

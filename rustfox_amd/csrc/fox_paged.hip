@@ -34,6 +34,8 @@ fox_gpu_status fox_paged_check(const char *what, const fox_gpu_paged *c, bool tr
         return fox_fail(FOX_GPU_ERR_ARG, "%s: the pools must be 16-byte aligned", what);
     if ((c->weight == nullptr) != (c->position == nullptr))
         return fox_fail(FOX_GPU_ERR_ARG, "%s: the cache has one of weight and position", what);
+    if ((uintptr_t)c->weight % 16 || (uintptr_t)c->position % 16)
+        return fox_fail(FOX_GPU_ERR_ARG, "%s: weight and position must be 16-byte aligned", what);
     if (track && !c->weight)
         return fox_fail(FOX_GPU_ERR_ARG, "%s: the cache has no weight and position", what);
     *out = {};

@@ -51,7 +51,7 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x)
     return x;
 }
 
-// the greatest x of all lanes
+// The greatest x of all lanes, and floats' maximum and sum.
 __device__ __forceinline__ uint32_t wave_max(uint32_t x)
 {
 #define FOX_DPP(ctrl, rows) x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, rows, 0xF, false))
@@ -63,4 +63,30 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t x)
     FOX_DPP(0x143, 0xC);
 #undef FOX_DPP
     return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+}
+__device__ __forceinline__ float wave_max(float x)
+{
+#define FOX_DPP(ctrl, rows) \
+    x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp((int)0xFF800000, __float_as_int(x), ctrl, rows, 0xF, false)))
+    FOX_DPP(0x111, 0xF);
+    FOX_DPP(0x112, 0xF);
+    FOX_DPP(0x114, 0xF);
+    FOX_DPP(0x118, 0xF);
+    FOX_DPP(0x142, 0xA);
+    FOX_DPP(0x143, 0xC);
+#undef FOX_DPP
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+}
+__device__ __forceinline__ float wave_sum(float x)
+{
+#define FOX_DPP(ctrl, rows) \
+    x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), ctrl, rows, 0xF, false))
+    FOX_DPP(0x111, 0xF);
+    FOX_DPP(0x112, 0xF);
+    FOX_DPP(0x114, 0xF);
+    FOX_DPP(0x118, 0xF);
+    FOX_DPP(0x142, 0xA);
+    FOX_DPP(0x143, 0xC);
+#undef FOX_DPP
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
 }

@@ -37,7 +37,7 @@ typedef uint32_t u2v __attribute__((ext_vector_type(2)));
 #define PA_TILE 16
 #define PA_UNIT (PA_TILE * PA_WAVES)
 #define PA_ROOM 8.0f             // how far scores may pass the running maximum
-#define PA_CHUNK 2048            // positions that a workgroup weighs
+#define PA_CHUNK 2048            // positions that a workgroup weighs: four a thread
 
 struct PagedAttnArgs {
     PagedDev C;
@@ -131,9 +131,10 @@ struct PagedWork {
     }
 };
 
+template <int THREADS = PA_THREADS>
 __device__ __forceinline__ PagedWork divide(const PagedAttnArgs &A, uint64_t *start)
 {
-    __shared__ uint64_t sums[PA_WAVES];
+    __shared__ uint64_t sums[THREADS / 64];
     const uint32_t tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     PagedWork D;
     D.start = start;
@@ -145,7 +146,7 @@ __device__ __forceinline__ PagedWork divide(const PagedAttnArgs &A, uint64_t *st
         D.before = x - D.units;
         D.total = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)x, (int)A.M - 1) * D.items;
     } else {
-        const uint32_t each = (A.M + PA_THREADS - 1) / PA_THREADS;  // (at most 4)
+        const uint32_t each = (A.M + THREADS - 1) / THREADS;        // (at most 4)
         uint64_t mine = 0;
         for (uint32_t i = 0; i < each; i++) {
             const uint32_t t = tid * each + i;
@@ -166,7 +167,7 @@ __device__ __forceinline__ PagedWork divide(const PagedAttnArgs &A, uint64_t *st
             start[t] = before;
             before += units_of(row_length(A, t));
         }
-        if (tid == PA_THREADS - 1) start[A.M] = before;
+        if (tid == THREADS - 1) start[A.M] = before;
         __syncthreads();
         D.total = start[A.M] * D.items;
     }
@@ -264,6 +265,9 @@ struct Tile {
     u2v u[4];
 };
 
+// ONCE: every row is read by one workgroup of the call (a token of each sequence, one tile of heads), so it need
+// not stay in the caches (the instruction's nt bit): attn-27b-64 298 -> 277 us, attn-4b-1-long 101 -> 90.
+// Of 512 tokens of one sequence, which share its rows, 360 -> 546.
 #define PA_NOWHERE 0x40000000u   // an offset past any descriptor's end
 
 template <int W, bool FULL>
@@ -294,16 +298,16 @@ __device__ __forceinline__ uint32_t here(uint32_t x)
     return x;
 }
 
-template <int W, bool FULL>
+template <int W, bool FULL, bool ONCE>
 __device__ __forceinline__ void load_keys(Tile<W> &T, __amdgpu_buffer_rsrc_t at, const Offsets<W, FULL> &O)
 {
     const uint32_t k = here(O.k[0]);
 #pragma unroll
     for (int c = 0; c < W / 32; c++)
-        T.k[c] = __builtin_amdgcn_raw_buffer_load_b128(at, FULL ? k + 64 * c : O.k[FULL ? 0 : c], 0, 0);
+        T.k[c] = __builtin_amdgcn_raw_buffer_load_b128(at, FULL ? k + 64 * c : O.k[FULL ? 0 : c], 0, ONCE ? 2 : 0);
 }
 
-template <int W, bool FULL>
+template <int W, bool FULL, bool ONCE>
 __device__ __forceinline__ void load_values(Tile<W> &T, __amdgpu_buffer_rsrc_t at, const Offsets<W, FULL> &O, uint32_t hd)
 {
     const uint32_t row = FULL ? W * 2 : hd * 2;
@@ -311,12 +315,12 @@ __device__ __forceinline__ void load_values(Tile<W> &T, __amdgpu_buffer_rsrc_t a
     for (int b = 0; b < W / 128; b++) {
         const uint32_t v = here(O.v[FULL ? 0 : b]) + (FULL ? 256 * b : 0);
 #pragma unroll
-        for (int r = 0; r < 4; r++) T.v[b][r] = __builtin_amdgcn_raw_buffer_load_b128(at, v + r * row, 0, 0);
+        for (int r = 0; r < 4; r++) T.v[b][r] = __builtin_amdgcn_raw_buffer_load_b128(at, v + r * row, 0, ONCE ? 2 : 0);
     }
     if (W % 128) {
         const uint32_t u = here(O.u);
 #pragma unroll
-        for (int r = 0; r < 4; r++) T.u[r] = __builtin_amdgcn_raw_buffer_load_b64(at, u + r * row, 0, 0);
+        for (int r = 0; r < 4; r++) T.u[r] = __builtin_amdgcn_raw_buffer_load_b64(at, u + r * row, 0, ONCE ? 2 : 0);
     }
 }
 
@@ -328,8 +332,8 @@ __device__ __forceinline__ void load_values(Tile<W> &T, __amdgpu_buffer_rsrc_t a
 // column its head's whole score.  The second is then sixteen products of 4x4x1 (a quarter of the
 // matrix unit's time): block b multiplies what its four lanes hold, V's dimensions of
 // one position and the weights of the four heads there.
-template <bool BF, int W, bool FULL, int HG>
-__global__ __launch_bounds__(PA_THREADS, HG == 4 && W <= 128 ? 3 : 2) void paged_attn_k(PagedAttnArgs A)
+template <bool BF, int W, bool FULL, int HG, bool ONCE>
+__global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_k(PagedAttnArgs A)
 {
     constexpr int NC = W / 32, NP = HG == 4 ? 1 : BF ? 3 : 2, NB = W / 128, NU = W % 128 ? 4 : 0, NA = NB * 8 + NU;
     constexpr bool QLDS = W > (HG == 4 ? 192 : 128);     // queries' parts stay in LDS
@@ -356,11 +360,10 @@ __global__ __launch_bounds__(PA_THREADS, HG == 4 && W <= 128 ? 3 : 2) void paged
         end = min(u + D.run, D.total);
     }
     while (u < end) {                                       // (uniform)
-        uint32_t t, item, k0 = 0, k1, units;
+        uint32_t t, item, k0 = 0, k1 = 0, units = 0;
         if (A.whole) {
             t = blockIdx.x / items;
             item = blockIdx.x - t * items;
-            units = k1 = units_of(row_length(A, t));
         } else {
             uint64_t first;
             t = D.row_of(u, first, units);
@@ -372,10 +375,11 @@ __global__ __launch_bounds__(PA_THREADS, HG == 4 && W <= 128 ? 3 : 2) void paged
         t = __builtin_amdgcn_readfirstlane(t);
         item = __builtin_amdgcn_readfirstlane(item);
         k0 = __builtin_amdgcn_readfirstlane(k0);
-        k1 = __builtin_amdgcn_readfirstlane(k1);
         const uint32_t h = item / A.tiles, h0 = item % A.tiles * A.per, heads = min(A.per, A.G - h0);
-        const uint32_t sq = A.seq ? word(A.seq, t) : t;
-        const uint32_t n = sq < A.C.n_seqs ? min(word(A.length, t), A.C.cap) : 0, s = n ? sq : 0;
+        const uint32_t sq = A.seq ? word(A.seq, t) : t, length = word(A.length, t);
+        const uint32_t n = sq < A.C.n_seqs ? min(length, A.C.cap) : 0, s = n ? sq : 0;
+        if (A.whole) units = k1 = units_of(n);
+        k1 = __builtin_amdgcn_readfirstlane(k1);
         const uint32_t *table = A.C.table + (size_t)s * A.C.max_pages;
 
         // the queries' rows and the first tile are asked for together
@@ -391,22 +395,24 @@ __global__ __launch_bounds__(PA_THREADS, HG == 4 && W <= 128 ? 3 : 2) void paged
         Tile<W> one, two;
         const uint32_t in_page = (1u << A.C.shift) - 1, stop = min(n, k1 * PA_UNIT);
         uint32_t p0 = k0 * PA_UNIT + wave * PA_TILE;
-        auto page_of = [&](uint32_t p) -> uint32_t { return p < stop ? word(table, p >> A.C.shift) : ~0u; };
+        // (no branches, so that loads are asked for together: places behind the run give some page of the
+        // sequence and no rows, and an address that is none is not used)
+        auto page_of = [&](uint32_t p) -> uint32_t { return word(table, min(p, A.C.cap - 1) >> A.C.shift); };
         auto rows_of = [&](uint32_t p, uint32_t page) -> uint32_t {   // that are seen
             return p < stop && page < A.C.n_pages ? min(n - p, (uint32_t)PA_TILE) : 0;
         };
         auto tile_at = [&](const void *pool, uint32_t p, uint32_t page) -> __amdgpu_buffer_rsrc_t {
             const uint32_t rows = rows_of(p, page);
-            const size_t at = rows ? ((((size_t)page * A.C.n_kv + h) << A.C.shift) + (p & in_page)) * hd : 0;
+            const size_t at = ((((size_t)page * A.C.n_kv + h) << A.C.shift) + (p & in_page)) * hd;
             return __builtin_amdgcn_make_buffer_rsrc((uint16_t *)pool + at, 0, rows * hd * 2, 0x00027000);
         };
         uint32_t pages[4];       // of this tile and the three after it
 #pragma unroll
         for (int x = 0; x < 4; x++) pages[x] = page_of(p0 + x * PA_UNIT);
-        load_keys<W, FULL>(one, tile_at(A.C.k, p0, pages[0]), O);
-        load_values<W, FULL>(one, tile_at(A.C.v, p0, pages[0]), O, hd);
-        load_keys<W, FULL>(two, tile_at(A.C.k, p0 + PA_UNIT, pages[1]), O);
-        load_values<W, FULL>(two, tile_at(A.C.v, p0 + PA_UNIT, pages[1]), O, hd);
+        load_keys<W, FULL, ONCE>(one, tile_at(A.C.k, p0, pages[0]), O);
+        load_values<W, FULL, ONCE>(one, tile_at(A.C.v, p0, pages[0]), O, hd);
+        load_keys<W, FULL, ONCE>(two, tile_at(A.C.k, p0 + PA_UNIT, pages[1]), O);
+        load_values<W, FULL, ONCE>(two, tile_at(A.C.v, p0 + PA_UNIT, pages[1]), O, hd);
 
         uint4 q[QLDS ? 1 : NC][NP];
         float factor;
@@ -449,7 +455,7 @@ __global__ __launch_bounds__(PA_THREADS, HG == 4 && W <= 128 ? 3 : 2) void paged
 #pragma unroll
                 for (int k = 0; k < NP; k++)
                     S = mfma_16<BF>(T.k[c], QLDS ? qlds[(c * NP + k) * 64 + lane] : q[QLDS ? 0 : c][k], S);
-            load_keys<W, FULL>(T, tile_at(A.C.k, after, pages[2]), O);
+            load_keys<W, FULL, ONCE>(T, tile_at(A.C.k, after, pages[2]), O);
             float sc[4];
             const int mine = (int)seen - 4 * (int)g;
 #pragma unroll
@@ -481,7 +487,7 @@ __global__ __launch_bounds__(PA_THREADS, HG == 4 && W <= 128 ? 3 : 2) void paged
                                      : __builtin_amdgcn_mfma_f32_16x16x4f32(v, w, acc[a], 0, 0, 0);
                 }
             }
-            load_values<W, FULL>(T, tile_at(A.C.v, after, pages[2]), O, hd);
+            load_values<W, FULL, ONCE>(T, tile_at(A.C.v, after, pages[2]), O, hd);
             p0 += PA_UNIT;
 #pragma unroll
             for (int x = 0; x < 3; x++) pages[x] = pages[x + 1];
@@ -521,25 +527,29 @@ __global__ __launch_bounds__(PA_THREADS, HG == 4 && W <= 128 ? 3 : 2) void paged
         __syncthreads();
         const bool whole = k0 == 0 && k1 == units;
         const size_t slot = (size_t)(A.whole ? 0 : blockIdx.x) + (size_t)t * items + item;
-        for (uint32_t x = tid; x < heads * hd; x += PA_THREADS) {
+        for (uint32_t x = tid * 4; x < heads * hd; x += PA_THREADS * 4) {
             const uint32_t j = x / hd, d = x - j * hd;
-            float y = 0.0f;
+            f4v y = {0, 0, 0, 0};
 #pragma unroll
-            for (int w = 0; w < PARTS; w++) y += sums[(size_t)w * A.per * hd + x];
+            for (int w = 0; w < PARTS; w++) y += *(const f4v *)(sums + (size_t)w * A.per * hd + x);
             float top = wm[0][j], all = 0.0f;
 #pragma unroll
             for (int w = 1; w < PA_WAVES; w++) top = fmaxf(top, wm[w][j]);
 #pragma unroll
             for (int w = 0; w < PA_WAVES; w++)
                 all += wm[w][j] == -INFINITY ? wl[w][j] : wl[w][j] * __builtin_amdgcn_exp2f(wm[w][j] - top);
-            if (whole)
-                A.out[t * A.out_stride + (size_t)(h * A.G + h0 + j) * hd + d] = all == 0.0f ? 0.0f : y / all;
-            else
-                A.part[(slot * A.per + j) * hd + d] = y;
-            if (d == 0) {
-                A.stats[(slot * A.per + j) * 2] = top;
-                A.stats[(slot * A.per + j) * 2 + 1] = all;
+            if (whole) {
+                float *to = A.out + t * A.out_stride + (size_t)(h * A.G + h0 + j) * hd + d;
+                if (all == 0.0f) y = f4v{0, 0, 0, 0};
+                else y /= all;
+                if (A.out_wide) *(f4v *)to = y;
+                else
+#pragma unroll
+                    for (int k = 0; k < 4; k++) to[k] = y[k];
+            } else {
+                *(f4v *)(A.part + (slot * A.per + j) * hd + d) = y;
             }
+            if (d == 0) *(float2 *)(A.stats + (slot * A.per + j) * 2) = float2{top, all};
         }
         if (A.whole) return;
         __syncthreads();
@@ -549,38 +559,18 @@ __global__ __launch_bounds__(PA_THREADS, HG == 4 && W <= 128 ? 3 : 2) void paged
 
 // ------------------------------------------------------------------- merge
 
-// A head's maximum and sum over its parts, first .. last, by a wave: a lane a part.
-// `stats` of the head in part 0.
-__device__ __forceinline__ void all_parts(const float *stats, size_t stride, uint32_t first, uint32_t last, float &top,
-                                          float &all)
-{
-    const uint32_t lane = threadIdx.x & 63;
-    top = -INFINITY;
-    all = 0.0f;
-    for (uint32_t w = first + lane; w <= last; w += 64) {
-        const float m = stats[w * stride], l = stats[w * stride + 1], mx = fmaxf(top, m);
-        all = (top == -INFINITY ? all : all * __builtin_amdgcn_exp2f(top - mx)) +
-              (m == -INFINITY ? l : l * __builtin_amdgcn_exp2f(m - mx));
-        top = mx;
-    }
-    float mx = top;
-#pragma unroll
-    for (int x = 1; x < 64; x <<= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
-    if (top != -INFINITY) all *= __builtin_amdgcn_exp2f(top - mx);
-    top = mx;
-#pragma unroll
-    for (int x = 1; x < 64; x <<= 1) all += __shfl_xor(all, x);
-}
+#define PM_THREADS 512
+#define PM_DEEP 4                // parts that a thread has on the way
 
-// A workgroup a query head: its parts at one maximum, added.  A wave takes every
-// fourth part, a lane four dimensions.
-__global__ __launch_bounds__(PA_THREADS) void paged_merge_k(PagedAttnArgs A)
+// A workgroup a query head: its parts at one maximum, added.  32 lanes (64 past 128 dimensions)
+// take every 16th (8th) part, four dimensions a lane, each at the maximum met so far; then
+// those sums are added.  Everything a part has is asked for at once: one wait for 64 parts.
+__device__ __forceinline__ void merge_head(const PagedAttnArgs &A, const PagedWork &D, uint32_t t, uint32_t head, float *sums,
+                                           float *tops, float *alls)
 {
-    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    __shared__ __attribute__((aligned(16))) float sums[PA_WAVES][256];
-    const PagedWork D = divide(A, (uint64_t *)lds);
-    const uint32_t t = blockIdx.y, head = blockIdx.x, h = head / A.G, j = head % A.G, tid = threadIdx.x;
-    const uint32_t wave = tid >> 6, d = (tid & 63) * 4, hd = A.C.hd;
+    const uint32_t h = head / A.G, j = head % A.G, tid = threadIdx.x;
+    const uint32_t hd = A.C.hd, lanes = hd <= 128 ? 32 : 64, groups = PM_THREADS / lanes, group = tid / lanes;
+    const uint32_t d = tid % lanes * 4;
     const uint32_t item = h * A.tiles + j / A.per;
     uint64_t at;
     uint32_t units, first, last;
@@ -590,65 +580,136 @@ __global__ __launch_bounds__(PA_THREADS) void paged_merge_k(PagedAttnArgs A)
     if (first == last) return;
     const size_t slot = (size_t)t * D.items + item;
     const float *stats = A.stats + (slot * A.per + j % A.per) * 2;
-    const float *part = A.part + (slot * A.per + j % A.per) * hd + d;
-    float top, all;
-    all_parts(stats, A.per * 2, first, last, top, all);
-    float4 y = {0, 0, 0, 0};
-    if (d < hd)
-#pragma unroll 4
-        for (uint32_t w = first + wave; w <= last; w += PA_WAVES) {
-            const float m = stats[(size_t)w * A.per * 2], f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - top);
-            const float4 x = *(const float4 *)(part + (size_t)w * A.per * hd);
-            y.x += x.x * f;
-            y.y += x.y * f;
-            y.z += x.z * f;
-            y.w += x.w * f;
+    const float *part = A.part + (slot * A.per + j % A.per) * hd + (d < hd ? d : 0);
+    float top = -INFINITY, all = 0.0f;
+    f4v y = {0, 0, 0, 0};
+    for (uint32_t w = first + group; w <= last; w += PM_DEEP * groups) {
+        float m[PM_DEEP], l[PM_DEEP], mx = top;
+        f4v x[PM_DEEP];
+#pragma unroll
+        for (int k = 0; k < PM_DEEP; k++) {
+            const uint32_t at = min(w + k * groups, last);
+            m[k] = stats[(size_t)at * A.per * 2];
+            l[k] = stats[(size_t)at * A.per * 2 + 1];
+            x[k] = *(const f4v *)(part + (size_t)at * A.per * hd);
         }
-    *(float4 *)(sums[wave] + d) = y;
+#pragma unroll
+        for (int k = 0; k < PM_DEEP; k++)
+            if (w + k * groups <= last) mx = fmaxf(mx, m[k]);
+        if (top != -INFINITY) {
+            const float f = __builtin_amdgcn_exp2f(top - mx);
+            all *= f;
+            y *= f;
+        }
+#pragma unroll
+        for (int k = 0; k < PM_DEEP; k++)
+            if (w + k * groups <= last) {
+                const float f = m[k] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[k] - mx);
+                all += l[k] * f;
+                y += x[k] * f;
+            }
+        top = mx;
+    }
+    if (d < hd) *(f4v *)(sums + group * lanes * 4 + d) = y;
+    if (d == 0) {
+        tops[group] = top;
+        alls[group] = all;
+    }
     __syncthreads();
-    if (tid < hd)
-        A.out[t * A.out_stride + (size_t)head * hd + tid] =
-            all == 0.0f ? 0.0f : (sums[0][tid] + sums[1][tid] + sums[2][tid] + sums[3][tid]) / all;
+    if (tid >= hd) return;
+    float mx = tops[0], out = 0.0f, sum = 0.0f;
+    for (uint32_t g = 1; g < groups; g++) mx = fmaxf(mx, tops[g]);
+    for (uint32_t g = 0; g < groups; g++) {
+        const float f = tops[g] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(tops[g] - mx);
+        sum += alls[g] * f;
+        out += sums[g * lanes * 4 + tid] * f;
+    }
+    A.out[t * A.out_stride + (size_t)head * hd + tid] = sum == 0.0f ? 0.0f : out / sum;
 }
 
-// A workgroup a kv head's PA_CHUNK positions: the group's weights of each, from the scores,
-// summed before they are added to what the row has.
-__global__ __launch_bounds__(PA_THREADS) void paged_weigh_k(PagedAttnArgs A)
+// A workgroup a kv head's PA_CHUNK positions, four a thread: the group's weights of each, from the scores,
+// summed in the heads' order before they are added to what the row has.  Eight heads at a time: a wave
+// adds up one head's parts while every thread has its eight scores on the way.
+__device__ __forceinline__ void weigh_chunk(const PagedAttnArgs &A, const PagedWork &D, uint32_t t, uint32_t h, uint32_t chunk,
+                                            float *tops, float *by)
+{
+    constexpr int WAVES = PM_THREADS / 64;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t n = min(word(A.length, t), A.C.cap), p = chunk * PA_CHUNK + tid * 4;
+    if (chunk * PA_CHUNK >= n) return;
+    const bool on = p < n && A.C.table[(size_t)t * A.C.max_pages + (p >> A.C.shift)] < A.C.n_pages;
+    float *weight = A.C.weight + ((size_t)t * A.C.n_kv + h) * A.C.cap + p;
+    const float *scores = A.scores + ((size_t)t * A.C.n_kv + h) * A.G * A.C.cap + p;
+    f4v sum = {0, 0, 0, 0}, had = sum, sc[WAVES];
+    if (on) had = *(const f4v *)weight;
+    for (uint32_t j0 = 0; j0 < A.G; j0 += WAVES) {
+#pragma unroll
+        for (int k = 0; k < WAVES; k++)
+            if (on && j0 + k < A.G) sc[k] = *(const f4v *)(scores + (size_t)(j0 + k) * A.C.cap);
+        const uint32_t j = j0 + wave;
+        if (j < A.G) {
+            const uint32_t item = h * A.tiles + j / A.per;
+            uint32_t first = 0, last = 0;
+            if (!A.whole) D.runs(t, item, first, last);
+            const float *stats = A.stats + (((size_t)t * A.C.n_kv * A.tiles + item) * A.per + j % A.per) * 2;
+            float top = -INFINITY, all = 0.0f;
+            for (uint32_t w = first + lane; w <= last; w += 64) {
+                const float2 ml = *(const float2 *)(stats + (size_t)w * A.per * 2);
+                const float mx = fmaxf(top, ml.x);
+                all = (top == -INFINITY ? all : all * __builtin_amdgcn_exp2f(top - mx)) +
+                      (ml.x == -INFINITY ? ml.y : ml.y * __builtin_amdgcn_exp2f(ml.x - mx));
+                top = mx;
+            }
+            const float mx = wave_max(top);
+            all = wave_sum(top == -INFINITY ? all : all * __builtin_amdgcn_exp2f(top - mx));
+            if (lane == 0) {
+                tops[wave] = mx;
+                by[wave] = all == 0.0f ? 0.0f : 1.0f / all;
+            }
+        }
+        __syncthreads();
+        if (on)
+#pragma unroll
+            for (int k = 0; k < WAVES; k++)
+                if (j0 + k < A.G) {
+                    const float top = tops[k] == -INFINITY ? 0.0f : tops[k];
+#pragma unroll
+                    for (int r = 0; r < 4; r++) sum[r] += __builtin_amdgcn_exp2f(sc[k][r] - top) * by[k];
+                }
+        __syncthreads();
+    }
+    if (!on) return;
+    if (p + 4 <= n) {
+        *(f4v *)weight = had + sum;
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            if (p + r < n) weight[r] = had[r] + sum[r];
+    }
+}
+
+// What follows the attention, in one launch: merges of the row's heads, and its kv heads' chunks weighed.
+__global__ __launch_bounds__(PM_THREADS) void paged_after_k(PagedAttnArgs A, uint32_t merges, uint32_t chunks)
 {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    __shared__ __attribute__((aligned(16))) float sums[16 * 128], tops[16], alls[16];
     PagedWork D;
-    if (!A.whole) D = divide(A, (uint64_t *)lds);
-    const uint32_t t = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
-    const uint32_t n = row_length(A, t), p0 = blockIdx.x * PA_CHUNK;
-    if (p0 >= n) return;
-    float sum[PA_CHUNK / PA_THREADS] = {};
-    for (uint32_t j = 0; j < A.G; j++) {
-        const uint32_t item = h * A.tiles + j / A.per;
-        uint32_t first = 0, last = 0;
-        if (!A.whole) D.runs(t, item, first, last);
-        float top, all;
-        all_parts(A.stats + (((size_t)t * A.C.n_kv * A.tiles + item) * A.per + j % A.per) * 2, A.per * 2, first, last, top, all);
-        const float *sc = A.scores + ((size_t)t * A.C.n_kv * A.G + h * A.G + j) * A.C.cap;
-        if (all == 0.0f) continue;
-#pragma unroll
-        for (int x = 0; x < PA_CHUNK / PA_THREADS; x++) {
-            const uint32_t p = p0 + x * PA_THREADS + tid;
-            if (p < n) sum[x] += __builtin_amdgcn_exp2f(sc[p] - top) / all;
-        }
-    }
-    float *weight = A.C.weight + ((size_t)t * A.C.n_kv + h) * A.C.cap;
-#pragma unroll
-    for (int x = 0; x < PA_CHUNK / PA_THREADS; x++) {
-        const uint32_t p = p0 + x * PA_THREADS + tid;
-        if (p < n && A.C.table[(size_t)t * A.C.max_pages + (p >> A.C.shift)] < A.C.n_pages) weight[p] += sum[x];
+    if (!A.whole) D = divide<PM_THREADS>(A, (uint64_t *)lds);
+    const uint32_t t = blockIdx.y;
+    if (blockIdx.x < merges) {
+        merge_head(A, D, t, blockIdx.x, sums, tops, alls);
+    } else {
+        const uint32_t x = blockIdx.x - merges;
+        weigh_chunk(A, D, t, x / chunks, x % chunks, tops, alls);
     }
 }
 
-template <bool BF, int HG>
+template <bool BF, int HG, bool ONCE>
 static const void *attn_kernel(size_t hd)
 {
-#define FOX_ATTN(w) (hd == w ? (const void *)paged_attn_k<BF, w, true, HG> : (const void *)paged_attn_k<BF, w, false, HG>)
-    return hd <= 64 ? FOX_ATTN(64) : hd <= 128 ? FOX_ATTN(128) : hd <= 192 ? FOX_ATTN(192) : FOX_ATTN(256);
+#define FOX_ATTN(w) (hd == w ? (const void *)paged_attn_k<BF, w, true, HG, ONCE> : (const void *)paged_attn_k<BF, w, false, HG, ONCE>)
+    return hd <= 64 ? FOX_ATTN(64) : hd <= 128 ? FOX_ATTN(128)
+         : hd <= 192 ? (const void *)paged_attn_k<BF, 192, false, HG, ONCE> : FOX_ATTN(256);
 #undef FOX_ATTN
 }
 
@@ -690,13 +751,13 @@ extern "C" fox_gpu_status fox_gpu_paged_attention(fox_gpu_ctx *ctx, const fox_gp
     // Short caches: a workgroup an item, one launch.
     A.whole = A.C.cap <= 512;
     const size_t most = items * ((A.C.cap + PA_UNIT - 1) / PA_UNIT);
-    const size_t fit = (size_t)(four && cache->head_dim <= 128 ? 3 : 2) * ctx->n_cu;
+    const size_t fit = (size_t)2 * ctx->n_cu;
     A.workers = (uint32_t)(A.whole ? items : most < fit ? most : fit);
     // parts, their maxima and sums, and the scores of rows that are weighed
     const size_t slots = A.whole ? items : items + A.workers;
     const size_t part = A.whole ? 0 : slots * A.per * cache->head_dim, stats = slots * A.per * 2;
     const size_t scores = weigh ? M * n_head * A.C.cap : 0;
-    if (scores > (size_t)1 << 34)
+    if (scores > (size_t)1 << 33)
         return fox_fail(FOX_GPU_ERR_ARG, "paged_attention: the weights of %zu tokens' %zu heads over %u rows are too "
                         "many", M, n_head, A.C.cap);
     if ((st = fox_ws_reserve(ctx, (scores + part + stats) * sizeof(float)))) return st;
@@ -705,19 +766,21 @@ extern "C" fox_gpu_status fox_gpu_paged_attention(fox_gpu_ctx *ctx, const fox_gp
     A.stats = A.part + part;
     FOX_HIP(hipSetDevice(ctx->device));
     const bool bf = cache->type == FOX_GPU_BF16;
-    const void *k = four ? bf ? attn_kernel<true, 4>(cache->head_dim) : attn_kernel<false, 4>(cache->head_dim)
-                         : bf ? attn_kernel<true, 16>(cache->head_dim) : attn_kernel<false, 16>(cache->head_dim);
+    const bool once = !seq && A.tiles == 1;
+#define FOX_ATTN(hg, o) (bf ? attn_kernel<true, hg, o>(cache->head_dim) : attn_kernel<false, hg, o>(cache->head_dim))
+    const void *k = four ? once ? FOX_ATTN(4, true) : FOX_ATTN(4, false) : once ? FOX_ATTN(16, true) : FOX_ATTN(16, false);
+#undef FOX_ATTN
     const size_t starts = M > 64 && !A.whole ? ((M + 1) * 8 + 15) / 16 * 16 : 0;
     const size_t lds = starts + (size_t)(four ? 4 : 1) * PA_WAVES * A.per * cache->head_dim * sizeof(float);
     void *args[] = {&A};
     FOX_HIP(hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
     FOX_HIP(hipLaunchKernel(k, dim3(A.workers), dim3(PA_THREADS), args, lds, ctx->stream));
-    if (!A.whole && A.workers > 1)
-        FOX_HIP(hipLaunchKernel((const void *)paged_merge_k, dim3((unsigned)n_head, (unsigned)M), dim3(PA_THREADS),
-                                args, starts, ctx->stream));
-    if (weigh)
-        FOX_HIP(hipLaunchKernel((const void *)paged_weigh_k,
-                                dim3((A.C.cap + PA_CHUNK - 1) / PA_CHUNK, (unsigned)cache->n_head_kv, (unsigned)M),
-                                dim3(PA_THREADS), args, starts, ctx->stream));
+    const uint32_t merges = A.whole || A.workers == 1 ? 0 : (uint32_t)n_head;
+    uint32_t chunks = weigh ? (A.C.cap + PA_CHUNK - 1) / PA_CHUNK : 0;
+    if (merges || chunks) {
+        void *after[] = {&A, (void *)&merges, &chunks};
+        FOX_HIP(hipLaunchKernel((const void *)paged_after_k, dim3((unsigned)(merges + chunks * cache->n_head_kv), (unsigned)M),
+                                dim3(PM_THREADS), after, starts, ctx->stream));
+    }
     return FOX_GPU_OK;
 }

@@ -22,7 +22,7 @@ BAD_CACHES = [(dict(type=0), UNSUPPORTED), (dict(type=4), UNSUPPORTED), (dict(k=
               (dict(v=P + 2), ARG), (dict(n_pages=(1 << 31) + 1), ARG), (dict(n_seqs=65536), ARG),
               (dict(n_head_kv=4097), ARG), (dict(n_seqs=1024, n_head_kv=1025), ARG),
               (dict(max_pages=(1 << 26) + 1), ARG), (dict(max_pages=2 ** 64 - 1), ARG), (dict(weight=None), ARG),
-              (dict(position=None), ARG)]
+              (dict(position=None), ARG), (dict(weight=P + 4), ARG), (dict(position=P + 8), ARG)]
 
 STORE = dict(ctx=C.addressof(CTX), cache=CACHE, q=P, qs=256, o=P, os=256, nh=4, k=P, ks=128, v=P, vs=128, M=3,
              qn=P, kn=P, eps=1e-6, pairs=0, n_rot=64, cos=P, sin=P, n_table=100, pos=P, seq=None, row=None)
