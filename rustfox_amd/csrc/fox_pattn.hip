@@ -47,7 +47,10 @@ struct PagedAttnArgs {
     const uint32_t *length, *seq;
     uint32_t G, M;               // query heads of a kv head; rows
     uint32_t per, tiles;         // query heads of a head tile (the last may have fewer); head tiles of a kv head
-    uint32_t workers;            // workgroups that share the units
+    // Workgroups that share the units: one a compute unit, two where a call is long. (A unit's rows arrive no
+    // faster for two, and each item has more parts: 16000 rows 23.0 / 25.2 us, 32 rows of 2000
+    // 45.9 / 49.9; more than 48 units each hide what rows' ends cost: attn-27b-64 283 / 273.)
+    uint32_t few, workers;
     bool whole;                  // no: a workgroup an item
     float score;                 // log2(e) / sqrt(hd)
     // of slot (worker + item): sums [slot][per][hd], maxima and weights' sums [slot][per][2]
@@ -171,7 +174,8 @@ __device__ __forceinline__ PagedWork divide(const PagedAttnArgs &A, uint64_t *st
         __syncthreads();
         D.total = start[A.M] * D.items;
     }
-    D.run = over(D.total + A.workers - 1, A.workers);
+    const uint32_t workers = D.total < (uint64_t)48 * A.workers ? A.few : A.workers;
+    D.run = over(D.total + workers - 1, workers);
     return D;
 }
 
@@ -748,11 +752,16 @@ extern "C" fox_gpu_status fox_gpu_paged_attention(fox_gpu_ctx *ctx, const fox_gp
     A.out_wide = (uintptr_t)out % 16 == 0 && (M == 1 || out_stride % 4 == 0);
     const size_t items = M * cache->n_head_kv * A.tiles;
     const bool four = A.per <= 4;
-    // Short caches: a workgroup an item, one launch.
-    A.whole = A.C.cap <= 512;
+    // Short caches: a workgroup an item, one launch.  How short depends on the items, since one alone
+    // draws rows at 55 GB/s (0.6 us for 64 of them): whole / divided, 8 items of 300 rows 8.7 / 11 us, of
+    // 640 11.8 / 11.0, of 1000 17.0 / 11.2; 64 of 640 14.5 / 16.2, of 1000 19.4 / 14.6; 256 of
+    // 1000 24.3 / 28.0, of 2000 42.4 / 45.9.
+    A.whole = A.C.cap <= 512 + 1536 * (items < (size_t)ctx->n_cu ? items : (size_t)ctx->n_cu) / ctx->n_cu;
     const size_t most = items * ((A.C.cap + PA_UNIT - 1) / PA_UNIT);
     const size_t fit = (size_t)2 * ctx->n_cu;
     A.workers = (uint32_t)(A.whole ? items : most < fit ? most : fit);
+    // (rows that are weighed are stored, too: attn-8b-24-weigh 70 / 64 us)
+    A.few = weigh || A.workers < (uint32_t)ctx->n_cu ? A.workers : (uint32_t)ctx->n_cu;
     // parts, their maxima and sums, and the scores of rows that are weighed
     const size_t slots = A.whole ? items : items + A.workers;
     const size_t part = A.whole ? 0 : slots * A.per * cache->head_dim, stats = slots * A.per * 2;
