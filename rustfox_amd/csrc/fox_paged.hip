@@ -7,6 +7,7 @@
 #include <cstring>
 
 typedef uint32_t u4v __attribute__((ext_vector_type(4)));
+typedef float f4v __attribute__((ext_vector_type(4)));
 
 #define PG_THREADS 256
 
@@ -56,33 +57,80 @@ fox_gpu_status fox_paged_check(const char *what, const fox_gpu_paged *c, bool tr
 
 // ------------------------------------------------------------------ tables
 
+#define RT_ROWS 4                // rows of a thread
+
 struct FreqArgs {
     double turn[128];             // turns a position, pair by pair
     double magnitude;
     const float *factors;
     float *cos_t, *sin_t;
-    uint32_t half, p0;
-    uint64_t total;               // n half
+    uint32_t half, p0, n;
+    bool wide;                    // rows take 16-byte stores
+};
+
+// (2 pi)^k / k!
+struct Terms {
+    double t[14];
+    constexpr __host__ __device__ Terms() : t()
+    {
+        t[0] = 1.0;
+        for (int k = 1; k < 14; k++) t[k] = t[k - 1] * 6.283185307179586476925 / k;
+    }
 };
 
 // Angles are counted in turns: what is left of p turn[j] after the nearest quarter is exact,
-// and within an eighth of a turn twelve terms of sine and cosine are good to 2^-36.
+// and within an eighth of a turn six and seven terms of sine and cosine are good to 2^-41.
 // (Angles in floats would be off by 2^-24 of all the turns made.)
+//
+// A thread has four pairs and RT_ROWS rows of them, so speeds are read once; the two tables are
+// all that moves, and their writes bound it: 131072 positions of 64 pairs (67 MB).
 __global__ __launch_bounds__(PG_THREADS) void rope_tables_k(FreqArgs A)
 {
-    const uint64_t at = (uint64_t)blockIdx.x * PG_THREADS + threadIdx.x;
-    if (at >= A.total) return;
-    const uint32_t j = (uint32_t)(at % A.half);
-    double w = A.turn[j];
-    if (A.factors) w = w / (double)A.factors[j];
-    const double a = (double)(A.p0 + at / A.half) * w, n = rint(4.0 * a);
-    const double x = __builtin_fma(-0.25, n, a) * 6.283185307179586;
-    const double s = sin(x), c = cos(x);
-    const int quarter = (int)((int64_t)n & 3);
-    const double cs = quarter == 0 ? c : quarter == 1 ? -s : quarter == 2 ? -c : s;
-    const double sn = quarter == 0 ? s : quarter == 1 ? c : quarter == 2 ? -s : -c;
-    A.cos_t[at] = (float)(A.magnitude * cs);
-    A.sin_t[at] = (float)(A.magnitude * sn);
+    const uint32_t quads = (A.half + 3) / 4, rows = PG_THREADS / quads;      // (quads <= 32)
+    const uint32_t side = threadIdx.x / quads, j0 = threadIdx.x % quads * 4;
+    if (side >= rows) return;
+    constexpr Terms T;
+    double turn[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t j = min(j0 + i, A.half - 1);
+        turn[i] = A.turn[j];
+        if (A.factors) turn[i] = turn[i] / (double)A.factors[j];
+    }
+#pragma unroll
+    for (int k = 0; k < RT_ROWS; k++) {
+        const uint64_t row = ((uint64_t)blockIdx.x * RT_ROWS + k) * rows + side;
+        if (row >= A.n) return;
+        float cs[4], sn[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const double a = (double)(A.p0 + row) * turn[i], n = rint(4.0 * a);
+            const double x = __builtin_fma(-0.25, n, a), y = x * x;
+            double s = T.t[13], c = T.t[12];
+            // (signs alternate: by -y)
+#pragma unroll
+            for (int m = 11; m > 0; m -= 2) s = __builtin_fma(s, -y, T.t[m]);
+#pragma unroll
+            for (int m = 10; m >= 0; m -= 2) c = __builtin_fma(c, -y, T.t[m]);
+            s *= x;
+            const uint32_t quarter = (uint32_t)(int64_t)n;
+            const float u = (float)(A.magnitude * (quarter & 1 ? s : c)), v = (float)(A.magnitude * (quarter & 1 ? c : s));
+            cs[i] = (quarter + 1) & 2 ? -u : u;
+            sn[i] = quarter & 2 ? -v : v;
+        }
+        const uint64_t at = row * A.half + j0;
+        if (A.wide) {
+            *(f4v *)(A.cos_t + at) = *(const f4v *)cs;
+            *(f4v *)(A.sin_t + at) = *(const f4v *)sn;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (j0 + i < A.half) {
+                    A.cos_t[at + i] = cs[i];
+                    A.sin_t[at + i] = sn[i];
+                }
+        }
+    }
 }
 
 extern "C" fox_gpu_status fox_gpu_rope_tables(fox_gpu_ctx *ctx, float *cos_t, float *sin_t, size_t p0, size_t n,
@@ -123,9 +171,11 @@ extern "C" fox_gpu_status fox_gpu_rope_tables(fox_gpu_ctx *ctx, float *cos_t, fl
     A.cos_t = cos_t;
     A.sin_t = sin_t;
     A.p0 = (uint32_t)p0;
-    A.total = (uint64_t)n * A.half;
+    A.n = (uint32_t)n;
+    A.wide = A.half % 4 == 0 && (uintptr_t)cos_t % 16 == 0 && (uintptr_t)sin_t % 16 == 0;
+    const size_t rows = PG_THREADS / ((A.half + 3) / 4) * RT_ROWS;
     FOX_HIP(hipSetDevice(ctx->device));
-    rope_tables_k<<<dim3((unsigned)((A.total + PG_THREADS - 1) / PG_THREADS)), dim3(PG_THREADS), 0, ctx->stream>>>(A);
+    rope_tables_k<<<dim3((unsigned)((n + rows - 1) / rows)), dim3(PG_THREADS), 0, ctx->stream>>>(A);
     FOX_LAUNCHED("rope_tables");
     return FOX_GPU_OK;
 }
@@ -143,51 +193,153 @@ struct PagedStoreArgs {
     int halves;
 };
 
-// One wave per (token, head): keys first, then values, then queries.
-template <bool BF>
+// the sum of x over LANES neighbouring lanes, in every one of them
+template <int LANES>
+__device__ __forceinline__ double sum_of(double x)
+{
+#define FOX_DPP(ctrl)                                                                                          \
+    {                                                                                                          \
+        const uint64_t u = __builtin_bit_cast(uint64_t, x);                                                    \
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)u, ctrl, 0xF, 0xF, true);        \
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(u >> 32), ctrl, 0xF, 0xF, true); \
+        x += __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);                                              \
+    }
+    FOX_DPP(0xB1)                // lane ^ 1, ^ 2, then the other half of 8 and of 16
+    FOX_DPP(0x4E)
+    FOX_DPP(0x141)
+    if (LANES > 8) FOX_DPP(0x140)
+    if (LANES > 16) x += __shfl_xor(x, 16);
+#undef FOX_DPP
+    return x;
+}
+
+__device__ __forceinline__ void load_eight(float x[8], const float *p, bool wide)
+{
+    if (wide) {
+        *(f4v *)x = *(const f4v *)p;
+        *(f4v *)(x + 4) = *(const f4v *)(p + 4);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = p[i];
+    }
+}
+
+// LANES lanes, of eight dimensions each, have one head's row of one token: keys' heads first, then
+// values', then queries'; a workgroup has rows of one token, so what tells where it goes is read once.
+// Norm and rotation are in double (a 16-bit key may hang on the last bit; the vector unit multiplies
+// doubles at the rate of floats).  A pair's other half is another lane's: it is read
+// again, from the first cache, not passed on.  All of a row is read before any of it
+// is written, so a query may be turned in place.
+//
+// FAST: rows, tables and weights take 16-byte accesses, and eight dimensions have eight (four) pairs' angles
+// that stand side by side.
+//
+// Bound by its reads and writes where there are many tokens: 1001 tokens of 32 + 16 + 16 heads of 128 (58 MB).
+template <bool BF, int LANES, bool FAST>
 __global__ __launch_bounds__(PG_THREADS) void paged_store_k(PagedStoreArgs A)
 {
-    __shared__ double lds[PG_THREADS / 64][256];
-    const uint32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6, hd = A.C.hd;
-    const uint32_t heads = A.n_head + 2 * A.C.n_kv;
-    const uint32_t at = blockIdx.y * (PG_THREADS / 64) + w, t = blockIdx.x;
-    const bool on = at < heads;
-    const uint32_t part = at < A.C.n_kv ? 0 : at < 2 * A.C.n_kv ? 1 : 2;
-    const uint32_t h = on ? at - part * A.C.n_kv : 0;
-    const uint32_t s = A.seq ? A.seq[t] : t, p = A.pos[t];
+    const uint32_t t = blockIdx.y, hd = A.C.hd, half = A.n_rot / 2;
+    const uint32_t at = blockIdx.x * (PG_THREADS / LANES) + threadIdx.x / LANES, d0 = threadIdx.x % LANES * 8;
+    const uint32_t s = A.seq ? A.seq[t] : t, p = A.pos[t], r = A.row ? A.row[t] : p;
     if (s >= A.C.n_seqs || p >= A.n_table) return;       // (uniform)
-    const float *src = part == 0 ? A.k + t * A.k_stride : part == 1 ? A.v + t * A.v_stride : A.q + t * A.q_stride;
-    const float *nw = part == 0 ? A.k_norm : part == 1 ? nullptr : A.q_norm;
-    double *x = lds[w];
-    double ss = 0.0;
-    if (on)
-        for (uint32_t d = lane; d < hd; d += 64) {
-            x[d] = (double)src[(size_t)h * hd + d];
-            ss += x[d] * x[d];
+    if (at >= A.n_head + 2 * A.C.n_kv) return;           // (of a whole row)
+    const uint32_t part = at < A.C.n_kv ? 0 : at < 2 * A.C.n_kv ? 1 : 2, h = at - part * A.C.n_kv;
+    const bool on = d0 < hd;
+    const float *row = part == 0 ? A.k + t * A.k_stride : part == 1 ? A.v + t * A.v_stride : A.q + t * A.q_stride;
+    const float *w = part == 0 ? A.k_norm : part == 1 ? nullptr : A.q_norm;
+    row += (size_t)h * hd;
+    float x[8] = {};
+    if (on) load_eight(x, row + d0, FAST);
+    if (part != 1) {
+        const bool turned = on && d0 < A.n_rot;
+        const float *cos_t = A.cos_t + (size_t)p * half, *sin_t = A.sin_t + (size_t)p * half;
+        // the other halves' values and weights, and the angles, dimension by dimension
+        float other[8] = {}, ws[8], wo[8], cs[8] = {}, sn[8] = {};
+        if (turned && FAST) {
+            if (A.halves) {
+                const uint32_t o = d0 < half ? d0 + half : d0 - half, j = d0 < half ? d0 : o;
+                load_eight(other, row + o, true);
+                if (w) load_eight(wo, w + o, true);
+                load_eight(cs, cos_t + j, true);
+                load_eight(sn, sin_t + j, true);
+            } else {
+                const f4v c = *(const f4v *)(cos_t + d0 / 2), z = *(const f4v *)(sin_t + d0 / 2);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    cs[i] = c[i / 2];
+                    sn[i] = z[i / 2];
+                }
+            }
         }
-    for (int m = 32; m; m >>= 1) ss += __shfl_xor(ss, m);
-    __syncthreads();
-    if (!on) return;
-    const double inv = nw ? 1.0 / sqrt(ss / (double)hd + (double)A.eps) : 1.0;
-    const uint32_t r = A.row ? A.row[t] : p, half = A.n_rot / 2;
-    const size_t to = part == 2 || r >= A.C.cap ? ~(size_t)0 : paged_row(A.C, s, h, r);
-    if (part != 2 && to == ~(size_t)0) return;
-    for (uint32_t d = lane; d < hd; d += 64) {
-        double y = x[d] * inv;
-        if (nw) y *= (double)nw[d];
-        if (part != 1 && d < A.n_rot) {
-            const bool second = A.halves ? d >= half : d & 1;
-            const uint32_t o = A.halves ? (second ? d - half : d + half) : d ^ 1;
-            const uint32_t j = A.halves ? (second ? d - half : d) : d / 2;
-            double z = x[o] * inv;
-            if (nw) z *= (double)nw[o];
-            const double c = (double)A.cos_t[(size_t)p * half + j], sn = (double)A.sin_t[(size_t)p * half + j];
-            y = second ? z * sn + y * c : y * c - z * sn;
+        if (turned && !FAST)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const uint32_t d = d0 + i;
+                if (d < A.n_rot) {
+                    const uint32_t o = !A.halves ? d ^ 1 : d < half ? d + half : d - half;
+                    const uint32_t j = !A.halves ? d / 2 : d < half ? d : o;
+                    other[i] = row[o];
+                    if (w) wo[i] = w[o];
+                    cs[i] = cos_t[j];
+                    sn[i] = sin_t[j];
+                }
+            }
+        double y[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) y[i] = (double)x[i];
+        double z[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) z[i] = (double)other[i];
+        if (w) {
+            if (on) load_eight(ws, w + d0, FAST);
+            double ss = 0.0;
+#pragma unroll
+            for (int i = 0; i < 8; i++) ss += y[i] * y[i];
+            const double inv = 1.0 / sqrt(sum_of<LANES>(ss) / (double)hd + (double)A.eps);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                y[i] = y[i] * inv * (double)ws[i];
+                z[i] = z[i] * inv * (double)wo[i];
+            }
         }
-        if (part == 2) A.q_out[t * A.qo_stride + (size_t)h * hd + d] = (float)y;
-        else ((uint16_t *)(part ? A.C.v : A.C.k))[to + d] = paged_round<BF>((float)y);
+        if (turned) {
+            double out[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const uint32_t d = d0 + i;
+                const bool second = A.halves ? d >= half : i & 1;
+                const double b = FAST && !A.halves ? y[i ^ 1] : z[i], c = (double)cs[i], e = (double)sn[i];
+                const double turn = second ? b * e + y[i] * c : y[i] * c - b * e;
+                out[i] = FAST || d < A.n_rot ? turn : y[i];
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) y[i] = out[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = (float)y[i];
+        if (part == 2) {
+            float *to = A.q_out + t * A.qo_stride + (size_t)h * hd + d0;
+            if (!on) return;
+            if (FAST) {
+                *(f4v *)to = *(const f4v *)x;
+                *(f4v *)(to + 4) = *(const f4v *)(x + 4);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) to[i] = x[i];
+            }
+            return;
+        }
     }
-    if (part == 0 && lane == 0 && A.C.weight) {
+    if (r >= A.C.cap) return;
+    const size_t to = paged_row(A.C, s, h, r);
+    if (to == ~(size_t)0) return;
+    if (on) {
+        u4v o;
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[i] = paged_round<BF>(x[2 * i]) | (uint32_t)paged_round<BF>(x[2 * i + 1]) << 16;
+        *(u4v *)((uint16_t *)(part ? A.C.v : A.C.k) + to + d0) = o;
+    }
+    if (part == 0 && d0 == 0 && A.C.weight) {
         const size_t i = ((size_t)s * A.C.n_kv + h) * A.C.cap + r;
         A.C.weight[i] = 0.0f;
         A.C.position[i] = p;
@@ -241,12 +393,21 @@ extern "C" fox_gpu_status fox_gpu_paged_rope_store(
     A.eps = eps;
     A.halves = pairs == FOX_GPU_PAIRS_HALVES;
     FOX_HIP(hipSetDevice(ctx->device));
-    const dim3 grid((unsigned)M, (unsigned)((n_head + 2 * cache->n_head_kv + 3) / 4));
-    if (cache->type == FOX_GPU_BF16)
-        paged_store_k<true><<<grid, dim3(PG_THREADS), 0, ctx->stream>>>(A);
-    else
-        paged_store_k<false><<<grid, dim3(PG_THREADS), 0, ctx->stream>>>(A);
-    FOX_LAUNCHED("paged_rope_store");
+    // (eight dimensions of a lane are all turned or none, and their pairs' angles aligned)
+    auto wide = [](const float *x, size_t stride) { return (uintptr_t)x % 16 == 0 && stride % 4 == 0; };
+    const bool fast = n_rot % (A.halves ? 16 : 8) == 0 && wide(q, M > 1 ? q_stride : 0) &&
+                      wide(q_out, M > 1 ? q_out_stride : 0) && wide(k, M > 1 ? k_stride : 0) &&
+                      wide(v, M > 1 ? v_stride : 0) && wide(q_norm, 0) && wide(k_norm, 0) && wide(cos_t, 0) && wide(sin_t, 0);
+    const size_t lanes = cache->head_dim <= 64 ? 8 : cache->head_dim <= 128 ? 16 : 32, rows = PG_THREADS / lanes;
+#define FOX_STORE(bf, f)                                                                                  \
+    (lanes == 8 ? (const void *)paged_store_k<bf, 8, f> : lanes == 16 ? (const void *)paged_store_k<bf, 16, f> \
+                                                        : (const void *)paged_store_k<bf, 32, f>)
+    const void *kern = cache->type == FOX_GPU_BF16 ? fast ? FOX_STORE(true, true) : FOX_STORE(true, false)
+                                                   : fast ? FOX_STORE(false, true) : FOX_STORE(false, false);
+#undef FOX_STORE
+    void *args[] = {&A};
+    FOX_HIP(hipLaunchKernel(kern, dim3((unsigned)((n_head + 2 * cache->n_head_kv + rows - 1) / rows), (unsigned)M),
+                            dim3(PG_THREADS), args, 0, ctx->stream));
     return FOX_GPU_OK;
 }
 
