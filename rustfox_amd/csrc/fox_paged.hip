@@ -189,6 +189,7 @@ struct PagedStoreArgs {
     size_t q_stride, qo_stride, k_stride, v_stride;
     const uint32_t *pos, *seq, *row;
     uint32_t n_head, M, n_rot, n_table;
+    double by_hd;                 // 1 / head_dim
     float eps;
     int halves;
 };
@@ -295,7 +296,7 @@ __global__ __launch_bounds__(PG_THREADS) void paged_store_k(PagedStoreArgs A)
             double ss = 0.0;
 #pragma unroll
             for (int i = 0; i < 8; i++) ss += y[i] * y[i];
-            const double inv = 1.0 / sqrt(sum_of<LANES>(ss) / (double)hd + (double)A.eps);
+            const double inv = rsqrt(sum_of<LANES>(ss) * A.by_hd + (double)A.eps);
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 y[i] = y[i] * inv * (double)ws[i];
@@ -308,8 +309,8 @@ __global__ __launch_bounds__(PG_THREADS) void paged_store_k(PagedStoreArgs A)
             for (int i = 0; i < 8; i++) {
                 const uint32_t d = d0 + i;
                 const bool second = A.halves ? d >= half : i & 1;
-                const double b = FAST && !A.halves ? y[i ^ 1] : z[i], c = (double)cs[i], e = (double)sn[i];
-                const double turn = second ? b * e + y[i] * c : y[i] * c - b * e;
+                const double b = FAST && !A.halves ? y[i ^ 1] : z[i];
+                const double turn = y[i] * (double)cs[i] + b * (double)(second ? sn[i] : -sn[i]);
                 out[i] = FAST || d < A.n_rot ? turn : y[i];
             }
 #pragma unroll
@@ -390,6 +391,7 @@ extern "C" fox_gpu_status fox_gpu_paged_rope_store(
     A.M = (uint32_t)M;
     A.n_rot = (uint32_t)n_rot;
     A.n_table = (uint32_t)n_table;
+    A.by_hd = 1.0 / (double)cache->head_dim;
     A.eps = eps;
     A.halves = pairs == FOX_GPU_PAIRS_HALVES;
     FOX_HIP(hipSetDevice(ctx->device));
