@@ -56,16 +56,11 @@ struct PagedAttnArgs {
     // of slot (worker + item): sums [slot][per][hd], maxima and weights' sums [slot][per][2]
     float *part, *stats;
     float *scores;               // [row][head][cap], where rows are weighed
+    uint32_t *bounds;            // of every item its first and its last worker
     bool q_wide, out_wide;       // rows take 16-byte accesses
 };
 
 // ---------------------------------------------------------------- division
-
-__device__ __forceinline__ uint32_t row_length(const PagedAttnArgs &A, uint32_t t)
-{
-    const uint32_t s = A.seq ? A.seq[t] : t;
-    return s < A.C.n_seqs ? min(A.length[t], A.C.cap) : 0;
-}
 
 // A word that no kernel of the call writes, at an address that is the same for the wave: through the
 // scalar cache.  (As vector loads, page numbers would be waited for behind the rows' loads.)
@@ -86,27 +81,24 @@ __device__ __forceinline__ uint64_t over(uint64_t a, uint32_t b)
 struct PagedWork {
     const uint64_t *start;        // [M + 1], past 64 rows
     uint64_t run, total;          // units of a worker; of the call
-    uint32_t items, M, before, units;
+    uint32_t items, M, before, units, length, seq;
 
-    // the row that holds unit u of the call, and its first unit of one item
-    __device__ __forceinline__ uint32_t row_of(uint64_t u, uint64_t &first, uint32_t &n) const
+    // the row that holds unit u of the call
+    __device__ __forceinline__ uint32_t row_of(uint64_t u) const
     {
-        uint32_t t;
         if (M <= 64) {
             const uint32_t lane = threadIdx.x & 63;
-            t = 63 - __builtin_clzll(__ballot(lane < M && (uint64_t)before * items <= u));
-        } else {
-            uint32_t lo = 0, hi = M;                        // the last with start items <= u
-            while (hi - lo > 1) {
-                const uint32_t mid = (lo + hi) / 2;
-                if (start[mid] * items <= u) lo = mid;
-                else hi = mid;
-            }
-            t = __builtin_amdgcn_readfirstlane(lo);
+            return 63 - __builtin_clzll(__ballot(lane < M && (uint64_t)before * items <= u));
         }
-        row(t, first, n);
-        return t;
+        uint32_t lo = 0, hi = M;                            // the last with start items <= u
+        while (hi - lo > 1) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (start[mid] * items <= u) lo = mid;
+            else hi = mid;
+        }
+        return __builtin_amdgcn_readfirstlane(lo);
     }
+    // a row's first unit of one item, and how many it has
     __device__ __forceinline__ void row(uint32_t t, uint64_t &first, uint32_t &n) const
     {
         if (M <= 64) {
@@ -117,43 +109,38 @@ struct PagedWork {
             n = (uint32_t)(start[t + 1] - first);
         }
     }
-    // the workers whose runs hold an item's units: first and last
-    __device__ __forceinline__ void runs(uint32_t t, uint32_t item, uint32_t &a, uint32_t &b) const
-    {
-        uint64_t first;
-        uint32_t n;
-        row(t, first, n);
-        const uint64_t u = first * items + (uint64_t)item * n;
-        if (total >> 32 == 0) {
-            a = (uint32_t)u / (uint32_t)run;
-            b = (uint32_t)(u + n - 1) / (uint32_t)run;
-        } else {
-            a = (uint32_t)(u / run);
-            b = (uint32_t)((u + n - 1) / run);
-        }
-    }
 };
 
-template <int THREADS = PA_THREADS>
+// rows that row t sees, and its sequence
+__device__ __forceinline__ uint32_t row_length(const PagedAttnArgs &A, uint32_t t, uint32_t &s)
+{
+    s = A.seq ? A.seq[t] : t;
+    const uint32_t n = A.length[t];
+    return s < A.C.n_seqs ? min(n, A.C.cap) : 0;
+}
+
 __device__ __forceinline__ PagedWork divide(const PagedAttnArgs &A, uint64_t *start)
 {
-    __shared__ uint64_t sums[THREADS / 64];
+    __shared__ uint64_t sums[PA_WAVES];
     const uint32_t tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     PagedWork D;
     D.start = start;
     D.M = A.M;
     D.items = A.C.n_kv * A.tiles;
+    D.length = D.seq = 0;
     if (A.M <= 64) {
-        D.units = lane < A.M ? units_of(row_length(A, lane)) : 0;   // (64 of at most 2^24)
-        const uint32_t x = wave_scan(D.units);
+        if (lane < A.M) D.length = row_length(A, lane, D.seq);
+        D.units = units_of(D.length);                               // (64 of at most 2^24)
+        const uint32_t x = A.M > 1 ? wave_scan(D.units) : D.units;
         D.before = x - D.units;
         D.total = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)x, (int)A.M - 1) * D.items;
     } else {
-        const uint32_t each = (A.M + THREADS - 1) / THREADS;        // (at most 4)
+        const uint32_t each = (A.M + PA_THREADS - 1) / PA_THREADS;  // (at most 4)
         uint64_t mine = 0;
+        uint32_t s;
         for (uint32_t i = 0; i < each; i++) {
             const uint32_t t = tid * each + i;
-            if (t < A.M) mine += units_of(row_length(A, t));
+            if (t < A.M) mine += units_of(row_length(A, t, s));
         }
         uint64_t x = mine;
         for (uint32_t m = 1; m < 64; m <<= 1) {
@@ -168,9 +155,9 @@ __device__ __forceinline__ PagedWork divide(const PagedAttnArgs &A, uint64_t *st
             const uint32_t t = tid * each + i;
             if (t >= A.M) break;
             start[t] = before;
-            before += units_of(row_length(A, t));
+            before += units_of(row_length(A, t, s));
         }
-        if (tid == THREADS - 1) start[A.M] = before;
+        if (tid == PA_THREADS - 1) start[A.M] = before;
         __syncthreads();
         D.total = start[A.M] * D.items;
     }
@@ -357,8 +344,10 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_k(PagedAttnArgs A)
             uint64_t first;
             uint32_t n;
             D.row(t, first, n);
-            if (n == 0)
+            if (n == 0) {
                 for (uint32_t d = tid; d < width; d += PA_THREADS) A.out[t * A.out_stride + d] = 0.0f;
+                for (uint32_t i = tid; i < 2 * items; i += PA_THREADS) A.bounds[(size_t)t * items * 2 + i] = 0;
+            }
         }
         u = blockIdx.x * D.run;
         end = min(u + D.run, D.total);
@@ -370,7 +359,8 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_k(PagedAttnArgs A)
             item = blockIdx.x - t * items;
         } else {
             uint64_t first;
-            t = D.row_of(u, first, units);
+            t = D.row_of(u);
+            D.row(t, first, units);
             const uint64_t in_row = u - first * items;
             item = (uint32_t)over(in_row, units);
             k0 = (uint32_t)(in_row - (uint64_t)item * units);
@@ -379,9 +369,18 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_k(PagedAttnArgs A)
         t = __builtin_amdgcn_readfirstlane(t);
         item = __builtin_amdgcn_readfirstlane(item);
         k0 = __builtin_amdgcn_readfirstlane(k0);
-        const uint32_t h = item / A.tiles, h0 = item % A.tiles * A.per, heads = min(A.per, A.G - h0);
-        const uint32_t sq = A.seq ? word(A.seq, t) : t, length = word(A.length, t);
-        const uint32_t n = sq < A.C.n_seqs ? min(length, A.C.cap) : 0, s = n ? sq : 0;
+        const uint32_t h = A.tiles == 1 ? item : item / A.tiles, h0 = (item - h * A.tiles) * A.per;
+        const uint32_t heads = min(A.per, A.G - h0);
+        uint32_t n, s;
+        if (!A.whole && A.M <= 64) {
+            n = (uint32_t)__builtin_amdgcn_readlane((int)D.length, t);
+            s = (uint32_t)__builtin_amdgcn_readlane((int)D.seq, t);
+        } else {
+            s = A.seq ? word(A.seq, t) : t;
+            const uint32_t length = word(A.length, t);
+            n = s < A.C.n_seqs ? min(length, A.C.cap) : 0;
+            if (n == 0) s = 0;
+        }
         if (A.whole) units = k1 = units_of(n);
         k1 = __builtin_amdgcn_readfirstlane(k1);
         const uint32_t *table = A.C.table + (size_t)s * A.C.max_pages;
@@ -503,18 +502,12 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_k(PagedAttnArgs A)
         }
         if (p0 < stop) step(one);
 
-        // the waves' sums at one maximum, added
+        // the waves' sums, each at its maximum, then added at the greatest
         l = sum_of_groups(l);
         if (lane < HG) {
             wm[wave][i % HG] = m;
             wl[wave][i % HG] = l;
         }
-        __syncthreads();
-        float mx = wm[0][col];
-#pragma unroll
-        for (int w = 1; w < PA_WAVES; w++) mx = fmaxf(mx, wm[w][col]);
-        // (a wave that saw nothing has no sums, but a NaN among them must not hide)
-        const float f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mx);
         if (col < heads) {
             float *to = sums + ((size_t)(HG == 4 ? wave * 4 + g : wave) * A.per + col) * hd;
 #pragma unroll
@@ -525,23 +518,33 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_k(PagedAttnArgs A)
                     const uint32_t row = HG == 4 ? (i & 12) + r : 4 * g + r;
                     const uint32_t d = b < 2 * NB ? b / 2 * 128 + 8 * row + b % 2 * 4 : NB * 128 + 4 * row;
                     if (FULL || d < hd)
-                        *(f4v *)(to + d) = f4v{acc[4 * b][r], acc[4 * b + 1][r], acc[4 * b + 2][r], acc[4 * b + 3][r]} * f;
+                        *(f4v *)(to + d) = f4v{acc[4 * b][r], acc[4 * b + 1][r], acc[4 * b + 2][r], acc[4 * b + 3][r]};
                 }
         }
         __syncthreads();
         const bool whole = k0 == 0 && k1 == units;
-        const size_t slot = (size_t)(A.whole ? 0 : blockIdx.x) + (size_t)t * items + item;
+        const size_t at = (size_t)t * items + item, slot = (A.whole ? 0 : blockIdx.x) + at;
+        if (tid == 0 && !A.whole) {
+            if (k0 == 0) A.bounds[2 * at] = blockIdx.x;
+            if (k1 == units) A.bounds[2 * at + 1] = blockIdx.x;
+        }
         for (uint32_t x = tid * 4; x < heads * hd; x += PA_THREADS * 4) {
             const uint32_t j = x / hd, d = x - j * hd;
-            f4v y = {0, 0, 0, 0};
-#pragma unroll
-            for (int w = 0; w < PARTS; w++) y += *(const f4v *)(sums + (size_t)w * A.per * hd + x);
             float top = wm[0][j], all = 0.0f;
 #pragma unroll
             for (int w = 1; w < PA_WAVES; w++) top = fmaxf(top, wm[w][j]);
+            f4v y = {0, 0, 0, 0};
 #pragma unroll
-            for (int w = 0; w < PA_WAVES; w++)
-                all += wm[w][j] == -INFINITY ? wl[w][j] : wl[w][j] * __builtin_amdgcn_exp2f(wm[w][j] - top);
+            for (int w = 0; w < PA_WAVES; w++) {
+                // (a wave that saw nothing has no sums, but a NaN among them must not hide)
+                const float f = wm[w][j] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(wm[w][j] - top);
+                f4v part = {0, 0, 0, 0};
+#pragma unroll
+                for (int k = 0; k < PARTS / PA_WAVES; k++)
+                    part += *(const f4v *)(sums + (size_t)(w * (PARTS / PA_WAVES) + k) * A.per * hd + x);
+                y += part * f;
+                all += wl[w][j] * f;
+            }
             if (whole) {
                 float *to = A.out + t * A.out_stride + (size_t)(h * A.G + h0 + j) * hd + d;
                 if (all == 0.0f) y = f4v{0, 0, 0, 0};
@@ -569,20 +572,15 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_k(PagedAttnArgs A)
 // A workgroup a query head: its parts at one maximum, added.  32 lanes (64 past 128 dimensions)
 // take every 16th (8th) part, four dimensions a lane, each at the maximum met so far; then
 // those sums are added.  Everything a part has is asked for at once: one wait for 64 parts.
-__device__ __forceinline__ void merge_head(const PagedAttnArgs &A, const PagedWork &D, uint32_t t, uint32_t head, float *sums,
-                                           float *tops, float *alls)
+__device__ __forceinline__ void merge_head(const PagedAttnArgs &A, uint32_t t, uint32_t head, float *sums, float *tops,
+                                           float *alls)
 {
     const uint32_t h = head / A.G, j = head % A.G, tid = threadIdx.x;
     const uint32_t hd = A.C.hd, lanes = hd <= 128 ? 32 : 64, groups = PM_THREADS / lanes, group = tid / lanes;
     const uint32_t d = tid % lanes * 4;
-    const uint32_t item = h * A.tiles + j / A.per;
-    uint64_t at;
-    uint32_t units, first, last;
-    D.row(t, at, units);
-    if (units == 0) return;
-    D.runs(t, item, first, last);
+    const size_t slot = (size_t)t * A.C.n_kv * A.tiles + h * A.tiles + j / A.per;
+    const uint32_t first = word(A.bounds, 2 * slot), last = word(A.bounds, 2 * slot + 1);
     if (first == last) return;
-    const size_t slot = (size_t)t * D.items + item;
     const float *stats = A.stats + (slot * A.per + j % A.per) * 2;
     const float *part = A.part + (slot * A.per + j % A.per) * hd + (d < hd ? d : 0);
     float top = -INFINITY, all = 0.0f;
@@ -634,8 +632,8 @@ __device__ __forceinline__ void merge_head(const PagedAttnArgs &A, const PagedWo
 // A workgroup a kv head's PA_CHUNK positions, four a thread: the group's weights of each, from the scores,
 // summed in the heads' order before they are added to what the row has.  Eight heads at a time: a wave
 // adds up one head's parts while every thread has its eight scores on the way.
-__device__ __forceinline__ void weigh_chunk(const PagedAttnArgs &A, const PagedWork &D, uint32_t t, uint32_t h, uint32_t chunk,
-                                            float *tops, float *by)
+__device__ __forceinline__ void weigh_chunk(const PagedAttnArgs &A, uint32_t t, uint32_t h, uint32_t chunk, float *tops,
+                                            float *by)
 {
     constexpr int WAVES = PM_THREADS / 64;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -652,10 +650,9 @@ __device__ __forceinline__ void weigh_chunk(const PagedAttnArgs &A, const PagedW
             if (on && j0 + k < A.G) sc[k] = *(const f4v *)(scores + (size_t)(j0 + k) * A.C.cap);
         const uint32_t j = j0 + wave;
         if (j < A.G) {
-            const uint32_t item = h * A.tiles + j / A.per;
-            uint32_t first = 0, last = 0;
-            if (!A.whole) D.runs(t, item, first, last);
-            const float *stats = A.stats + (((size_t)t * A.C.n_kv * A.tiles + item) * A.per + j % A.per) * 2;
+            const size_t slot = (size_t)t * A.C.n_kv * A.tiles + h * A.tiles + j / A.per;
+            const uint32_t first = A.whole ? 0 : word(A.bounds, 2 * slot), last = A.whole ? 0 : word(A.bounds, 2 * slot + 1);
+            const float *stats = A.stats + (slot * A.per + j % A.per) * 2;
             float top = -INFINITY, all = 0.0f;
             for (uint32_t w = first + lane; w <= last; w += 64) {
                 const float2 ml = *(const float2 *)(stats + (size_t)w * A.per * 2);
@@ -695,16 +692,13 @@ __device__ __forceinline__ void weigh_chunk(const PagedAttnArgs &A, const PagedW
 // What follows the attention, in one launch: merges of the row's heads, and its kv heads' chunks weighed.
 __global__ __launch_bounds__(PM_THREADS) void paged_after_k(PagedAttnArgs A, uint32_t merges, uint32_t chunks)
 {
-    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     __shared__ __attribute__((aligned(16))) float sums[16 * 128], tops[16], alls[16];
-    PagedWork D;
-    if (!A.whole) D = divide<PM_THREADS>(A, (uint64_t *)lds);
     const uint32_t t = blockIdx.y;
     if (blockIdx.x < merges) {
-        merge_head(A, D, t, blockIdx.x, sums, tops, alls);
+        merge_head(A, t, blockIdx.x, sums, tops, alls);
     } else {
         const uint32_t x = blockIdx.x - merges;
-        weigh_chunk(A, D, t, x / chunks, x % chunks, tops, alls);
+        weigh_chunk(A, t, x / chunks, x % chunks, tops, alls);
     }
 }
 
@@ -769,10 +763,12 @@ extern "C" fox_gpu_status fox_gpu_paged_attention(fox_gpu_ctx *ctx, const fox_gp
     if (scores > (size_t)1 << 33)
         return fox_fail(FOX_GPU_ERR_ARG, "paged_attention: the weights of %zu tokens' %zu heads over %u rows are too "
                         "many", M, n_head, A.C.cap);
-    if ((st = fox_ws_reserve(ctx, (scores + part + stats) * sizeof(float)))) return st;
+    const size_t bounds = A.whole ? 0 : 2 * items;
+    if ((st = fox_ws_reserve(ctx, (scores + part + stats + bounds) * sizeof(float)))) return st;
     A.scores = weigh ? (float *)ctx->ws : nullptr;
     A.part = (float *)ctx->ws + scores;
     A.stats = A.part + part;
+    A.bounds = (uint32_t *)(A.stats + stats);
     FOX_HIP(hipSetDevice(ctx->device));
     const bool bf = cache->type == FOX_GPU_BF16;
     const bool once = !seq && A.tiles == 1;
@@ -789,7 +785,7 @@ extern "C" fox_gpu_status fox_gpu_paged_attention(fox_gpu_ctx *ctx, const fox_gp
     if (merges || chunks) {
         void *after[] = {&A, (void *)&merges, &chunks};
         FOX_HIP(hipLaunchKernel((const void *)paged_after_k, dim3((unsigned)(merges + chunks * cache->n_head_kv), (unsigned)M),
-                                dim3(PM_THREADS), after, starts, ctx->stream));
+                                dim3(PM_THREADS), after, 0, ctx->stream));
     }
     return FOX_GPU_OK;
 }
