@@ -417,6 +417,7 @@ extern "C" fox_gpu_status fox_gpu_paged_rope_store(
 
 #define EV_COPIES 2              // of a histogram: lanes that meet in one place wait for each other
 #define EV_FEW 64                // so many rows are moved by the workgroup that finds them
+#define EV_ONES 8                // so many rows to give up are found one by one
 #define EV_DEEP 2                // rows that a thread of the mover has on the way (4: 22 us instead of 17.5, for registers)
 
 struct EvictArgs {
@@ -554,7 +555,7 @@ __device__ __forceinline__ uint32_t scan_counts(const uint32_t *cnt, uint32_t *p
 // Rows above it and the first of those equal to it are kept; the places and the rows that fill
 // them are listed in order: each wave's 64 rows are counted by a ballot, the counts
 // summed once.  Keys stay in registers, HELD a thread; of longer sequences
-// each turn reads weights and positions anew.  FEW: moves the rows, too.
+// each turn reads weights and positions anew.  Few rows are moved here; FEW: there are never more.
 //
 // It waits, for loads, LDS and other waves, more than it works.
 template <bool FEW, int THREADS, int HELD>
@@ -563,7 +564,7 @@ __global__ __launch_bounds__(THREADS) void evict_select_k(EvictArgs A)
     constexpr int WAVES = THREADS / 64, ROWS = THREADS * HELD;
     static_assert(WAVES * HELD % 64 == 0, "scan_counts");
     __shared__ uint32_t high[EV_COPIES][4096], low[2][EV_COPIES][1024], shares[3][WAVES], cnt[2][HELD * WAVES], pre[2][HELD * WAVES], red[WAVES];
-    __shared__ uint32_t few[FEW ? 2 * EV_FEW : 1];
+    __shared__ uint32_t few[2 * EV_FEW], ones[2][2][WAVES];
     const uint32_t h = blockIdx.x, s = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const size_t head = (size_t)s * A.C.n_kv + h;
@@ -615,6 +616,74 @@ __global__ __launch_bounds__(THREADS) void evict_select_k(EvictArgs A)
         }
     };
 
+    const uint32_t pieces = A.C.hd / 8, side = THREADS / (2 * pieces);
+    auto move_few = [&](uint32_t rows) {                     // the places and rows of few[]
+        for (uint32_t m = tid / (2 * pieces); m < rows; m += side * EV_DEEP) {
+            uint32_t t[EV_DEEP], f[EV_DEEP];
+#pragma unroll
+            for (int i = 0; i < EV_DEEP; i++) {
+                const bool in = m + i * side < rows;
+                t[i] = in ? few[m + i * side] : ~0u;
+                f[i] = in ? few[EV_FEW + m + i * side] : 0u;
+            }
+            move_piece(A, head, s, h, t, f, tid % (2 * pieces), pieces, tid < side * 2 * pieces);
+        }
+    };
+
+    // A step's one row too many (a few): the least key, of equal ones the highest row, is found and
+    // taken out, as often as rows have to go.  evict-step-8b 12.0 us by histograms, 8 so.
+    if (held && n - A.keep <= EV_ONES) {
+        const uint32_t go = n - A.keep;
+        uint32_t out = 0, gone[EV_ONES];                     // a bit a row
+#pragma unroll
+        for (int e = 0; e < EV_ONES; e++) {
+            gone[e] = ~0u;
+            if (e >= go) continue;                           // (uniform)
+            uint32_t k = 0xFFFFFFFFu, r = 0;
+            bool any = false;
+#pragma unroll
+            for (int c = 0; c < HELD; c++)
+                if (c * THREADS < n && c * THREADS + tid < n && !(out >> c & 1) && key[c] <= k) {
+                    k = key[c];                              // (rows rise with c)
+                    r = c * THREADS + tid;
+                    any = true;
+                }
+            const uint32_t least = ~wave_max(~k);
+            const uint32_t most = wave_max(any && k == least ? r + 1 : 0);   // 0: no row is left
+            if (lane == 0) {
+                ones[e & 1][0][wave] = least;
+                ones[e & 1][1][wave] = most;
+            }
+            __syncthreads();
+            const uint32_t kw = lane < WAVES && ones[e & 1][1][lane % WAVES] ? ones[e & 1][0][lane % WAVES] : 0xFFFFFFFFu;
+            const uint32_t all = ~wave_max(~kw);
+            gone[e] = wave_max(lane < WAVES && kw == all ? ones[e & 1][1][lane % WAVES] : 0) - 1;
+            if (gone[e] % THREADS == tid) out |= 1u << (gone[e] / THREADS);
+        }
+        // of the rows from keep on, those that are not gone fill the places below it, both in order
+        uint32_t rows = 0;
+#pragma unroll
+        for (int e = 0; e < EV_ONES; e++) {
+            uint32_t rank = 0, moves = 0;
+            bool left = A.keep + e < n;
+#pragma unroll
+            for (int x = 0; x < EV_ONES; x++) {
+                rank += gone[x] < gone[e];
+                left = left && gone[x] != A.keep + e;
+                moves += gone[x] >= A.keep && gone[x] < A.keep + e;
+            }
+            if (gone[e] < A.keep) {
+                rows++;
+                if (tid == 0) few[rank] = gone[e];
+            }
+            if (left && tid == 0) few[EV_FEW + e - moves] = A.keep + e;
+        }
+        if (!FEW && tid == 0) A.count[head] = 0;
+        __syncthreads();
+        move_few(rows);
+        return;
+    }
+
     uint32_t least = 0, want = A.keep, in;   // the bits found; rows still to take among those that share them
     const uint32_t copy = lane % EV_COPIES;
     for (uint32_t base = 0; base < n; base += ROWS) {
@@ -640,7 +709,7 @@ __global__ __launch_bounds__(THREADS) void evict_select_k(EvictArgs A)
         every = in == want;
     }
 
-    uint32_t *to = FEW ? few : A.list + head * 2 * A.room, *from = FEW ? few + EV_FEW : to + A.room;
+    uint32_t *to = FEW ? nullptr : A.list + head * 2 * A.room, *from = FEW ? nullptr : to + A.room;
     uint32_t ties = 0, places = 0, moves = 0;
     for (uint32_t base = 0; base < n; base += ROWS) {
         if (base) __syncthreads();
@@ -690,12 +759,14 @@ __global__ __launch_bounds__(THREADS) void evict_select_k(EvictArgs A)
                 if (r0 < A.keep) {
                     const bool place = !stay && r0 + lane < A.keep;
                     const uint32_t a = places + (x & 0xFFFFu) + lanes_below(__ballot(place));
-                    if (place && a < A.room) to[a] = r0 + lane;
+                    if (place && a < EV_FEW) few[a] = r0 + lane;
+                    if (!FEW && place && a < A.room) to[a] = r0 + lane;
                 }
                 if (r0 + 64 > A.keep) {
                     const bool mover = stay && r0 + lane >= A.keep;
                     const uint32_t b = moves + (x >> 16) + lanes_below(__ballot(mover));
-                    if (mover && b < A.room) from[b] = r0 + lane;
+                    if (mover && b < EV_FEW) few[EV_FEW + b] = r0 + lane;
+                    if (!FEW && mover && b < A.room) from[b] = r0 + lane;
                 }
             }
         }
@@ -703,22 +774,10 @@ __global__ __launch_bounds__(THREADS) void evict_select_k(EvictArgs A)
         moves += all >> 16;
     }
     const uint32_t rows = min(min(places, moves), A.room);   // (places and moves are equal)
-    if (!FEW) {
-        if (tid == 0) A.count[head] = rows;
-        return;
-    }
+    if (!FEW && tid == 0) A.count[head] = rows > EV_FEW ? rows : 0;
+    if (rows > EV_FEW) return;
     __syncthreads();
-    const uint32_t pieces = A.C.hd / 8, side = THREADS / (2 * pieces);
-    for (uint32_t m = tid / (2 * pieces); m < rows; m += side * EV_DEEP) {
-        uint32_t t[EV_DEEP], f[EV_DEEP];
-#pragma unroll
-        for (int i = 0; i < EV_DEEP; i++) {
-            const bool in = m + i * side < rows;
-            t[i] = in ? to[m + i * side] : ~0u;
-            f[i] = in ? from[m + i * side] : 0u;
-        }
-        move_piece(A, head, s, h, t, f, tid % (2 * pieces), pieces, tid < side * 2 * pieces);
-    }
+    move_few(rows);
 }
 
 // Rows to their places: no place is another's row, so in any order.  A thread has EV_DEEP
