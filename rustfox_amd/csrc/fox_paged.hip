@@ -174,6 +174,8 @@ extern "C" fox_gpu_status fox_gpu_rope_tables(fox_gpu_ctx *ctx, float *cos_t, fl
     A.n = (uint32_t)n;
     A.wide = A.half % 4 == 0 && (uintptr_t)cos_t % 16 == 0 && (uintptr_t)sin_t % 16 == 0;
     const size_t rows = PG_THREADS / ((A.half + 3) / 4) * RT_ROWS;
+    if ((n + rows - 1) / rows > 0xFFFFFFFFu / PG_THREADS)
+        return fox_fail(FOX_GPU_ERR_ARG, "rope_tables: %zu positions of %zu pairs are too many", n, n_rot / 2);
     FOX_HIP(hipSetDevice(ctx->device));
     rope_tables_k<<<dim3((unsigned)((n + rows - 1) / rows)), dim3(PG_THREADS), 0, ctx->stream>>>(A);
     FOX_LAUNCHED("rope_tables");

@@ -53,7 +53,9 @@ struct PagedAttnArgs {
     uint32_t few, workers;
     bool whole;                  // no: a workgroup an item
     float score;                 // log2(e) / sqrt(hd)
-    // of slot (worker + item): sums [slot][per][hd], maxima and weights' sums [slot][per][2]
+    // Parts: sums [part][per][hd], maxima and weights' sums [part][per][2].  A worker has two at most:
+    // of the item that its run begins in (2 worker) and of the one that it ends in (2 worker + 1).
+    // Behind them, where rows are weighed, the maxima and sums of whole items.
     float *part, *stats;
     float *scores;               // [row][head][cap], where rows are weighed
     uint32_t *bounds;            // of every item its first and its last worker
@@ -523,7 +525,8 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_k(PagedAttnArgs A)
         }
         __syncthreads();
         const bool whole = k0 == 0 && k1 == units;
-        const size_t at = (size_t)t * items + item, slot = (A.whole ? 0 : blockIdx.x) + at;
+        const size_t at = (size_t)t * items + item;
+        const size_t slot = !whole ? 2 * (size_t)blockIdx.x + (k0 == 0) : (A.whole ? 0 : 2 * (size_t)A.workers) + at;
         if (tid == 0 && !A.whole) {
             if (k0 == 0) A.bounds[2 * at] = blockIdx.x;
             if (k1 == units) A.bounds[2 * at + 1] = blockIdx.x;
@@ -556,7 +559,7 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_k(PagedAttnArgs A)
             } else {
                 *(f4v *)(A.part + (slot * A.per + j) * hd + d) = y;
             }
-            if (d == 0) *(float2 *)(A.stats + (slot * A.per + j) * 2) = float2{top, all};
+            if (d == 0 && (!whole || A.scores)) *(float2 *)(A.stats + (slot * A.per + j) * 2) = float2{top, all};
         }
         if (A.whole) return;
         __syncthreads();
@@ -578,11 +581,11 @@ __device__ __forceinline__ void merge_head(const PagedAttnArgs &A, uint32_t t, u
     const uint32_t h = head / A.G, j = head % A.G, tid = threadIdx.x;
     const uint32_t hd = A.C.hd, lanes = hd <= 128 ? 32 : 64, groups = PM_THREADS / lanes, group = tid / lanes;
     const uint32_t d = tid % lanes * 4;
-    const size_t slot = (size_t)t * A.C.n_kv * A.tiles + h * A.tiles + j / A.per;
-    const uint32_t first = word(A.bounds, 2 * slot), last = word(A.bounds, 2 * slot + 1);
+    const size_t item = (size_t)t * A.C.n_kv * A.tiles + h * A.tiles + j / A.per;
+    const uint32_t first = word(A.bounds, 2 * item), last = word(A.bounds, 2 * item + 1);
     if (first == last) return;
-    const float *stats = A.stats + (slot * A.per + j % A.per) * 2;
-    const float *part = A.part + (slot * A.per + j % A.per) * hd + (d < hd ? d : 0);
+    const float *stats = A.stats + j % A.per * 2;
+    const float *part = A.part + j % A.per * (size_t)hd + (d < hd ? d : 0);
     float top = -INFINITY, all = 0.0f;
     f4v y = {0, 0, 0, 0};
     for (uint32_t w = first + group; w <= last; w += PM_DEEP * groups) {
@@ -590,7 +593,7 @@ __device__ __forceinline__ void merge_head(const PagedAttnArgs &A, uint32_t t, u
         f4v x[PM_DEEP];
 #pragma unroll
         for (int k = 0; k < PM_DEEP; k++) {
-            const uint32_t at = min(w + k * groups, last);
+            const uint32_t worker = min(w + k * groups, last), at = 2 * worker + (worker == first);
             m[k] = stats[(size_t)at * A.per * 2];
             l[k] = stats[(size_t)at * A.per * 2 + 1];
             x[k] = *(const f4v *)(part + (size_t)at * A.per * hd);
@@ -650,12 +653,13 @@ __device__ __forceinline__ void weigh_chunk(const PagedAttnArgs &A, uint32_t t, 
             if (on && j0 + k < A.G) sc[k] = *(const f4v *)(scores + (size_t)(j0 + k) * A.C.cap);
         const uint32_t j = j0 + wave;
         if (j < A.G) {
-            const size_t slot = (size_t)t * A.C.n_kv * A.tiles + h * A.tiles + j / A.per;
-            const uint32_t first = A.whole ? 0 : word(A.bounds, 2 * slot), last = A.whole ? 0 : word(A.bounds, 2 * slot + 1);
-            const float *stats = A.stats + (slot * A.per + j % A.per) * 2;
+            const size_t item = (size_t)t * A.C.n_kv * A.tiles + h * A.tiles + j / A.per;
+            const uint32_t first = A.whole ? 0 : word(A.bounds, 2 * item), last = A.whole ? 0 : word(A.bounds, 2 * item + 1);
+            const float *stats = A.stats + j % A.per * 2;
             float top = -INFINITY, all = 0.0f;
             for (uint32_t w = first + lane; w <= last; w += 64) {
-                const float2 ml = *(const float2 *)(stats + (size_t)w * A.per * 2);
+                const size_t at = first != last ? 2 * (size_t)w + (w == first) : (A.whole ? 0 : 2 * (size_t)A.workers) + item;
+                const float2 ml = *(const float2 *)(stats + at * A.per * 2);
                 const float mx = fmaxf(top, ml.x);
                 all = (top == -INFINITY ? all : all * __builtin_amdgcn_exp2f(top - mx)) +
                       (ml.x == -INFINITY ? ml.y : ml.y * __builtin_amdgcn_exp2f(ml.x - mx));
@@ -757,19 +761,19 @@ extern "C" fox_gpu_status fox_gpu_paged_attention(fox_gpu_ctx *ctx, const fox_gp
     // (rows that are weighed are stored, too: attn-8b-24-weigh 70 / 64 us)
     A.few = weigh || A.workers < (uint32_t)ctx->n_cu ? A.workers : (uint32_t)ctx->n_cu;
     // parts, their maxima and sums, and the scores of rows that are weighed
-    const size_t slots = A.whole ? items : items + A.workers;
-    const size_t part = A.whole ? 0 : slots * A.per * cache->head_dim, stats = slots * A.per * 2;
+    const size_t parts = A.whole ? 0 : 2 * (size_t)A.workers;
+    const size_t part = parts * A.per * cache->head_dim, stats = (parts + (weigh ? items : 0)) * A.per * 2;
     const size_t scores = weigh ? M * n_head * A.C.cap : 0;
     if (scores > (size_t)1 << 33)
         return fox_fail(FOX_GPU_ERR_ARG, "paged_attention: the weights of %zu tokens' %zu heads over %u rows are too "
                         "many", M, n_head, A.C.cap);
     const size_t bounds = A.whole ? 0 : 2 * items;
+    FOX_HIP(hipSetDevice(ctx->device));
     if ((st = fox_ws_reserve(ctx, (scores + part + stats + bounds) * sizeof(float)))) return st;
     A.scores = weigh ? (float *)ctx->ws : nullptr;
     A.part = (float *)ctx->ws + scores;
     A.stats = A.part + part;
     A.bounds = (uint32_t *)(A.stats + stats);
-    FOX_HIP(hipSetDevice(ctx->device));
     const bool bf = cache->type == FOX_GPU_BF16;
     const bool once = !seq && A.tiles == 1;
 #define FOX_ATTN(hg, o) (bf ? attn_kernel<true, hg, o>(cache->head_dim) : attn_kernel<false, hg, o>(cache->head_dim))

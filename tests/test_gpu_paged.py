@@ -248,6 +248,60 @@ def test_attention(gpu, kind, case, weigh):
     check(gpu, c, q, n_head, weigh=weigh, pad=3, lead=1)
 
 
+WIDE = [(n_head, hd) for n_head in (2, 8, 34) for hd in (64, 56, 128, 104, 192, 136, 256, 200)]
+
+
+@pytest.mark.parametrize("case", WIDE, ids=str)
+@pytest.mark.parametrize("kind", KINDS)
+def test_every_kernel(gpu, kind, case):
+    """Up to 4, 16 and more heads over a kv head, every width, whole and ragged: divided among workers
+    and not, rows of one sequence each and of sequences given."""
+    n_head, hd = case
+    rng = np.random.default_rng(n_head * hd)
+    for lengths, page in (([1100, 0, 63, 64, 65, 1, 2049], 32), ([40, 333, 16], 16)):
+        c = Paged(gpu, rng, kind, 2, hd, page, lengths, room=100)
+        q = (1.5 * rng.standard_normal((len(lengths), n_head * hd))).astype(np.float32)
+        got = check(gpu, c, q, n_head, weigh=True)
+        assert np.array_equal(got, check(gpu, c, q, n_head, seq=np.arange(len(lengths))))
+
+
+@pytest.mark.parametrize("cap", [512, 528, 1104, 2048, 2064])
+def test_short_caches(gpu, cap):
+    """A workgroup a head or a run of units, on both sides of where that changes, for few and many
+    items; more sequences than a wave has lanes, some without rows."""
+    rng = np.random.default_rng(cap)
+    for n, n_kv in ((2, 4), (66, 4)):
+        lengths = [int(x) for x in rng.integers(0, cap + 1, n)]
+        lengths[0], lengths[-1] = cap, 0
+        c = Paged(gpu, rng, rf.BF16, n_kv, 64, 16, lengths)
+        q = rng.standard_normal((n, 2 * n_kv * 64)).astype(np.float32)
+        check(gpu, c, q, 2 * n_kv, weigh=True)
+
+
+def test_the_most_heads(gpu):
+    """65535 heads of one kv head, and 4096 kv heads: the largest grids and tiles."""
+    rng = np.random.default_rng(31)
+    for n_head, n_kv, lengths in ((65535, 1, [70, 600]), (8192, 4096, [20]), (4096, 4096, [530])):
+        c = Paged(gpu, rng, rf.F16, n_kv, 8, 16, lengths, track=n_kv > 1)
+        q = rng.standard_normal((len(lengths), n_head * 8)).astype(np.float32)
+        got = attend(gpu, c, q, n_head, weigh=n_kv > 1)
+        some = np.unique(np.concatenate([[0, n_head - 1], rng.integers(0, n_head, 60)]))
+        cols = (some[:, None] * 8 + np.arange(8)).reshape(-1)
+        for t, n in enumerate(lengths):
+            for h in some:
+                g = h // (n_head // n_kv)
+                pools = [p[:, g:g + 1] for p in c.pools]
+                want, sizes, _ = pr.attention(q[t:t + 1, h * 8:h * 8 + 8], *pools, c.table, c.kind, 1, [n], [t])
+                assert (np.abs(got[t:t + 1, h * 8:h * 8 + 8] - want) <= pr.attention_bound(sizes)).all()
+
+
+def test_the_largest_pages(gpu):
+    rng = np.random.default_rng(32)
+    c = Paged(gpu, rng, rf.F16, 2, 64, 4096, [9000, 4096, 17])
+    q = rng.standard_normal((3, 8 * 64)).astype(np.float32)
+    check(gpu, c, q, 8, weigh=True)
+
+
 def test_a_long_row(gpu):
     """Many splits of one sequence, beside short ones."""
     rng = np.random.default_rng(3)
@@ -386,6 +440,46 @@ def test_evict(gpu, kind, case, values):
     c.length = m
     gpu.paged_evict(c.c, dev(gpu, m), kept, keep, recent)
     assert np.array_equal(c.k.numpy(), k) and np.array_equal(kept.numpy(), m)
+
+
+@pytest.mark.parametrize("cap", [400, 5000, 40000])
+@pytest.mark.parametrize("equal", [False, True])
+def test_evict_by_ones_and_twos(gpu, cap, equal):
+    """From one row too many to a dozen, in caches with little and much room, in keys all equal too."""
+    rng = np.random.default_rng(cap)
+    for keep in (1, 2, 5, 63, 64, 65, 380):
+        lengths = [keep + x for x in range(0, 13)]
+        c = Paged(gpu, rng, rf.F16, 1, 16, 16, lengths, room=cap - max(lengths))
+        if equal:
+            c.weight[:] = rng.integers(0, 2, c.weight.shape)
+        for s, n in enumerate(lengths):
+            c.position[s, 0, :n] = rng.permutation(n)
+        c.upload()
+        kept = dev(gpu, np.zeros(len(lengths), np.uint32))
+        gpu.paged_evict(c.c, c.d_length, kept, keep, min(keep, 3))
+        k, v, w, p, m = pr.evict(*c.pools, c.table, c.weight, c.position, c.length, keep, min(keep, 3))
+        assert np.array_equal(kept.numpy(), m)
+        assert np.array_equal(c.d_position.numpy(), p) and np.array_equal(c.d_weight.numpy(), w)
+        assert np.array_equal(c.k.numpy(), k) and np.array_equal(c.v.numpy(), v)
+
+
+@pytest.mark.parametrize("values", ["spread", "equal"])
+@pytest.mark.parametrize("keep,recent", [(59999, 100), (59000, 0), (30000, 30000), (24576, 77), (100, 5), (1, 0)])
+def test_evict_longer_than_registers(gpu, keep, recent, values):
+    """Rows past those that a workgroup holds, read anew in every turn."""
+    rng = np.random.default_rng(keep)
+    c = Paged(gpu, rng, rf.BF16, 1, 8, 128, [60000, 24577, 24576], spare=0)
+    c.weight[:] = np.exp(2 * rng.standard_normal(c.weight.shape)) if values == "spread" else \
+        rng.integers(0, 2, c.weight.shape)
+    for s, n in enumerate(c.length):
+        c.position[s, 0, :n] = rng.permutation(int(n))
+    c.upload()
+    kept = dev(gpu, np.zeros(3, np.uint32))
+    gpu.paged_evict(c.c, c.d_length, kept, keep, recent)
+    k, v, w, p, m = pr.evict(*c.pools, c.table, c.weight, c.position, c.length, keep, recent)
+    assert np.array_equal(kept.numpy(), m)
+    assert np.array_equal(c.d_position.numpy(), p) and np.array_equal(c.d_weight.numpy(), w)
+    assert np.array_equal(c.k.numpy(), k) and np.array_equal(c.v.numpy(), v)
 
 
 def test_evict_positions_alike_or_far(gpu):

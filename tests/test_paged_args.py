@@ -53,7 +53,7 @@ CALLS = {
         (dict(ctx=None), ARG), (dict(cos=None), ARG), (dict(sin=None), ARG), (dict(freq=None), ARG), (dict(n=0), ARG),
         (dict(n_rot=0), ARG), (dict(n_rot=63), UNSUPPORTED), (dict(n_rot=258), UNSUPPORTED),
         (dict(n=(1 << 30) + 1), ARG), (dict(p0=(1 << 30) + 1), ARG), (dict(p0=1 << 30, n=1), ARG),
-        (dict(p0=2 ** 64 - 1, n=2), ARG)] +
+        (dict(p0=2 ** 64 - 1, n=2), ARG), (dict(n=1 << 30, n_rot=256), ARG)] +
         [(dict(freq=dict(FREQ, **f)), ARG) for f in (
             dict(base=0.0), dict(base=-1.0), dict(base=NAN), dict(base=INF), dict(scale=NAN), dict(scale=INF),
             dict(ext=NAN), dict(magnitude=INF), dict(ext=1.0), dict(ext=1.0, orig_ctx=64.0, base=1.0),
