@@ -88,6 +88,7 @@ struct PagedWork {
     // the row that holds unit u of the call
     __device__ __forceinline__ uint32_t row_of(uint64_t u) const
     {
+        if (M == 1) return 0;
         if (M <= 64) {
             const uint32_t lane = threadIdx.x & 63;
             return 63 - __builtin_clzll(__ballot(lane < M && (uint64_t)before * items <= u));
@@ -130,10 +131,17 @@ __device__ __forceinline__ PagedWork divide(const PagedAttnArgs &A, uint64_t *st
     D.M = A.M;
     D.items = A.C.n_kv * A.tiles;
     D.length = D.seq = 0;
-    if (A.M <= 64) {
+    if (A.M == 1) {                                                 // (by the scalar unit)
+        D.seq = A.seq ? word(A.seq, 0) : 0;
+        const uint32_t n = word(A.length, 0);
+        D.length = D.seq < A.C.n_seqs ? min(n, A.C.cap) : 0;
+        D.units = units_of(D.length);
+        D.before = 0;
+        D.total = (uint64_t)D.units * D.items;
+    } else if (A.M <= 64) {
         if (lane < A.M) D.length = row_length(A, lane, D.seq);
         D.units = units_of(D.length);                               // (64 of at most 2^24)
-        const uint32_t x = A.M > 1 ? wave_scan(D.units) : D.units;
+        const uint32_t x = wave_scan(D.units);
         D.before = x - D.units;
         D.total = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)x, (int)A.M - 1) * D.items;
     } else {
@@ -326,8 +334,15 @@ __device__ __forceinline__ void load_values(Tile<W> &T, __amdgpu_buffer_rsrc_t a
 // matrix unit's time): block b multiplies what its four lanes hold, V's dimensions of
 // one position and the weights of the four heads there.
 template <bool BF, int W, bool FULL, int HG, bool ONCE>
-__global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_k(PagedAttnArgs A)
+__global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_k(const uint32_t *length0, const uint32_t *seq0, uint32_t M0,
+                                                             uint32_t n_seqs0, uint32_t cap0, PagedAttnArgs A)
 {
+    // (what the first reads need comes in registers: the rest is read beside them)
+    A.length = length0;
+    A.seq = seq0;
+    A.M = M0;
+    A.C.n_seqs = n_seqs0;
+    A.C.cap = cap0;
     constexpr int NC = W / 32, NP = HG == 4 ? 1 : BF ? 3 : 2, NB = W / 128, NU = W % 128 ? 4 : 0, NA = NB * 8 + NU;
     constexpr bool QLDS = W > (HG == 4 ? 192 : 128);     // queries' parts stay in LDS
     constexpr int PARTS = HG == 4 ? 4 * PA_WAVES : PA_WAVES;   // partial sums of a workgroup
@@ -578,14 +593,15 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_k(PagedAttnArgs A)
 __device__ __forceinline__ void merge_head(const PagedAttnArgs &A, uint32_t t, uint32_t head, float *sums, float *tops,
                                            float *alls)
 {
-    const uint32_t h = head / A.G, j = head % A.G, tid = threadIdx.x;
+    const uint32_t h = head / A.G, j = head - h * A.G, tid = threadIdx.x;
+    const uint32_t tile = A.tiles == 1 ? 0 : j / A.per, in_tile = j - tile * A.per;
     const uint32_t hd = A.C.hd, lanes = hd <= 128 ? 32 : 64, groups = PM_THREADS / lanes, group = tid / lanes;
     const uint32_t d = tid % lanes * 4;
-    const size_t item = (size_t)t * A.C.n_kv * A.tiles + h * A.tiles + j / A.per;
+    const size_t item = (size_t)t * A.C.n_kv * A.tiles + h * A.tiles + tile;
     const uint32_t first = word(A.bounds, 2 * item), last = word(A.bounds, 2 * item + 1);
     if (first == last) return;
-    const float *stats = A.stats + j % A.per * 2;
-    const float *part = A.part + j % A.per * (size_t)hd + (d < hd ? d : 0);
+    const float *stats = A.stats + in_tile * 2;
+    const float *part = A.part + in_tile * (size_t)hd + (d < hd ? d : 0);
     float top = -INFINITY, all = 0.0f;
     f4v y = {0, 0, 0, 0};
     for (uint32_t w = first + group; w <= last; w += PM_DEEP * groups) {
@@ -694,8 +710,14 @@ __device__ __forceinline__ void weigh_chunk(const PagedAttnArgs &A, uint32_t t, 
 }
 
 // What follows the attention, in one launch: merges of the row's heads, and its kv heads' chunks weighed.
-__global__ __launch_bounds__(PM_THREADS) void paged_after_k(PagedAttnArgs A, uint32_t merges, uint32_t chunks)
+__global__ __launch_bounds__(PM_THREADS) void paged_after_k(const uint32_t *bounds0, uint32_t merges, uint32_t chunks, uint32_t n_kv0,
+                                                            uint32_t G0, uint32_t tiles0, uint32_t per0, PagedAttnArgs A)
 {
+    A.bounds = (uint32_t *)bounds0;                          // (in registers from the start, as above)
+    A.C.n_kv = n_kv0;
+    A.G = G0;
+    A.tiles = tiles0;
+    A.per = per0;
     __shared__ __attribute__((aligned(16))) float sums[16 * 128], tops[16], alls[16];
     const uint32_t t = blockIdx.y;
     if (blockIdx.x < merges) {
@@ -781,13 +803,13 @@ extern "C" fox_gpu_status fox_gpu_paged_attention(fox_gpu_ctx *ctx, const fox_gp
 #undef FOX_ATTN
     const size_t starts = M > 64 && !A.whole ? ((M + 1) * 8 + 15) / 16 * 16 : 0;
     const size_t lds = starts + (size_t)(four ? 4 : 1) * PA_WAVES * A.per * cache->head_dim * sizeof(float);
-    void *args[] = {&A};
+    void *args[] = {&A.length, &A.seq, &A.M, &A.C.n_seqs, &A.C.cap, &A};
     FOX_HIP(hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
     FOX_HIP(hipLaunchKernel(k, dim3(A.workers), dim3(PA_THREADS), args, lds, ctx->stream));
     const uint32_t merges = A.whole || A.workers == 1 ? 0 : (uint32_t)n_head;
     uint32_t chunks = weigh ? (A.C.cap + PA_CHUNK - 1) / PA_CHUNK : 0;
     if (merges || chunks) {
-        void *after[] = {&A, (void *)&merges, &chunks};
+        void *after[] = {&A.bounds, (void *)&merges, &chunks, &A.C.n_kv, &A.G, &A.tiles, &A.per, &A};
         FOX_HIP(hipLaunchKernel((const void *)paged_after_k, dim3((unsigned)(merges + chunks * cache->n_head_kv), (unsigned)M),
                                 dim3(PM_THREADS), after, 0, ctx->stream));
     }
