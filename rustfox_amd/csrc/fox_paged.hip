@@ -83,7 +83,8 @@ struct Terms {
 // (Angles in floats would be off by 2^-24 of all the turns made.)
 //
 // A thread has four pairs and RT_ROWS rows of them, so speeds are read once; the two tables are
-// all that moves, and their writes bound it: 131072 positions of 64 pairs (67 MB).
+// all that moves, and their writes bound it: 131072 positions of 64 pairs (67 MB) 15.1 us, 4.4 TB/s
+// (with the library's sine and cosine in double, a value a thread, 43).
 __global__ __launch_bounds__(PG_THREADS) void rope_tables_k(FreqArgs A)
 {
     const uint32_t quads = (A.half + 3) / 4, rows = PG_THREADS / quads;      // (quads <= 32)
@@ -237,7 +238,8 @@ __device__ __forceinline__ void load_eight(float x[8], const float *p, bool wide
 // FAST: rows, tables and weights take 16-byte accesses, and eight dimensions have eight (four) pairs' angles
 // that stand side by side.
 //
-// Bound by its reads and writes where there are many tokens: 1001 tokens of 32 + 16 + 16 heads of 128 (58 MB).
+// Bound by its reads and writes where there are many tokens: 1001 tokens of 32 + 16 + 16 heads of 128 (58 MB)
+// 14.5 us, 4.0 TB/s; 12.5 without norms. (A wave a row, a value a lane: 33.5.)
 template <bool BF, int LANES, bool FAST>
 __global__ __launch_bounds__(PG_THREADS) void paged_store_k(PagedStoreArgs A)
 {
@@ -559,7 +561,9 @@ __device__ __forceinline__ uint32_t scan_counts(const uint32_t *cnt, uint32_t *p
 // summed once.  Keys stay in registers, HELD a thread; of longer sequences
 // each turn reads weights and positions anew.  Few rows are moved here; FEW: there are never more.
 //
-// It waits, for loads, LDS and other waves, more than it works.
+// It waits, for loads, LDS and other waves, more than it works: 48 kv heads of up to 20011 rows 19 us
+// (of it 3.5 us the rows' way to one compute unit, 4 the histograms, 6 the lists), one row too many of
+// 2049 in 128 kv heads 6.3 us.
 template <bool FEW, int THREADS, int HELD>
 __global__ __launch_bounds__(THREADS) void evict_select_k(EvictArgs A)
 {
@@ -783,7 +787,8 @@ __global__ __launch_bounds__(THREADS) void evict_select_k(EvictArgs A)
 }
 
 // Rows to their places: no place is another's row, so in any order.  A thread has EV_DEEP
-// rows' pieces on the way, since each waits for the list, the table and the row in turn.
+// rows' pieces on the way, since each waits for the list, the table and the row in turn: 71 MB read and
+// written in 17.5 us, 4.1 TB/s.
 __global__ __launch_bounds__(PG_THREADS) void evict_move_k(EvictArgs A)
 {
     const uint32_t head = blockIdx.x / A.movers, part = blockIdx.x % A.movers, h = head % A.C.n_kv, s = head / A.C.n_kv;

@@ -4,14 +4,14 @@
 // Arithmetic.  A tile is 16 positions of one kv head, by the (up to 16) query heads that
 // share it:
 //   S[pos][head] = sum_d K[pos][d] q[head][d]          16x16x32 products of 16 bits
-//   O[dim][head] += sum_pos V[pos][dim] P[pos][head]   16x16x4 products of 32 bits
+//   O[dim][head] += sum_pos V[pos][dim] P[pos][head]   16x16x4 or 4x4x1 products of 32 bits
 // The cache's values are multiplied as they are.  A query is the sum of two halves (its head's row
 // first brought to 2^14 .. 2^15 by a power of two) or of three bfloat16 (exact), each
 // its own product into the same float sums.  Weights stay floats: a 16-bit second
 // product would need V by columns, eight positions of a dimension to a lane, where pages hold
 // rows; of the 32-bit one, a lane of S holds four positions of one head, which are the
 // operands of four products as they stand, and a row of V is read whole by 16 lanes.  Its rate is
-// enough: a tile of 128 dimensions takes 1100 clocks of one SIMD's matrix unit, and
+// enough: a tile of 128 dimensions and 16 heads takes 1100 clocks of one SIMD's matrix unit, and
 // 8 KB at the copy's rate 1600 clocks of a SIMD's share.
 // The running maximum only follows scores that pass it by 8 (in powers of two), so
 // between updates no lane needs another's.
@@ -19,7 +19,14 @@
 // Division.  A row's heads have ceil(length / 64) units of 64 positions, one tile for
 // each wave of a workgroup.  All units of a call, in order of row, head, position, are
 // cut into equal runs, one a workgroup, whatever the lengths, which only the device knows; a
-// head whose units lie in several runs is merged by a second launch.
+// head whose units lie in several runs is merged by a second launch.  (Merged by the last workgroup
+// to arrive, one launch less takes four times as long: before it counts itself each must write its
+// part past its XCD's cache, and the fence for that empties it.)
+//
+// Bound by reads: 64 sequences of 8192 rows and fewer, 16 kv heads of 128 (1.64 GB), 270 us, 6.1 TB/s
+// (a plain read reaches 6.5); one of 131071, 8 kv heads (537 MB), 86 us; matrix units are
+// busy a tenth of the time.  Short calls by their way in and out, straight code
+// that each workgroup meets cold: 4097 rows of 8 kv heads (17 MB) 15 us, 11 of them the first launch.
 #include "fox_paged_dev.h"
 
 #include <cfloat>
@@ -71,15 +78,15 @@ __device__ __forceinline__ uint32_t word(const uint32_t *p, size_t i) { return (
 
 __device__ __forceinline__ uint32_t units_of(uint32_t n) { return (n + PA_UNIT - 1) / PA_UNIT; }
 
-// Where the units of each row begin, counted for one of its heads (an item): up to 64
-// rows by every wave for itself, lane t row t, without LDS or a barrier; more by the
-// workgroup, in LDS.
 // a / b; most calls' units are below 2^32, where a quotient takes 20 instructions, not 150
 __device__ __forceinline__ uint64_t over(uint64_t a, uint32_t b)
 {
     return a >> 32 ? a / b : (uint32_t)a / b;
 }
 
+// Where the units of each row begin, counted for one of its heads (an item): up to 64
+// rows by every wave for itself, lane t row t, without LDS or a barrier; more by the
+// workgroup, in LDS.
 struct PagedWork {
     const uint64_t *start;        // [M + 1], past 64 rows
     uint64_t run, total;          // units of a worker; of the call

@@ -332,6 +332,28 @@ def test_tokens_of_one_sequence(gpu, kind):
     assert (got[-3:] == 0).all()
 
 
+def test_many_tokens_and_rows_behind_them(gpu):
+    """More tokens than a wave has lanes, of few sequences and of some that are none; what lies behind
+    the last token stays."""
+    rng = np.random.default_rng(33)
+    c = Paged(gpu, rng, rf.BF16, 2, 64, 16, [700, 60, 1])
+    seq = rng.integers(0, 5, 130).astype(np.uint32)
+    seq[5] = 2 ** 32 - 1
+    length = rng.integers(0, 700, 130)
+    length[seq < 3] = np.minimum(length, c.length[np.minimum(seq, 2)])[seq < 3]
+    q = rng.standard_normal((130, 8 * 64)).astype(np.float32)
+    check(gpu, c, q, 8, length, seq)
+    out = dev(gpu, np.full((140, 8 * 64), 9.25, np.float32))
+    gpu.paged_attention(c.c, out, dev(gpu, q), 8, 130, dev(gpu, length, np.uint32), seq=dev(gpu, seq))
+    got = out.numpy()
+    assert (got[130:] == 9.25).all() and (got[:130][seq >= 3] == 0).all()
+    before = c.d_weight.numpy()
+    gpu.paged_attention(c.c, out, dev(gpu, q), 8, 2, dev(gpu, [0, 7], np.uint32), weigh=True)
+    after = c.d_weight.numpy()
+    assert np.array_equal(after[0], before[0]) and np.array_equal(after[2], before[2])
+    assert np.array_equal(after[1, :, 7:], before[1, :, 7:]) and (after[1, :, :7] > before[1, :, :7]).any()
+
+
 @pytest.mark.parametrize("kind", KINDS)
 def test_pages_that_are_none(gpu, kind):
     """Rows without a page are hidden, whole sequences too; a length past the table's rows means all
