@@ -36,6 +36,7 @@ typedef _Float16 h8v __attribute__((ext_vector_type(8)));
 typedef short s8v __attribute__((ext_vector_type(8)));
 typedef __bf16 b8v __attribute__((ext_vector_type(8)));
 typedef float f4v __attribute__((ext_vector_type(4)));
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));   // (rows of any alignment)
 typedef uint32_t u4v __attribute__((ext_vector_type(4)));
 typedef uint32_t u2v __attribute__((ext_vector_type(2)));
 
@@ -66,7 +67,6 @@ struct PagedAttnArgs {
     float *part, *stats;
     float *scores;               // [row][head][cap], where rows are weighed
     uint32_t *bounds;            // of every item its first and its last worker
-    bool q_wide, out_wide;       // rows take 16-byte accesses
 };
 
 // ---------------------------------------------------------------- division
@@ -185,28 +185,15 @@ __device__ __forceinline__ PagedWork divide(const PagedAttnArgs &A, uint64_t *st
 
 // ------------------------------------------------------------------- tiles
 
-// eight floats of a query's row from dimension d on (zero past hd)
-__device__ __forceinline__ void load_q(float x[8], const float *row, uint32_t d, uint32_t hd, bool on, bool wide)
-{
-    on = on && d < hd;
-    if (wide) {
-        *(float4 *)x = on ? *(const float4 *)(row + d) : float4{0, 0, 0, 0};
-        *(float4 *)(x + 4) = on ? *(const float4 *)(row + d + 4) : float4{0, 0, 0, 0};
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = on ? row[d + i] : 0.0f;
-}
-
 // the parts of eight query values: two halves of x 2^e, or three bfloat16
 template <bool BF>
-__device__ __forceinline__ void split_q(uint4 part[BF ? 3 : 2], const float x[8], int e)
+__device__ __forceinline__ void split_q(uint4 part[BF ? 3 : 2], const f4v x[2], int e)
 {
     uint32_t w[3][4] = {};
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         if (BF) {
-            float r = x[i];
+            float r = x[i / 4][i % 4];
 #pragma unroll
             for (int k = 0; k < 3; k++) {                // (truncated: what is left is exact)
                 const uint32_t u = __float_as_uint(r) & 0xFFFF0000u;
@@ -214,7 +201,7 @@ __device__ __forceinline__ void split_q(uint4 part[BF ? 3 : 2], const float x[8]
                 r -= __uint_as_float(u);
             }
         } else {
-            const float y = ldexpf(x[i], e);
+            const float y = ldexpf(x[i / 4][i % 4], e);
             const _Float16 hi = (_Float16)y, lo = (_Float16)(y - (float)hi);
             w[0][i / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, hi) << (16 * (i & 1));
             w[1][i / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, lo) << (16 * (i & 1));
@@ -410,11 +397,18 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_k(const uint32_t *le
         const uint32_t *table = A.C.table + (size_t)s * A.C.max_pages;
 
         // the queries' rows and the first tile are asked for together
-        float x[NC][8];
+        // (heads past the tile's read as zeros behind its end, and so do dimensions past the row's)
+        f4v x[NC][2];
         {
-            const float *row = A.q + t * A.q_stride + (size_t)(h * A.G + h0 + (col < heads ? col : 0)) * hd;
+            const __amdgpu_buffer_rsrc_t at = __builtin_amdgcn_make_buffer_rsrc(
+                (float *)A.q + t * A.q_stride + (size_t)(h * A.G + h0) * hd, 0, heads * hd * 4, 0x00027000);
 #pragma unroll
-            for (int c = 0; c < NC; c++) load_q(x[c], row, 32 * c + 8 * g, hd, col < heads, A.q_wide);
+            for (int c = 0; c < NC; c++) {
+                const uint32_t d = 32 * c + 8 * g, o = FULL || d < hd ? (col * hd + d) * 4 : PA_NOWHERE;
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+                    x[c][k] = __builtin_bit_cast(f4v, __builtin_amdgcn_raw_buffer_load_b128(at, o + 16 * k, 0, 0));
+            }
         }
         // Tiles of this wave: p0, p0 + PA_UNIT, ...; two are held, and as soon as one's keys
         // (values) are used, those of the tile after the next are asked for in their place.
@@ -450,7 +444,7 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_k(const uint32_t *le
 #pragma unroll
                 for (int c = 0; c < NC; c++)
 #pragma unroll
-                    for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(x[c][j]));
+                    for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(x[c][j / 4][j % 4]));
                 top = max_of_groups(top);
                 // (top is in 2^-149 .. 2^128; an infinity stays one)
                 e = top > 0.0f && top <= FLT_MAX ? 15 - (ilogbf(top) + 1) : 0;
@@ -574,10 +568,7 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_k(const uint32_t *le
                 float *to = A.out + t * A.out_stride + (size_t)(h * A.G + h0 + j) * hd + d;
                 if (all == 0.0f) y = f4v{0, 0, 0, 0};
                 else y /= all;
-                if (A.out_wide) *(f4v *)to = y;
-                else
-#pragma unroll
-                    for (int k = 0; k < 4; k++) to[k] = y[k];
+                *(f4u *)to = y;
             } else {
                 *(f4v *)(A.part + (slot * A.per + j) * hd + d) = y;
             }
@@ -775,8 +766,6 @@ extern "C" fox_gpu_status fox_gpu_paged_attention(fox_gpu_ctx *ctx, const fox_gp
     A.tiles = (A.G + 15) / 16;
     A.per = (A.G + A.tiles - 1) / A.tiles;
     A.score = (float)(1.4426950408889634 / std::sqrt((double)cache->head_dim));
-    A.q_wide = (uintptr_t)q % 16 == 0 && (M == 1 || q_stride % 4 == 0);
-    A.out_wide = (uintptr_t)out % 16 == 0 && (M == 1 || out_stride % 4 == 0);
     const size_t items = M * cache->n_head_kv * A.tiles;
     const bool four = A.per <= 4;
     // Short caches: a workgroup an item, one launch.  How short depends on the items, since one alone
