@@ -32,13 +32,14 @@
 #include <cfloat>
 #include <cmath>
 
+typedef _Float16 h2v __attribute__((ext_vector_type(2)));
 typedef _Float16 h8v __attribute__((ext_vector_type(8)));
-typedef short s8v __attribute__((ext_vector_type(8)));
 typedef __bf16 b8v __attribute__((ext_vector_type(8)));
 typedef float f4v __attribute__((ext_vector_type(4)));
 typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));   // (rows of any alignment)
 typedef uint32_t u4v __attribute__((ext_vector_type(4)));
 typedef uint32_t u2v __attribute__((ext_vector_type(2)));
+typedef float f2v __attribute__((ext_vector_type(2)));
 
 #define PA_WAVES 4
 #define PA_THREADS (64 * PA_WAVES)
@@ -189,22 +190,24 @@ __device__ __forceinline__ PagedWork divide(const PagedAttnArgs &A, uint64_t *st
 template <bool BF>
 __device__ __forceinline__ void split_q(uint4 part[BF ? 3 : 2], const f4v x[2], int e)
 {
-    uint32_t w[3][4] = {};
+    uint32_t w[3][4];
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        if (BF) {
-            float r = x[i / 4][i % 4];
+    for (int i = 0; i < 4; i++) {                        // two values a word
+        const float a = x[i / 2][i % 2 * 2], b = x[i / 2][i % 2 * 2 + 1];
+        if (BF) {                                        // (truncated: what is left is exact)
+            uint32_t u = __float_as_uint(a), v = __float_as_uint(b);
 #pragma unroll
-            for (int k = 0; k < 3; k++) {                // (truncated: what is left is exact)
-                const uint32_t u = __float_as_uint(r) & 0xFFFF0000u;
-                w[k][i / 2] |= i & 1 ? u : u >> 16;
-                r -= __uint_as_float(u);
+            for (int k = 0; k < 3; k++) {
+                w[k][i] = __builtin_amdgcn_perm(v, u, 0x07060302);
+                u = __float_as_uint(__uint_as_float(u) - __uint_as_float(u & 0xFFFF0000u));
+                v = __float_as_uint(__uint_as_float(v) - __uint_as_float(v & 0xFFFF0000u));
             }
         } else {
-            const float y = ldexpf(x[i / 4][i % 4], e);
-            const _Float16 hi = (_Float16)y, lo = (_Float16)(y - (float)hi);
-            w[0][i / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, hi) << (16 * (i & 1));
-            w[1][i / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, lo) << (16 * (i & 1));
+            const f2v y = {ldexpf(a, e), ldexpf(b, e)};
+            const h2v hi = __builtin_convertvector(y, h2v);
+            const h2v lo = __builtin_convertvector(y - __builtin_convertvector(hi, f2v), h2v);
+            w[0][i] = __builtin_bit_cast(uint32_t, hi);
+            w[1][i] = __builtin_bit_cast(uint32_t, lo);
         }
     }
 #pragma unroll
