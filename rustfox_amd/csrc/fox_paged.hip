@@ -571,6 +571,7 @@ __global__ __launch_bounds__(THREADS) void evict_select_k(EvictArgs A)
     static_assert(WAVES * HELD % 64 == 0, "scan_counts");
     __shared__ uint32_t high[EV_COPIES][4096], low[2][EV_COPIES][1024], shares[3][WAVES], cnt[2][HELD * WAVES], pre[2][HELD * WAVES], red[WAVES];
     __shared__ uint32_t few[2 * EV_FEW], ones[2][2][WAVES];
+    __shared__ uint64_t words[HELD * WAVES];
     const uint32_t h = blockIdx.x, s = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const size_t head = (size_t)s * A.C.n_kv + h;
@@ -742,17 +743,20 @@ __global__ __launch_bounds__(THREADS) void evict_select_k(EvictArgs A)
                 }
             ties += all;
         }
-        // places in the low half, rows to move in the high half (a wave's 64 rows are mostly one or the other)
+        // A wave's rows as masks, kept by lane c, then counted by a thread a mask: places in the low half, rows
+        // to move in the high half.
+        uint64_t mine = 0;
 #pragma unroll
         for (int c = 0; c < HELD; c++) {
-            const uint32_t r0 = base + c * THREADS + wave * 64;
-            uint32_t x = 0;
-            if (r0 < n) {
-                const bool stay = stays >> c & 1;
-                if (r0 < A.keep) x = __popcll(__ballot(!stay && r0 + lane < A.keep));
-                if (r0 + 64 > A.keep) x |= __popcll(__ballot(stay && r0 + lane >= A.keep)) << 16;
-            }
-            if (lane == 0) cnt[1][c * WAVES + wave] = x;
+            const uint64_t mask = __ballot(stays >> c & 1);
+            mine = lane == c ? mask : mine;
+        }
+        if (lane < HELD) words[lane * WAVES + wave] = mine;
+        __syncthreads();
+        if (tid < HELD * WAVES) {
+            const uint32_t r0 = base + tid * 64;
+            const uint64_t low = r0 >= A.keep ? 0 : A.keep - r0 >= 64 ? ~(uint64_t)0 : ((uint64_t)1 << (A.keep - r0)) - 1;
+            cnt[1][tid] = __popcll(~words[tid] & low) | __popcll(words[tid] & ~low) << 16;
         }
         __syncthreads();
         const uint32_t all = scan_counts<HELD * WAVES>(cnt[1], pre[1]);
