@@ -420,7 +420,9 @@ extern "C" fox_gpu_status fox_gpu_paged_rope_store(
 // ---------------------------------------------------------------- eviction
 
 #define EV_COPIES 2              // of a histogram: lanes that meet in one place wait for each other
-#define EV_FEW 64                // so many rows are moved by the workgroup that finds them
+// So many rows are moved by the workgroup that finds them (100 of 128 dimensions: 13 to 15 us in one
+// launch, 13.0 in two; one, where 100 could: 7.8 and 9.3; 240: 19.5 and 13.3).
+#define EV_FEW 128
 #define EV_ONES 8                // so many rows to give up are found one by one
 #define EV_DEEP 2                // rows that a thread of the mover has on the way (4: 22 us instead of 17.5, for registers)
 
@@ -693,12 +695,18 @@ __global__ __launch_bounds__(THREADS) void evict_select_k(EvictArgs A)
 
     uint32_t least = 0, want = A.keep, in;   // the bits found; rows still to take among those that share them
     const uint32_t copy = lane % EV_COPIES;
+    uint32_t newer = 0;                      // rows of the greatest key, one place for all: added up first
     for (uint32_t base = 0; base < n; base += ROWS) {
         read(base);
 #pragma unroll
         for (int c = 0; c < HELD; c++)
-            if (base + c * THREADS < n && base + c * THREADS + tid < n) atomicAdd(&high[copy][key[c] >> 20], 1u);
+            if (base + c * THREADS < n && base + c * THREADS + tid < n) {
+                if (key[c] == 0xFFFFFFFFu) newer++;
+                else atomicAdd(&high[copy][key[c] >> 20], 1u);
+            }
     }
+    newer = wave_scan(newer);
+    if (lane == 63) atomicAdd(&high[0][4095], newer);
     least = find_bin<4096, WAVES>(high, shares[0], want, in) << 20;
     bool every = in == want;                 // those are all taken
 #pragma unroll
@@ -830,12 +838,15 @@ extern "C" fox_gpu_status fox_gpu_paged_evict(fox_gpu_ctx *ctx, const fox_gpu_pa
     // at most so many rows can move
     A.room = A.C.cap - A.keep < A.keep ? A.C.cap - A.keep : A.keep;
     const size_t heads = cache->n_seqs * cache->n_head_kv;
-    // Short sequences by 512 threads of 8 rows, long ones by 1024 of 24; the few rows that a step
-    // can give up are moved in the same launch.
-    const bool few = A.room <= EV_FEW, brief = A.C.cap <= 4096;
-    const void *k = few ? brief ? (const void *)evict_select_k<true, 512, 8> : (const void *)evict_select_k<true, 1024, 24>
-                        : brief ? (const void *)evict_select_k<false, 512, 8> : (const void *)evict_select_k<false, 1024, 24>;
-    const dim3 grid((unsigned)cache->n_head_kv, (unsigned)cache->n_seqs), block(brief ? 512 : 1024);
+    // Short sequences by 512 threads of 8 rows, longer ones by 1024 of 8 or 24 (4631 rows, 1915 of them kept:
+    // 13.6 us by 8, 18.1 by 24: less code to meet); the few rows that a step can give up are moved in the same launch.
+    const bool few = A.room <= EV_FEW;
+#define FOX_SELECT(f)                                                                               \
+    (A.C.cap <= 4096 ? (const void *)evict_select_k<f, 512, 8> : A.C.cap <= 8192 ? (const void *)evict_select_k<f, 1024, 8> \
+                                                               : (const void *)evict_select_k<f, 1024, 24>)
+    const void *k = few ? FOX_SELECT(true) : FOX_SELECT(false);
+#undef FOX_SELECT
+    const dim3 grid((unsigned)cache->n_head_kv, (unsigned)cache->n_seqs), block(A.C.cap <= 4096 ? 512 : 1024);
     void *args[] = {&A};
     FOX_HIP(hipSetDevice(ctx->device));
     if (few) {
