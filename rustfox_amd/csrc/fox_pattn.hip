@@ -23,7 +23,7 @@
 // to arrive, one launch less takes four times as long: before it counts itself each must write its
 // part past its XCD's cache, and the fence for that empties it.)
 //
-// Bound by reads: 64 sequences of 8192 rows and fewer, 16 kv heads of 128 (1.64 GB), 270 us, 6.1 TB/s
+// Bound by reads: 64 sequences of 8192 rows and fewer, 16 kv heads of 128 (1.64 GB), 266 us, 6.2 TB/s
 // (a plain read reaches 6.5); one of 131071, 8 kv heads (537 MB), 86 us; matrix units are
 // busy a tenth of the time.  Short calls by their way in and out, straight code
 // that each workgroup meets cold: 4097 rows of 8 kv heads (17 MB) 15 us, 11 of them the first launch.
@@ -575,9 +575,35 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_k(const uint32_t *le
             } else {
                 *(f4v *)(A.part + (slot * A.per + j) * hd + d) = y;
             }
-            if (d == 0 && (!whole || A.scores)) *(float2 *)(A.stats + (slot * A.per + j) * 2) = float2{top, all};
+            if (d == 0 && (!whole || (A.scores && A.tiles > 1))) *(float2 *)(A.stats + (slot * A.per + j) * 2) = float2{top, all};
         }
-        if (A.whole) return;
+        if (A.whole) {
+            if (!A.scores || A.tiles > 1) return;
+            // the rows' weights, from the scores that this workgroup has stored, summed in the heads' order
+            // before they are added to what the row has
+            __shared__ float tops[HG], by[HG];
+            if (tid < heads) {
+                float top = wm[0][tid], all = 0.0f;
+#pragma unroll
+                for (int w = 1; w < PA_WAVES; w++) top = fmaxf(top, wm[w][tid]);
+#pragma unroll
+                for (int w = 0; w < PA_WAVES; w++)
+                    all += wm[w][tid] == -INFINITY ? wl[w][tid] : wl[w][tid] * __builtin_amdgcn_exp2f(wm[w][tid] - top);
+                tops[tid] = top == -INFINITY ? 0.0f : top;
+                by[tid] = all == 0.0f ? 0.0f : 1.0f / all;
+            }
+            __syncthreads();
+            float *weight = A.C.weight + ((size_t)t * A.C.n_kv + h) * A.C.cap;
+            const float *scores = A.scores + ((size_t)t * A.C.n_kv + h) * A.G * A.C.cap;
+            for (uint32_t p = tid; p < n; p += PA_THREADS) {
+                if (table[p >> A.C.shift] >= A.C.n_pages) continue;
+                float sum = 0.0f;
+                for (uint32_t j = 0; j < heads; j++)
+                    sum += __builtin_amdgcn_exp2f(scores[(size_t)j * A.C.cap + p] - tops[j]) * by[j];
+                weight[p] += sum;
+            }
+            return;
+        }
         __syncthreads();
         u += k1 - k0;
     }
@@ -806,7 +832,9 @@ extern "C" fox_gpu_status fox_gpu_paged_attention(fox_gpu_ctx *ctx, const fox_gp
     FOX_HIP(hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
     FOX_HIP(hipLaunchKernel(k, dim3(A.workers), dim3(PA_THREADS), args, lds, ctx->stream));
     const uint32_t merges = A.whole || A.workers == 1 ? 0 : (uint32_t)n_head;
-    uint32_t chunks = weigh ? (A.C.cap + PA_CHUNK - 1) / PA_CHUNK : 0;
+    // (a workgroup that has all of an item and its group adds its weights itself: 2 rows of 11, 8 kv heads,
+    // 7.8 us, by another launch 9.5)
+    uint32_t chunks = weigh && !(A.whole && A.tiles == 1) ? (A.C.cap + PA_CHUNK - 1) / PA_CHUNK : 0;
     if (merges || chunks) {
         void *after[] = {&A.bounds, (void *)&merges, &chunks, &A.C.n_kv, &A.G, &A.tiles, &A.per, &A};
         FOX_HIP(hipLaunchKernel((const void *)paged_after_k, dim3((unsigned)(merges + chunks * cache->n_head_kv), (unsigned)M),
