@@ -575,7 +575,7 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_k(const uint32_t *le
             } else {
                 *(f4v *)(A.part + (slot * A.per + j) * hd + d) = y;
             }
-            if (d == 0 && (!whole || (A.scores && A.tiles > 1))) *(float2 *)(A.stats + (slot * A.per + j) * 2) = float2{top, all};
+            if (d == 0 && (!whole || A.scores)) *(float2 *)(A.stats + (slot * A.per + j) * 2) = float2{top, all};
         }
         if (A.whole) {
             if (!A.scores || A.tiles > 1) return;
