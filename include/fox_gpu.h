@@ -512,7 +512,7 @@ typedef struct {
  * beta_fast times within orig_ctx positions keep their speed and those of less
  * than beta_slow turns are slowed; with ext = 0 the last three are not looked at.  `factors`
  * (device memory) divides each pair's speed by its own.  Computed in double and rounded
- * once. */
+ * once.  n * n_rot / 2 values past one launch (about 2^32) are refused. */
 typedef struct {
     double       base, scale, ext, beta_fast, beta_slow, orig_ctx, magnitude;
     const float *factors;
@@ -547,8 +547,12 @@ fox_gpu_status fox_gpu_paged_rope_store(
  * zeros.  Hidden rows may hold anything.  weigh != 0 (seq NULL, the cache has weight): every
  * row's softmax weights, summed over the query heads of its kv head, are
  * added to cache->weight.  The cache's values are multiplied as they are; scores, maxima, weights
- * and sums are in 32 bits.  A query's value is held to 2^-22 of it (and
- * halves' to 2^-38 of its head's largest).  A score past a float's range gives NaN.
+ * and sums are in 32 bits.  A query's value is held to 2^-22 of it (and halves' to 2^-38 of its head's
+ * largest).  A visible row's infinite or NaN key, an infinite or NaN query and a score above a
+ * float's range give NaN; scores below it have no weight, and a token that has no others gets zeros.
+ * Sums are divided last and hold up to 2^8 of a row's value: bfloat16 values beyond 2^119 over the
+ * number of rows may pass a float's range.  Weights of M * n_head * max_pages * page_size above
+ * 2^33 are refused.
  * n_head is a multiple of n_head_kv, at most 65535.  out must not overlap q. */
 fox_gpu_status fox_gpu_paged_attention(fox_gpu_ctx *ctx, const fox_gpu_paged *cache, float *out,
                                        size_t out_stride, const float *q, size_t q_stride,

@@ -504,6 +504,24 @@ def test_evict_longer_than_registers(gpu, keep, recent, values):
     assert np.array_equal(c.k.numpy(), k) and np.array_equal(c.v.numpy(), v)
 
 
+@pytest.mark.parametrize("cap", [320, 5008, 9008])
+@pytest.mark.parametrize("keep", [127, 128, 129])
+def test_evict_mostly_the_newest(gpu, keep, cap):
+    """Nearly all of the rows kept are the newest, and as many move as one launch takes, one less and one more."""
+    rng = np.random.default_rng(keep + cap)
+    for recent in (keep, keep - 1, keep - 30):
+        c = Paged(gpu, rng, rf.F16, 2, 40, 16, [2 * keep + 20, keep + 9, 2 * keep], room=cap - 2 * keep - 20)
+        for s, n in enumerate(c.length):
+            c.position[s, :, :n] = np.arange(n)
+        c.upload()
+        kept = dev(gpu, np.zeros(3, np.uint32))
+        gpu.paged_evict(c.c, c.d_length, kept, keep, recent)
+        k, v, w, p, m = pr.evict(*c.pools, c.table, c.weight, c.position, c.length, keep, recent)
+        assert np.array_equal(kept.numpy(), m)
+        assert np.array_equal(c.d_position.numpy(), p) and np.array_equal(c.d_weight.numpy(), w)
+        assert np.array_equal(c.k.numpy(), k) and np.array_equal(c.v.numpy(), v)
+
+
 def test_evict_positions_alike_or_far(gpu):
     """Positions that say nothing (all the same, more of the newest than are kept, past 2^31): still
     `keep` rows, and nothing out of place."""
