@@ -18,7 +18,8 @@
 //
 // Division.  A row's heads have ceil(length / 64) units of 64 positions, one tile for
 // each wave of a workgroup.  All units of a call, in order of row, head, position, are
-// cut into equal runs, one a workgroup, whatever the lengths, which only the device knows; a
+// cut into equal runs, one a workgroup (or each head's, where that wastes little), whatever the
+// lengths, which only the device knows; a
 // head whose units lie in several runs is merged by a second launch.  (Merged by the last workgroup
 // to arrive, one launch less takes four times as long: before it counts itself each must write its
 // part past its XCD's cache, and the fence for that empties it.)
@@ -26,7 +27,7 @@
 // Bound by reads: 64 sequences of 8192 rows and fewer, 16 kv heads of 128 (1.64 GB), 266 us, 6.2 TB/s
 // (a plain read reaches 6.5); one of 131071, 8 kv heads (537 MB), 86 us; matrix units are
 // busy a tenth of the time.  Short calls by their way in and out, straight code
-// that each workgroup meets cold: 4097 rows of 8 kv heads (17 MB) 15 us, 11 of them the first launch.
+// that each workgroup meets cold: 4097 rows of 8 kv heads (17 MB) 12.8 us, 9 of them the first launch.
 #include "fox_paged_dev.h"
 
 #include <cfloat>
@@ -85,15 +86,17 @@ __device__ __forceinline__ uint64_t over(uint64_t a, uint32_t b)
     return a >> 32 ? a / b : (uint32_t)a / b;
 }
 
-// Where the units of each row begin, counted for one of its heads (an item): up to 64
+// Where the pieces of each row begin, counted for one of its heads (an item): up to 64
 // rows by every wave for itself, lane t row t, without LDS or a barrier; more by the
-// workgroup, in LDS.
+// workgroup, in LDS.  A piece is `size` units, or what an item has left: one unit, or all of a worker's
+// where every run can end with its item, so that no worker has two ways in and out.
 struct PagedWork {
     const uint64_t *start;        // [M + 1], past 64 rows
-    uint64_t run, total;          // units of a worker; of the call
-    uint32_t items, M, before, units, length, seq;
+    uint64_t run, total;          // pieces of a worker; of the call
+    uint32_t size;
+    uint32_t items, M, before, pieces, length, seq;
 
-    // the row that holds unit u of the call
+    // the row that holds piece u of the call
     __device__ __forceinline__ uint32_t row_of(uint64_t u) const
     {
         if (M == 1) return 0;
@@ -109,12 +112,12 @@ struct PagedWork {
         }
         return __builtin_amdgcn_readfirstlane(lo);
     }
-    // a row's first unit of one item, and how many it has
+    // a row's first piece of one item, and how many it has
     __device__ __forceinline__ void row(uint32_t t, uint64_t &first, uint32_t &n) const
     {
         if (M <= 64) {
             first = (uint32_t)__builtin_amdgcn_readlane((int)before, t);
-            n = (uint32_t)__builtin_amdgcn_readlane((int)units, t);
+            n = (uint32_t)__builtin_amdgcn_readlane((int)pieces, t);
         } else {
             first = start[t];
             n = (uint32_t)(start[t + 1] - first);
@@ -139,18 +142,19 @@ __device__ __forceinline__ PagedWork divide(const PagedAttnArgs &A, uint64_t *st
     D.M = A.M;
     D.items = A.C.n_kv * A.tiles;
     D.length = D.seq = 0;
+    D.size = 1;
     if (A.M == 1) {                                                 // (by the scalar unit)
         D.seq = A.seq ? word(A.seq, 0) : 0;
         const uint32_t n = word(A.length, 0);
         D.length = D.seq < A.C.n_seqs ? min(n, A.C.cap) : 0;
-        D.units = units_of(D.length);
+        D.pieces = units_of(D.length);
         D.before = 0;
-        D.total = (uint64_t)D.units * D.items;
+        D.total = (uint64_t)D.pieces * D.items;
     } else if (A.M <= 64) {
         if (lane < A.M) D.length = row_length(A, lane, D.seq);
-        D.units = units_of(D.length);                               // (64 of at most 2^24)
-        const uint32_t x = wave_scan(D.units);
-        D.before = x - D.units;
+        D.pieces = units_of(D.length);                              // (64 of at most 2^24)
+        const uint32_t x = wave_scan(D.pieces);
+        D.before = x - D.pieces;
         D.total = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)x, (int)A.M - 1) * D.items;
     } else {
         const uint32_t each = (A.M + PA_THREADS - 1) / PA_THREADS;  // (at most 4)
@@ -179,8 +183,55 @@ __device__ __forceinline__ PagedWork divide(const PagedAttnArgs &A, uint64_t *st
         __syncthreads();
         D.total = start[A.M] * D.items;
     }
-    const uint32_t workers = D.total < (uint64_t)48 * A.workers ? A.few : A.workers;
+    // (more items than workers take twice the workers: 24 rows of 150 to 3000, 16 kv heads, 61 / 54.6 us)
+    uint32_t workers = D.total < (uint64_t)48 * A.workers && A.M * D.items <= A.few ? A.few : A.workers;
     D.run = over(D.total + workers - 1, workers);
+    // Runs that end with their items, where runs a fifth or three units longer leave workers enough for them; if
+    // not, with twice the workers: attn-8b-1 15.2 / 12.8 us, 16 rows of 150 to 3000 28.6 / 22.2,
+    // 32 of 125 to 2500 50.3 / 34.1.  (Twice the workers without that: 32 rows of 4000 82.8 / 85.4.)
+    if (A.M == 1) {
+        const uint32_t units = D.pieces, run = (uint32_t)D.run, most = workers / D.items;
+        if (run > 1 && most) {
+            const uint32_t size = (units + most - 1) / most;
+            if (size <= run + 3 * (1 + run / 16)) {
+                D.size = size;
+                D.pieces = (units + size - 1) / size;
+                D.total = D.pieces * D.items;
+                D.run = 1;
+            }
+        }
+    } else if (A.M <= 64 && D.run > 1 && A.M * D.items <= workers) {
+        const uint32_t units = D.pieces;
+        for (;; workers = A.workers) {
+            const uint32_t run = (uint32_t)over(D.total + workers - 1, workers), step = 1 + run / 16;
+            // four sizes at once, two sums a word (64 of at most 1023; workers are fewer)
+            uint32_t x[2], y[2], all = 0;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const uint32_t size = run + k * step, n = min((units + size - 1) / size, 1023u);
+                if (k & 1) y[k / 2] |= n << 16;
+                else y[k / 2] = n;
+            }
+#pragma unroll
+            for (int k = 0; k < 2; k++) x[k] = wave_scan(y[k]);
+#pragma unroll
+            for (int k = 3; k >= 0; k--) {
+                const uint32_t at = (uint32_t)__builtin_amdgcn_readlane((int)x[k / 2], (int)A.M - 1) >> k % 2 * 16 & 0xFFFFu;
+                if (at * D.items <= workers) {
+                    D.size = run + k * step;
+                    D.pieces = y[k / 2] >> k % 2 * 16 & 0xFFFFu;
+                    D.before = (x[k / 2] - y[k / 2]) >> k % 2 * 16 & 0xFFFFu;
+                    all = at;
+                }
+            }
+            if (all) {
+                D.total = all * D.items;
+                D.run = 1;
+                return D;
+            }
+            if (workers == A.workers) break;
+        }
+    }
     return D;
 }
 
@@ -367,22 +418,21 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_k(const uint32_t *le
         end = min(u + D.run, D.total);
     }
     while (u < end) {                                       // (uniform)
-        uint32_t t, item, k0 = 0, k1 = 0, units = 0;
+        uint32_t t, item, k0 = 0, k1 = 0, part = 0, parts = 1;
         if (A.whole) {
             t = blockIdx.x / items;
             item = blockIdx.x - t * items;
         } else {
             uint64_t first;
             t = D.row_of(u);
-            D.row(t, first, units);
+            D.row(t, first, parts);
             const uint64_t in_row = u - first * items;
-            item = (uint32_t)over(in_row, units);
-            k0 = (uint32_t)(in_row - (uint64_t)item * units);
-            k1 = (uint32_t)min((uint64_t)units, k0 + (end - u));
+            item = (uint32_t)over(in_row, parts);
+            part = (uint32_t)(in_row - (uint64_t)item * parts);
+            parts = (uint32_t)min((uint64_t)parts - part, end - u);
         }
         t = __builtin_amdgcn_readfirstlane(t);
         item = __builtin_amdgcn_readfirstlane(item);
-        k0 = __builtin_amdgcn_readfirstlane(k0);
         const uint32_t h = A.tiles == 1 ? item : item / A.tiles, h0 = (item - h * A.tiles) * A.per;
         const uint32_t heads = min(A.per, A.G - h0);
         uint32_t n, s;
@@ -395,7 +445,14 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_k(const uint32_t *le
             n = s < A.C.n_seqs ? min(length, A.C.cap) : 0;
             if (n == 0) s = 0;
         }
-        if (A.whole) units = k1 = units_of(n);
+        const uint32_t units = units_of(n);
+        if (A.whole) {
+            k1 = units;
+        } else {
+            k0 = part * D.size;
+            k1 = min(units, k0 + parts * D.size);
+        }
+        k0 = __builtin_amdgcn_readfirstlane(k0);
         k1 = __builtin_amdgcn_readfirstlane(k1);
         const uint32_t *table = A.C.table + (size_t)s * A.C.max_pages;
 
@@ -605,7 +662,7 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_k(const uint32_t *le
             return;
         }
         __syncthreads();
-        u += k1 - k0;
+        u += parts;
     }
 }
 
