@@ -855,10 +855,13 @@ extern "C" fox_gpu_status fox_gpu_paged_attention(fox_gpu_ctx *ctx, const fox_gp
     const size_t items = M * cache->n_head_kv * A.tiles;
     const bool four = A.per <= 4;
     // Short caches: a workgroup an item, one launch.  How short depends on the items, since one alone
-    // draws rows at 55 GB/s (0.6 us for 64 of them): whole / divided, 8 items of 300 rows 8.7 / 11 us, of
-    // 640 11.8 / 11.0, of 1000 17.0 / 11.2; 64 of 640 14.5 / 16.2, of 1000 19.4 / 14.6; 256 of
-    // 1000 24.3 / 28.0, of 2000 42.4 / 45.9.
-    A.whole = A.C.cap <= 512 + 1536 * (items < (size_t)ctx->n_cu ? items : (size_t)ctx->n_cu) / ctx->n_cu;
+    // draws rows at 55 GB/s (0.6 us for 64 of them), and many fill the compute units anyway.  Whole / divided, us, all
+    // as long as the cache (and of 1/20 of it to all): 8 items of 300 rows 8.9 / 10.3, of 600 13.1 / 10.4; 128 of 300
+    // 9.8 / 13.1, of 600 14.4 / 15.6 (13.5 / 13.0), of 1000 20.2 / 19.0 (18.8 / 14.0); 192 of 800 18.2 / 21.2
+    // (16.3 / 16.6); 256 of 2000 42.3 / 45.4 (33.8 / 29.7); 512 of 2500 100 / 104 (66 / 71),
+    // of 4000 157 / 161 (102 / 84).
+    const double full = (double)items / ctx->n_cu;
+    A.whole = A.C.cap <= (full < 1.0 ? 400.0 + 1648.0 * full * full * full : 1536.0 + 512.0 * (full < 4.0 ? full : 4.0));
     const size_t most = items * ((A.C.cap + PA_UNIT - 1) / PA_UNIT);
     const size_t fit = (size_t)2 * ctx->n_cu;
     A.workers = (uint32_t)(A.whole ? items : most < fit ? most : fit);
