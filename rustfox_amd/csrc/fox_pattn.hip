@@ -57,9 +57,9 @@ struct PagedAttnArgs {
     const uint32_t *length, *seq;
     uint32_t G, M;               // query heads of a kv head; rows
     uint32_t per, tiles;         // query heads of a head tile (the last may have fewer); head tiles of a kv head
-    // Workgroups that share the units: one a compute unit, two where a call is long. (A unit's rows arrive no
-    // faster for two, and each item has more parts: 16000 rows 23.0 / 25.2 us, 32 rows of 2000
-    // 45.9 / 49.9; more than 48 units each hide what rows' ends cost: attn-27b-64 283 / 273.)
+    // Workgroups that share the units: one a compute unit; two where a call is long or has many items. (A
+    // unit's rows arrive no faster for two, and each item has more parts; more than 48 units each
+    // hide what rows' ends cost: attn-27b-64 283 / 273.)
     uint32_t few, workers;
     bool whole;                  // no: a workgroup an item
     float score;                 // log2(e) / sqrt(hd)
@@ -865,8 +865,7 @@ extern "C" fox_gpu_status fox_gpu_paged_attention(fox_gpu_ctx *ctx, const fox_gp
     const size_t most = items * ((A.C.cap + PA_UNIT - 1) / PA_UNIT);
     const size_t fit = (size_t)2 * ctx->n_cu;
     A.workers = (uint32_t)(A.whole ? items : most < fit ? most : fit);
-    // (rows that are weighed are stored, too: attn-8b-24-weigh 70 / 64 us)
-    A.few = weigh || A.workers < (uint32_t)ctx->n_cu ? A.workers : (uint32_t)ctx->n_cu;
+    A.few = A.workers < (uint32_t)ctx->n_cu ? A.workers : (uint32_t)ctx->n_cu;
     // parts, their maxima and sums, and the scores of rows that are weighed
     const size_t parts = A.whole ? 0 : 2 * (size_t)A.workers;
     const size_t part = parts * A.per * cache->head_dim, stats = (parts + (weigh ? items : 0)) * A.per * 2;
