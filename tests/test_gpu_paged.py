@@ -278,6 +278,22 @@ def test_short_caches(gpu, cap):
         check(gpu, c, q, 2 * n_kv, weigh=True)
 
 
+@pytest.mark.parametrize("case", [
+    (1, 3, [64 * 85 * 3, 64 * 85 * 3 + 1, 64 * 85 * 4 - 1]), (1, 8, [64 * 32 * 2, 64 * 32 * 2 + 1, 3001]), (3, 8, None),
+    (20, 8, None), (32, 8, None), (32, 8, [2300] * 32), (31, 8, [0, 2600] * 15 + [1]), (50, 8, None), (60, 8, [2500] * 60),
+    (60, 10, None), (64, 4, None), (64, 4, [64 * k for k in range(64)])], ids=lambda c: "%d-%d-%s" % (c[0], c[1], c[2] and c[2][0]))
+def test_runs_that_end_with_their_heads(gpu, case):
+    """Work divided so that runs end with the heads or not, for fewer heads than compute units, fewer than
+    twice as many, and more."""
+    n, n_kv, lengths = case
+    rng = np.random.default_rng(n + n_kv)
+    for these in [[x] for x in lengths] if n == 1 else [lengths or [int(x) for x in rng.integers(0, 2700, n)]]:
+        c = Paged(gpu, rng, rf.F16, n_kv, 8, 64, these, room=max(0, 2700 - max(these)))
+        q = rng.standard_normal((n, n_kv * 8)).astype(np.float32)
+        got = check(gpu, c, q, n_kv, weigh=True)
+        assert np.array_equal(got, check(gpu, c, q, n_kv, seq=np.arange(n)))
+
+
 def test_the_most_heads(gpu):
     """65535 heads of one kv head, and 4096 kv heads: the largest grids and tiles."""
     rng = np.random.default_rng(31)
