@@ -859,9 +859,12 @@ extern "C" fox_gpu_status fox_gpu_paged_attention(fox_gpu_ctx *ctx, const fox_gp
     // as long as the cache (and of 1/20 of it to all): 8 items of 300 rows 8.9 / 10.3, of 600 13.1 / 10.4; 128 of 300
     // 9.8 / 13.1, of 600 14.4 / 15.6 (13.5 / 13.0), of 1000 20.2 / 19.0 (18.8 / 14.0); 192 of 800 18.2 / 21.2
     // (16.3 / 16.6); 256 of 2000 42.3 / 45.4 (33.8 / 29.7); 512 of 2500 100 / 104 (66 / 71),
-    // of 4000 157 / 161 (102 / 84).
+    // of 4000 157 / 161 (102 / 84).  Tokens that are sure to share rows are as long as each other, and in the items'
+    // order a kv head's rows are read by few XCDs' caches: 512 tokens of one sequence at 2048 268 / 314, at 9000
+    // 1208 / 2050, 48 at 9000 160 / 221 (300 of 2 kv heads 234 / 214).
     const double full = (double)items / ctx->n_cu;
-    A.whole = A.C.cap <= (full < 1.0 ? 400.0 + 1648.0 * full * full * full : 1536.0 + 512.0 * (full < 4.0 ? full : 4.0));
+    A.whole = A.C.cap <= (full < 1.0 ? 400.0 + 1648.0 * full * full * full : 1536.0 + 512.0 * (full < 4.0 ? full : 4.0)) ||
+              (seq && M > cache->n_seqs && full >= 1.0);
     const size_t most = items * ((A.C.cap + PA_UNIT - 1) / PA_UNIT);
     const size_t fit = (size_t)2 * ctx->n_cu;
     A.workers = (uint32_t)(A.whole ? items : most < fit ? most : fit);

@@ -294,6 +294,19 @@ def test_runs_that_end_with_their_heads(gpu, case):
         assert np.array_equal(got, check(gpu, c, q, n_kv, seq=np.arange(n)))
 
 
+@pytest.mark.parametrize("n_head,n_kv,hd", [(8, 8, 40), (12, 4, 64), (20, 2, 16)])
+def test_a_prompt_on_a_long_cache(gpu, n_head, n_kv, hd):
+    """More tokens than sequences, on both sides of as many heads as compute units."""
+    rng = np.random.default_rng(n_head)
+    c = Paged(gpu, rng, rf.BF16, n_kv, hd, 64, [4200, 2300])
+    for M in (9, 130):
+        seq = rng.integers(0, 3, M)                          # (sequence 2 is none)
+        length = np.where(seq == 0, 4200 - M, 2300 - M) + np.arange(M)
+        length[3] = 0
+        q = rng.standard_normal((M, n_head * hd)).astype(np.float32)
+        check(gpu, c, q, n_head, length=length, seq=seq)
+
+
 def test_the_most_heads(gpu):
     """65535 heads of one kv head, and 4096 kv heads: the largest grids and tiles."""
     rng = np.random.default_rng(31)
