@@ -212,6 +212,18 @@ struct PagedDev {
 };
 fox_gpu_status fox_paged_check(const char *what, const fox_gpu_paged *cache, bool track, PagedDev *out);
 
+// How attention over a paged cache is launched (fox_pattn.hip): a workgroup an item (a head tile of a kv head of
+// a token), or the items' units divided among workers, or, `either`, whichever the lengths and sequences on the device
+// say; fox_paged_plan_whole says the same of arrays on the host.
+struct PagedPlan {
+    bool whole, either;
+    uint32_t tiles, per;          // head tiles of a kv head; query heads of a tile
+    uint32_t workers, few;
+    size_t items;
+};
+PagedPlan fox_paged_plan(size_t n_head, size_t n_head_kv, size_t M, size_t cap, bool seq, int n_cu);
+bool fox_paged_plan_whole(const PagedPlan &p, size_t M, size_t cap, size_t n_seqs, const uint32_t *length, const uint32_t *seq);
+
 // How attention over a quantised cache is launched (fox_kvattn.hip): a kernel's
 // rows and positions as they are divided, and which of the two kernels run.
 struct KvqParts {

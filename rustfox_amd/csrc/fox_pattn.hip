@@ -62,6 +62,7 @@ struct PagedAttnArgs {
     // hide what rows' ends cost: attn-27b-64 283 / 273.)
     uint32_t few, workers;
     bool whole;                  // no: a workgroup an item
+    bool either;                 // the device decides that: workgroups for both are launched
     float score;                 // log2(e) / sqrt(hd)
     // Parts: sums [part][per][hd], maxima and weights' sums [part][per][2].  A worker has two at most:
     // of the item that its run begins in (2 worker) and of the one that it ends in (2 worker + 1).
@@ -95,6 +96,7 @@ struct PagedWork {
     uint64_t run, total;          // pieces of a worker; of the call
     uint32_t size;
     uint32_t items, M, before, pieces, length, seq;
+    bool whole;                   // no division: a workgroup an item
 
     // the row that holds piece u of the call
     __device__ __forceinline__ uint32_t row_of(uint64_t u) const
@@ -133,6 +135,64 @@ __device__ __forceinline__ uint32_t row_length(const PagedAttnArgs &A, uint32_t 
     return s < A.C.n_seqs ? min(n, A.C.cap) : 0;
 }
 
+// Whether a call whose tokens share rows (`alike` of the M are of the sequence of the one before, with rows) takes
+// a workgroup an item all the same.  In the items' order a kv head's rows are read by few XCDs' caches, by
+// neighbouring tokens at once, which the runs of a division do not; but an item is no faster for what
+// else is done, so the longest may take twice an equal share of all units, no more.  Whole / divided, us, 32 heads
+// over 8 kv heads of 128: 512 tokens of one sequence at 9000 rows 1222 / 2080, at 2048 276 / 314, 48 at 9000 164 / 222
+// (the longest 1.3 shares), 8 of each of 5 sequences of 4000 79 / 103 (1.6); 1000 tokens from the first on 211 / 725;
+// 300 over 2 kv heads at 9000 239 / 214.  30 sequences of 1000, one of 100000 and 16 tokens of a
+// prompt 1055 / 106 (43 shares).
+__host__ __device__ inline bool paged_whole(uint32_t M, uint32_t alike, uint64_t units, uint32_t longest, uint32_t workers)
+{
+    return 2 * alike >= M && (uint64_t)longest * workers <= 2 * units;
+}
+
+// That of more than 64 rows, by the workgroup
+__device__ __forceinline__ bool whole_rows(const PagedAttnArgs &A, uint32_t items)
+{
+    constexpr int EACH = FOX_GPU_BATCH_TOKENS / PA_THREADS;
+    static_assert(EACH * PA_THREADS == FOX_GPU_BATCH_TOKENS, "a thread has EACH rows");
+    __shared__ uint32_t units[PA_WAVES], longest[PA_WAVES], alike[PA_WAVES];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    uint32_t n[EACH], s[EACH], before[EACH];
+#pragma unroll
+    for (int i = 0; i < EACH; i++) {                         // (asked for together)
+        const uint32_t t = min(tid + i * PA_THREADS, A.M - 1);
+        n[i] = A.length[t];
+        s[i] = A.seq[t];
+        before[i] = A.seq[t ? t - 1 : 0];
+    }
+    uint32_t all = 0, most = 0, same = 0;
+#pragma unroll
+    for (int i = 0; i < EACH; i++) {
+        const uint32_t t = tid + i * PA_THREADS;
+        const uint32_t u = t < A.M && s[i] < A.C.n_seqs ? units_of(min(n[i], A.C.cap)) : 0;
+        all += (u + 1) / 2;                                  // (256 of at most 2^23)
+        most = max(most, u);
+        same += u && t && s[i] == before[i];
+    }
+    all = wave_scan(all);
+    most = wave_max(most);
+    same = wave_scan(same);
+    if (lane == 63) {
+        units[w] = all;
+        longest[w] = most;
+        alike[w] = same;
+    }
+    __syncthreads();
+    uint64_t total = 0;
+    most = same = 0;
+    for (int i = 0; i < PA_WAVES; i++) {
+        total += (uint64_t)units[i] * 2 * items;
+        most = max(most, longest[i]);
+        same += alike[i];
+    }
+    return paged_whole(A.M, same, total, most, A.workers);
+}
+
+// SEQ: the tokens' sequences may be given
+template <bool SEQ>
 __device__ __forceinline__ PagedWork divide(const PagedAttnArgs &A, uint64_t *start)
 {
     __shared__ uint64_t sums[PA_WAVES];
@@ -143,6 +203,7 @@ __device__ __forceinline__ PagedWork divide(const PagedAttnArgs &A, uint64_t *st
     D.items = A.C.n_kv * A.tiles;
     D.length = D.seq = 0;
     D.size = 1;
+    D.whole = false;
     if (A.M == 1) {                                                 // (by the scalar unit)
         D.seq = A.seq ? word(A.seq, 0) : 0;
         const uint32_t n = word(A.length, 0);
@@ -156,7 +217,17 @@ __device__ __forceinline__ PagedWork divide(const PagedAttnArgs &A, uint64_t *st
         const uint32_t x = wave_scan(D.pieces);
         D.before = x - D.pieces;
         D.total = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)x, (int)A.M - 1) * D.items;
+        if (SEQ && A.either) {
+            const uint32_t ahead = __shfl_up(D.seq, 1);
+            const uint32_t alike = __popcll(__ballot(lane > 0 && D.pieces && D.seq == ahead));
+            D.whole = paged_whole(A.M, alike, D.total, wave_max(D.pieces), A.workers);
+            if (D.whole) return D;
+        }
     } else {
+        if (SEQ && A.either) {
+            D.whole = whole_rows(A, D.items);
+            if (D.whole) return D;
+        }
         const uint32_t each = (A.M + PA_THREADS - 1) / PA_THREADS;  // (at most 4)
         uint64_t mine = 0;
         uint32_t s;
@@ -403,8 +474,13 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_k(const uint32_t *le
     const uint32_t hd = FULL ? W : A.C.hd, width = A.C.n_kv * A.G * hd, items = A.C.n_kv * A.tiles;
     PagedWork D;
     uint64_t u = 0, end = 1;
+    bool whole_item = A.whole;                              // (a workgroup's item is its number)
     if (!A.whole) {
-        D = divide(A, (uint64_t *)lds);
+        D = divide<!ONCE>(A, (uint64_t *)lds);
+        if (!ONCE) whole_item = D.whole;
+    }
+    if (!ONCE && whole_item && blockIdx.x >= A.M * items) return;
+    if (!whole_item) {
         for (uint32_t t = blockIdx.x; t < A.M; t += gridDim.x) {
             uint64_t first;
             uint32_t n;
@@ -419,7 +495,7 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_k(const uint32_t *le
     }
     while (u < end) {                                       // (uniform)
         uint32_t t, item, k0 = 0, k1 = 0, part = 0, parts = 1;
-        if (A.whole) {
+        if (whole_item) {
             t = blockIdx.x / items;
             item = blockIdx.x - t * items;
         } else {
@@ -436,17 +512,17 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_k(const uint32_t *le
         const uint32_t h = A.tiles == 1 ? item : item / A.tiles, h0 = (item - h * A.tiles) * A.per;
         const uint32_t heads = min(A.per, A.G - h0);
         uint32_t n, s;
-        if (!A.whole && A.M <= 64) {
+        if (!A.whole && A.M <= 64) {                        // (divided or not)
             n = (uint32_t)__builtin_amdgcn_readlane((int)D.length, t);
             s = (uint32_t)__builtin_amdgcn_readlane((int)D.seq, t);
         } else {
             s = A.seq ? word(A.seq, t) : t;
             const uint32_t length = word(A.length, t);
             n = s < A.C.n_seqs ? min(length, A.C.cap) : 0;
-            if (n == 0) s = 0;
         }
+        if (n == 0) s = 0;                                  // (a sequence that is none has no table)
         const uint32_t units = units_of(n);
-        if (A.whole) {
+        if (whole_item) {
             k1 = units;
         } else {
             k0 = part * D.size;
@@ -662,7 +738,7 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_k(const uint32_t *le
             return;
         }
         __syncthreads();
-        u += parts;
+        u += parts;                                         // (one, of a whole item)
     }
 }
 
@@ -795,7 +871,7 @@ __device__ __forceinline__ void weigh_chunk(const PagedAttnArgs &A, uint32_t t, 
 
 // What follows the attention, in one launch: merges of the row's heads, and its kv heads' chunks weighed.
 __global__ __launch_bounds__(PM_THREADS) void paged_after_k(const uint32_t *bounds0, uint32_t merges, uint32_t chunks, uint32_t n_kv0,
-                                                            uint32_t G0, uint32_t tiles0, uint32_t per0, PagedAttnArgs A)
+                                                            uint32_t G0, uint32_t tiles0, uint32_t per0, uint32_t group, PagedAttnArgs A)
 {
     A.bounds = (uint32_t *)bounds0;                          // (in registers from the start, as above)
     A.C.n_kv = n_kv0;
@@ -805,7 +881,18 @@ __global__ __launch_bounds__(PM_THREADS) void paged_after_k(const uint32_t *boun
     __shared__ __attribute__((aligned(16))) float sums[16 * 128], tops[16], alls[16];
     const uint32_t t = blockIdx.y;
     if (blockIdx.x < merges) {
-        merge_head(A, t, blockIdx.x, sums, tops, alls);
+        if (group == 1) return merge_head(A, t, blockIdx.x, sums, tops, alls);
+        // those of the group that have parts, found by a lane each
+        const uint32_t lane = threadIdx.x & 63, mine = blockIdx.x * group + lane;
+        uint2 b = {0, 0};
+        if (lane < group && mine < n_kv0 * G0) {
+            const uint32_t tile = mine / G0 * tiles0 + mine % G0 / per0;
+            b = *(const uint2 *)(bounds0 + 2 * ((size_t)t * n_kv0 * tiles0 + tile));
+        }
+        for (uint64_t left = __ballot(b.x != b.y); left; left &= left - 1) {
+            merge_head(A, t, blockIdx.x * group + (uint32_t)__ffsll((unsigned long long)left) - 1, sums, tops, alls);
+            __syncthreads();
+        }
     } else {
         const uint32_t x = blockIdx.x - merges;
         weigh_chunk(A, t, x / chunks, x % chunks, tops, alls);
@@ -819,6 +906,42 @@ static const void *attn_kernel(size_t hd)
     return hd <= 64 ? FOX_ATTN(64) : hd <= 128 ? FOX_ATTN(128)
          : hd <= 192 ? (const void *)paged_attn_k<BF, 192, false, HG, ONCE> : FOX_ATTN(256);
 #undef FOX_ATTN
+}
+
+PagedPlan fox_paged_plan(size_t n_head, size_t n_head_kv, size_t M, size_t cap, bool seq, int n_cu)
+{
+    PagedPlan p = {};
+    const size_t G = n_head / n_head_kv;
+    p.tiles = (uint32_t)((G + 15) / 16);
+    p.per = (uint32_t)((G + p.tiles - 1) / p.tiles);
+    p.items = M * n_head_kv * p.tiles;
+    // Short caches: a workgroup an item, one launch.  How short depends on the items, since one alone
+    // draws rows at 55 GB/s (0.6 us for 64 of them), and many fill the compute units anyway.  Whole / divided, us, all
+    // as long as the cache (and of 1/20 of it to all): 8 items of 300 rows 8.9 / 10.3, of 600 13.1 / 10.4; 128 of 300
+    // 9.8 / 13.1, of 600 14.4 / 15.6 (13.5 / 13.0), of 1000 20.2 / 19.0 (18.8 / 14.0); 192 of 800 18.2 / 21.2
+    // (16.3 / 16.6); 256 of 2000 42.3 / 45.4 (33.8 / 29.7); 512 of 2500 100 / 104 (66 / 71),
+    // of 4000 157 / 161 (102 / 84).  Calls of many items whose tokens may share rows are decided on the device.
+    const double full = (double)p.items / n_cu;
+    p.whole = cap <= (full < 1.0 ? 400.0 + 1648.0 * full * full * full : 1536.0 + 512.0 * (full < 4.0 ? full : 4.0));
+    p.either = !p.whole && seq && M > 1 && full >= 1.0;
+    const size_t most = p.items * ((cap + PA_UNIT - 1) / PA_UNIT), fit = (size_t)2 * n_cu;
+    p.workers = (uint32_t)(p.whole ? p.items : most < fit ? most : fit);
+    p.few = p.workers < (uint32_t)n_cu ? p.workers : (uint32_t)n_cu;
+    return p;
+}
+
+bool fox_paged_plan_whole(const PagedPlan &p, size_t M, size_t cap, size_t n_seqs, const uint32_t *length, const uint32_t *seq)
+{
+    if (!p.either) return p.whole;
+    uint64_t units = 0;
+    uint32_t longest = 0, alike = 0;
+    for (size_t t = 0; t < M; t++) {
+        const uint32_t n = seq[t] < n_seqs ? ((length[t] < cap ? length[t] : (uint32_t)cap) + PA_UNIT - 1) / PA_UNIT : 0;
+        units += n;
+        if (n > longest) longest = n;
+        if (n && t && seq[t] == seq[t - 1]) alike++;
+    }
+    return paged_whole((uint32_t)M, alike, units * (p.items / M), longest, p.workers);
 }
 
 extern "C" fox_gpu_status fox_gpu_paged_attention(fox_gpu_ctx *ctx, const fox_gpu_paged *cache, float *out,
@@ -847,28 +970,18 @@ extern "C" fox_gpu_status fox_gpu_paged_attention(fox_gpu_ctx *ctx, const fox_gp
     A.out_stride = out_stride;
     A.length = length;
     A.seq = seq;
+    const PagedPlan p = fox_paged_plan(n_head, cache->n_head_kv, M, A.C.cap, seq != nullptr, ctx->n_cu);
     A.G = (uint32_t)(n_head / cache->n_head_kv);
     A.M = (uint32_t)M;
-    A.tiles = (A.G + 15) / 16;
-    A.per = (A.G + A.tiles - 1) / A.tiles;
+    A.tiles = p.tiles;
+    A.per = p.per;
     A.score = (float)(1.4426950408889634 / std::sqrt((double)cache->head_dim));
-    const size_t items = M * cache->n_head_kv * A.tiles;
+    A.whole = p.whole;
+    A.either = p.either;
+    A.workers = p.workers;
+    A.few = p.few;
+    const size_t items = p.items;
     const bool four = A.per <= 4;
-    // Short caches: a workgroup an item, one launch.  How short depends on the items, since one alone
-    // draws rows at 55 GB/s (0.6 us for 64 of them), and many fill the compute units anyway.  Whole / divided, us, all
-    // as long as the cache (and of 1/20 of it to all): 8 items of 300 rows 8.9 / 10.3, of 600 13.1 / 10.4; 128 of 300
-    // 9.8 / 13.1, of 600 14.4 / 15.6 (13.5 / 13.0), of 1000 20.2 / 19.0 (18.8 / 14.0); 192 of 800 18.2 / 21.2
-    // (16.3 / 16.6); 256 of 2000 42.3 / 45.4 (33.8 / 29.7); 512 of 2500 100 / 104 (66 / 71),
-    // of 4000 157 / 161 (102 / 84).  Tokens that are sure to share rows are as long as each other, and in the items'
-    // order a kv head's rows are read by few XCDs' caches: 512 tokens of one sequence at 2048 268 / 314, at 9000
-    // 1208 / 2050, 48 at 9000 160 / 221 (300 of 2 kv heads 234 / 214).
-    const double full = (double)items / ctx->n_cu;
-    A.whole = A.C.cap <= (full < 1.0 ? 400.0 + 1648.0 * full * full * full : 1536.0 + 512.0 * (full < 4.0 ? full : 4.0)) ||
-              (seq && M > cache->n_seqs && full >= 1.0);
-    const size_t most = items * ((A.C.cap + PA_UNIT - 1) / PA_UNIT);
-    const size_t fit = (size_t)2 * ctx->n_cu;
-    A.workers = (uint32_t)(A.whole ? items : most < fit ? most : fit);
-    A.few = A.workers < (uint32_t)ctx->n_cu ? A.workers : (uint32_t)ctx->n_cu;
     // parts, their maxima and sums, and the scores of rows that are weighed
     const size_t parts = A.whole ? 0 : 2 * (size_t)A.workers;
     const size_t part = parts * A.per * cache->head_dim, stats = (parts + (weigh ? items : 0)) * A.per * 2;
@@ -892,13 +1005,17 @@ extern "C" fox_gpu_status fox_gpu_paged_attention(fox_gpu_ctx *ctx, const fox_gp
     const size_t lds = starts + (size_t)(four ? 4 : 1) * PA_WAVES * A.per * cache->head_dim * sizeof(float);
     void *args[] = {&A.length, &A.seq, &A.M, &A.C.n_seqs, &A.C.cap, &A};
     FOX_HIP(hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-    FOX_HIP(hipLaunchKernel(k, dim3(A.workers), dim3(PA_THREADS), args, lds, ctx->stream));
-    const uint32_t merges = A.whole || A.workers == 1 ? 0 : (uint32_t)n_head;
+    FOX_HIP(hipLaunchKernel(k, dim3((unsigned)(A.either && items > A.workers ? items : A.workers)), dim3(PA_THREADS), args, lds,
+                            ctx->stream));
+    // (query heads of a workgroup: many that may have nothing to merge are looked through by fewer; 1000 tokens of 32
+    // heads 23 us one by one, 4.7 by eight)
+    const uint32_t group = A.either && M > 64 ? 8 : 1;
+    const uint32_t merges = A.whole || A.workers == 1 ? 0 : ((uint32_t)n_head + group - 1) / group;
     // (a workgroup that has all of an item and its group adds its weights itself: 2 rows of 11, 8 kv heads,
     // 7.8 us, by another launch 9.5)
     uint32_t chunks = weigh && !(A.whole && A.tiles == 1) ? (A.C.cap + PA_CHUNK - 1) / PA_CHUNK : 0;
     if (merges || chunks) {
-        void *after[] = {&A.bounds, (void *)&merges, &chunks, &A.C.n_kv, &A.G, &A.tiles, &A.per, &A};
+        void *after[] = {&A.bounds, (void *)&merges, &chunks, &A.C.n_kv, &A.G, &A.tiles, &A.per, (void *)&group, &A};
         FOX_HIP(hipLaunchKernel((const void *)paged_after_k, dim3((unsigned)(merges + chunks * cache->n_head_kv), (unsigned)M),
                                 dim3(PM_THREADS), after, 0, ctx->stream));
     }

@@ -146,3 +146,14 @@ extern "C" void fox_gpu_kvq_plan_probe(size_t hd, size_t n_head, size_t n_head_k
                           (int64_t)p.many_blocks, p.many_parts.splits};
     for (int i = 0; i < 8; i++) out[i] = v[i];
 }
+
+// whether a workgroup takes an item, its workers, and the items, of a paged attention; seq may be null
+extern "C" void fox_gpu_paged_plan_probe(size_t n_head, size_t n_head_kv, size_t M, size_t cap, size_t n_seqs,
+                                         const uint32_t *length, const uint32_t *seq, int n_cu, int64_t *out)
+{
+    const PagedPlan p = fox_paged_plan(n_head, n_head_kv, M, cap, seq != nullptr, n_cu);
+    out[0] = fox_paged_plan_whole(p, M, cap, n_seqs, length, seq);
+    out[1] = p.either;
+    out[2] = p.workers;
+    out[3] = (int64_t)p.items;
+}
