@@ -548,8 +548,9 @@ fox_gpu_status fox_gpu_paged_rope_store(
  * row's softmax weights, summed over the query heads of its kv head, are
  * added to cache->weight.  The cache's values are multiplied as they are; scores, maxima, weights
  * and sums are in 32 bits.  A query's value is held to 2^-22 of it (and halves' to 2^-38 of its head's
- * largest).  A visible row's infinite or NaN key, an infinite or NaN query and a score above a
- * float's range give NaN; scores below it have no weight, and a token that has no others gets zeros.
+ * largest).  A visible row's NaN key, an infinite or NaN query and a score above a float's range
+ * give NaN; scores below it have no weight, and a token that has no others gets zeros.  An
+ * infinite key gives NaN, but where its score is negative infinity it may have no weight instead.
  * Sums are divided last and hold up to 2^8 of a row's value: bfloat16 values beyond 2^119 over the
  * number of rows may pass a float's range.  Weights of M * n_head * max_pages * page_size above
  * 2^33 are refused.
