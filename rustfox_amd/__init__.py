@@ -196,6 +196,11 @@ class PagedCache:
                        max_pages, weight.ptr if weight else None, position.ptr if position else None)
 
 
+def _paged(cache) -> Paged:
+    """The struct of a PagedCache, or one that a caller has filled."""
+    return cache.c if isinstance(cache, PagedCache) else cache
+
+
 class DeviceArray:
     """A device allocation with a numpy dtype and shape (no compute)."""
 
@@ -507,7 +512,8 @@ class Gpu:
                                               q_stride or w, kv_type, cache.ptr, n_head, n_head_kv,
                                               head_dim, M, pos.ptr, n_ctx))
 
-    # -- paged caches (many sequences; strides default to the row's width)
+    # -- paged caches (many sequences; strides default to the row's width; a cache is a PagedCache, or a
+    # Paged struct whose arrays the caller keeps)
     def rope_tables(self, cos_t: DeviceArray, sin_t: DeviceArray, n, n_rot, p0=0, base=10000.0, scale=1.0,
                     ext=0.0, beta_fast=32.0, beta_slow=1.0, orig_ctx=0.0, magnitude=1.0,
                     factors: DeviceArray = None):
@@ -526,7 +532,7 @@ class Gpu:
         of any sequences into their pages."""
         nq, nk = n_head * cache.head_dim, cache.n_head_kv * cache.head_dim
         _check(self.lib.fox_gpu_paged_rope_store(
-            self.ctx, C.byref(cache.c), q.ptr, q_stride or nq, q_out.ptr, q_out_stride or nq, n_head, k.ptr,
+            self.ctx, C.byref(_paged(cache)), q.ptr, q_stride or nq, q_out.ptr, q_out_stride or nq, n_head, k.ptr,
             k_stride or nk, v.ptr, v_stride or nk, M, q_norm.ptr if q_norm else None,
             k_norm.ptr if k_norm else None, eps, pairs, n_rot, cos_t.ptr, sin_t.ptr, n_table, pos.ptr,
             seq.ptr if seq else None, row.ptr if row else None))
@@ -536,13 +542,13 @@ class Gpu:
                         q_stride=None):
         """Attention of M tokens over the first length[i] rows of their sequences."""
         w = n_head * cache.head_dim
-        _check(self.lib.fox_gpu_paged_attention(self.ctx, C.byref(cache.c), out.ptr, out_stride or w, q.ptr,
+        _check(self.lib.fox_gpu_paged_attention(self.ctx, C.byref(_paged(cache)), out.ptr, out_stride or w, q.ptr,
                                                 q_stride or w, n_head, M, length.ptr,
                                                 seq.ptr if seq else None, int(weigh)))
 
     def paged_evict(self, cache: PagedCache, length: DeviceArray, kept: DeviceArray, keep, recent=0):
         """Every sequence of more than `keep` rows cut back to those, the least weighed given up."""
-        _check(self.lib.fox_gpu_paged_evict(self.ctx, C.byref(cache.c), length.ptr, kept.ptr, keep, recent))
+        _check(self.lib.fox_gpu_paged_evict(self.ctx, C.byref(_paged(cache)), length.ptr, kept.ptr, keep, recent))
 
     def event(self):
         e = C.c_void_p()
