@@ -527,7 +527,7 @@ fox_gpu_status fox_gpu_rope_tables(fox_gpu_ctx *ctx, float *cos_t, float *sin_t,
  * at position pos[i] (a row of the tables, n_table rows of n_rot/2) and
  * becomes row row[i] of the sequence (row NULL: pos[i]; after an eviction
  * the two differ).  As fox_gpu_norm_rope_store, in double, rounded to float once: queries
- * to q_out (which may be q, with its stride), keys and values then to the cache's type, to the
+ * to q_out (which may be q, with its stride, and else overlaps no row of q, k or v), keys and values then to the cache's type, to the
  * nearest, ties to even (halves end at 65504, also where a value is infinite; a NaN stays one).
  * Where the cache has weight and position, the row's become 0 and pos[i].  A token whose sequence is not
  * below n_seqs or whose position is not below n_table is neither turned nor stored; one whose row
@@ -554,7 +554,7 @@ fox_gpu_status fox_gpu_paged_rope_store(
  * Sums are divided last and hold up to 2^8 of a row's value: bfloat16 values beyond 2^119 over the
  * number of rows may pass a float's range.  Weights of M * n_head * max_pages * page_size above
  * 2^33 are refused.
- * n_head is a multiple of n_head_kv, at most 65535.  out must not overlap q. */
+ * n_head is a multiple of n_head_kv, at most 65535.  out's rows must not overlap q's. */
 fox_gpu_status fox_gpu_paged_attention(fox_gpu_ctx *ctx, const fox_gpu_paged *cache, float *out,
                                        size_t out_stride, const float *q, size_t q_stride,
                                        size_t n_head, size_t M, const uint32_t *length,

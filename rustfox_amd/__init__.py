@@ -62,6 +62,7 @@ def probe_lib() -> C.CDLL:
         L.fox_gpu_kvq_plan_probe.restype = None
         L.fox_gpu_paged_plan_probe.argtypes = [sz, sz, sz, sz, sz, vp, vp, C.c_int, vp]
         L.fox_gpu_paged_plan_probe.restype = None
+        L.fox_gpu_rows_overlap_probe.argtypes = [sz] * 7
         _probe = L
     return _probe
 

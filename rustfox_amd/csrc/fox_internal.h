@@ -210,6 +210,8 @@ struct PagedDev {
     uint32_t n_pages, n_seqs, max_pages, n_kv, hd, shift;   // page_size = 1 << shift
     uint32_t cap;                                           // rows of a sequence
 };
+// whether a row of a and one of b, M rows of each at their strides (no less than the widths), have a float in common
+bool fox_rows_overlap(const float *a, size_t a_stride, size_t a_width, const float *b, size_t b_stride, size_t b_width, size_t M);
 fox_gpu_status fox_paged_check(const char *what, const fox_gpu_paged *cache, bool track, PagedDev *out);
 
 // How attention over a paged cache is launched (fox_pattn.hip): a workgroup an item (a head tile of a kv head of

@@ -55,6 +55,22 @@ fox_gpu_status fox_paged_check(const char *what, const fox_gpu_paged *c, bool tr
     return FOX_GPU_OK;
 }
 
+bool fox_rows_overlap(const float *a, size_t a_stride, size_t a_width, const float *b, size_t b_stride, size_t b_width, size_t M)
+{
+    const uintptr_t a0 = (uintptr_t)a, b0 = (uintptr_t)b;
+    const size_t as = (M > 1 ? a_stride : a_width) * sizeof(float), bs = (M > 1 ? b_stride : b_width) * sizeof(float);
+    const size_t aw = a_width * sizeof(float), bw = b_width * sizeof(float);
+    if (a0 >= b0 + (M - 1) * bs + bw || b0 >= a0 + (M - 1) * as + aw) return false;
+    // (rows may lie between each other's: a row of a meets the last of b's that begins before it ends, or none)
+    for (size_t i = 0; i < M; i++) {
+        const uintptr_t lo = a0 + i * as, hi = lo + aw;
+        if (hi <= b0) continue;
+        const size_t j = (hi - 1 - b0) / bs < M - 1 ? (hi - 1 - b0) / bs : M - 1;
+        if (b0 + j * bs + bw > lo) return true;
+    }
+    return false;
+}
+
 // ------------------------------------------------------------------ tables
 
 #define RT_ROWS 4                // rows of a thread
@@ -376,6 +392,11 @@ extern "C" fox_gpu_status fox_gpu_paged_rope_store(
         return fox_fail(FOX_GPU_ERR_ARG, "paged_rope_store: a stride below the row's width");
     if (!seq && M > cache->n_seqs)
         return fox_fail(FOX_GPU_ERR_ARG, "paged_rope_store: %zu tokens for %zu sequences", M, cache->n_seqs);
+    if ((q_out != q || (M > 1 && q_out_stride != q_stride)) && fox_rows_overlap(q_out, q_out_stride, nq, q, q_stride, nq, M))
+        return fox_fail(FOX_GPU_ERR_ARG, "paged_rope_store: q_out overlaps q and is not q with its stride");
+    if (fox_rows_overlap(q_out, q_out_stride, nq, k, k_stride, nkv, M) ||
+        fox_rows_overlap(q_out, q_out_stride, nq, v, v_stride, nkv, M))
+        return fox_fail(FOX_GPU_ERR_ARG, "paged_rope_store: q_out overlaps k or v");
     A.q = q;
     A.k = k;
     A.v = v;

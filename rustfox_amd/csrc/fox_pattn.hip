@@ -964,6 +964,8 @@ extern "C" fox_gpu_status fox_gpu_paged_attention(fox_gpu_ctx *ctx, const fox_gp
     if (weigh && seq)
         return fox_fail(FOX_GPU_ERR_ARG, "paged_attention: weights are added to for a token of each sequence, "
                         "without seq");
+    if (fox_rows_overlap(out, out_stride, width, q, q_stride, width, M))
+        return fox_fail(FOX_GPU_ERR_ARG, "paged_attention: out overlaps q");
     A.q = q;
     A.out = out;
     A.q_stride = q_stride;

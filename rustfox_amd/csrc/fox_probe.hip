@@ -157,3 +157,9 @@ extern "C" void fox_gpu_paged_plan_probe(size_t n_head, size_t n_head_kv, size_t
     out[2] = p.workers;
     out[3] = (int64_t)p.items;
 }
+
+extern "C" int fox_gpu_rows_overlap_probe(size_t a, size_t a_stride, size_t a_width, size_t b, size_t b_stride, size_t b_width,
+                                          size_t M)
+{
+    return fox_rows_overlap((const float *)a, a_stride, a_width, (const float *)b, b_stride, b_width, M);
+}
