@@ -512,7 +512,7 @@ typedef struct {
  * beta_fast times within orig_ctx positions keep their speed and those of less
  * than beta_slow turns are slowed; with ext = 0 the last three are not looked at.  `factors`
  * (device memory) divides each pair's speed by its own.  Computed in double and rounded
- * once.  n * n_rot / 2 values past one launch (about 2^32) are refused. */
+ * once.  n * n_rot / 2 values past one launch (about 2^36) are refused. */
 typedef struct {
     double       base, scale, ext, beta_fast, beta_slow, orig_ctx, magnitude;
     const float *factors;
@@ -546,7 +546,8 @@ fox_gpu_status fox_gpu_paged_rope_store(
  * a token that sees no row (length 0, no page, a sequence not below n_seqs) gets
  * zeros.  Hidden rows may hold anything.  weigh != 0 (seq NULL, the cache has weight): every
  * row's softmax weights, summed over the query heads of its kv head, are
- * added to cache->weight.  The cache's values are multiplied as they are; scores, maxima, weights
+ * added to cache->weight (by way of a workspace of M * n_head * max_pages * page_size floats, whatever the
+ * lengths).  The cache's values are multiplied as they are; scores, maxima, weights
  * and sums are in 32 bits.  A query's value is held to 2^-22 of it (and halves' to 2^-38 of its head's
  * largest).  A visible row's NaN key, an infinite or NaN query and a score above a float's range
  * give NaN; scores below it have no weight, and a token that has no others gets zeros.  An
@@ -566,9 +567,11 @@ fox_gpu_status fox_gpu_paged_attention(fox_gpu_ctx *ctx, const fox_gpu_paged *ca
  * greater than 0, a NaN too, counts as 0), of equal ones the lower row.  Kept rows from `keep` on, in
  * order, take the places of the rows that are not kept below `keep`, in order:
  * keys, values, weights and positions; the others stay where they are, so few rows move.
- * kept[i] = min(length[i], keep), rows from there on are free.  Sequences that are cut
- * must not share pages.  keep >= 1, recent <= keep; the cache has weight
- * and position; kept is another array than length. */
+ * kept[i] = min(length[i], keep), rows from there on are free; a length past the table's rows
+ * means all of them.  Rows without a page count like others, but where a kept row or its place has
+ * none, weight and position move and keys and values do not: a sequence that is cut should have
+ * pages for all its rows.  Sequences that are cut must not share pages.  keep >= 1, recent <= keep;
+ * the cache has weight and position; kept is another array than length. */
 fox_gpu_status fox_gpu_paged_evict(fox_gpu_ctx *ctx, const fox_gpu_paged *cache,
                                    const uint32_t *length, uint32_t *kept, size_t keep,
                                    size_t recent);
