@@ -95,7 +95,7 @@ struct Terms {
 };
 
 // Angles are counted in turns: what is left of p turn[j] after the nearest quarter is exact,
-// and within an eighth of a turn six and seven terms of sine and cosine are good to 2^-41.
+// and within an eighth of a turn seven terms each of sine and cosine are good to 2^-41.
 // (Angles in floats would be off by 2^-24 of all the turns made.)
 //
 // A thread has four pairs and RT_ROWS rows of them, so speeds are read once; the two tables are
@@ -207,7 +207,7 @@ struct PagedStoreArgs {
     float *q_out;
     size_t q_stride, qo_stride, k_stride, v_stride;
     const uint32_t *pos, *seq, *row;
-    uint32_t n_head, M, n_rot, n_table;
+    uint32_t n_head, n_rot, n_table;
     double by_hd;                 // 1 / head_dim
     float eps;
     int halves;
@@ -413,7 +413,6 @@ extern "C" fox_gpu_status fox_gpu_paged_rope_store(
     A.seq = seq;
     A.row = row;
     A.n_head = (uint32_t)n_head;
-    A.M = (uint32_t)M;
     A.n_rot = (uint32_t)n_rot;
     A.n_table = (uint32_t)n_table;
     A.by_hd = 1.0 / (double)cache->head_dim;

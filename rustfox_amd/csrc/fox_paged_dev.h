@@ -30,12 +30,6 @@ __device__ __forceinline__ uint16_t paged_round(float x)
     return __builtin_bit_cast(uint16_t, (_Float16)x);
 }
 
-template <bool BF>
-__device__ __forceinline__ float paged_float(uint16_t x)
-{
-    return BF ? __uint_as_float((uint32_t)x << 16) : (float)__builtin_bit_cast(_Float16, x);
-}
-
 // Lane l gets the sum of x over lanes 0 .. l, in six adds between neighbours (row shifts, then a
 // row's last lane to the rows after it): a shuffle through LDS takes ten times an add.
 __device__ __forceinline__ uint32_t wave_scan(uint32_t x)
