@@ -76,3 +76,40 @@ def test_a_captured_call_is_divided_anew(gpu):
         assert np.array_equal(out.numpy(), want[i])
     gpu.sync()
     lib.fox_gpu_graph_free(g)
+
+
+@pytest.mark.parametrize("n,n_head,n_kv,hd", [(2, 8, 4, 64), (24, 8, 8, 40), (66, 8, 4, 64), (100, 16, 8, 16)], ids=str)
+def test_caches_on_both_sides(gpu, n, n_head, n_kv, hd):
+    """The longest caches of which a workgroup takes a head, and the shortest that are divided, for few and many
+    heads; more sequences than a wave has lanes, some without rows."""
+    rng = np.random.default_rng(n)
+    caps = [cap for cap in range(32, 4096, 16)
+            if plan(n_head, n_kv, cap, n, [cap] * n)["whole"] != plan(n_head, n_kv, cap + 16, n, [cap] * n)["whole"]]
+    assert len(caps) == 1
+    for cap in (caps[0], caps[0] + 16):
+        lengths = [int(x) for x in cap * rng.random(n) ** 2]
+        lengths[0], lengths[-1] = cap, 0
+        c = Paged(gpu, rng, rf.BF16, n_kv, hd, 16, lengths)
+        assert plan(n_head, n_kv, c.cap, n, lengths)["whole"] == (cap == caps[0])
+        q = rng.standard_normal((n, n_head * hd)).astype(np.float32)
+        check(gpu, c, q, n_head, weigh=True)
+
+
+@pytest.mark.parametrize("n,n_head,n_kv,hd", [(65, 4, 4, 64), (96, 32, 4, 16), (300, 20, 1, 40), (256, 2, 2, 72), (257, 8, 2, 8),
+                                              (1000, 3, 1, 16)], ids=str)
+@pytest.mark.parametrize("kind", [rf.F16, rf.BF16])
+def test_divided_past_a_waves_lanes(gpu, kind, n, n_head, n_kv, hd):
+    """Many sequences' rows in equal runs, found through LDS: some sequences long, most short, some empty (the
+    first and the last, neighbours), rows weighed."""
+    rng = np.random.default_rng(n + hd)
+    lengths = rng.integers(0, 90, n)
+    lengths[rng.integers(0, n, 4)] = [3700, 3000, 64, 129]
+    lengths[rng.integers(1, n, n // 8)] = 0
+    lengths[[0, -1, -2]] = 0
+    c = Paged(gpu, rng, kind, n_kv, hd, 128, [int(x) for x in lengths], room=3800 - int(lengths.max()))
+    assert not plan(n_head, n_kv, c.cap, n, lengths)["whole"]
+    q = rng.standard_normal((n, n_head * hd)).astype(np.float32)
+    got = check(gpu, c, q, n_head, weigh=True)
+    assert (got[lengths == 0] == 0).all()
+    # (sequences given, in their order: divided alike)
+    assert np.array_equal(got, check(gpu, c, q, n_head, seq=np.arange(n)))
