@@ -19,7 +19,8 @@
 // Division.  A row's heads have ceil(length / 64) units of 64 positions, one tile for
 // each wave of a workgroup.  All units of a call, in order of row, head, position, are
 // cut into equal runs, one a workgroup (or each head's, where that wastes little), whatever the
-// lengths, which only the device knows; a
+// lengths, which only the device knows (short caches, and tokens that share rows and are much
+// of a length, are not divided: a workgroup has all of a head); a
 // head whose units lie in several runs is merged by a second launch.  (Merged by the last workgroup
 // to arrive, one launch less takes four times as long: before it counts itself each must write its
 // part past its XCD's cache, and the fence for that empties it.)
@@ -168,7 +169,7 @@ __device__ __forceinline__ bool whole_rows(const PagedAttnArgs &A, uint32_t item
     for (int i = 0; i < EACH; i++) {
         const uint32_t t = tid + i * PA_THREADS;
         const uint32_t u = t < A.M && s[i] < A.C.n_seqs ? units_of(min(n[i], A.C.cap)) : 0;
-        all += (u + 1) / 2;                                  // (256 of at most 2^23)
+        all += min(u, (1u << 24) - 1);                       // (a wave's 256 fit: a row has at most 2^24)
         most = max(most, u);
         same += u && t && s[i] == before[i];
     }
@@ -184,7 +185,7 @@ __device__ __forceinline__ bool whole_rows(const PagedAttnArgs &A, uint32_t item
     uint64_t total = 0;
     most = same = 0;
     for (int i = 0; i < PA_WAVES; i++) {
-        total += (uint64_t)units[i] * 2 * items;
+        total += (uint64_t)units[i] * items;
         most = max(most, longest[i]);
         same += alike[i];
     }
