@@ -252,7 +252,8 @@ __device__ __forceinline__ void load_eight(float x[8], const float *p, bool wide
 // is written, so a query may be turned in place.
 //
 // FAST: rows, tables and weights take 16-byte accesses, and eight dimensions have eight (four) pairs' angles
-// that stand side by side.
+// that stand side by side.  Without, values come one by one: the prompt below takes 49 us with rows that are
+// not aligned, 36 with 120 dimensions turned.
 //
 // Bound by its reads and writes where there are many tokens: 1001 tokens of 32 + 16 + 16 heads of 128 (58 MB)
 // 14.5 us, 4.0 TB/s; 12.5 without norms. (A wave a row, a value a lane: 33.5.)
